@@ -98,6 +98,11 @@ RA_API int ra_debug_step_form(void);
  * current device and those of the cache, the stream and the two sources (-1: not device memory). */
 RA_API int ra_debug_append_route(int device, int cache_device, int stream_device, int k_device, int v_device);
 
+/* Index of row `slot` of a sequence among the rows of KV head 0 of its page, pages one after the other, -1 where there is none
+ * (see ra_paged_kv); `table` is host memory. For tests: it is what the kernels compute. */
+RA_API long long ra_debug_paged_row(const int* table, int max_pages, int num_pages, int page_size, int kv_heads,
+                                    long long slot);
+
 /* ------------------------------------------------------------------ prefill ---- */
 
 /* out = 0, l = 0, m = -inf. Replaces launch_attention_init (src/attention.hpp:73,
@@ -308,6 +313,86 @@ RA_API void ra_kv_cache_reset(ra_kv_cache* c);
 RA_API int ra_local_decode_step(const void* q, const ra_kv_cache* cache, int heads,
                                 int q_pos_global, int cache_k_offset, int causal, float* out,
                                 ra_stream stream);
+
+/* ------------------------------------------- norms and position rotation of Q and K ---- */
+
+/* Rows of every head, (batch, heads, seq, head_dim): the elements of a row are contiguous, rows, heads and batches are this
+ * many elements apart (a projection's token-major output as well as the layout of the attention entry points). */
+typedef struct ra_rows {
+  void* data;
+  long long batch_stride, head_stride, row_stride;
+} ra_rows;
+
+/* A position rotation: pair i of a row, elements (i, i + rot_dim / 2), or (2 i, 2 i + 1) if interleaved, turns by
+ * position * frequency i; elements from rot_dim on stay as they are. turns[i] is the part of a full turn that a position adds,
+ * in units of 2^-64: position * turns modulo 2^64 is the angle's place in its turn, as exact at position 2^31 as at 1. Host
+ * memory, filled by ra_rope_init (frequencies base^(-2 i / rot_dim) * scale) or ra_rope_init_freqs (rot_dim / 2 frequencies in
+ * radians a position). rot_dim: a multiple of 16, up to 256. No counterpart in the reference, which has no rotation. */
+#define RA_ROPE_MAX_PAIRS 128
+typedef struct ra_rope {
+  int rot_dim, interleaved;
+  unsigned long long turns[RA_ROPE_MAX_PAIRS];
+} ra_rope;
+RA_API int ra_rope_init(ra_rope* rope, int rot_dim, int interleaved, double base, double scale);
+RA_API int ra_rope_init_freqs(ra_rope* rope, int rot_dim, int interleaved, const double* freqs);
+
+/* What happens to a row of Q or K: x -> rotate(x / sqrt(mean(x^2) + eps) * weight). A NULL weight: no norm; a NULL rope: no
+ * rotation. Weights: head_dim elements of weight_dtype (that of the rows, or RA_F32). Positions: `positions` (device,
+ * (batch, seq), pos_batch_stride apart) if not NULL, else those of `segmap` and pos_stride, as in ra_attention_step_ex. */
+typedef struct ra_norm_rope {
+  const void* q_weight;
+  const void* k_weight;
+  int weight_dtype;
+  float eps;
+  const ra_rope* rope;
+  const ra_segmap* segmap;
+  int pos_stride;
+  const int* positions;
+  long long pos_batch_stride;
+} ra_norm_rope;
+
+/* Norms of queries and keys for each head with the position rotation in the same pass: q -> q_out (shape->heads heads) and
+ * k -> k_out (kv heads), shape->seq_q = shape->seq_k rows each; q and q_out, or k and k_out, may be NULL. Sums, norms and angles
+ * are held in 32 bits and each result is rounded once to dtype. An output is its input (same address and strides) or shares no
+ * memory with any row that the call reads. head_dim 32, 64, 128 or 256. */
+RA_API int ra_qk_norm_rope(int dtype, const ra_rows* q, const ra_rows* k, const ra_rows* q_out, const ra_rows* k_out,
+                           const ra_shape* shape, const ra_norm_rope* how, ra_stream stream);
+
+/* Its backward pass: from the inputs q, k and the gradients dq_out, dk_out of the results, the gradients dq, dk of the inputs
+ * (rounded once to dtype) and dq_weight, dk_weight of the weights (fp32, head_dim each, overwritten; NULL: not wanted). q and k
+ * are needed where there is a weight and may be NULL elsewhere, with the whole side absent if its gradient is. dq may be dq_out
+ * or q, dk likewise. The weights' gradients are summed in a fixed order, so the same call gives the same bits.
+ * `workspace`: ra_qk_norm_rope_backward_workspace_bytes(head_dim) bytes (needed where a weight's gradient is wanted). */
+RA_API size_t ra_qk_norm_rope_backward_workspace_bytes(int head_dim);
+RA_API int ra_qk_norm_rope_backward(int dtype, const ra_rows* q, const ra_rows* k, const ra_rows* dq_out,
+                                    const ra_rows* dk_out, const ra_rows* dq, const ra_rows* dk, float* dq_weight,
+                                    float* dk_weight, const ra_shape* shape, const ra_norm_rope* how, void* workspace,
+                                    size_t workspace_bytes, ra_stream stream);
+
+/* ------------------------------------------------------------------ paged KV cache ---- */
+
+/* K and V of many sequences in pages of page_size rows: (num_pages, kv_heads, page_size, head_dim), 16-byte aligned. Row j of
+ * sequence b is row j % page_size of page page_table[b * table_stride + j / page_size] (device memory, max_pages entries of a
+ * sequence are read). A page number outside [0, num_pages), such as -1, holds nothing: rows are not written there and its
+ * keys are not seen. `lens` (device, batch): rows of each sequence; one of 0 or less has none. page_size: 16, 32, 64, 128 or 256.
+ * Beside ra_kv_cache, which holds every sequence at full length; no counterpart in the reference. */
+typedef struct ra_paged_kv {
+  int dtype, num_pages, kv_heads, page_size, head_dim;
+  void* k;
+  void* v;
+  int batch, max_pages;
+  long long table_stride;
+  const int* page_table;
+  const int* lens;
+} ra_paged_kv;
+
+/* Appends new rows: row t of k and v ((batch, kv_heads, rows, head_dim) each) becomes row lens[b] + t of sequence b, for
+ * t < counts[b] (device; NULL: all rows; other rows are neither read nor written). K is normed and rotated on the way as `how`
+ * says (NULL: as it is), at position lens[b] + t or how->positions (how->segmap is not used), V is copied. With q, its rows of the
+ * same tokens ((batch, heads, rows, head_dim)) go to q_out in the same launch. Rows that would go behind max_pages or into a page
+ * number out of range are dropped. `lens` is not changed. No two rows of a call may have the same place. */
+RA_API int ra_paged_append(const ra_paged_kv* cache, const ra_rows* k, const ra_rows* v, int rows, const int* counts,
+                           const ra_rows* q, const ra_rows* q_out, int heads, const ra_norm_rope* how, ra_stream stream);
 
 /* ---------------------------------------------------------------- partition ---- */
 

@@ -18,6 +18,7 @@ RA_STEP_CTA_PAIR = 32
 RA_STEP_KEY_SPLIT_SHIFT = 8
 RA_STEP_SPREAD_KEYS = 2048
 RA_MAX_SEG = 16
+RA_ROPE_MAX_PAIRS = 128
 
 STATUS_NAMES = {0: "RA_OK", 1: "RA_ERR_INVALID", 2: "RA_ERR_CUDA", 3: "RA_ERR_UNSUPPORTED",
                 4: "RA_ERR_NCCL", 5: "RA_ERR_DEVICE_WAIT", 6: "RA_ERR_OVERFLOW"}
@@ -59,6 +60,48 @@ class RingResult(C.Structure):
                 ("total_ms", C.c_double)]
 
 
+class Rope(C.Structure):
+    """ra_rope: a position rotation (see ``make`` and ``from_freqs``)."""
+    _fields_ = [("rot_dim", C.c_int), ("interleaved", C.c_int), ("turns", C.c_ulonglong * RA_ROPE_MAX_PAIRS)]
+
+    @classmethod
+    def make(cls, rot_dim, base=10000.0, interleaved=False, scale=1.0):
+        """Pair i of a row turns by ``base ** (-2 * i / rot_dim) * scale`` radians a position."""
+        r = cls()
+        check(lib().ra_rope_init(C.byref(r), rot_dim, int(interleaved), base, scale))
+        return r
+
+    @classmethod
+    def from_freqs(cls, freqs, interleaved=False):
+        """Pair i of a row turns by ``freqs[i]`` radians a position; the first 2 * len(freqs) elements turn."""
+        freqs = [float(f) for f in freqs]
+        if len(freqs) > RA_ROPE_MAX_PAIRS:
+            raise ValueError(f"up to {RA_ROPE_MAX_PAIRS} frequencies, got {len(freqs)}")
+        r = cls()
+        check(lib().ra_rope_init_freqs(C.byref(r), 2 * len(freqs), int(interleaved), (C.c_double * len(freqs))(*freqs)))
+        return r
+
+
+class Rows(C.Structure):
+    """ra_rows: rows of every head, with the strides of batches, heads and rows in elements."""
+    _fields_ = [("data", C.c_void_p), ("batch_stride", C.c_longlong), ("head_stride", C.c_longlong),
+                ("row_stride", C.c_longlong)]
+
+
+class NormRope(C.Structure):
+    """ra_norm_rope: what happens to a row of Q or K."""
+    _fields_ = [("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("weight_dtype", C.c_int), ("eps", C.c_float),
+                ("rope", C.POINTER(Rope)), ("segmap", C.POINTER(SegMap)), ("pos_stride", C.c_int),
+                ("positions", C.c_void_p), ("pos_batch_stride", C.c_longlong)]
+
+
+class PagedKV(C.Structure):
+    """ra_paged_kv: a paged KV cache and the sequences in it."""
+    _fields_ = [("dtype", C.c_int), ("num_pages", C.c_int), ("kv_heads", C.c_int), ("page_size", C.c_int),
+                ("head_dim", C.c_int), ("k", C.c_void_p), ("v", C.c_void_p), ("batch", C.c_int), ("max_pages", C.c_int),
+                ("table_stride", C.c_longlong), ("page_table", C.c_void_p), ("lens", C.c_void_p)]
+
+
 class RingAttentionError(RuntimeError):
     def __init__(self, code, msg):
         super().__init__(f"{STATUS_NAMES.get(code, code)}: {msg}")
@@ -66,6 +109,7 @@ class RingAttentionError(RuntimeError):
 
 
 _P = C.c_void_p
+_ROWS = C.POINTER(Rows)
 _SIG = {
     "ra_last_error": (C.c_char_p, []),
     "ra_version": (C.c_int, []),
@@ -156,6 +200,15 @@ _SIG = {
     "ra_debug_stall_producer_after": (None, [C.c_int]),
     "ra_debug_set_block_order": (None, [C.c_int]),
     "ra_debug_step_form": (C.c_int, []),
+    "ra_rope_init": (C.c_int, [C.POINTER(Rope), C.c_int, C.c_int, C.c_double, C.c_double]),
+    "ra_rope_init_freqs": (C.c_int, [C.POINTER(Rope), C.c_int, C.c_int, C.POINTER(C.c_double)]),
+    "ra_qk_norm_rope": (C.c_int, [C.c_int, _ROWS, _ROWS, _ROWS, _ROWS, C.POINTER(Shape), C.POINTER(NormRope), _P]),
+    "ra_qk_norm_rope_backward_workspace_bytes": (C.c_size_t, [C.c_int]),
+    "ra_qk_norm_rope_backward": (C.c_int, [C.c_int, _ROWS, _ROWS, _ROWS, _ROWS, _ROWS, _ROWS, _P, _P, C.POINTER(Shape),
+                                           C.POINTER(NormRope), _P, C.c_size_t, _P]),
+    "ra_paged_append": (C.c_int, [C.POINTER(PagedKV), _ROWS, _ROWS, C.c_int, _P, _ROWS, _ROWS, C.c_int,
+                                  C.POINTER(NormRope), _P]),
+    "ra_debug_paged_row": (C.c_longlong, [C.POINTER(C.c_int), C.c_int, C.c_int, C.c_int, C.c_int, C.c_longlong]),
     "ra_debug_append_route": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
 }
 

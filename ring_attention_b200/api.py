@@ -15,7 +15,7 @@ import torch
 
 from . import _lib
 from ._lib import (RA_BF16, RA_F16, RA_F32, RA_STEP_CAUSAL, RA_STEP_FINALIZE, RA_STEP_FORCE_SIMT,
-                   RA_STEP_FRESH, RingConfig, RingResult, SegMap, Shape, check, lib)
+                   RA_STEP_FRESH, NormRope, PagedKV, RingConfig, RingResult, Rope, Rows, SegMap, Shape, check, lib)
 
 _DT = {torch.float32: RA_F32, torch.float16: RA_F16, torch.bfloat16: RA_BF16}
 
@@ -471,3 +471,152 @@ class Ring:
                                         owner_rank, cache._h, lens, _ptr(out), _stream(),
                                         C.byref(res) if timed else None))
         return res if timed else None
+
+
+# ---- norms and position rotation of queries and keys; the paged cache ----------------------------
+
+
+def _on_device(*tensors):
+    """Refuses tensors that the kernels of the current device cannot read on its current stream."""
+    dev = _current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError("expected tensors of the current CUDA device")
+
+
+def _rows(t, shape, dtype, out=False):
+    """ra_rows of a (batch, heads, seq, head_dim) tensor with strides of its own and contiguous elements of a row."""
+    if t is None:
+        return None
+    if t.shape != shape or t.dtype != dtype:
+        raise ValueError(f"expected a tensor of {tuple(shape)} in {dtype}, got {tuple(t.shape)} in {t.dtype}")
+    sb, sh, ss, sd = t.stride()
+    if sd != 1:
+        raise ValueError("the elements of a row must be contiguous")
+    if out and (sb == 0 and shape[0] > 1 or sh == 0 and shape[1] > 1 or ss == 0 and shape[2] > 1):
+        raise ValueError("rows of a result must not share memory")
+    return Rows(t.data_ptr(), sb, sh, ss)
+
+
+def _int32(t, shape, name):
+    if t.dtype != torch.int32 or t.shape != shape or shape and t.stride(-1) != 1:
+        raise ValueError(f"{name}: expected an int32 tensor of {tuple(shape)} with contiguous rows")
+    return t.data_ptr()
+
+
+def _norm_rope(dtype, B, S, D, q_weight, k_weight, eps, rope, segmap, pos_stride, positions):
+    """ra_norm_rope of the arguments that the functions below share."""
+    h = NormRope(eps=eps, pos_stride=pos_stride)
+    w_dtype = None
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is None:
+            continue
+        if w.shape != (D,) or w.stride(0) != 1 or w.dtype not in (dtype, torch.float32) or w_dtype not in (None, w.dtype):
+            raise ValueError(f"{name}: expected {D} contiguous elements, of the rows' dtype or fp32, alike for Q and K")
+        w_dtype = w.dtype
+        setattr(h, name, w.data_ptr())
+    if w_dtype is not None:
+        h.weight_dtype = _DT[w_dtype]
+    if rope is not None:
+        h.rope = C.pointer(rope)
+        if positions is not None:
+            if positions.dim() == 1:
+                positions = positions.unsqueeze(0).expand(B, -1)
+            h.positions = _int32(positions, (B, S), "positions")
+            h.pos_batch_stride = positions.stride(0)
+        elif segmap is not None:
+            h.segmap = C.pointer(segmap)
+    return h
+
+
+def qk_norm_rope(q, k, q_out, k_out, *, q_weight=None, k_weight=None, eps=1e-6, rope=None, segmap=None, pos_stride=1,
+                 positions=None):
+    """Norms of queries and keys for each head with the position rotation in the same pass: ``q_out = rotate(q / rms(q) *
+    q_weight)``, ``k_out`` likewise; without a weight no norm, without ``rope`` (a ``Rope``) no rotation. q is (batch, heads,
+    seq, head_dim) and k (batch, kv_heads, seq, head_dim), with any strides but contiguous rows, so a transposed view of a
+    projection's token-major output goes in as it is; either may be None with its result. Results may be the inputs.
+    Row i is at position ``segmap`` / ``pos_stride`` say (``RingPartition.step_maps``), at ``positions`` ((batch, seq) or (seq,),
+    int32), or at i."""
+    one = q if q is not None else k
+    if one is None or (q is None) != (q_out is None) or (k is None) != (k_out is None):
+        raise ValueError("qk_norm_rope: rows without a result, or a result without rows")
+    B, _, S, D = one.shape
+    dt = one.dtype
+    H, kvH = (t.shape[1] if t is not None else 0 for t in (q, k))
+    _on_device(q, k, q_out, k_out, q_weight, k_weight, positions)
+    if rope is not None and segmap is None and positions is None:
+        segmap = SegMap.make([0], S)
+    how = _norm_rope(dt, B, S, D, q_weight, k_weight, eps, rope, segmap, pos_stride, positions)
+    qs, ks = (B, H, S, D), (B, kvH, S, D)
+    check(lib().ra_qk_norm_rope(_dtype(one), _rows(q, qs, dt), _rows(k, ks, dt), _rows(q_out, qs, dt, True),
+                                _rows(k_out, ks, dt, True), Shape(B, H or 1, S, S, D, kvH), how, _stream()))
+
+
+def qk_norm_rope_backward(q, k, dq_out, dk_out, dq, dk, *, dq_weight=None, dk_weight=None, q_weight=None, k_weight=None,
+                          eps=1e-6, rope=None, segmap=None, pos_stride=1, positions=None, workspace=None):
+    """The gradients of ``qk_norm_rope`` with the same keywords: from its inputs q and k (needed where there is a weight) and
+    the gradients dq_out, dk_out of its results into dq, dk (which may be dq_out, dk_out) and, where wanted, dq_weight,
+    dk_weight (fp32, head_dim; overwritten, summed over all rows in a fixed order)."""
+    one = dq_out if dq_out is not None else dk_out
+    if one is None or (dq is None) != (dq_out is None) or (dk is None) != (dk_out is None):
+        raise ValueError("qk_norm_rope_backward: a gradient of the result without one of the rows, or the other way round")
+    B, _, S, D = one.shape
+    dt = one.dtype
+    H, kvH = (t.shape[1] if t is not None else 0 for t in (dq_out, dk_out))
+    _on_device(q, k, dq_out, dk_out, dq, dk, dq_weight, dk_weight, q_weight, k_weight, positions, workspace)
+    if rope is not None and segmap is None and positions is None:
+        segmap = SegMap.make([0], S)
+    how = _norm_rope(dt, B, S, D, q_weight, k_weight, eps, rope, segmap, pos_stride, positions)
+    need = 0
+    for w in (dq_weight, dk_weight):
+        if w is not None:
+            if w.shape != (D,) or w.dtype != torch.float32 or w.stride(0) != 1:
+                raise ValueError(f"gradients of weights are {D} contiguous elements in fp32")
+            need = lib().ra_qk_norm_rope_backward_workspace_bytes(D)
+    if need and workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=one.device)
+    qs, ks = (B, H, S, D), (B, kvH, S, D)
+    check(lib().ra_qk_norm_rope_backward(
+        _dtype(one), _rows(q if q_weight is not None else None, qs, dt), _rows(k if k_weight is not None else None, ks, dt),
+        _rows(dq_out, qs, dt), _rows(dk_out, ks, dt), _rows(dq, qs, dt, True), _rows(dk, ks, dt, True), _ptr(dq_weight),
+        _ptr(dk_weight), Shape(B, H or 1, S, S, D, kvH), how, _ptr(workspace) if need else None,
+        workspace.numel() * workspace.element_size() if need else 0, _stream()))
+
+
+def _paged_kv(k_pages, v_pages, page_table, lens):
+    """ra_paged_kv of the tensors (see ``paged_append``)."""
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or \
+            not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise ValueError("k_pages and v_pages: expected contiguous (num_pages, kv_heads, page_size, head_dim) tensors alike")
+    n, kvH, page, D = k_pages.shape
+    if page_table.dim() != 2:
+        raise ValueError("page_table: expected (batch, max_pages)")
+    B, most = page_table.shape
+    return PagedKV(_dtype(k_pages), n, kvH, page, D, k_pages.data_ptr(), v_pages.data_ptr(), B, most, page_table.stride(0),
+                   _int32(page_table, (B, most), "page_table"), _int32(lens, (B,), "lens"))
+
+
+def paged_append(k, v, k_pages, v_pages, page_table, lens, *, counts=None, rope=None, positions=None, k_weight=None, q=None,
+                 q_out=None, q_weight=None, eps=1e-6):
+    """Appends rows to a paged KV cache, K normed and rotated on the way (see ``qk_norm_rope``; row t at position lens[b] + t
+    or positions[b, t]). k_pages and v_pages are (num_pages, kv_heads, page_size, head_dim); row j of sequence b is in page
+    page_table[b, j // page_size] ((batch, max_pages), int32; a number out of range, such as -1, holds nothing and rows that
+    would go there are dropped). k and v are (batch, kv_heads, rows, head_dim) with any strides but contiguous rows; row t of
+    the first counts[b] (int32; None: all) becomes row lens[b] + t. With q ((batch, heads, rows, head_dim)) the queries of
+    the same tokens go to q_out in the same launch. ``lens`` (int32) stays as it is: the caller adds the counts."""
+    B, kvH, T, D = k.shape
+    dt = k_pages.dtype
+    _on_device(k, v, k_pages, v_pages, page_table, lens, counts, positions, k_weight, q, q_out, q_weight)
+    cache = _paged_kv(k_pages, v_pages, page_table, lens)
+    if (B, kvH, D) != (page_table.shape[0], cache.kv_heads, cache.head_dim):
+        raise ValueError("paged_append: k does not fit the cache")
+    if (q is None) != (q_out is None):
+        raise ValueError("paged_append: queries without a result, or a result without queries")
+    how = None
+    if rope is not None or k_weight is not None or q_weight is not None:
+        how = _norm_rope(dt, B, T, D, q_weight, k_weight, eps, rope, None, 1, positions)
+    H = q.shape[1] if q is not None else 0
+    ks, qs = (B, kvH, T, D), (B, H, T, D)
+    check(lib().ra_paged_append(cache, _rows(k, ks, dt), _rows(v, ks, dt), T,
+                                _int32(counts, (B,), "counts") if counts is not None else None, _rows(q, qs, dt),
+                                _rows(q_out, qs, dt, True), H, how, _stream()))

@@ -35,8 +35,8 @@ def _stale(target, deps):
 
 def _compile(src, verbose):
     obj = os.path.join(OBJ, src[:-3] + ".o")
-    deps = [os.path.join(CSRC, src), os.path.join(CSRC, "common.cuh"), os.path.join(CSRC, "tc_common.cuh"),
-            os.path.join(HERE, "..", "include", "ring_attention_b200.h")]
+    deps = [os.path.join(CSRC, src), os.path.join(HERE, "..", "include", "ring_attention_b200.h")]
+    deps += [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".cuh")]
     if not _stale(obj, deps):
         return obj, ""
     cmd = [NVCC, *FLAGS, "-c", os.path.join(CSRC, src), "-o", obj]
