@@ -394,6 +394,20 @@ typedef struct ra_paged_kv {
 RA_API int ra_paged_append(const ra_paged_kv* cache, const ra_rows* k, const ra_rows* v, int rows, const int* counts,
                            const ra_rows* q, const ra_rows* q_out, int heads, const ra_norm_rope* how, ra_stream stream);
 
+/* Decode attention, one query row a sequence, over the paged cache: out[b, h] = softmax(q[b, h] . K / sqrt(head_dim)) V over
+ * rows j < lens[b] of sequence b (as far as its table reaches); q and out are (batch, heads, head_dim) of the cache's dtype, lse
+ * (batch, heads; fp32, or NULL) gets the log of the sum of exponentials, with which results of other caches or ranks merge. A row
+ * that sees no key gives zeros and -inf. Sums are held in 32 bits; 16-bit caches round the weights of the sum over V to their type,
+ * as ra_attention_decode_step does, and the result once. 16-byte aligned q and out; heads 1 to 4096.
+ * shared_pages: the pages of the first shared_len rows (a multiple of page_size; 0: none) of every sequence that has at least
+ * that many, as a long common prompt has them. They are read once for all sequences instead of once for each; the tables still
+ * have an entry for them, which sequences with fewer rows use.
+ * `workspace`: ra_paged_decode_workspace_bytes(...) bytes, 16-byte aligned, of this call's launches alone. Lengths, tables
+ * and pages are read by the launches: a captured call follows them. */
+RA_API size_t ra_paged_decode_workspace_bytes(const ra_paged_kv* cache, int heads, int shared_len);
+RA_API int ra_paged_decode(const ra_paged_kv* cache, const void* q, int heads, const int* shared_pages, int shared_len,
+                           void* out, float* lse, void* workspace, size_t workspace_bytes, ra_stream stream);
+
 /* ---------------------------------------------------------------- partition ---- */
 
 /* Index maps of RingPartition (src/ring_partition.hpp:11-75, src/ring_partition.cpp:41-108).

@@ -499,7 +499,7 @@ def _rows(t, shape, dtype, out=False):
 
 
 def _int32(t, shape, name):
-    if t.dtype != torch.int32 or t.shape != shape or shape and t.stride(-1) != 1:
+    if t.dtype != torch.int32 or t.shape != shape or shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name}: expected an int32 tensor of {tuple(shape)} with contiguous rows")
     return t.data_ptr()
 
@@ -620,3 +620,25 @@ def paged_append(k, v, k_pages, v_pages, page_table, lens, *, counts=None, rope=
     check(lib().ra_paged_append(cache, _rows(k, ks, dt), _rows(v, ks, dt), T,
                                 _int32(counts, (B,), "counts") if counts is not None else None, _rows(q, qs, dt),
                                 _rows(q_out, qs, dt, True), H, how, _stream()))
+
+
+def paged_decode(q, k_pages, v_pages, page_table, lens, out, *, lse=None, shared_pages=None, workspace=None):
+    """Decode attention of one query row a sequence over a paged KV cache (see ``paged_append``): q and out are (batch, heads,
+    head_dim) in the cache's dtype, query head h reads KV head h % kv_heads, sequence b sees its first lens[b] rows. ``lse``
+    ((batch, heads), fp32) gets the log-sum-exp. A sequence without rows gives zeros and -inf. ``shared_pages`` (int32):
+    the pages that every sequence with at least that many rows begins with; they are read once for all of them."""
+    _on_device(q, k_pages, v_pages, page_table, lens, out, lse, shared_pages, workspace)
+    cache = _paged_kv(k_pages, v_pages, page_table, lens)
+    if q.dim() != 3 or q.dtype != k_pages.dtype or (q.shape[0], q.shape[2]) != (page_table.shape[0], cache.head_dim):
+        raise ValueError("paged_decode: q does not fit the cache")
+    if out.shape != q.shape or out.dtype != q.dtype or \
+            lse is not None and (lse.shape != q.shape[:2] or lse.dtype != torch.float32):
+        raise ValueError("paged_decode: out is like q, lse (batch, heads) in fp32")
+    H, shared_len, pages = q.shape[1], 0, None
+    if shared_pages is not None:
+        shared_len = shared_pages.numel() * cache.page_size
+        pages = _int32(shared_pages, (shared_pages.numel(),), "shared_pages")
+    if workspace is None:
+        workspace = torch.empty(lib().ra_paged_decode_workspace_bytes(cache, H, shared_len), dtype=torch.uint8, device=q.device)
+    check(lib().ra_paged_decode(cache, _ptr(q), H, pages, shared_len, _ptr(out), _ptr(lse), _ptr(workspace),
+                                workspace.numel() * workspace.element_size(), _stream()))

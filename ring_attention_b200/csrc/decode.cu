@@ -33,6 +33,7 @@
 #include <mutex>
 #include <type_traits>
 
+#include "mma16.cuh"
 #include "tc_common.cuh"
 
 namespace rab {
@@ -54,18 +55,6 @@ constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kStages = 4;
 constexpr int kMaxSplits = 128;
-
-__device__ inline void cp_async16(void* smem_dst, const void* gsrc, int src_bytes) {
-  const unsigned d = static_cast<unsigned>(__cvta_generic_to_shared(smem_dst));
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(gsrc),
-               "r"(src_bytes)
-               : "memory");
-}
-__device__ inline void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ inline void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 
 // Unpack one 16-byte piece into floats.
 template <typename T>
@@ -836,49 +825,6 @@ __global__ void __launch_bounds__(GroupCfg<T, D, GB>::kThreads)
 // piece c of row r is stored at piece c ^ (r & 7), so that the ldmatrix reads (8 rows at a
 // fixed column) touch all banks once.
 constexpr int kMmaKeysPerWarp = 16;
-
-template <typename T>
-__device__ inline void mma16816(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1);
-template <>
-__device__ inline void mma16816<__half>(float (&c)[4], const unsigned (&a)[4], unsigned b0,
-                                        unsigned b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <>
-__device__ inline void mma16816<__nv_bfloat16>(float (&c)[4], const unsigned (&a)[4], unsigned b0,
-                                               unsigned b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ inline void ldmatrix_x4(unsigned (&r)[4], unsigned saddr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(saddr));
-}
-__device__ inline void ldmatrix_x4_trans(unsigned (&r)[4], unsigned saddr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(saddr));
-}
-template <typename T>
-__device__ inline unsigned pack_pair(float lo, float hi);
-template <>
-__device__ inline unsigned pack_pair<__half>(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const unsigned*>(&h);
-}
-template <>
-__device__ inline unsigned pack_pair<__nv_bfloat16>(float lo, float hi) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const unsigned*>(&h);
-}
 
 template <int D>
 struct MmaCfg {

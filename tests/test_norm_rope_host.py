@@ -175,6 +175,38 @@ def test_append_refusals():
     assert call(n=0) == 0 and call(c=paged(batch=0)) == 0
 
 
+def test_decode_refusals():
+    L = lib()
+    need = L.ra_paged_decode_workspace_bytes(paged(), 4, 0)
+    assert need > 0 and L.ra_paged_decode_workspace_bytes(paged(), 4, 32) > need
+    assert L.ra_paged_decode_workspace_bytes(None, 4, 0) == 0 and L.ra_paged_decode_workspace_bytes(paged(page_size=7), 4, 0) == 0
+
+    def call(c=paged(), q=P, heads=4, pages=None, n=0, out=P, ws=P, room=1 << 40):
+        return L.ra_paged_decode(c, q, heads, pages, n, out, None, ws, room, None)
+
+    refused(call(c=None), 1, "null")
+    refused(call(q=None), 1, "null")
+    refused(call(out=None), 1, "null")
+    refused(call(q=P + 8), 1, "aligned")
+    refused(call(out=P + 4), 1, "aligned")
+    refused(call(c=paged(dtype=3)), 1, "dtype")
+    refused(call(c=paged(head_dim=80)), 3, "head_dim=80")
+    refused(call(c=paged(page_size=24)), 3, "page_size")
+    refused(call(c=paged(v=None)), 1, "null")
+    refused(call(c=paged(lens=None)), 1, "null")
+    refused(call(heads=1), 1, "heads")
+    refused(call(heads=4097), 1, "heads")
+    refused(call(c=paged(batch=1 << 23)), 1, "rows")
+    refused(call(n=16), 1, "shared")
+    refused(call(pages=P, n=17), 1, "whole")
+    refused(call(pages=P, n=-16), 1, "whole")
+    refused(call(ws=None), 6, "workspace")
+    refused(call(ws=P + 8), 6, "workspace")
+    refused(call(room=need - 1), 6, "workspace")
+    refused(call(c=paged(max_pages=2 ** 31 - 1, batch=4000)), 1, "too many keys")
+    assert call(c=paged(batch=0)) == 0
+
+
 def test_structures_are_those_of_the_header(tmp_path):
     """Sizes and offsets of the fields as a C compiler lays them out."""
     names = {"ra_rope": Rope, "ra_rows": Rows, "ra_norm_rope": NormRope, "ra_paged_kv": PagedKV}
