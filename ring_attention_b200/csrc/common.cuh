@@ -167,6 +167,27 @@ int step_stacked(int dtype, const void* q, const void* k, const void* v, float* 
                  int pos_stride, unsigned flags, long long doc_len, cudaStream_t stream);
 bool step_stacked_supported(int dtype, int head_dim);
 
+// Decode rows of a batch on the shared pages of a 16-bit paged cache (step_tc.cu): every query row that has all of the shared
+// rows, against them. A query block is tiles_per_block tiles of 128 rows, a tile the rows of `pack` heads of all sequences, or
+// (pack 1) 128 sequences of one head; share i of block j leaves (O, m in log2 units, l) of its rows at part
+// (kv head * blocks + j) * shares + i, of tiles_per_block * 128 rows.
+struct SharedPrefix {
+  const void* q;
+  const void* k;
+  const void* v;
+  int B, H, kvH, D;
+  const int* pages;
+  const int* lens;
+  int shared_len, num_pages, max_pages, shift;
+};
+struct SharedPlan {
+  int tiles_per_block, pack, blocks, shares;
+};
+bool plan_shared_prefix(int B, int H, int kvH, int D, int shared_len, SharedPlan* plan);  // false: not by that kernel
+size_t shared_part_rows(const SharedPlan& plan, int kvH);
+int launch_shared_prefix(int dtype, const SharedPrefix& p, const SharedPlan& plan, float* part_o, float2* part_ml,
+                         cudaStream_t stream);
+
 // seq_q == 1 split-K decode step (decode.cu); workspace NULL = per-device buffer.
 int decode_step(int dtype, const void* q, const void* k, const void* v, float* out, float* m,
                 float* l, const ra_shape& s, int q_offset, int k_offset, int causal,

@@ -51,6 +51,11 @@ struct PagedArgs {
   long long* head;  // {stages of a share, first stage of every sequence}
   float2* part_ml;  // (m in log2 units, l) of rs rows, a part after the other
   float* part_o;
+  // shared pages by the tensor-core kernel (step_tc.cu; RB is 0 then): its parts, see SharedPrefix
+  SharedPlan shared;
+  float2* shared_ml;  // NULL: not by it
+  float* shared_o;
+  const int* status;
 };
 
 // Keys [start, end) of a sequence that its own table holds: behind the shared pages if it has all of them.
@@ -182,6 +187,16 @@ __device__ inline int find_share(const PagedArgs& a, Walk<SR>* w, long long* per
   return static_cast<int>(stages);
 }
 
+// Behind the kernel of the shared pages, whose blocks let this one begin when all that came before them has completed, nothing
+// waits for that kernel itself but the end: the fold, which waits for this grid, then finds both kernels' parts.
+__device__ inline void begin_main(const PagedArgs& a) {
+  let_next_start();
+  if (a.shared_ml == nullptr) wait_for_previous();
+}
+__device__ inline void end_main(const PagedArgs& a) {
+  if (a.shared_ml != nullptr) wait_for_previous();
+}
+
 // Query row r of a unit: sequence and head; false where the unit has no such row.
 template <int RU, int SR>
 __device__ inline bool unit_row(const PagedArgs& a, const Walk<SR>& w, int r, int* b, int* h) {
@@ -305,12 +320,14 @@ __global__ void __launch_bounds__(PagedMma<D>::kThreads) paged_mma_kernel(PagedA
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, tq = lane & 3;  // fragment row (and row + 8), column pair
 
-  let_next_start();
-  wait_for_previous();
+  begin_main(a);
   Walk<SR> wc;
   long long per;
   const int total = find_share<SR, C::kThreads>(a, &wc, &per);
-  if (total == 0) return;
+  if (total == 0) {
+    end_main(a);
+    return;
+  }
   Walk<SR> wi = wc;  // ahead of wc by what the ring holds
   Loader<T, D, SR, C::kThreads> load;
   load.look_up(a, wi);
@@ -496,6 +513,7 @@ __global__ void __launch_bounds__(PagedMma<D>::kThreads) paged_mma_kernel(PagedA
     if (s + 1 < total) wc.next(a);
   }
   cp_async_wait<0>();
+  end_main(a);
 }
 
 // ---- fp32 caches --------------------------------------------------------------------
@@ -534,12 +552,14 @@ __global__ void __launch_bounds__(128) paged_f32_kernel(PagedArgs a) {
   int* const ok_ring = reinterpret_cast<int*>(smem + C::kOffOk);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
-  let_next_start();
-  wait_for_previous();
+  begin_main(a);
   Walk<SR> wc;
   long long per;
   const int total = find_share<SR, kThreads>(a, &wc, &per);
-  if (total == 0) return;
+  if (total == 0) {
+    end_main(a);
+    return;
+  }
   Walk<SR> wi = wc;
   Loader<float, D, SR, kThreads> load;
   load.look_up(a, wi);
@@ -677,6 +697,7 @@ __global__ void __launch_bounds__(128) paged_f32_kernel(PagedArgs a) {
     if (s + 1 < total) wc.next(a);
   }
   cp_async_wait<0>();
+  end_main(a);
 }
 
 // ---- fold ---------------------------------------------------------------------------
@@ -717,18 +738,39 @@ __global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const PagedArg
     pre_lo = (c0 + uid) * a.rs + i % RU;
     pre_n = static_cast<int>(c1 - c0) + 1;
   }
-  const bool done = own_n == 1 && start == 0;  // by the block that had the unit
+  long long pre_step = a.rs;
+  const float2* pre_ml = a.part_ml;
+  const float* pre_o = a.part_o;
+  bool lost = false;  // the kernel of the shared pages gave up: the rows stay as they are
+  if (a.shared_ml) {
+    lost = *reinterpret_cast<const volatile int*>(a.status) != 0;
+    if (mine && start > 0) {
+      const SharedPlan& s = a.shared;
+      const int tile = s.pack > 1 ? g / s.pack : b / 128 * a.G + g, at = s.pack > 1 ? g % s.pack * a.B + b : b % 128;
+      pre_step = s.tiles_per_block * 128;
+      pre_lo = (static_cast<long long>(kvh) * s.blocks + tile / s.tiles_per_block) * s.shares * pre_step +
+               tile % s.tiles_per_block * 128 + at;
+      pre_n = s.shares;
+      pre_ml = a.shared_ml;
+      pre_o = a.shared_o;
+    }
+  }
+  const bool done = lost || (own_n == 1 && start == 0);  // by the block that had the unit
   const int parts = mine && !done ? own_n + pre_n : 0;
-  auto part = [&](int i) { return i < pre_n ? pre_lo + static_cast<long long>(i) * a.rs : own_lo + static_cast<long long>(i - pre_n) * a.rs; };
+  auto ml_of_part = [&](int i) { return i < pre_n ? pre_ml[pre_lo + i * pre_step] : a.part_ml[own_lo + static_cast<long long>(i - pre_n) * a.rs]; };
+  auto o_of_part = [&](int i) {
+    const float* const o = i < pre_n ? pre_o + (pre_lo + i * pre_step) * D : a.part_o + (own_lo + static_cast<long long>(i - pre_n) * a.rs) * D;
+    return *reinterpret_cast<const float4*>(o + col * 4);
+  };
   float m_all = -INFINITY;
 #pragma unroll 4
-  for (int i = slice; i < parts; i += kSlices) m_all = fmaxf(m_all, a.part_ml[part(i)].x);
+  for (int i = slice; i < parts; i += kSlices) m_all = fmaxf(m_all, ml_of_part(i).x);
   float l_all = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int i = slice; i < parts; i += kSlices) {
-    const float2 ml = a.part_ml[part(i)];
-    const float4 o = *reinterpret_cast<const float4*>(a.part_o + part(i) * D + col * 4);
+    const float2 ml = ml_of_part(i);
+    const float4 o = o_of_part(i);
     if (ml.y == 0.f) continue;  // saw nothing
     const float f = ml.x > -INFINITY ? ex2(ml.x - m_all) : 1.f;
     l_all += f * ml.y;
@@ -775,8 +817,11 @@ __global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const PagedArg
 // block c's of unit u is part c + u: both only grow along the list, so no two meet.
 struct PagedPlan {
   int RU, SR, blocks;
+  bool tc;  // shared pages by the tensor-core kernel
+  SharedPlan shared;
   double most;  // stages that there can be
-  size_t parts, head_bytes, ml_bytes, bytes;
+  int rs;  // rows of a part
+  size_t parts, head_bytes, ml_bytes, o_bytes, shared_rows, shared_ml_bytes, bytes;
 };
 
 constexpr int kBlocksPerSm = 2;  // of both kernels: 96 KB of ring each
@@ -784,13 +829,15 @@ constexpr int kBlocksPerSm = 2;  // of both kernels: 96 KB of ring each
 int fp32_rows(int G) { return G <= 1 ? 1 : G <= 2 ? 2 : G <= 4 ? 4 : 8; }
 
 PagedPlan make_plan(const ra_paged_kv& c, int heads, int shared_len) {
-  PagedPlan p;
+  PagedPlan p = {};
   const int G = (heads + c.kv_heads - 1) / c.kv_heads;
   const bool f32 = c.dtype == RA_F32;
   const long long rows_shared = shared_len > 0 ? static_cast<long long>(c.batch) * G : 0;
   p.RU = f32 ? fp32_rows(static_cast<int>(std::max<long long>(std::min<long long>(rows_shared, 8), G))) : 16;
   p.SR = f32 ? (c.head_dim == 256 ? 16 : 32) : c.head_dim == 256 ? 32 : 64;
-  const long long HB = (G + p.RU - 1) / p.RU, RB = (rows_shared + p.RU - 1) / p.RU;
+  p.tc = !f32 && rows_shared > 0 && static_cast<long long>(c.num_pages) * c.kv_heads < (1ll << 31) - 1 && c.num_pages > 0 &&
+         plan_shared_prefix(c.batch, heads, c.kv_heads, c.head_dim, shared_len, &p.shared);
+  const long long HB = (G + p.RU - 1) / p.RU, RB = p.tc ? 0 : (rows_shared + p.RU - 1) / p.RU;
   const long long units = c.kv_heads * (RB + c.batch * HB);
   // stages that there are at most: as many as the tables have room for
   const long long room = static_cast<long long>(c.max_pages) * c.page_size;
@@ -799,10 +846,15 @@ PagedPlan make_plan(const ra_paged_kv& c, int heads, int shared_len) {
   const int wave = kBlocksPerSm * sm_count();
   p.blocks = p.most < wave ? static_cast<int>(p.most) : wave;
   p.parts = static_cast<size_t>(units) + p.blocks;
-  const size_t rs = shared_len > 0 ? p.RU : std::min(p.RU, G);
-  p.head_bytes = ((1 + static_cast<size_t>(c.batch)) * 8 + 127) & ~static_cast<size_t>(127);
-  p.ml_bytes = (p.parts * rs * sizeof(float2) + 127) & ~static_cast<size_t>(127);
-  p.bytes = p.head_bytes + p.ml_bytes + p.parts * rs * c.head_dim * sizeof(float);
+  p.rs = RB > 0 ? p.RU : std::min(p.RU, G);
+  const size_t rs = p.rs;
+  auto whole = [](size_t n) { return (n + 127) & ~static_cast<size_t>(127); };
+  p.head_bytes = whole((1 + static_cast<size_t>(c.batch)) * 8);
+  p.ml_bytes = whole(p.parts * rs * sizeof(float2));
+  p.o_bytes = whole(p.parts * rs * c.head_dim * sizeof(float));
+  p.shared_rows = p.tc ? shared_part_rows(p.shared, c.kv_heads) : 0;
+  p.shared_ml_bytes = whole(p.shared_rows * sizeof(float2));
+  p.bytes = p.head_bytes + p.ml_bytes + p.o_bytes + p.shared_ml_bytes + p.shared_rows * c.head_dim * sizeof(float);
   return p;
 }
 
@@ -926,8 +978,8 @@ int ra_paged_decode(const ra_paged_kv* cache, const void* q, int heads, const in
   a.kvH = c.kv_heads;
   a.G = (heads + c.kv_heads - 1) / c.kv_heads;
   a.HB = (a.G + p.RU - 1) / p.RU;
-  a.RB = shared_len > 0 ? static_cast<int>((static_cast<long long>(a.B) * a.G + p.RU - 1) / p.RU) : 0;
-  a.rs = shared_len > 0 ? p.RU : std::min(p.RU, a.G);
+  a.RB = shared_len > 0 && !p.tc ? static_cast<int>((static_cast<long long>(a.B) * a.G + p.RU - 1) / p.RU) : 0;
+  a.rs = p.rs;
   a.min_per = 1;
   a.scale_log2 = kLog2e / std::sqrt(static_cast<float>(c.head_dim));
   unsigned char* const ws = static_cast<unsigned char*>(workspace);
@@ -935,6 +987,18 @@ int ra_paged_decode(const ra_paged_kv* cache, const void* q, int heads, const in
   a.part_ml = reinterpret_cast<float2*>(ws + p.head_bytes);
   a.part_o = reinterpret_cast<float*>(ws + p.head_bytes + p.ml_bytes);
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  a.shared = p.shared;
+  a.shared_ml = nullptr;
+  a.shared_o = nullptr;
+  a.status = nullptr;
+  if (p.tc) {
+    a.shared_ml = reinterpret_cast<float2*>(ws + p.head_bytes + p.ml_bytes + p.o_bytes);
+    a.shared_o = reinterpret_cast<float*>(ws + p.head_bytes + p.ml_bytes + p.o_bytes + p.shared_ml_bytes);
+    a.status = device_status_ptr();
+    const SharedPrefix s{q, c.k, c.v, a.B, a.H, a.kvH, c.head_dim, shared_pages, c.lens, shared_len, c.num_pages, c.max_pages, a.shift};
+    const int rc2 = launch_shared_prefix(c.dtype, s, p.shared, a.shared_o, a.shared_ml, stream);
+    if (rc2 != RA_OK) return rc2;
+  }
   if (c.head_dim == 32) return launch_head_dim<32>(c.dtype, a, p, stream);
   if (c.head_dim == 64) return launch_head_dim<64>(c.dtype, a, p, stream);
   if (c.head_dim == 128) return launch_head_dim<128>(c.dtype, a, p, stream);

@@ -64,6 +64,7 @@
 // of the next launch, which overlap this one) see it in front of their first V and leave the state as it is.
 #include <atomic>
 #include <climits>
+#include <type_traits>
 
 #include "tc_common.cuh"
 
@@ -183,8 +184,10 @@ __device__ inline RingPos ring_pos(int which, int t, int sub) {
 // states through distributed shared memory (see pick_key_split).
 // kFold: the two query tiles of a block are a light and a heavy one of the head (see fold_rows).
 // kSpread: a block takes a share of the key tiles of two query tiles of a KV head, into a workspace (see plan_spread).
+// kPaged: that form on the shared pages of a paged cache, with the sequences of a decode batch as the query rows (see
+// launch_shared_prefix).
 template <int D, bool kBf16, bool kPInTmem, int DR, bool kPair = false, bool kSplit = false, bool kFold = false,
-          bool kSpread = false>
+          bool kSpread = false, bool kPaged = false>
 __global__ void __launch_bounds__((TcCfg<D, kPInTmem, kPair, kSplit, kFold>::kThreads), 1)
     step_tc_kernel(const __grid_constant__ CUtensorMap tmap_q,
                    const __grid_constant__ CUtensorMap tmap_k,
@@ -222,7 +225,7 @@ __global__ void __launch_bounds__((TcCfg<D, kPInTmem, kPair, kSplit, kFold>::kTh
 
   // The status word (see below) is on its way while the block sets itself up.
   const int gone = tid == 0 ? *reinterpret_cast<volatile int*>(a.status) : 0;
-  let_next_start();
+  if constexpr (!kPaged) let_next_start();
 
   const bool causal = (a.flags & RA_STEP_CAUSAL) != 0;
   const bool fresh = (a.flags & RA_STEP_FRESH) != 0;
@@ -409,6 +412,8 @@ __global__ void __launch_bounds__((TcCfg<D, kPInTmem, kPair, kSplit, kFold>::kTh
   // Everything so far touched no memory but the status word. A word that is set says to leave; one that is not may
   // yet be set by a launch before this one, so the producer reads it again.
   wait_for_previous();
+  // (what follows may begin when every block is here, and need not wait for what came before: see paged_decode.cu)
+  if constexpr (kPaged) let_next_start();
   if (leave) {
     if (warp == 1)
       asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem_base) : "memory");
@@ -422,7 +427,62 @@ __global__ void __launch_bounds__((TcCfg<D, kPInTmem, kPair, kSplit, kFold>::kTh
     if constexpr (C::kTiles == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(RAB_REGS_LO));
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer ----
-    if (lane == 0 && n_tiles > 0) {
+    if constexpr (kPaged) {
+      // A key tile lies in up to eight pages, so the lanes of the warp issue its copies, a piece of a page and 64 columns
+      // each. Pieces behind the last page, and pages that there are not, are copied from out of bounds: zeros.
+      if (n_tiles > 0) {
+        const int lost = *reinterpret_cast<volatile int*>(a.status);
+        if (lane == 0) {
+          for (int w = 0; w < live; ++w) {
+            mbar_expect_tx(bar_q_full + 8 * w, C::kBoxes * (a.spread.pack > 1 ? a.spread.pack * a.Sq : kBM) * 128);
+            for (int bx = 0; bx < C::kBoxes; ++bx)
+              tma_load_5d(s_q + w * C::kTileBytes + bx * (kBM * 128), &tmap_q, bar_q_full + 8 * w, bx * 64, tile_row0(w),
+                          static_cast<int>(blockIdx.y), tile_head(w), 0);
+          }
+        }
+        const int shift = a.paged.shift, rows = min(1 << shift, kBN), pieces = kBN / rows;
+        const int piece = lane % pieces, bx = lane / pieces;
+        bool ok = true;
+        auto head_of = [&](int tile) {  // of this lane's piece
+          const int key = tile * kBN + piece * rows;
+          const int page = key < a.kmap.seg_len ? a.paged.pages[key >> shift] : -1;
+          return page >= 0 && page < a.paged.num_pages ? page * a.kvH + static_cast<int>(blockIdx.y) : a.paged.num_pages * a.kvH;
+        };
+        auto load_items = [&](int which, int j, int tile, int head) {
+          if (which == 1 && lost != 0) {
+            *abort_flag = 1;
+            ok = false;
+          }
+          for (int sub = 0; sub < C::kItemsPerTile && ok; ++sub) {
+            const RingPos pos = ring_pos<C>(which, j, sub);
+            if (pos.use >= 1)
+              ok = __all_sync(0xffffffffu, mbar_wait(bar_kv_empty + 8 * pos.slot, (pos.use + 1) & 1, abort_flag, a.status, 1, j,
+                                                     a.wait_ns)) != 0;
+            if (a.stall_after >= 0 && (2 * j + which) * C::kItemsPerTile + sub >= a.stall_after) ok = false;  // (test hook)
+            if (!ok) break;
+            if (lane == 0) mbar_expect_tx(bar_kv_full + 8 * pos.slot, C::kItemBytes);
+            __syncwarp();
+            if (bx < C::kBoxesPerItem)
+              tma_load_3d(s_kv + pos.slot * C::kItemBytes + bx * (kBN * 128) + piece * rows * 128, which == 0 ? &tmap_k : &tmap_v,
+                          bar_kv_full + 8 * pos.slot, (sub * C::kBoxesPerItem + bx) * 64,
+                          (tile * kBN + piece * rows) & ((1 << shift) - 1), head);
+          }
+        };
+        int head = head_of(share_beg), v_head = 0;
+        for (int j = 0; j < n_tiles && ok; ++j) {
+          const int tile = share_beg + j, next = j + 1 < n_tiles ? head_of(tile + 1) : 0;
+          load_items(0, j, tile, head);
+          if constexpr (C::kSplitRing) {
+            if (j > 0) load_items(1, j - 1, tile - 1, v_head);
+            v_head = head;
+          } else {
+            load_items(1, j, tile, head);
+          }
+          head = next;
+        }
+        if (C::kSplitRing && ok) load_items(1, n_tiles - 1, share_beg + n_tiles - 1, v_head);
+      }
+    } else if (lane == 0 && n_tiles > 0) {
       // The status word once more: `gone` was read while an earlier launch may still have been running. Behind one that
       // gave up no V comes, and the block unwinds without a store. (Read here, looked at in front of a V: nothing waits
       // for it. Read by the softmax warps under the last MMAs it cost a call 0.15 to 0.4 us.)
@@ -830,6 +890,18 @@ __global__ void __launch_bounds__((TcCfg<D, kPInTmem, kPair, kSplit, kFold>::kTh
         row_valid = w < live && g < a.spread.pack && tile_head(w) + g < group;
       }
     }
+    if constexpr (kPaged) {  // sequences that do not have all of the shared rows are not served here
+      const long long room = static_cast<long long>(a.paged.max_pages) << a.paged.shift;
+      row_valid = row_valid && min(static_cast<long long>(a.paged.lens[r_in_seg]), room) >= a.kmap.seg_len;
+    }
+    // 16-key blocks of a tile whose page is out of range; lane i looks at block i, a tile ahead of its use
+    [[maybe_unused]] auto no_page = [&](int t) {
+      const int key = t * kBN + lane * 16;
+      const int page = lane < kBN / 16 && key < a.kmap.seg_len ? a.paged.pages[key >> a.paged.shift] : 0;
+      return page < 0 || page >= a.paged.num_pages;
+    };
+    [[maybe_unused]] bool gone_next = false;
+    if constexpr (kPaged) gone_next = n_tiles > 0 && no_page(share_beg);
     const int qpos = a.qmap.base[tile_sq(w)] + r_in_seg * a.stride;
     const int n_own = kFold && w == 1 ? n_light : n_tiles;  // key tiles of this query tile
     const long long qdoc = a.doc_len > 0 ? qpos / a.doc_len : 0;
@@ -886,7 +958,13 @@ __global__ void __launch_bounds__((TcCfg<D, kPInTmem, kPair, kSplit, kFold>::kTh
         int c_lo = min(max(rel_lo - t * kBN, 0), kBN);
         int c_hi = min(max(rel_hi - t * kBN, 0), kBN);
         if (c_hi < c_lo) c_hi = c_lo;
-        const bool full = __all_sync(0xffffffffu, (kNoVote && !row_valid) || (c_lo == 0 && c_hi == kBN));
+        bool full = __all_sync(0xffffffffu, (kNoVote && !row_valid) || (c_lo == 0 && c_hi == kBN));
+        [[maybe_unused]] unsigned no_keys = 0;
+        if constexpr (kPaged) {
+          no_keys = __ballot_sync(0xffffffffu, gone_next);
+          gone_next = t + 1 < tr.hi && no_page(t + 1);
+          full = full && no_keys == 0;
+        }
 
         // (double S: buffer j & 1 and its barrier, used every other tile)
         const int sbuf = C::kDoubleS ? (j & 1) : 0;
@@ -912,7 +990,8 @@ __global__ void __launch_bounds__((TcCfg<D, kPInTmem, kPair, kSplit, kFold>::kTh
         if (!full) {
           // hidden columns become -inf, which the exponential below turns into exactly 0
 #pragma unroll
-          for (int i = 0; i < kBN; ++i) s[i] = (i >= c_lo && i < c_hi) ? s[i] : -INFINITY;
+          for (int i = 0; i < kBN; ++i)
+            s[i] = (i >= c_lo && i < c_hi && !(kPaged && (no_keys >> (i / 16) & 1u))) ? s[i] : -INFINITY;
         }
 
         // P = 2^(s * scale - m_ref), two columns at a time (packed fp32x2 multiply-add and add),
@@ -1392,6 +1471,55 @@ int launch_cfg(const StepArgs& a, cudaStream_t stream, int key_split = 1, const 
   return RA_OK;
 }
 
+// The kPaged form: rows are the sequences of a decode batch, every query block sees all keys and has `n` shares.
+template <int D, bool kBf16, int DR>
+int launch_paged(const SharedPrefix& p, const SharedPlan& plan, float* part_o, float2* part_ml, cudaStream_t stream) {
+  using C = TcCfg<D, true>;
+  CUtensorMap mq, mk, mv;
+  const int dtype = kBf16 ? RA_BF16 : RA_F16;
+  int rc = make_decode_query_map(&mq, dtype, p.q, p.D, p.B, p.H, p.kvH, plan.pack > 1 ? p.B : kBM, plan.pack);
+  if (rc != RA_OK) return rc;
+  const int page = 1 << p.shift;
+  const long long heads = static_cast<long long>(p.num_pages) * p.kvH;
+  rc = make_map(&mk, dtype, p.k, p.D, page, heads, static_cast<long long>(page) * p.D, std::min(page, kBN));
+  if (rc != RA_OK) return rc;
+  rc = make_map(&mv, dtype, p.v, p.D, page, heads, static_cast<long long>(page) * p.D, std::min(page, kBN));
+  if (rc != RA_OK) return rc;
+  TcArgs t;
+  std::memset(&t, 0, sizeof(t));
+  t.H = p.H;
+  t.kvH = p.kvH;
+  t.Sq = p.B;
+  t.n_qblocks_per_seg = (p.B + kBM - 1) / kBM;
+  t.qmap = affine_posmap(0, p.B);
+  t.kmap = affine_posmap(0, p.shared_len);
+  t.stride = 1;
+  t.status = device_status_ptr();
+  RAB_REQUIRE(t.status != nullptr, RA_ERR_CUDA, "paged_decode: no device status word");
+  t.wait_ns = g_wait_ns.load(std::memory_order_relaxed);
+  t.stall_after = g_stall_after.load(std::memory_order_relaxed);
+  t.key_split = 1;
+  t.spread.total = plan.blocks * plan.shares;
+  t.spread.pack = plan.pack;
+  for (int j = 0; j <= kMaxSpread; ++j)
+    t.spread.beg[j] = static_cast<unsigned char>(std::min(j, plan.blocks) * plan.shares);
+  t.part_o = part_o;
+  t.part_ml = part_ml;
+  t.paged = {p.pages, p.lens, p.num_pages, p.max_pages, p.shift};
+  auto kern = step_tc_kernel<D, kBf16, true, DR, false, false, false, true, true>;
+  static std::atomic<unsigned long long> smem_set{0};
+  int dev = 0;
+  RAB_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !(smem_set.load(std::memory_order_acquire) >> dev & 1ull)) {
+    RAB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
+    if (dev >= 0 && dev < 64) smem_set.fetch_or(1ull << dev, std::memory_order_release);
+  }
+  set_step_form(1 | 128);
+  RAB_CUDA(launch_overlapped(kern, dim3(static_cast<unsigned>(t.spread.total), static_cast<unsigned>(p.kvH)), dim3(C::kThreads),
+                             C::kSmemBytes, stream, mq, mk, mv, t));
+  return RA_OK;
+}
+
 template <int D, int DR>
 int launch_split(int dtype, const StepArgs& a, cudaStream_t stream, int n) {
   return dtype == RA_BF16 ? launch_cfg<D, true, true, DR, false, true>(a, stream, n)
@@ -1502,6 +1630,48 @@ bool step_tc_supported(int dtype, const StepArgs& a) {
        reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.out)) & 15u)
     return false;
   return true;
+}
+
+// Shares of a query block's key tiles, for the least time of the last block: a block costs its tiles and kBlock of prologue and
+// end. As many as fill the SMs once, or twice where more query blocks than SMs want it.
+bool plan_shared_prefix(int B, int H, int kvH, int D, int shared_len, SharedPlan* plan) {
+  if (H % kvH != 0) return false;
+  const int group = H / kvH, kTiles = D == 256 ? 1 : 2;
+  plan->pack = 2 * B <= kBM ? std::min(group, kBM / B) : 1;
+  const long long tiles = plan->pack > 1 ? (group + plan->pack - 1) / plan->pack : static_cast<long long>(group) * ((B + kBM - 1) / kBM);
+  const long long blocks = (tiles + kTiles - 1) / kTiles;
+  if (blocks > kMaxSpread) return false;
+  plan->tiles_per_block = kTiles;
+  plan->blocks = static_cast<int>(blocks);
+  const int keys = (shared_len + kBN - 1) / kBN, sms = sm_count();
+  constexpr int kBlock = 6;
+  plan->shares = 1;
+  long long best = -1;
+  for (int n = 1; n <= keys && n * blocks <= kMaxSpread; ++n) {
+    const long long waves = (n * blocks * kvH + sms - 1) / sms;
+    const long long cost = waves * ((keys + n - 1) / n + kBlock);
+    if (best < 0 || cost < best) {
+      best = cost;
+      plan->shares = n;
+    }
+  }
+  return true;
+}
+
+size_t shared_part_rows(const SharedPlan& plan, int kvH) {
+  return static_cast<size_t>(kvH) * plan.blocks * plan.shares * plan.tiles_per_block * kBM;
+}
+
+int launch_shared_prefix(int dtype, const SharedPrefix& p, const SharedPlan& plan, float* part_o, float2* part_ml,
+                         cudaStream_t stream) {
+  auto go = [&](auto bf16) {
+    constexpr bool kB = decltype(bf16)::value;
+    if (p.D == 32) return launch_paged<64, kB, 32>(p, plan, part_o, part_ml, stream);
+    if (p.D == 64) return launch_paged<64, kB, 64>(p, plan, part_o, part_ml, stream);
+    if (p.D == 128) return launch_paged<128, kB, 128>(p, plan, part_o, part_ml, stream);
+    return launch_paged<256, kB, 256>(p, plan, part_o, part_ml, stream);
+  };
+  return dtype == RA_BF16 ? go(std::true_type()) : go(std::false_type());
 }
 
 size_t step_tc_workspace_bytes(const StepArgs& a) {

@@ -550,6 +550,11 @@ struct TcArgs {
   Spread spread;               // spread form: the shares, and where their partial states go
   float* part_o;
   float2* part_ml;
+  struct {  // shared pages of a paged cache (see ra_paged_decode); kmap has their rows as one segment
+    const int* pages;
+    const int* lens;
+    int num_pages, max_pages, shift;
+  } paged;
 };
 
 // What a block does whose rows see no key: nothing, or the state of `rows` rows from row0 on is written empty
@@ -820,6 +825,24 @@ inline int make_query_map(CUtensorMap* map, int dtype, const StepArgs& a, int bo
   const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   const CUresult r = fn(map, dtype == RA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
                         const_cast<void*>(a.q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  RAB_REQUIRE(r == CUDA_SUCCESS, RA_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", static_cast<int>(r));
+  return RA_OK;
+}
+
+// The 16-bit queries of a decode batch, (sequences, heads, D), as (D, sequences, kv heads, heads that share one, 1).
+inline int make_decode_query_map(CUtensorMap* map, int dtype, const void* q, int D, int B, int H, int kvH, int box_rows,
+                                 int box_heads) {
+  EncodeTiledFn fn = encode_fn();
+  RAB_REQUIRE(fn != nullptr, RA_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t head = static_cast<cuuint64_t>(D) * 2;
+  const cuuint64_t dims[5] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(B), static_cast<cuuint64_t>(kvH),
+                              static_cast<cuuint64_t>(H / kvH), 1};
+  const cuuint64_t strides[4] = {head * H, head, head * kvH, head * H * B};
+  const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(box_rows), 1, static_cast<cuuint32_t>(box_heads), 1};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  const CUresult r = fn(map, dtype == RA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
+                        const_cast<void*>(q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   RAB_REQUIRE(r == CUDA_SUCCESS, RA_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", static_cast<int>(r));
   return RA_OK;
