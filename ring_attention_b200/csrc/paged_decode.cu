@@ -6,12 +6,19 @@
 // What bounds it is the cache: every row is read once. The work is cut into units, the up to RU query rows that read the same
 // keys: the heads of a KV head and a sequence, behind the shared pages where the sequence has them; and for the shared pages RU
 // rows of all sequences. A unit is a list of stages of SR keys, and all units' stages one after the other are dealt in equal
-// shares to the blocks of one wave, so that lengths do not matter to the balance. A block streams its share through a
-// shared-memory ring without a pause where units meet (16-byte cp.async; page numbers are read a stage ahead). A unit that lies in one
-// share is finished there; of others every share leaves (O, m, l) in the workspace, and a second kernel folds them.
+// shares to the blocks of one wave, so that lengths do not matter to the balance. A unit that lies in one share is finished
+// there; of others every share leaves (O, m, l) in the workspace, and a second kernel folds them.
+//
+// Inside a block one warp walks the list, looks the pages up a stage ahead and copies a stage's rows with TMA (a piece of a page
+// and 128 bytes of its rows a lane, 128-byte swizzle) into a ring of 96 KB, two blocks to an SM; it leaves beside each stage what
+// the other warps have to know of it. Each of those takes its own keys of a stage, with a running maximum, sum and O of
+// its own: nothing meets before the end of a unit, and the copies run on across units.
 //
 // 16-bit caches: both products on mma.sync m16n8k16, the unit's rows as its M rows, as in decode_mma_kernel (decode.cu). fp32:
-// plain multiply-adds, the scores of a stage by groups of lanes and its values by columns.
+// plain multiply-adds, four or eight lanes to a key for the scores, four columns a lane for the sum over V.
+//
+// Every wait on a barrier is bounded, as in the step kernels: when one runs out the block records it in the device status word
+// and leaves, and the fold leaves every row that it would have written as it is.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -31,8 +38,6 @@ using tcgen::kLog2e;
 
 struct PagedArgs {
   const void* q;
-  const void* k;
-  const void* v;
   void* out;
   float* lse;  // or NULL
   const int* table;
@@ -42,20 +47,20 @@ struct PagedArgs {
   int shared_len;  // rows in shared pages
   int num_pages, max_pages, shift;
   int B, H, kvH;
-  int G;          // heads of a KV head, at most
-  int HB;         // units of a KV head and a sequence
-  int RB;         // units of a KV head on the shared pages (0: not by this kernel)
-  int rs;         // rows of a part in the workspace
-  int min_per;    // stages of a share, at least
+  int G;   // heads of a KV head, at most
+  int HB;  // units of a KV head and a sequence
+  int RB;  // units of a KV head on the shared pages (0: not by this kernel)
+  int rs;  // rows of a part in the workspace
   float scale_log2;
-  long long* head;  // {stages of a share, first stage of every sequence}
-  float2* part_ml;  // (m in log2 units, l) of rs rows, a part after the other
+  int2* unit_parts;  // first block that has a part of a unit, and how many do
+  float2* part_ml;   // (m in log2 units, l) of rs rows, a part after the other
   float* part_o;
   // shared pages by the tensor-core kernel (step_tc.cu; RB is 0 then): its parts, see SharedPrefix
   SharedPlan shared;
   float2* shared_ml;  // NULL: not by it
   float* shared_o;
-  const int* status;
+  int* status;
+  unsigned long long wait_ns;
 };
 
 // Keys [start, end) of a sequence that its own table holds: behind the shared pages if it has all of them.
@@ -74,16 +79,16 @@ __device__ inline int own_stages(const PagedArgs& a, int b) {
 // A place in the list of stages.
 template <int SR>
 struct Walk {
-  int uid;          // number of the unit; units on the shared pages come first
-  int b, kvh, hb;   // b = -1: on the shared pages
-  int st, n;        // stage of the unit and how many it has
-  int start, end;   // its keys
-  __device__ inline int prefix_stages(const PagedArgs& a) const { return (a.shared_len + SR - 1) / SR; }
+  int uid;         // number of the unit; units on the shared pages come first
+  int b, kvh, hb;  // b = -1: on the shared pages
+  int st, n;       // stage of the unit and how many it has
+  int start, end;  // its keys
+  __device__ inline int shared_stages(const PagedArgs& a) const { return (a.shared_len + SR - 1) / SR; }
   __device__ inline void on_shared(const PagedArgs& a) {
     b = -1;
     start = 0;
     end = a.shared_len;
-    n = prefix_stages(a);
+    n = shared_stages(a);
   }
   __device__ inline void on_sequence(const PagedArgs& a, int seq) {
     b = seq;
@@ -91,6 +96,7 @@ struct Walk {
     n = static_cast<int>((static_cast<long long>(end) - start + SR - 1) / SR);
   }
   __device__ inline void number(const PagedArgs& a) { uid = b < 0 ? kvh * a.RB + hb : a.kvH * a.RB + (b * a.kvH + kvh) * a.HB + hb; }
+  __device__ inline int left() const { return end - start - st * SR; }  // keys from this stage on
   // On to the next stage; there has to be one.
   __device__ inline void next(const PagedArgs& a) {
     if (++st < n) return;
@@ -108,9 +114,17 @@ struct Walk {
   }
 };
 
+// Room of find_share.
+template <int kThreads>
+struct ScanRoom {
+  long long sums[kThreads / 32];
+  long long in_seq;
+  int seq;
+};
+
 // Sum over the block of a thread's v, and the sum over the threads before it.
 template <int kThreads>
-__device__ inline long long block_scan(long long v, long long* total, long long* room) {
+__device__ inline long long block_scan(long long v, long long* total, ScanRoom<kThreads>* room) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   long long incl = v;
 #pragma unroll
@@ -119,65 +133,59 @@ __device__ inline long long block_scan(long long v, long long* total, long long*
     if (lane >= i) incl += o;
   }
   __syncthreads();
-  if (lane == 31) room[warp] = incl;
+  if (lane == 31) room->sums[warp] = incl;
   __syncthreads();
   long long before = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) before += room[w];
-    all += room[w];
+    if (w < warp) before += room->sums[w];
+    all += room->sums[w];
   }
   *total = all;
   return before + incl - v;
 }
 
-// The block's share: its first place and how many stages; *per: stages of a share. Block 0 writes the head of the workspace.
+// The block's share: its first place, and how many stages; *per: stages of a whole share.
 template <int SR, int kThreads>
-__device__ inline int find_share(const PagedArgs& a, Walk<SR>* w, long long* per) {
-  __shared__ long long room[kThreads / 32];
-  __shared__ int seq;
-  __shared__ long long in_seq;
+__device__ inline int find_share(const PagedArgs& a, Walk<SR>* w, int* per, ScanRoom<kThreads>* room) {
   const int units = a.kvH * a.HB;
   long long shared_total = 0;
-  if (a.RB > 0) shared_total = static_cast<long long>(a.kvH) * a.RB * w->prefix_stages(a);
+  if (a.RB > 0) shared_total = static_cast<long long>(a.kvH) * a.RB * w->shared_stages(a);
   // the first chunk of sequences stays at hand
   const int mine = static_cast<int>(threadIdx.x) < a.B ? own_stages<SR>(a, threadIdx.x) : 0;
   long long sum = mine, total;
   for (int b = static_cast<int>(threadIdx.x) + kThreads; b < a.B; b += kThreads) sum += own_stages<SR>(a, b);
-  block_scan<kThreads>(sum, &total, room);
+  const long long before = block_scan<kThreads>(sum, &total, room);
   const long long all = shared_total + total * units;
-  *per = max(static_cast<long long>(a.min_per), (all + gridDim.x - 1) / gridDim.x);
-  const long long first = *per * blockIdx.x, stages = min(*per, all - first);
-  const bool writer = blockIdx.x == 0;
-  if (writer && threadIdx.x == 0) a.head[0] = *per;
-  if (stages <= 0 && !writer) return 0;
-  const bool on_shared = first < shared_total;
-  if (!on_shared || writer) {
-    long long base = shared_total;
-    for (int b0 = 0; b0 < a.B; b0 += kThreads) {
-      const int b = b0 + static_cast<int>(threadIdx.x);
-      const long long n = (b0 == 0 ? mine : b < a.B ? own_stages<SR>(a, b) : 0) * static_cast<long long>(units);
-      long long chunk;
-      const long long at = base + block_scan<kThreads>(n, &chunk, room);
-      if (writer && b < a.B) a.head[1 + b] = at;
-      if (first >= at && first < at + n) {
-        seq = b;
-        in_seq = first - at;
-      }
-      base += chunk;
-      if (!writer && first < base) break;
-    }
-    __syncthreads();
-  }
+  const long long share = max(1ll, (all + gridDim.x - 1) / gridDim.x);
+  *per = static_cast<int>(share);
+  const long long first = share * blockIdx.x, stages = min(share, all - first);
   if (stages <= 0) return 0;
-  if (on_shared) {
+  if (first < shared_total) {
     w->on_shared(a);
     const int u = static_cast<int>(first / w->n);
     w->st = static_cast<int>(first - static_cast<long long>(u) * w->n);
     w->kvh = u / a.RB;
     w->hb = u % a.RB;
   } else {
-    w->on_sequence(a, seq);
+    long long base = shared_total;
+    for (int b0 = 0; b0 < a.B && base <= first; b0 += kThreads) {
+      const int b = b0 + static_cast<int>(threadIdx.x);
+      long long n = mine, chunk = total, ahead = before;  // (of the only chunk)
+      if (a.B > kThreads) {
+        if (b0 > 0) n = b < a.B ? own_stages<SR>(a, b) : 0;
+        ahead = block_scan<kThreads>(n, &chunk, room);
+      }
+      const long long at = base + ahead * units;
+      if (first >= at && first < at + n * units) {
+        room->seq = b;
+        room->in_seq = first - at;
+      }
+      base += chunk * units;
+    }
+    __syncthreads();
+    w->on_sequence(a, room->seq);
+    const long long in_seq = room->in_seq;
     const int u = static_cast<int>(in_seq / w->n);
     w->st = static_cast<int>(in_seq - static_cast<long long>(u) * w->n);
     w->kvh = u / a.HB;
@@ -187,66 +195,23 @@ __device__ inline int find_share(const PagedArgs& a, Walk<SR>* w, long long* per
   return static_cast<int>(stages);
 }
 
-// Behind the kernel of the shared pages, whose blocks let this one begin when all that came before them has completed, nothing
-// waits for that kernel itself but the end: the fold, which waits for this grid, then finds both kernels' parts.
-__device__ inline void begin_main(const PagedArgs& a) {
-  let_next_start();
-  if (a.shared_ml == nullptr) wait_for_previous();
-}
-__device__ inline void end_main(const PagedArgs& a) {
-  if (a.shared_ml != nullptr) wait_for_previous();
-}
+// What the warps that compute have to know of a stage.
+struct StageInfo {
+  int b, kvh, hb, uid;
+  int keys;        // of the stage
+  unsigned pages;  // bit i: keys 16 i and on are there
+  int first;       // of the block's part of the unit
+  int last;        // the same; 2: and the part is the result, the unit being whole and no shared pages ahead of it
+};
 
 // Query row r of a unit: sequence and head; false where the unit has no such row.
-template <int RU, int SR>
-__device__ inline bool unit_row(const PagedArgs& a, const Walk<SR>& w, int r, int* b, int* h) {
-  const int i = w.hb * RU + r, g = w.b < 0 ? i % a.G : i;
-  *b = w.b < 0 ? i / a.G : w.b;
-  *h = w.kvh + a.kvH * g;
+template <int RU>
+__device__ inline bool unit_row(const PagedArgs& a, const StageInfo& u, int r, int* b, int* h) {
+  const int i = u.hb * RU + r, g = u.b < 0 ? i % a.G : i;
+  *b = u.b < 0 ? i / a.G : u.b;
+  *h = u.kvh + a.kvH * g;
   return *b < a.B && *h < a.H;
 }
-
-// Row indexes in the cache of the 16-key blocks of a stage (-1: none), and the asynchronous copies of a stage.
-template <typename T, int D, int SR, int kThreads>
-struct Loader {
-  static constexpr int kPieces = D * static_cast<int>(sizeof(T)) / 16;
-  static constexpr int kBlocks = SR / 16;
-  long long at[kBlocks];
-  // a 16-byte piece's place in its row, so that neither the rows of an ldmatrix nor the lanes that share out a row meet in a bank
-  __device__ static inline int place(int r, int c) {
-    if constexpr (sizeof(T) == 4) return c ^ ((r & 1) << 2);
-    else return kPieces == 4 ? c ^ ((r >> 1) & 3) : c ^ (r & 7);
-  }
-  __device__ inline void look_up(const PagedArgs& a, const Walk<SR>& w) {
-    const int* table = w.b < 0 ? a.shared_pages : a.table + w.b * a.table_stride;
-    const int most = w.b < 0 ? a.shared_len >> a.shift : a.max_pages;
-#pragma unroll
-    for (int i = 0; i < kBlocks; ++i) {
-      const long long slot = static_cast<long long>(w.start) + static_cast<long long>(w.st) * SR + 16 * i;
-      const long long row = slot < w.end ? paged_row(table, most, a.num_pages, a.shift, a.kvH, slot) : -1;
-      at[i] = row < 0 ? -1 : row + (static_cast<long long>(w.kvh) << a.shift);
-    }
-  }
-  __device__ inline void issue(const PagedArgs& a, const Walk<SR>& w, unsigned char* k_slot, unsigned char* v_slot, int* ok) const {
-    const int tid = threadIdx.x;
-    const int left = w.end - w.start - w.st * SR;
-#pragma unroll
-    for (int i = 0; i < kBlocks; ++i)
-      if (tid == i) ok[i] = at[i] >= 0;
-#pragma unroll
-    for (int i = 0; i < SR * kPieces / kThreads; ++i) {
-      const int p = tid + i * kThreads, r = p / kPieces, c = p % kPieces;
-      long long row = at[0];
-#pragma unroll
-      for (int j = 1; j < kBlocks; ++j) row = (r >> 4) == j ? at[j] : row;
-      const bool there = row >= 0 && r < left;
-      const size_t off = there ? (static_cast<size_t>(row + (r & 15)) * kPieces + c) * 16 : 0;
-      const int dst = (r * kPieces + place(r, c)) * 16;
-      cp_async16(k_slot + dst, static_cast<const unsigned char*>(a.k) + off, there ? 16 : 0);
-      cp_async16(v_slot + dst, static_cast<const unsigned char*>(a.v) + off, there ? 16 : 0);
-    }
-  }
-};
 
 template <typename T>
 __device__ inline void put4(T* dst, float4 v);
@@ -263,23 +228,22 @@ __device__ inline void put4<__nv_bfloat16>(__nv_bfloat16* dst, float4 v) {
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack_pair<__nv_bfloat16>(v.x, v.y), pack_pair<__nv_bfloat16>(v.z, v.w));
 }
 
-// The end of a unit, or of the block's part of it: `rows` rows of (m, l) and O in shared memory, O relative to m and summed over
-// nothing any more. A unit that the block has whole, and no shared pages ahead of it, is the result; others go to the workspace.
-template <typename T, int D, int RU, int SR, int kThreads>
-__device__ inline void put_unit(const PagedArgs& a, const Walk<SR>& w, bool whole, const float* m, const float* l, const float* o) {
+// The end of the block's part of a unit, by `threads` threads: rows of (m, l) and O in shared memory. (l is 0 where no key was
+// seen, and NaN where one that is not finite was.)
+template <typename T, int D, int RU>
+__device__ inline void put_unit(const PagedArgs& a, const StageInfo& u, const float* m, const float* l, const float* o, int threads) {
   constexpr int kVec = D / 4;
-  const bool direct = whole && w.b >= 0 && w.start == 0;
-  const size_t part = (static_cast<size_t>(blockIdx.x) + w.uid) * a.rs;
-  for (int i = threadIdx.x; i < RU * kVec; i += kThreads) {
+  const size_t part = (static_cast<size_t>(blockIdx.x) + u.uid) * a.rs;
+  for (int i = threadIdx.x; i < RU * kVec; i += threads) {
     const int r = i / kVec, col = i % kVec * 4;
     int b, h;
-    if (!unit_row<RU>(a, w, r, &b, &h)) continue;
-    float4 v = *reinterpret_cast<const float4*>(o + r * D + col);
-    if (direct) {
-      const float inv = l[r] > 0.f ? 1.f / l[r] : 0.f;
+    if (!unit_row<RU>(a, u, r, &b, &h)) continue;
+    const float4 v = *reinterpret_cast<const float4*>(o + r * D + col);
+    if (u.last == 2) {
+      const float inv = 1.f / l[r];
       const size_t row = static_cast<size_t>(b) * a.H + h;
-      put4(static_cast<T*>(a.out) + row * D + col, l[r] == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                                              : make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+      put4(static_cast<T*>(a.out) + row * D + col,
+           l[r] == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
       if (a.lse && col == 0) a.lse[row] = l[r] > 0.f ? m[r] * kLn2 + logf(l[r]) : l[r] == 0.f ? -INFINITY : l[r];
     } else {
       *reinterpret_cast<float4*>(a.part_o + (part + r) * D + col) = v;
@@ -288,426 +252,521 @@ __device__ inline void put_unit(const PagedArgs& a, const Walk<SR>& w, bool whol
   }
 }
 
-// ---- 16-bit caches ------------------------------------------------------------------
-
-template <int D>
-struct PagedMma {
-  static constexpr int RU = 16;
-  static constexpr int kWarps = D == 256 ? 2 : 4;
-  static constexpr int kThreads = kWarps * 32;
-  static constexpr int SR = kWarps * 16;
-  static constexpr int kStageBytes = SR * D * 2;  // per tensor
-  // 96 KB of ring and two blocks an SM, as in decode_mma_kernel
-  static constexpr int kStages = 96 * 1024 / (2 * kStageBytes) < 8 ? 96 * 1024 / (2 * kStageBytes) : 8;
-  static constexpr int kOffMerge = 2 * kStages * kStageBytes;
-  static constexpr int kMergeRows = 16 * (kWarps / 2);
-  static constexpr int kOffMl = kOffMerge + kMergeRows * D * 4;
-  static constexpr int kOffOk = kOffMl + (kWarps + 1) * 32 * 4;
-  static constexpr int kSmemBytes = kOffOk + kStages * (SR / 16) * 4;
+// Shared memory of a block of either kernel: kWarps warps that compute, then the one that copies. A stage's tensor is kBoxes boxes
+// of SR rows of 128 bytes, 16-byte piece c of a row's box at c ^ (row & 7).
+template <typename T, int D, int kWarps_, int SR_, int kRows_, int kExtra>
+struct PagedBlock {
+  static constexpr int kWarps = kWarps_, SR = SR_, RU = kRows_, kThreads = (kWarps + 1) * 32;
+  static constexpr int kEs = static_cast<int>(sizeof(T));
+  static constexpr int kBoxes = D * kEs > 128 ? D * kEs / 128 : 1, kBoxCols = 128 / kEs;
+  static constexpr int kTileBytes = SR * kBoxes * 128;  // per tensor
+  static constexpr int kStages = 96 * 1024 / (2 * kTileBytes) < 8 ? 96 * 1024 / (2 * kTileBytes) : 8;
+  static constexpr int kOffMerge = 2 * kStages * kTileBytes;  // O of the warps, summed up
+  static constexpr int kOffExtra = kOffMerge + RU * D * 4;
+  static constexpr int kOffMl = kOffExtra + kExtra;           // m of every warp's rows and of all, then l
+  static constexpr int kOffInfo = (kOffMl + (kWarps + 1) * RU * 8 + 15) & ~15;
+  static constexpr int kOffBar = kOffInfo + kStages * static_cast<int>(sizeof(StageInfo));
+  static constexpr int kOffRoom = kOffBar + (2 * kStages + 1) * 8;
+  static constexpr int kOffFlag = kOffRoom + static_cast<int>(sizeof(ScanRoom<kThreads>));
+  static constexpr int kSmemBytes = kOffFlag + 8;
+  static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two blocks to an SM");
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(PagedMma<D>::kThreads) paged_mma_kernel(PagedArgs a) {
-  using C = PagedMma<D>;
-  constexpr int SR = C::SR, RU = C::RU, kStages = C::kStages;
-  extern __shared__ __align__(16) unsigned char smem[];
-  unsigned char* const k_ring = smem;
-  unsigned char* const v_ring = smem + kStages * C::kStageBytes;
-  float* const merge = reinterpret_cast<float*>(smem + C::kOffMerge);
-  float* const red_m = reinterpret_cast<float*>(smem + C::kOffMl);  // [warps + 1][16], then l likewise
-  float* const red_l = red_m + (C::kWarps + 1) * 16;
-  int* const ok_ring = reinterpret_cast<int*>(smem + C::kOffOk);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane >> 2, tq = lane & 3;  // fragment row (and row + 8), column pair
+__device__ inline bool warp_wait(const PagedArgs& a, unsigned bar, unsigned parity, volatile int* gave_up, int which, int at) {
+  return __all_sync(0xffffffffu, tcgen::mbar_wait(bar, parity, gave_up, a.status, which, at, a.wait_ns)) != 0;
+}
 
-  begin_main(a);
-  Walk<SR> wc;
-  long long per;
-  const int total = find_share<SR, C::kThreads>(a, &wc, &per);
-  if (total == 0) {
-    end_main(a);
-    return;
-  }
-  Walk<SR> wi = wc;  // ahead of wc by what the ring holds
-  Loader<T, D, SR, C::kThreads> load;
-  load.look_up(a, wi);
-  int issued = 0;
-  auto issue = [&]() {
-    if (issued < total) {
-      const int slot = issued % kStages;
-      load.issue(a, wi, k_ring + slot * C::kStageBytes, v_ring + slot * C::kStageBytes, ok_ring + slot * (SR / 16));
-      if (++issued < total) {
-        wi.next(a);
-        load.look_up(a, wi);
-      }
-    }
-    cp_async_commit();
+// The warp that copies: `total` stages from the place w on.
+template <typename C>
+__device__ inline void copy_stages(const PagedArgs& a, const CUtensorMap* map_k, const CUtensorMap* map_v, Walk<C::SR> w, int total,
+                                   int per, unsigned char* smem, unsigned base, volatile int* gave_up) {
+  constexpr int SR = C::SR;
+  const int lane = threadIdx.x & 31;
+  const unsigned bar_full = base + C::kOffBar, bar_empty = bar_full + 8 * C::kStages;
+  // a lane's copies: a piece of the stage's rows, a box of one tensor (no more than 32: SR / 16 times kBoxes is at most 8)
+  static_assert(2 * C::kBoxes * (SR / 16) <= 32, "a copy a lane");
+  const int rows = min(1 << a.shift, SR), pieces = SR / rows;
+  const int piece = lane % pieces, box = lane / pieces % C::kBoxes, tensor = lane / pieces / C::kBoxes;
+  // the page of this lane's piece, as the head its rows are in the tensor map; -1 where there is none
+  auto look_up = [&]() {
+    if (piece * rows >= w.left()) return -1;
+    const int at = (w.start + w.st * SR + piece * rows) >> a.shift;
+    const int* const table = w.b < 0 ? a.shared_pages : a.table + w.b * a.table_stride;
+    if (at >= (w.b < 0 ? a.shared_len >> a.shift : a.max_pages)) return -1;
+    const int page = table[at];
+    return page >= 0 && page < a.num_pages ? page * a.kvH + w.kvh : -1;
   };
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) issue();
-
-  unsigned qa[D / 16][4];
-  float o[D / 8][4];
-  float m_run[2], l_run[2];
-  const int mi = lane >> 3, r8 = lane & 7, key0 = warp * 16;
-  const unsigned k_row_off = static_cast<unsigned>((key0 + (mi >> 1) * 8 + r8) * D * 2);
-  const unsigned v_row_off = static_cast<unsigned>((key0 + (mi & 1) * 8 + r8) * D * 2);
-  int first_st = wc.st;  // first stage of the block's part of the unit
+  int head = look_up(), first_st = w.st;
   for (int s = 0; s < total; ++s) {
-    if (s == 0 || wc.st == 0) {
-      first_st = wc.st;
-      // Q as A fragments: reg0 (row g, k 2tq..), reg1 (row g+8, same k), reg2 / reg3 the same at k+8
-      int b0, h0, b1, h1;
-      const bool is0 = unit_row<RU>(a, wc, g, &b0, &h0), is1 = unit_row<RU>(a, wc, g + 8, &b1, &h1);
-      const T* const q0 = static_cast<const T*>(a.q) + (is0 ? static_cast<size_t>(b0) * a.H + h0 : 0) * D + 2 * tq;
-      const T* const q1 = static_cast<const T*>(a.q) + (is1 ? static_cast<size_t>(b1) * a.H + h1 : 0) * D + 2 * tq;
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        qa[ks][0] = is0 ? *reinterpret_cast<const unsigned*>(q0 + ks * 16) : 0u;
-        qa[ks][1] = is1 ? *reinterpret_cast<const unsigned*>(q1 + ks * 16) : 0u;
-        qa[ks][2] = is0 ? *reinterpret_cast<const unsigned*>(q0 + ks * 16 + 8) : 0u;
-        qa[ks][3] = is1 ? *reinterpret_cast<const unsigned*>(q1 + ks * 16 + 8) : 0u;
-      }
-#pragma unroll
-      for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-      m_run[0] = m_run[1] = -INFINITY;
-      l_run[0] = l_run[1] = 0.f;  // this lane's share of the row sums
+    const int slot = s % C::kStages, use = s / C::kStages;
+    if (w.st == 0) {
+      first_st = 0;
+      // the block with a unit's first stage says which blocks have parts of it: this one and those that the rest reaches into
+      const int here = min(w.n, total - s);
+      if (lane == 0) a.unit_parts[w.uid] = make_int2(static_cast<int>(blockIdx.x), 1 + (w.n - here + per - 1) / per);
     }
-    cp_async_wait<kStages - 2>();
-    __syncthreads();
-    issue();
-    const int slot = s % kStages;
-    const int n_valid = wc.end - wc.start - wc.st * SR - key0;  // keys of this warp's block
-    if (n_valid > 0 && ok_ring[slot * (SR / 16) + warp]) {
-      const unsigned kt = static_cast<unsigned>(__cvta_generic_to_shared(k_ring + slot * C::kStageBytes));
-      const unsigned vt = static_cast<unsigned>(__cvta_generic_to_shared(v_ring + slot * C::kStageBytes));
-      // S = Q K^T for 16 keys: s0 = keys 0..7, s1 = keys 8..15
-      float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+    const int row = (w.start + w.st * SR + piece * rows) & ((1 << a.shift) - 1);
+    const int my_head = head;
+    const unsigned there = __ballot_sync(0xffffffffu, my_head >= 0 && lane < pieces);
+    StageInfo info;
+    info.b = w.b, info.kvh = w.kvh, info.hb = w.hb, info.uid = w.uid;
+    info.keys = min(SR, w.left());
+    info.pages = 0;
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        unsigned kb[4];
-        ldmatrix_x4(kb, kt + k_row_off + (load.place(r8, 2 * ks + (mi & 1)) << 4));
-        mma16816<T>(s0, qa[ks], kb[0], kb[1]);
-        mma16816<T>(s1, qa[ks], kb[2], kb[3]);
-      }
-      float v[8] = {s0[0], s0[1], s1[0], s1[1], s0[2], s0[3], s1[2], s1[3]};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int col = ((i >> 1) & 1) * 8 + 2 * tq + (i & 1);
-        v[i] = col < n_valid ? v[i] * a.scale_log2 : -INFINITY;
-      }
-      float mx0 = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
-      float mx1 = fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7]));
-      mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-      mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-      mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-      mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-      if (__any_sync(0xffffffffu, mx0 > m_run[0] || mx1 > m_run[1])) {  // rare after the first blocks
-        const float mn0 = fmaxf(m_run[0], mx0), mn1 = fmaxf(m_run[1], mx1);
-        const float a0 = m_run[0] == -INFINITY ? 0.f : ex2(m_run[0] - mn0);
-        const float a1 = m_run[1] == -INFINITY ? 0.f : ex2(m_run[1] - mn1);
-        l_run[0] *= a0;
-        l_run[1] *= a1;
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n) {
-          o[n][0] *= a0;
-          o[n][1] *= a0;
-          o[n][2] *= a1;
-          o[n][3] *= a1;
-        }
-        m_run[0] = mn0;
-        m_run[1] = mn1;
-      }
-      const float ms0 = m_run[0] == -INFINITY ? 0.f : m_run[0];
-      const float ms1 = m_run[1] == -INFINITY ? 0.f : m_run[1];
-      float p[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p[i] = ex2(v[i] - ms0);
-        p[4 + i] = ex2(v[4 + i] - ms1);
-      }
-      l_run[0] += (p[0] + p[1]) + (p[2] + p[3]);
-      l_run[1] += (p[4] + p[5]) + (p[6] + p[7]);
-      // P as the A fragment of the second product, rounded to the cache's type as the products want it
-      unsigned pa[4];
-      pa[0] = pack_pair<T>(p[0], p[1]);
-      pa[1] = pack_pair<T>(p[4], p[5]);
-      pa[2] = pack_pair<T>(p[2], p[3]);
-      pa[3] = pack_pair<T>(p[6], p[7]);
-#pragma unroll
-      for (int c2 = 0; c2 < D / 16; ++c2) {
-        unsigned vb[4];
-        ldmatrix_x4_trans(vb, vt + v_row_off + (load.place(r8, 2 * c2 + (mi >> 1)) << 4));
-        mma16816<T>(o[2 * c2], pa, vb[0], vb[1]);
-        mma16816<T>(o[2 * c2 + 1], pa, vb[2], vb[3]);
-      }
+    for (int i = 0; i < SR / 16; ++i) info.pages |= (there >> (i * 16 / rows) & 1u) << i;
+    const bool ends = w.st == w.n - 1;
+    info.first = w.st == first_st;
+    info.last = ends && first_st == 0 && w.b >= 0 && w.start == 0 ? 2 : ends || s == total - 1;
+    // on to the next stage: its page numbers are on their way while this one waits for its place
+    if (s + 1 < total) {
+      w.next(a);
+      head = look_up();
     }
-    if (wc.st == wc.n - 1 || s == total - 1) {
-      // the lanes of a row, then the warps, in pairs: the upper half of the warps stages its O
-      const bool whole = first_st == 0 && wc.st == wc.n - 1;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 1);
-        l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 2);
-      }
-      if (tq == 0) {
-        red_m[warp * 16 + g] = m_run[0];
-        red_m[warp * 16 + g + 8] = m_run[1];
-        red_l[warp * 16 + g] = l_run[0];
-        red_l[warp * 16 + g + 8] = l_run[1];
-      }
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float m_all = -INFINITY, l_all = 0.f;
-#pragma unroll
-        for (int w = 0; w < C::kWarps; ++w) m_all = fmaxf(m_all, red_m[w * 16 + g + 8 * i]);
-#pragma unroll
-        for (int w = 0; w < C::kWarps; ++w) {
-          const float mw = red_m[w * 16 + g + 8 * i];
-          l_all += (mw == -INFINITY ? (red_l[w * 16 + g + 8 * i] == 0.f ? 0.f : 1.f) : ex2(mw - m_all)) * red_l[w * 16 + g + 8 * i];
-        }
-        const float f = m_run[i] == -INFINITY ? 1.f : ex2(m_run[i] - m_all);
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n) {
-          o[n][2 * i] *= f;
-          o[n][2 * i + 1] *= f;
-        }
-        if (warp == 0 && tq == 0) {
-          red_m[C::kWarps * 16 + g + 8 * i] = m_all;
-          red_l[C::kWarps * 16 + g + 8 * i] = l_all;
-        }
-      }
-      auto stage = [&](int at, bool add) {
-        float* const dst = merge + at * 16 * D;
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float2* const x = reinterpret_cast<float2*>(dst + (g + 8 * i) * D + n * 8 + 2 * tq);
-            float2 y = make_float2(o[n][2 * i], o[n][2 * i + 1]);
-            if (add) {
-              const float2 z = *x;
-              y.x += z.x;
-              y.y += z.y;
-            }
-            *x = y;
-          }
-      };
-      constexpr int kHalf = C::kWarps / 2;
-      if (warp >= kHalf) stage(warp - kHalf, false);
-      __syncthreads();
-      if (warp < kHalf) stage(warp, true);
-      __syncthreads();
-      if constexpr (kHalf == 2) {
-        for (int i = threadIdx.x; i < 16 * D / 4; i += C::kThreads) {
-          float4* const x = reinterpret_cast<float4*>(merge) + i;
-          const float4 y = *x, z = reinterpret_cast<const float4*>(merge + 16 * D)[i];
-          *x = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
-        }
-        __syncthreads();
-      }
-      put_unit<T, D, RU, SR, C::kThreads>(a, wc, whole, red_m + C::kWarps * 16, red_l + C::kWarps * 16, merge);
-      __syncthreads();
+    if (use >= 1 && !warp_wait(a, bar_empty + 8 * slot, (use + 1) & 1, gave_up, 1, s)) break;
+    if (lane == 0) {
+      *reinterpret_cast<StageInfo*>(smem + C::kOffInfo + slot * sizeof(StageInfo)) = info;
+      tcgen::mbar_expect_tx(bar_full + 8 * slot, 2 * C::kBoxes * 128 * rows * __popc(there));
     }
-    if (s + 1 < total) wc.next(a);
+    __syncwarp();
+    if (tensor < 2 && my_head >= 0)
+      tcgen::tma_load_3d(base + (tensor * C::kStages + slot) * C::kTileBytes + (box * SR + piece * rows) * 128,
+                         tensor == 0 ? map_k : map_v, bar_full + 8 * slot, box * C::kBoxCols, row, my_head);
   }
-  cp_async_wait<0>();
-  end_main(a);
+}
+
+// What every block does around its walk. `compute(warp, total, base, smem, gave_up)` runs in the warps that compute.
+template <typename C, typename Compute>
+__device__ inline void paged_block(const PagedArgs& a, const CUtensorMap* map_k, const CUtensorMap* map_v, unsigned char* smem,
+                                   Compute compute) {
+  const unsigned base = tcgen::smem_u32(smem);
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  volatile int* const gave_up = reinterpret_cast<volatile int*>(smem + C::kOffFlag);
+  const unsigned bars = base + C::kOffBar;
+  let_next_start();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      tcgen::mbar_init(bars + 8 * s, 1);                          // full
+      tcgen::mbar_init(bars + 8 * (C::kStages + s), C::kWarps);   // empty
+    }
+    tcgen::mbar_init(bars + 16 * C::kStages, C::kWarps);          // a meeting of the warps that compute
+    *gave_up = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    tcgen::prefetch_map(map_k);
+    tcgen::prefetch_map(map_v);
+  }
+  // Behind the kernel of the shared pages, whose blocks let this one begin when all that came before them has completed,
+  // nothing waits for that kernel itself but the end: the fold, which waits for this grid, then finds both kernels' parts.
+  if (a.shared_ml == nullptr) wait_for_previous();
+  Walk<C::SR> w;
+  int per = 1;
+  int total = find_share<C::SR, C::kThreads>(a, &w, &per, reinterpret_cast<ScanRoom<C::kThreads>*>(smem + C::kOffRoom));
+  // (behind a launch that gave up nothing is computed; the fold writes nothing then either)
+  if (*reinterpret_cast<volatile int*>(a.status) != 0) total = 0;
+  total = __syncthreads_or(total == 0) ? 0 : total;
+  if (total > 0) {
+    if (warp == C::kWarps) copy_stages<C>(a, map_k, map_v, w, total, per, smem, base, gave_up);
+    else compute(warp, total, base, gave_up);
+    __syncthreads();
+    if (*gave_up) {  // give copies in flight time to land
+      const unsigned long long t0 = tcgen::global_ns();
+      while (tcgen::global_ns() - t0 < 1000000ull) __nanosleep(1000);
+    }
+  }
+  if (a.shared_ml != nullptr) wait_for_previous();
+}
+
+// A meeting of the warps that compute; false when some warp gave up.
+template <typename C>
+struct Meeting {
+  unsigned bar;
+  unsigned phase = 0;
+  __device__ inline bool meet(const PagedArgs& a, volatile int* gave_up, int at) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) tcgen::mbar_arrive(bar);
+    const bool ok = warp_wait(a, bar, phase, gave_up, 2, at);
+    phase ^= 1;
+    return ok;
+  }
+};
+
+// ---- 16-bit caches ------------------------------------------------------------------
+
+template <typename T, int D>
+using MmaBlock = PagedBlock<T, D, D == 256 ? 2 : 4, D == 256 ? 32 : 64, 16, 0>;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(MmaBlock<T, D>::kThreads, 2)
+    paged_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                     const __grid_constant__ PagedArgs a) {
+  using C = MmaBlock<T, D>;
+  constexpr int SR = C::SR, RU = C::RU;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  paged_block<C>(a, &map_k, &map_v, smem, [&](int warp, int total, unsigned base, volatile int* gave_up) {
+    float* const merge = reinterpret_cast<float*>(smem + C::kOffMerge);
+    float* const red_m = reinterpret_cast<float*>(smem + C::kOffMl);  // [warps + 1][16]
+    float* const red_l = red_m + (C::kWarps + 1) * 16;
+    const unsigned bar_full = base + C::kOffBar, bar_empty = bar_full + 8 * C::kStages;
+    Meeting<C> all{bar_empty + 8 * C::kStages};
+    const int lane = threadIdx.x & 31;
+    const int g = lane >> 2, tq = lane & 3;  // fragment row (and row + 8), column pair
+    const int mi = lane >> 3, r8 = lane & 7, key0 = warp * 16;
+    // a lane's rows of the ldmatrix tiles, and the swizzled offsets of its pieces c = 2 i + (0 or 1) of a box
+    const unsigned k_row = base + static_cast<unsigned>(key0 + (mi >> 1) * 8 + r8) * 128;
+    const unsigned v_row = base + static_cast<unsigned>(C::kStages * C::kTileBytes + (key0 + (mi & 1) * 8 + r8) * 128);
+    unsigned k_off[4], v_off[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      k_off[i] = ((2 * i + (mi & 1)) ^ r8) << 4;
+      v_off[i] = ((2 * i + (mi >> 1)) ^ r8) << 4;
+    }
+    unsigned qa[D / 16][4];
+    float o[D / 8][4];
+    float m_run[2], l_run[2];
+    for (int s = 0; s < total; ++s) {
+      const int slot = s % C::kStages;
+      if (!warp_wait(a, bar_full + 8 * slot, (s / C::kStages) & 1, gave_up, 3, s)) return;
+      const StageInfo u = *reinterpret_cast<const StageInfo*>(smem + C::kOffInfo + slot * sizeof(StageInfo));
+      if (u.first) {
+        // Q as A fragments: reg0 (row g, k 2tq..), reg1 (row g+8, same k), reg2 / reg3 the same at k+8
+        int b0, h0, b1, h1;
+        const bool is0 = unit_row<RU>(a, u, g, &b0, &h0), is1 = unit_row<RU>(a, u, g + 8, &b1, &h1);
+        const T* const q0 = static_cast<const T*>(a.q) + (is0 ? static_cast<size_t>(b0) * a.H + h0 : 0) * D + 2 * tq;
+        const T* const q1 = static_cast<const T*>(a.q) + (is1 ? static_cast<size_t>(b1) * a.H + h1 : 0) * D + 2 * tq;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          qa[ks][0] = is0 ? *reinterpret_cast<const unsigned*>(q0 + ks * 16) : 0u;
+          qa[ks][1] = is1 ? *reinterpret_cast<const unsigned*>(q1 + ks * 16) : 0u;
+          qa[ks][2] = is0 ? *reinterpret_cast<const unsigned*>(q0 + ks * 16 + 8) : 0u;
+          qa[ks][3] = is1 ? *reinterpret_cast<const unsigned*>(q1 + ks * 16 + 8) : 0u;
+        }
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+        m_run[0] = m_run[1] = -INFINITY;
+        l_run[0] = l_run[1] = 0.f;  // this lane's share of the row sums
+      }
+      const int n_valid = u.keys - key0;  // keys of this warp
+      if (n_valid > 0 && (u.pages >> warp & 1u)) {
+        const unsigned kt = k_row + slot * C::kTileBytes, vt = v_row + slot * C::kTileBytes;
+        if (n_valid < 16) {
+          // what a page holds behind the sequence's end has weight 0, but may be anything: out of V's rows with it
+          unsigned char* const v_tile = smem + (C::kStages + slot) * C::kTileBytes;
+          for (int i = lane; i < (16 - n_valid) * C::kBoxes * 8; i += 32)
+            *reinterpret_cast<uint4*>(v_tile + (i / 8 % C::kBoxes * SR + key0 + n_valid + i / 8 / C::kBoxes) * 128 + i % 8 * 16) =
+                make_uint4(0u, 0u, 0u, 0u);
+          __syncwarp();
+        }
+        // S = Q K^T for 16 keys: s0 = keys 0..7, s1 = keys 8..15
+        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          unsigned kb[4];
+          ldmatrix_x4(kb, kt + ks / 4 * (SR * 128) + k_off[ks % 4]);
+          mma16816<T>(s0, qa[ks], kb[0], kb[1]);
+          mma16816<T>(s1, qa[ks], kb[2], kb[3]);
+        }
+        float v[8] = {s0[0], s0[1], s1[0], s1[1], s0[2], s0[3], s1[2], s1[3]};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int col = ((i >> 1) & 1) * 8 + 2 * tq + (i & 1);
+          v[i] = col < n_valid ? v[i] * a.scale_log2 : -INFINITY;
+        }
+        float mx0 = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+        float mx1 = fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7]));
+        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
+        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
+        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
+        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+        if (__any_sync(0xffffffffu, mx0 > m_run[0] || mx1 > m_run[1])) {  // rare after the first stages
+          const float mn0 = fmaxf(m_run[0], mx0), mn1 = fmaxf(m_run[1], mx1);
+          const float a0 = m_run[0] == -INFINITY ? 0.f : ex2(m_run[0] - mn0);
+          const float a1 = m_run[1] == -INFINITY ? 0.f : ex2(m_run[1] - mn1);
+          l_run[0] = m_run[0] == -INFINITY ? l_run[0] : l_run[0] * a0;  // (0, or NaN to keep)
+          l_run[1] = m_run[1] == -INFINITY ? l_run[1] : l_run[1] * a1;
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) {
+            o[n][0] *= a0;
+            o[n][1] *= a0;
+            o[n][2] *= a1;
+            o[n][3] *= a1;
+          }
+          m_run[0] = mn0;
+          m_run[1] = mn1;
+        }
+        const float ms0 = m_run[0] == -INFINITY ? 0.f : m_run[0];
+        const float ms1 = m_run[1] == -INFINITY ? 0.f : m_run[1];
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[i] = ex2(v[i] - ms0);
+          p[4 + i] = ex2(v[4 + i] - ms1);
+        }
+        l_run[0] += (p[0] + p[1]) + (p[2] + p[3]);
+        l_run[1] += (p[4] + p[5]) + (p[6] + p[7]);
+        // P as the A fragment of the second product, rounded to the cache's type as the products want it
+        unsigned pa[4];
+        pa[0] = pack_pair<T>(p[0], p[1]);
+        pa[1] = pack_pair<T>(p[4], p[5]);
+        pa[2] = pack_pair<T>(p[2], p[3]);
+        pa[3] = pack_pair<T>(p[6], p[7]);
+#pragma unroll
+        for (int c2 = 0; c2 < D / 16; ++c2) {
+          unsigned vb[4];
+          ldmatrix_x4_trans(vb, vt + c2 / 4 * (SR * 128) + v_off[c2 % 4]);
+          mma16816<T>(o[2 * c2], pa, vb[0], vb[1]);
+          mma16816<T>(o[2 * c2 + 1], pa, vb[2], vb[3]);
+        }
+        if (n_valid < 16) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next copy lands behind those zeros
+      }
+      __syncwarp();
+      if (lane == 0) tcgen::mbar_arrive(bar_empty + 8 * slot);
+      if (u.last) {
+        // the lanes of a row, then the warps one after the other
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 1);
+          l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 2);
+        }
+        if (tq == 0) {
+          red_m[warp * 16 + g] = m_run[0];
+          red_m[warp * 16 + g + 8] = m_run[1];
+          red_l[warp * 16 + g] = l_run[0];
+          red_l[warp * 16 + g + 8] = l_run[1];
+        }
+        if (!all.meet(a, gave_up, s)) return;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float m_all = -INFINITY, l_all = 0.f;
+#pragma unroll
+          for (int w = 0; w < C::kWarps; ++w) m_all = fmaxf(m_all, red_m[w * 16 + g + 8 * i]);
+#pragma unroll
+          for (int w = 0; w < C::kWarps; ++w) {
+            const float mw = red_m[w * 16 + g + 8 * i];
+            l_all += (mw == -INFINITY ? 1.f : ex2(mw - m_all)) * red_l[w * 16 + g + 8 * i];
+          }
+          const float f = m_run[i] == -INFINITY ? 1.f : ex2(m_run[i] - m_all);
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) {
+            o[n][2 * i] *= f;
+            o[n][2 * i + 1] *= f;
+          }
+          if (warp == 0 && tq == 0) {
+            red_m[C::kWarps * 16 + g + 8 * i] = m_all;
+            red_l[C::kWarps * 16 + g + 8 * i] = l_all;
+          }
+        }
+#pragma unroll 1
+        for (int w = 0; w < C::kWarps; ++w) {
+          if (warp == w) {
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                float2* const x = reinterpret_cast<float2*>(merge + (g + 8 * i) * D + n * 8 + 2 * tq);
+                const float2 y = w == 0 ? make_float2(0.f, 0.f) : *x;
+                *x = make_float2(y.x + o[n][2 * i], y.y + o[n][2 * i + 1]);
+              }
+          }
+          if (!all.meet(a, gave_up, s)) return;
+        }
+        put_unit<T, D, RU>(a, u, red_m + C::kWarps * 16, red_l + C::kWarps * 16, merge, C::kWarps * 32);
+        if (!all.meet(a, gave_up, s)) return;
+      }
+    }
+  });
 }
 
 // ---- fp32 caches --------------------------------------------------------------------
 
 template <int D, int kRows>
-struct PagedF32 {
-  static constexpr int RU = kRows;
-  static constexpr int kThreads = 128;
-  static constexpr int SR = D == 256 ? 16 : 32;
-  static constexpr int kParts = kThreads / SR;       // lanes that share out a key's row
-  static constexpr int kVec = D / 4;                 // columns of the second product, four at a time
-  static constexpr int kSlices = kThreads / kVec;    // threads that share out a column's keys
-  static constexpr int kStageBytes = SR * D * 4;     // per tensor
-  static constexpr int kStages = 96 * 1024 / (2 * kStageBytes) < 6 ? 96 * 1024 / (2 * kStageBytes) : 6;
-  static constexpr int kOffQ = 2 * kStages * kStageBytes;
-  static constexpr int kOffP = kOffQ + RU * D * 4;
-  static constexpr int kOffMl = kOffP + RU * SR * 4;
-  static constexpr int kOffMerge = kOffMl + 4 * RU * 4;
-  static constexpr int kOffOk = kOffMerge + RU * D * 4;
-  static constexpr int kSmemBytes = kOffOk + kStages * (SR / 16) * 4;
-};
+using F32Block = PagedBlock<float, D, 4, D == 256 ? 16 : 32, kRows, kRows * D * 4>;
 
 template <int D, int kRows>
-__global__ void __launch_bounds__(128) paged_f32_kernel(PagedArgs a) {
-  using C = PagedF32<D, kRows>;
-  constexpr int SR = C::SR, RU = C::RU, kStages = C::kStages, kThreads = C::kThreads;
-  extern __shared__ __align__(16) unsigned char smem[];
-  unsigned char* const k_ring = smem;
-  unsigned char* const v_ring = smem + kStages * C::kStageBytes;
-  float* const q_s = reinterpret_cast<float*>(smem + C::kOffQ);        // [row][D], times scale
-  float* const p_s = reinterpret_cast<float*>(smem + C::kOffP);        // [key][row]
-  float* const m_s = reinterpret_cast<float*>(smem + C::kOffMl);       // running (m, l) and the stage's factor of every row
-  float* const l_s = m_s + RU;
-  float* const f_s = l_s + RU;
-  float* const merge = reinterpret_cast<float*>(smem + C::kOffMerge);  // [row][D]
-  int* const ok_ring = reinterpret_cast<int*>(smem + C::kOffOk);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-
-  begin_main(a);
-  Walk<SR> wc;
-  long long per;
-  const int total = find_share<SR, kThreads>(a, &wc, &per);
-  if (total == 0) {
-    end_main(a);
-    return;
-  }
-  Walk<SR> wi = wc;
-  Loader<float, D, SR, kThreads> load;
-  load.look_up(a, wi);
-  int issued = 0;
-  auto issue = [&]() {
-    if (issued < total) {
-      const int slot = issued % kStages;
-      load.issue(a, wi, k_ring + slot * C::kStageBytes, v_ring + slot * C::kStageBytes, ok_ring + slot * (SR / 16));
-      if (++issued < total) {
-        wi.next(a);
-        load.look_up(a, wi);
-      }
-    }
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) issue();
-
-  const int key = tid / C::kParts, part = tid % C::kParts;         // first product
-  const int col = tid % C::kVec, slice = tid / C::kVec;            // second product
-  float4 o[RU];
-  int first_st = wc.st;
-  for (int s = 0; s < total; ++s) {
-    if (s == 0 || wc.st == 0) {
-      first_st = wc.st;
-      for (int i = tid; i < RU * C::kVec; i += kThreads) {
-        int b, h;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (unit_row<RU>(a, wc, i / C::kVec, &b, &h))
-          x = reinterpret_cast<const float4*>(a.q)[(static_cast<size_t>(b) * a.H + h) * C::kVec + i % C::kVec];
-        reinterpret_cast<float4*>(q_s)[i] = x;
-      }
-      if (tid < RU) {
-        m_s[tid] = -INFINITY;
-        l_s[tid] = 0.f;
-      }
-#pragma unroll
-      for (int r = 0; r < RU; ++r) o[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    cp_async_wait<kStages - 2>();
-    __syncthreads();
-    issue();
-    const int slot = s % kStages;
-    const int n_valid = wc.end - wc.start - wc.st * SR;
-    // scores: kParts lanes a key, every kParts-th piece each
-    {
-      const float4* const row = reinterpret_cast<const float4*>(k_ring + slot * C::kStageBytes) + key * C::kVec;
-      float sc[RU];
-#pragma unroll
-      for (int r = 0; r < RU; ++r) sc[r] = 0.f;
-#pragma unroll 4
-      for (int j = 0; j < C::kVec / C::kParts; ++j) {
-        const int c = j * C::kParts + part;
-        const float4 x = row[load.place(key, c)];
+__global__ void __launch_bounds__(F32Block<D, kRows>::kThreads, 2)
+    paged_f32_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                     const __grid_constant__ PagedArgs a) {
+  using C = F32Block<D, kRows>;
+  constexpr int SR = C::SR, RU = C::RU, kVec = D / 4;
+  constexpr int kKeys = SR / 4;                       // of a warp and stage
+  constexpr int kParts = 32 / kKeys;                  // lanes that share out a key's row
+  constexpr int kCols = kVec < 32 ? kVec : 32;        // lanes side by side on a row of V
+  constexpr int kAt = 32 / kCols, kEach = kVec / kCols;  // rows of V at a time, 16-byte pieces of one a lane
+  extern __shared__ __align__(1024) unsigned char smem[];
+  paged_block<C>(a, &map_k, &map_v, smem, [&](int warp, int total, unsigned base, volatile int* gave_up) {
+    float* const merge = reinterpret_cast<float*>(smem + C::kOffMerge);
+    const float4* const q_s = reinterpret_cast<const float4*>(smem + C::kOffExtra);  // [row][D / 4]
+    float* const red_m = reinterpret_cast<float*>(smem + C::kOffMl);                 // [warps + 1][RU]
+    float* const red_l = red_m + (C::kWarps + 1) * RU;
+    const unsigned bar_full = base + C::kOffBar, bar_empty = bar_full + 8 * C::kStages;
+    Meeting<C> all{bar_empty + 8 * C::kStages};
+    const int lane = threadIdx.x & 31;
+    const int key = lane / kParts, part = lane % kParts;  // scores
+    const int col = lane % kCols, sub = lane / kCols;     // sum over V
+    const int key0 = warp * kKeys;
+    float4 o[RU][kEach];
+    float m_run[RU], l_run[RU];
+    for (int s = 0; s < total; ++s) {
+      const int slot = s % C::kStages;
+      if (!warp_wait(a, bar_full + 8 * slot, (s / C::kStages) & 1, gave_up, 3, s)) return;
+      const StageInfo u = *reinterpret_cast<const StageInfo*>(smem + C::kOffInfo + slot * sizeof(StageInfo));
+      if (u.first) {
+        for (int i = threadIdx.x; i < RU * kVec; i += C::kWarps * 32) {
+          int b, h;
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (unit_row<RU>(a, u, i / kVec, &b, &h))
+            x = static_cast<const float4*>(a.q)[(static_cast<size_t>(b) * a.H + h) * kVec + i % kVec];
+          reinterpret_cast<float4*>(smem + C::kOffExtra)[i] = x;
+        }
 #pragma unroll
         for (int r = 0; r < RU; ++r) {
-          const float4 y = reinterpret_cast<const float4*>(q_s)[r * C::kVec + c];
-          sc[r] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, sc[r]))));
+          m_run[r] = -INFINITY;
+          l_run[r] = 0.f;
+#pragma unroll
+          for (int i = 0; i < kEach; ++i) o[r][i] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
+        if (!all.meet(a, gave_up, s)) return;
       }
-      const bool seen = key < n_valid && ok_ring[slot * (SR / 16) + (key >> 4)];
+      const int n_valid = u.keys - key0;
+      if (n_valid > 0 && (u.pages >> (key0 / 16) & 1u)) {
+        const unsigned char* const kt = smem + slot * C::kTileBytes + (key0 + key) * 128;
+        const unsigned char* const vt = smem + (C::kStages + slot) * C::kTileBytes + key0 * 128;
+        float sc[RU];
 #pragma unroll
-      for (int r = 0; r < RU; ++r) {
-#pragma unroll
-        for (int i = 1; i < C::kParts; i *= 2) sc[r] += __shfl_xor_sync(0xffffffffu, sc[r], i);
-        if (part == r % C::kParts) p_s[key * RU + r] = seen ? sc[r] * a.scale_log2 : -INFINITY;
-      }
-    }
-    __syncthreads();
-    // a warp a row: maximum, weights, sum
-    for (int r = warp; r < RU; r += 4) {
-      const float v = lane < SR ? p_s[lane * RU + r] : -INFINITY;
-      float mx = v;
-#pragma unroll
-      for (int i = 16; i > 0; i /= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, i));
-      const float m_old = m_s[r], m_new = fmaxf(m_old, mx);
-      const float p = ex2(v - (m_new == -INFINITY ? 0.f : m_new));
-      float sum = p;
-#pragma unroll
-      for (int i = 16; i > 0; i /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, i);
-      if (lane < SR) p_s[lane * RU + r] = p;
-      __syncwarp();
-      if (lane == 0) {
-        const float f = m_old == -INFINITY ? (l_s[r] == 0.f ? 0.f : 1.f) : ex2(m_old - m_new);
-        f_s[r] = f;
-        l_s[r] = l_s[r] * f + sum;
-        m_s[r] = m_new;
-      }
-    }
-    __syncthreads();
-    // values: a thread has four columns and every kSlices-th key
-    {
-      const float4* const v_s = reinterpret_cast<const float4*>(v_ring + slot * C::kStageBytes);
-#pragma unroll
-      for (int r = 0; r < RU; ++r) {
-        const float f = f_s[r];
-        o[r].x *= f;
-        o[r].y *= f;
-        o[r].z *= f;
-        o[r].w *= f;
-      }
-      const int* const ok = ok_ring + slot * (SR / 16);
+        for (int r = 0; r < RU; ++r) sc[r] = 0.f;
+        // A lane's pieces: every other one of a box, so that the two keys of eight neighbouring lanes, a bank apart by their
+        // swizzle, do not meet; with eight lanes to a key they are neighbours.
 #pragma unroll 4
-      for (int i = 0; i < SR / C::kSlices; ++i) {
-        const int j = i * C::kSlices + slice;
-        if (j >= n_valid || !ok[j >> 4]) continue;
-        const float4 x = v_s[j * C::kVec + load.place(j, col)];
-#pragma unroll
-        for (int r = 0; r < RU; ++r) {
-          const float p = p_s[j * RU + r];
-          o[r].x = fmaf(p, x.x, o[r].x);
-          o[r].y = fmaf(p, x.y, o[r].y);
-          o[r].z = fmaf(p, x.z, o[r].z);
-          o[r].w = fmaf(p, x.w, o[r].w);
-        }
-      }
-    }
-    if (wc.st == wc.n - 1 || s == total - 1) {
-      const bool whole = first_st == 0 && wc.st == wc.n - 1;
-      // the slices of a column one after the other
-      for (int i = 0; i < C::kSlices; ++i) {
-        if (slice == i) {
+        for (int j = 0; j < kVec / kParts; ++j) {
+          const int c = kParts == 4 ? (j >> 1) * 8 + 2 * part + (j & 1) : j * kParts + part;
+          const float4 x = *reinterpret_cast<const float4*>(kt + c / 8 * (SR * 128) + ((c % 8) ^ ((key0 + key) & 7)) * 16);
 #pragma unroll
           for (int r = 0; r < RU; ++r) {
-            float4* const x = reinterpret_cast<float4*>(merge) + r * C::kVec + col;
-            const float4 y = i == 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *x;
-            *x = make_float4(y.x + o[r].x, y.y + o[r].y, y.z + o[r].z, y.w + o[r].w);
+            const float4 y = q_s[r * kVec + c];
+            sc[r] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, sc[r]))));
           }
         }
-        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < RU; ++r) {
+#pragma unroll
+          for (int i = 1; i < kParts; i *= 2) sc[r] += __shfl_xor_sync(0xffffffffu, sc[r], i);
+          sc[r] = key < n_valid ? sc[r] * a.scale_log2 : -INFINITY;
+        }
+        float mx[RU];
+        bool moved = false;
+#pragma unroll
+        for (int r = 0; r < RU; ++r) {
+          mx[r] = sc[r];
+#pragma unroll
+          for (int i = kParts; i < 32; i *= 2) mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], i));
+          moved = moved || mx[r] > m_run[r];
+        }
+        if (moved) {  // (the same in all lanes)
+#pragma unroll
+          for (int r = 0; r < RU; ++r) {
+            const float mn = fmaxf(m_run[r], mx[r]);
+            const float f = m_run[r] == -INFINITY ? 0.f : ex2(m_run[r] - mn);
+            l_run[r] = m_run[r] == -INFINITY ? l_run[r] : l_run[r] * f;
+            m_run[r] = mn;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) o[r][i] = make_float4(o[r][i].x * f, o[r][i].y * f, o[r][i].z * f, o[r][i].w * f);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < RU; ++r) {
+          sc[r] = ex2(sc[r] - (m_run[r] == -INFINITY ? 0.f : m_run[r]));
+          l_run[r] += sc[r];  // of this lane's key
+        }
+#pragma unroll
+        for (int i = 0; i < kKeys / kAt; ++i) {
+          const int row = i * kAt + sub;
+          float p[RU];
+#pragma unroll
+          for (int r = 0; r < RU; ++r) p[r] = __shfl_sync(0xffffffffu, sc[r], row * kParts);
+          if (row < n_valid) {  // (rows behind the end may hold anything)
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+              const int c = e * kCols + col;
+              const float4 x = *reinterpret_cast<const float4*>(vt + (c / 8 * SR + row) * 128 + ((c % 8) ^ ((key0 + row) & 7)) * 16);
+#pragma unroll
+              for (int r = 0; r < RU; ++r) {
+                o[r][e].x = fmaf(p[r], x.x, o[r][e].x);
+                o[r][e].y = fmaf(p[r], x.y, o[r][e].y);
+                o[r][e].z = fmaf(p[r], x.z, o[r][e].z);
+                o[r][e].w = fmaf(p[r], x.w, o[r][e].w);
+              }
+            }
+          }
+        }
       }
-      put_unit<float, D, RU, SR, kThreads>(a, wc, whole, m_s, l_s, merge);
-      __syncthreads();
+      __syncwarp();
+      if (lane == 0) tcgen::mbar_arrive(bar_empty + 8 * slot);
+      if (u.last) {
+        // the lanes of a row, then the warps one after the other
+#pragma unroll
+        for (int r = 0; r < RU; ++r) {
+#pragma unroll
+          for (int i = kParts; i < 32; i *= 2) l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], i);
+#pragma unroll
+          for (int e = 0; e < kEach; ++e)
+#pragma unroll
+            for (int i = kCols; i < 32; i *= 2) {
+              o[r][e].x += __shfl_xor_sync(0xffffffffu, o[r][e].x, i);
+              o[r][e].y += __shfl_xor_sync(0xffffffffu, o[r][e].y, i);
+              o[r][e].z += __shfl_xor_sync(0xffffffffu, o[r][e].z, i);
+              o[r][e].w += __shfl_xor_sync(0xffffffffu, o[r][e].w, i);
+            }
+          if (lane == 0) {
+            red_m[warp * RU + r] = m_run[r];
+            red_l[warp * RU + r] = l_run[r];
+          }
+        }
+        if (!all.meet(a, gave_up, s)) return;
+#pragma unroll
+        for (int r = 0; r < RU; ++r) {
+          float m_all = -INFINITY, l_all = 0.f;
+#pragma unroll
+          for (int w = 0; w < C::kWarps; ++w) m_all = fmaxf(m_all, red_m[w * RU + r]);
+#pragma unroll
+          for (int w = 0; w < C::kWarps; ++w) {
+            const float mw = red_m[w * RU + r];
+            l_all += (mw == -INFINITY ? 1.f : ex2(mw - m_all)) * red_l[w * RU + r];
+          }
+          const float f = m_run[r] == -INFINITY ? 1.f : ex2(m_run[r] - m_all);
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) o[r][e] = make_float4(o[r][e].x * f, o[r][e].y * f, o[r][e].z * f, o[r][e].w * f);
+          if (threadIdx.x == 0) {
+            red_m[C::kWarps * RU + r] = m_all;
+            red_l[C::kWarps * RU + r] = l_all;
+          }
+        }
+#pragma unroll 1
+        for (int w = 0; w < C::kWarps; ++w) {
+          if (warp == w && sub == 0) {
+#pragma unroll
+            for (int r = 0; r < RU; ++r)
+#pragma unroll
+              for (int e = 0; e < kEach; ++e) {
+                float4* const x = reinterpret_cast<float4*>(merge) + r * kVec + e * kCols + col;
+                const float4 y = w == 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *x;
+                *x = make_float4(y.x + o[r][e].x, y.y + o[r][e].y, y.z + o[r][e].z, y.w + o[r][e].w);
+              }
+          }
+          if (!all.meet(a, gave_up, s)) return;
+        }
+        put_unit<float, D, RU>(a, u, red_m + C::kWarps * RU, red_l + C::kWarps * RU, merge, C::kWarps * 32);
+        if (!all.meet(a, gave_up, s)) return;
+      }
     }
-    if (s + 1 < total) wc.next(a);
-  }
-  cp_async_wait<0>();
-  end_main(a);
+  });
 }
 
 // ---- fold ---------------------------------------------------------------------------
 
-// Parts of the rows that no block finished. A row has D / 4 threads, four columns each, times kSlices, which take every
-// kSlices-th part.
+// Parts of the rows that no block finished, and rows without keys. A row has D / 4 threads, four columns each, times kSlices, which
+// take every kSlices-th part; a thread asks for eight parts at a time.
 constexpr int kFoldThreads = 256;
-template <typename T, int D, int SR, int RU, int kSlices>
-__global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const PagedArgs a) {
-  constexpr int kVec = D / 4, kRowsPer = kFoldThreads / kVec / kSlices;
+template <typename T, int D, int RU, int kSlices>
+__global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const __grid_constant__ PagedArgs a) {
+  constexpr int kVec = D / 4, kRowsPer = kFoldThreads / kVec / kSlices, kBatch = 8;
   __shared__ float4 acc_of[kSlices > 1 ? kFoldThreads : 1];
   __shared__ float2 ml_of[kSlices > 1 ? kFoldThreads / kVec : 1];
   let_next_start();
@@ -715,36 +774,21 @@ __global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const PagedArg
   const int row = static_cast<int>(blockIdx.x) * kRowsPer + lane_row / kSlices;
   const bool mine = row < a.B * a.H;
   const int b = mine ? row / a.H : 0, h = mine ? row - b * a.H : 0, kvh = h % a.kvH, g = h / a.kvH;
+  const int own_uid = a.kvH * a.RB + (b * a.kvH + kvh) * a.HB + g / RU;
+  const int of_all = b * a.G + g, shared_uid = a.RB > 0 ? kvh * a.RB + of_all / RU : own_uid;
   wait_for_previous();
+  const bool lost = *reinterpret_cast<const volatile int*>(a.status) != 0;  // some wait ran out: the rows stay as they are
+  const int2 own = a.unit_parts[own_uid], pre = a.unit_parts[shared_uid];
   int start = 0, end = 0;
   if (mine) own_keys(a, b, &start, &end);
-  const int n = static_cast<int>((static_cast<long long>(end) - start + SR - 1) / SR);
-  const long long per = a.head[0];
-  // parts [lo, lo + count) of a unit: those of the blocks that its stages lie with
-  long long own_lo = 0, pre_lo = 0;
-  int own_n = 0, pre_n = 0;
-  if (mine && n > 0) {
-    const int hb = g / RU;
-    const long long beg = a.head[1 + b] + static_cast<long long>(kvh * a.HB + hb) * n;
-    const long long c0 = beg / per, c1 = (beg + n - 1) / per;
-    const long long uid = static_cast<long long>(a.kvH) * a.RB + (static_cast<long long>(b) * a.kvH + kvh) * a.HB + hb;
-    own_lo = (c0 + uid) * a.rs + g % RU;
-    own_n = static_cast<int>(c1 - c0) + 1;
-  }
-  if (mine && start > 0 && a.RB > 0) {
-    const int i = b * a.G + g, tile = i / RU, stages = (a.shared_len + SR - 1) / SR;
-    const long long uid = static_cast<long long>(kvh) * a.RB + tile, beg = uid * stages;
-    const long long c0 = beg / per, c1 = (beg + stages - 1) / per;
-    pre_lo = (c0 + uid) * a.rs + i % RU;
-    pre_n = static_cast<int>(c1 - c0) + 1;
-  }
-  long long pre_step = a.rs;
+  const int own_n = end > start ? own.y : 0;
+  const long long own_lo = (static_cast<long long>(own.x) + own_uid) * a.rs + g % RU;
+  int pre_n = 0;
+  long long pre_lo = 0, pre_step = a.rs;
   const float2* pre_ml = a.part_ml;
   const float* pre_o = a.part_o;
-  bool lost = false;  // the kernel of the shared pages gave up: the rows stay as they are
-  if (a.shared_ml) {
-    lost = *reinterpret_cast<const volatile int*>(a.status) != 0;
-    if (mine && start > 0) {
+  if (start > 0) {
+    if (a.shared_ml) {
       const SharedPlan& s = a.shared;
       const int tile = s.pack > 1 ? g / s.pack : b / 128 * a.G + g, at = s.pack > 1 ? g % s.pack * a.B + b : b % 128;
       pre_step = s.tiles_per_block * 128;
@@ -753,42 +797,58 @@ __global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const PagedArg
       pre_n = s.shares;
       pre_ml = a.shared_ml;
       pre_o = a.shared_o;
+    } else {
+      pre_lo = (static_cast<long long>(pre.x) + shared_uid) * a.rs + of_all % RU;
+      pre_n = pre.y;
     }
   }
   const bool done = lost || (own_n == 1 && start == 0);  // by the block that had the unit
   const int parts = mine && !done ? own_n + pre_n : 0;
-  auto ml_of_part = [&](int i) { return i < pre_n ? pre_ml[pre_lo + i * pre_step] : a.part_ml[own_lo + static_cast<long long>(i - pre_n) * a.rs]; };
-  auto o_of_part = [&](int i) {
-    const float* const o = i < pre_n ? pre_o + (pre_lo + i * pre_step) * D : a.part_o + (own_lo + static_cast<long long>(i - pre_n) * a.rs) * D;
-    return *reinterpret_cast<const float4*>(o + col * 4);
-  };
-  float m_all = -INFINITY;
-#pragma unroll 4
-  for (int i = slice; i < parts; i += kSlices) m_all = fmaxf(m_all, ml_of_part(i).x);
-  float l_all = 0.f;
+  float m_all = -INFINITY, l_all = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = slice; i < parts; i += kSlices) {
-    const float2 ml = ml_of_part(i);
-    const float4 o = o_of_part(i);
-    if (ml.y == 0.f) continue;  // saw nothing
-    const float f = ml.x > -INFINITY ? ex2(ml.x - m_all) : 1.f;
-    l_all += f * ml.y;
-    acc.x += f * o.x;
-    acc.y += f * o.y;
-    acc.z += f * o.z;
-    acc.w += f * o.w;
+  for (int i0 = slice; i0 < parts; i0 += kSlices * kBatch) {
+    float2 ml[kBatch];
+    float4 o[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int i = i0 + j * kSlices;
+      ml[j] = make_float2(-INFINITY, 0.f);
+      o[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < parts) {
+        const bool is_pre = i < pre_n;
+        const long long at = is_pre ? pre_lo + i * pre_step : own_lo + static_cast<long long>(i - pre_n) * a.rs;
+        ml[j] = (is_pre ? pre_ml : a.part_ml)[at];
+        o[j] = *reinterpret_cast<const float4*>((is_pre ? pre_o : a.part_o) + at * D + col * 4);
+      }
+    }
+    float m_new = m_all;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) m_new = fmaxf(m_new, ml[j].x);
+    const float f_old = m_all == -INFINITY ? 1.f : ex2(m_all - m_new);
+    l_all *= f_old;
+    acc = make_float4(acc.x * f_old, acc.y * f_old, acc.z * f_old, acc.w * f_old);
+    m_all = m_new;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if (ml[j].y == 0.f) continue;  // saw nothing, and may have left no O
+      const float f = ml[j].x > -INFINITY ? ex2(ml[j].x - m_all) : 1.f;
+      l_all += f * ml[j].y;
+      acc.x += f * o[j].x;
+      acc.y += f * o[j].y;
+      acc.z += f * o[j].z;
+      acc.w += f * o[j].w;
+    }
   }
   if constexpr (kSlices > 1) {
     acc_of[threadIdx.x] = acc;
     if (col == 0) ml_of[lane_row] = make_float2(m_all, l_all);
     __syncthreads();
     if (slice == 0) {
-      const float2 own = make_float2(m_all, l_all);
+      const float2 first = make_float2(m_all, l_all);
 #pragma unroll
       for (int i = 1; i < kSlices; ++i) m_all = fmaxf(m_all, ml_of[lane_row + i].x);
-      const float f0 = own.x > -INFINITY ? ex2(own.x - m_all) : 1.f;
-      l_all = f0 * own.y;
+      const float f0 = first.x > -INFINITY ? ex2(first.x - m_all) : 1.f;
+      l_all = f0 * first.y;
       acc = make_float4(f0 * acc.x, f0 * acc.y, f0 * acc.z, f0 * acc.w);
 #pragma unroll
       for (int i = 1; i < kSlices; ++i) {
@@ -813,20 +873,20 @@ __global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const PagedArg
 
 // ---- host side ----------------------------------------------------------------------
 
-// Which kernel a call runs, and its room: header, (m, l) and O of every part. A block leaves at most one part a unit, and
-// block c's of unit u is part c + u: both only grow along the list, so no two meet.
-struct PagedPlan {
-  int RU, SR, blocks;
-  bool tc;  // shared pages by the tensor-core kernel
-  SharedPlan shared;
-  double most;  // stages that there can be
-  int rs;  // rows of a part
-  size_t parts, head_bytes, ml_bytes, o_bytes, shared_rows, shared_ml_bytes, bytes;
-};
-
-constexpr int kBlocksPerSm = 2;  // of both kernels: 96 KB of ring each
+constexpr int kBlocksPerSm = 2;  // of both kernels
 
 int fp32_rows(int G) { return G <= 1 ? 1 : G <= 2 ? 2 : G <= 4 ? 4 : 8; }
+
+// How a call runs, and its room: which blocks have parts of a unit, and (m, l) and O of every part. A block leaves at most one
+// part of a unit, and block c's of unit u is part c + u: both only grow along the list, so no two meet.
+struct PagedPlan {
+  int RU, SR, HB, RB, blocks;
+  int rs;       // rows of a part
+  double most;  // stages that there can be
+  bool tc;      // shared pages by the tensor-core kernel
+  SharedPlan shared;
+  size_t unit_bytes, ml_bytes, o_bytes, shared_ml_bytes, bytes;
+};
 
 PagedPlan make_plan(const ra_paged_kv& c, int heads, int shared_len) {
   PagedPlan p = {};
@@ -835,84 +895,80 @@ PagedPlan make_plan(const ra_paged_kv& c, int heads, int shared_len) {
   const long long rows_shared = shared_len > 0 ? static_cast<long long>(c.batch) * G : 0;
   p.RU = f32 ? fp32_rows(static_cast<int>(std::max<long long>(std::min<long long>(rows_shared, 8), G))) : 16;
   p.SR = f32 ? (c.head_dim == 256 ? 16 : 32) : c.head_dim == 256 ? 32 : 64;
-  p.tc = !f32 && rows_shared > 0 && static_cast<long long>(c.num_pages) * c.kv_heads < (1ll << 31) - 1 && c.num_pages > 0 &&
-         plan_shared_prefix(c.batch, heads, c.kv_heads, c.head_dim, shared_len, &p.shared);
-  const long long HB = (G + p.RU - 1) / p.RU, RB = p.tc ? 0 : (rows_shared + p.RU - 1) / p.RU;
-  const long long units = c.kv_heads * (RB + c.batch * HB);
-  // stages that there are at most: as many as the tables have room for
+  p.tc = !f32 && rows_shared > 0 && plan_shared_prefix(c.batch, heads, c.kv_heads, c.head_dim, shared_len, &p.shared);
+  p.HB = (G + p.RU - 1) / p.RU;
+  p.RB = p.tc ? 0 : static_cast<int>((rows_shared + p.RU - 1) / p.RU);
+  const size_t units = static_cast<size_t>(c.kv_heads) * (p.RB + static_cast<size_t>(c.batch) * p.HB);
+  // as many stages as the tables have room for
   const long long room = static_cast<long long>(c.max_pages) * c.page_size;
-  p.most = static_cast<double>(c.kv_heads) * (static_cast<double>(c.batch) * HB * ((room + p.SR - 1) / p.SR) +
-                                                   static_cast<double>(RB) * ((shared_len + p.SR - 1) / p.SR));
+  p.most = static_cast<double>(c.kv_heads) * (static_cast<double>(c.batch) * p.HB * ((room + p.SR - 1) / p.SR) +
+                                              static_cast<double>(p.RB) * ((shared_len + p.SR - 1) / p.SR));
   const int wave = kBlocksPerSm * sm_count();
   p.blocks = p.most < wave ? static_cast<int>(p.most) : wave;
-  p.parts = static_cast<size_t>(units) + p.blocks;
-  p.rs = RB > 0 ? p.RU : std::min(p.RU, G);
-  const size_t rs = p.rs;
+  p.rs = p.RB > 0 ? p.RU : std::min(p.RU, G);
   auto whole = [](size_t n) { return (n + 127) & ~static_cast<size_t>(127); };
-  p.head_bytes = whole((1 + static_cast<size_t>(c.batch)) * 8);
-  p.ml_bytes = whole(p.parts * rs * sizeof(float2));
-  p.o_bytes = whole(p.parts * rs * c.head_dim * sizeof(float));
-  p.shared_rows = p.tc ? shared_part_rows(p.shared, c.kv_heads) : 0;
-  p.shared_ml_bytes = whole(p.shared_rows * sizeof(float2));
-  p.bytes = p.head_bytes + p.ml_bytes + p.o_bytes + p.shared_ml_bytes + p.shared_rows * c.head_dim * sizeof(float);
+  const size_t rows = (units + p.blocks) * p.rs, shared_rows = p.tc ? shared_part_rows(p.shared, c.kv_heads) : 0;
+  p.unit_bytes = whole(units * sizeof(int2));
+  p.ml_bytes = whole(rows * sizeof(float2));
+  p.o_bytes = whole(rows * c.head_dim * sizeof(float));
+  p.shared_ml_bytes = whole(shared_rows * sizeof(float2));
+  p.bytes = p.unit_bytes + p.ml_bytes + p.o_bytes + p.shared_ml_bytes + shared_rows * c.head_dim * sizeof(float);
   return p;
 }
 
-template <void (*kern)(PagedArgs)>
-int launch_main(int threads, int smem, int blocks, const PagedArgs& a, cudaStream_t stream) {
+template <void (*kern)(CUtensorMap, CUtensorMap, PagedArgs), typename C>
+int launch_main(const CUtensorMap& k, const CUtensorMap& v, int blocks, const PagedArgs& a, cudaStream_t stream) {
   static std::atomic<unsigned long long> smem_set{0};  // once per device and instantiation
   int dev = 0;
   RAB_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !(smem_set.load(std::memory_order_acquire) >> dev & 1ull)) {
-    RAB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    RAB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
     if (dev >= 0 && dev < 64) smem_set.fetch_or(1ull << dev, std::memory_order_release);
   }
-  RAB_CUDA(launch_overlapped(kern, dim3(static_cast<unsigned>(blocks)), dim3(threads), smem, stream, a));
+  RAB_CUDA(launch_overlapped(kern, dim3(static_cast<unsigned>(blocks)), dim3(C::kThreads), C::kSmemBytes, stream, k, v, a));
   return RA_OK;
 }
 
-template <typename T, int D, int SR, int RU>
-int launch_fold(const PagedArgs& a, int blocks, cudaStream_t stream) {
+template <typename T, int D, int RU>
+int launch_fold(const PagedArgs& a, cudaStream_t stream) {
   const long long rows = static_cast<long long>(a.B) * a.H;
-  constexpr int kPer = kFoldThreads / (D / 4);
-  if (rows * 4 <= blocks) {
-    RAB_CUDA(launch_overlapped(paged_fold_kernel<T, D, SR, RU, 4>, dim3(static_cast<unsigned>((rows + kPer / 4 - 1) / (kPer / 4))),
+  constexpr int kPer = kFoldThreads / (D / 4), kMany = kPer < 8 ? kPer : 8;
+  // few rows: their parts are shared out, since the blocks of a wave may all have parts of the same row
+  if (rows <= static_cast<long long>(sm_count()) * kPer) {
+    RAB_CUDA(launch_overlapped(paged_fold_kernel<T, D, RU, kMany>, dim3(static_cast<unsigned>((rows * kMany + kPer - 1) / kPer)),
                                dim3(kFoldThreads), 0, stream, a));
   } else {
-    RAB_CUDA(launch_overlapped(paged_fold_kernel<T, D, SR, RU, 1>, dim3(static_cast<unsigned>((rows + kPer - 1) / kPer)),
+    RAB_CUDA(launch_overlapped(paged_fold_kernel<T, D, RU, 1>, dim3(static_cast<unsigned>((rows + kPer - 1) / kPer)),
                                dim3(kFoldThreads), 0, stream, a));
   }
   return RA_OK;
 }
 
-template <typename T, int D>
-int launch_16(const PagedArgs& a, const PagedPlan& p, cudaStream_t stream) {
-  using C = PagedMma<D>;
+template <typename T, int D, int RU>
+int launch_rows(const ra_paged_kv& c, const PagedArgs& a, const PagedPlan& p, cudaStream_t stream) {
   if (p.blocks > 0) {
-    const int rc = launch_main<paged_mma_kernel<T, D>>(C::kThreads, C::kSmemBytes, p.blocks, a, stream);
+    CUtensorMap k, v;
+    const long long heads = static_cast<long long>(a.num_pages) * a.kvH, stride = static_cast<long long>(c.page_size) * D;
+    const int box = std::min(c.page_size, p.SR);
+    int rc = tcgen::make_map(&k, c.dtype, c.k, D, c.page_size, heads, stride, box);
+    if (rc == RA_OK) rc = tcgen::make_map(&v, c.dtype, c.v, D, c.page_size, heads, stride, box);
+    if (rc == RA_OK) {
+      if constexpr (sizeof(T) == 4) rc = launch_main<paged_f32_kernel<D, RU>, F32Block<D, RU>>(k, v, p.blocks, a, stream);
+      else rc = launch_main<paged_mma_kernel<T, D>, MmaBlock<T, D>>(k, v, p.blocks, a, stream);
+    }
     if (rc != RA_OK) return rc;
   }
-  return launch_fold<T, D, C::SR, C::RU>(a, p.blocks, stream);
-}
-
-template <int D, int RU>
-int launch_32(const PagedArgs& a, const PagedPlan& p, cudaStream_t stream) {
-  using C = PagedF32<D, RU>;
-  if (p.blocks > 0) {
-    const int rc = launch_main<paged_f32_kernel<D, RU>>(C::kThreads, C::kSmemBytes, p.blocks, a, stream);
-    if (rc != RA_OK) return rc;
-  }
-  return launch_fold<float, D, C::SR, RU>(a, p.blocks, stream);
+  return launch_fold<T, D, RU>(a, stream);
 }
 
 template <int D>
-int launch_head_dim(int dtype, const PagedArgs& a, const PagedPlan& p, cudaStream_t stream) {
-  if (dtype == RA_F16) return launch_16<__half, D>(a, p, stream);
-  if (dtype == RA_BF16) return launch_16<__nv_bfloat16, D>(a, p, stream);
-  if (p.RU == 1) return launch_32<D, 1>(a, p, stream);
-  if (p.RU == 2) return launch_32<D, 2>(a, p, stream);
-  if (p.RU == 4) return launch_32<D, 4>(a, p, stream);
-  return launch_32<D, 8>(a, p, stream);
+int launch_head_dim(const ra_paged_kv& c, const PagedArgs& a, const PagedPlan& p, cudaStream_t stream) {
+  if (c.dtype == RA_F16) return launch_rows<__half, D, 16>(c, a, p, stream);
+  if (c.dtype == RA_BF16) return launch_rows<__nv_bfloat16, D, 16>(c, a, p, stream);
+  if (p.RU == 1) return launch_rows<float, D, 1>(c, a, p, stream);
+  if (p.RU == 2) return launch_rows<float, D, 2>(c, a, p, stream);
+  if (p.RU == 4) return launch_rows<float, D, 4>(c, a, p, stream);
+  return launch_rows<float, D, 8>(c, a, p, stream);
 }
 
 int check_decode(const ra_paged_kv& c, int heads, const int* shared_pages, int shared_len) {
@@ -924,9 +980,16 @@ int check_decode(const ra_paged_kv& c, int heads, const int* shared_pages, int s
   if (rc != RA_OK) return rc;
   RAB_REQUIRE(heads >= c.kv_heads && heads <= 4096, RA_ERR_INVALID, "%s: bad heads", what);
   RAB_REQUIRE(static_cast<long long>(c.batch) * heads < (1ll << 24), RA_ERR_INVALID, "%s: too many rows", what);
+  RAB_REQUIRE(static_cast<long long>(c.num_pages) * c.kv_heads < (1ll << 31) - 1, RA_ERR_INVALID, "%s: too many pages", what);
   RAB_REQUIRE(shared_len >= 0 && shared_len % c.page_size == 0 && (shared_len == 0 || shared_pages), RA_ERR_INVALID,
               "%s: shared pages are whole: shared_len=%d, page_size=%d", what, shared_len, c.page_size);
   return RA_OK;
+}
+
+// A cache without pages holds no keys, whatever the tables say.
+ra_paged_kv without_pages(ra_paged_kv c, int* shared_len) {
+  if (c.num_pages == 0) c.max_pages = *shared_len = 0;
+  return c;
 }
 
 }  // namespace
@@ -937,32 +1000,31 @@ using namespace rab;
 extern "C" {
 
 size_t ra_paged_decode_workspace_bytes(const ra_paged_kv* cache, int heads, int shared_len) {
-  if (!cache) return 0;
-  ra_paged_kv c = *cache;
   int none = 0;
-  if (check_decode(c, heads, &none, shared_len) != RA_OK) return 0;
+  if (!cache || check_decode(*cache, heads, &none, shared_len) != RA_OK) return 0;
+  const ra_paged_kv c = without_pages(*cache, &shared_len);
   return make_plan(c, heads, shared_len).bytes;
 }
 
 int ra_paged_decode(const ra_paged_kv* cache, const void* q, int heads, const int* shared_pages, int shared_len, void* out,
                     float* lse, void* workspace, size_t workspace_bytes, ra_stream stream_) {
   RAB_REQUIRE(cache != nullptr, RA_ERR_INVALID, "paged_decode: null argument");
-  const ra_paged_kv& c = *cache;
-  const int rc = check_decode(c, heads, shared_pages, shared_len);
+  int rc = check_decode(*cache, heads, shared_pages, shared_len);
   if (rc != RA_OK) return rc;
-  if (c.batch == 0) return RA_OK;
+  if (cache->batch == 0) return RA_OK;
   RAB_REQUIRE(q && out, RA_ERR_INVALID, "paged_decode: null argument");
   RAB_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0, RA_ERR_INVALID,
               "paged_decode: q and out must be 16-byte aligned");
+  const ra_paged_kv c = without_pages(*cache, &shared_len);
   const PagedPlan p = make_plan(c, heads, shared_len);
   // (a share is counted in 32 bits; tables that name a page over and over could ask for more)
   RAB_REQUIRE(p.most < 2147483648.0 * std::max(p.blocks, 1), RA_ERR_INVALID, "paged_decode: too many keys");
   RAB_REQUIRE(workspace && workspace_bytes >= p.bytes && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, RA_ERR_OVERFLOW,
               "paged_decode: workspace too small or not 16-byte aligned");
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  unsigned char* const ws = static_cast<unsigned char*>(workspace);
   PagedArgs a;
   a.q = q;
-  a.k = c.k;
-  a.v = c.v;
   a.out = out;
   a.lse = lse;
   a.table = c.page_table;
@@ -977,32 +1039,30 @@ int ra_paged_decode(const ra_paged_kv* cache, const void* q, int heads, const in
   a.H = heads;
   a.kvH = c.kv_heads;
   a.G = (heads + c.kv_heads - 1) / c.kv_heads;
-  a.HB = (a.G + p.RU - 1) / p.RU;
-  a.RB = shared_len > 0 && !p.tc ? static_cast<int>((static_cast<long long>(a.B) * a.G + p.RU - 1) / p.RU) : 0;
+  a.HB = p.HB;
+  a.RB = p.RB;
   a.rs = p.rs;
-  a.min_per = 1;
   a.scale_log2 = kLog2e / std::sqrt(static_cast<float>(c.head_dim));
-  unsigned char* const ws = static_cast<unsigned char*>(workspace);
-  a.head = reinterpret_cast<long long*>(ws);
-  a.part_ml = reinterpret_cast<float2*>(ws + p.head_bytes);
-  a.part_o = reinterpret_cast<float*>(ws + p.head_bytes + p.ml_bytes);
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  a.unit_parts = reinterpret_cast<int2*>(ws);
+  a.part_ml = reinterpret_cast<float2*>(ws + p.unit_bytes);
+  a.part_o = reinterpret_cast<float*>(ws + p.unit_bytes + p.ml_bytes);
   a.shared = p.shared;
   a.shared_ml = nullptr;
   a.shared_o = nullptr;
-  a.status = nullptr;
+  a.status = device_status_ptr();
+  RAB_REQUIRE(a.status != nullptr, RA_ERR_CUDA, "paged_decode: no device status word");
+  a.wait_ns = tcgen::tc_wait_limit_ns();
   if (p.tc) {
-    a.shared_ml = reinterpret_cast<float2*>(ws + p.head_bytes + p.ml_bytes + p.o_bytes);
-    a.shared_o = reinterpret_cast<float*>(ws + p.head_bytes + p.ml_bytes + p.o_bytes + p.shared_ml_bytes);
-    a.status = device_status_ptr();
+    a.shared_ml = reinterpret_cast<float2*>(ws + p.unit_bytes + p.ml_bytes + p.o_bytes);
+    a.shared_o = reinterpret_cast<float*>(ws + p.unit_bytes + p.ml_bytes + p.o_bytes + p.shared_ml_bytes);
     const SharedPrefix s{q, c.k, c.v, a.B, a.H, a.kvH, c.head_dim, shared_pages, c.lens, shared_len, c.num_pages, c.max_pages, a.shift};
-    const int rc2 = launch_shared_prefix(c.dtype, s, p.shared, a.shared_o, a.shared_ml, stream);
-    if (rc2 != RA_OK) return rc2;
+    rc = launch_shared_prefix(c.dtype, s, p.shared, a.shared_o, a.shared_ml, stream);
+    if (rc != RA_OK) return rc;
   }
-  if (c.head_dim == 32) return launch_head_dim<32>(c.dtype, a, p, stream);
-  if (c.head_dim == 64) return launch_head_dim<64>(c.dtype, a, p, stream);
-  if (c.head_dim == 128) return launch_head_dim<128>(c.dtype, a, p, stream);
-  return launch_head_dim<256>(c.dtype, a, p, stream);
+  if (c.head_dim == 32) return launch_head_dim<32>(c, a, p, stream);
+  if (c.head_dim == 64) return launch_head_dim<64>(c, a, p, stream);
+  if (c.head_dim == 128) return launch_head_dim<128>(c, a, p, stream);
+  return launch_head_dim<256>(c, a, p, stream);
 }
 
 }  // extern "C"
