@@ -6,18 +6,19 @@
 // What bounds it is the cache: every row is read once. The work is cut into units, the up to RU query rows that read the same
 // keys: the heads of a KV head and a sequence, behind the shared pages where the sequence has them; and for the shared pages RU
 // rows of all sequences. A unit is a list of stages of SR keys, and all units' stages one after the other are dealt in equal
-// shares to the blocks of one wave, so that lengths do not matter to the balance. A unit that lies in one share is finished
+// shares to the warps of one wave, so that lengths do not matter to the balance. A unit that lies in one share is finished
 // there; of others every share leaves (O, m, l) in the workspace, and a second kernel folds them.
 //
-// Inside a block one warp walks the list, looks the pages up a stage ahead and copies a stage's rows with TMA (a piece of a page
-// and 128 bytes of its rows a lane, 128-byte swizzle) into a ring of 96 KB, two blocks to an SM; it leaves beside each stage what
-// the other warps have to know of it. Each of those takes its own keys of a stage, with a running maximum, sum and O of
-// its own: nothing meets before the end of a unit, and the copies run on across units.
+// A warp works alone: it walks its share, looks the pages up a stage ahead and copies the rows of a stage with TMA (a piece of a
+// page and 128 bytes of its rows a lane, 128-byte swizzle) into a ring of its own, 192 KB for the warps of an SM. Where a unit
+// ends and the next one's queries come, and where it waits for a copy, the others of the SM run on. us a pass, four sequences of
+// 131072 to 262144 rows (H32/kvH8 D128 fp16) and 256 of 300 to 600: 16-byte cp.async of all threads and a barrier a stage
+// 854; a copying warp to four that meet where a unit ends 502 and 103; so 499 and 80.
 //
 // 16-bit caches: both products on mma.sync m16n8k16, the unit's rows as its M rows, as in decode_mma_kernel (decode.cu). fp32:
-// plain multiply-adds, four or eight lanes to a key for the scores, four columns a lane for the sum over V.
+// plain multiply-adds, four lanes to a key for the scores, four columns a lane for the sum over V.
 //
-// Every wait on a barrier is bounded, as in the step kernels: when one runs out the block records it in the device status word
+// Every wait on a barrier is bounded, as in the step kernels: when one runs out the warp records it in the device status word
 // and leaves, and the fold leaves every row that it would have written as it is.
 #include <algorithm>
 #include <atomic>
@@ -52,7 +53,7 @@ struct PagedArgs {
   int RB;  // units of a KV head on the shared pages (0: not by this kernel)
   int rs;  // rows of a part in the workspace
   float scale_log2;
-  int2* unit_parts;  // first block that has a part of a unit, and how many do
+  int2* unit_parts;  // first share that has a part of a unit, and how many do
   float2* part_ml;   // (m in log2 units, l) of rs rows, a part after the other
   float* part_o;
   // shared pages by the tensor-core kernel (step_tc.cu; RB is 0 then): its parts, see SharedPrefix
@@ -115,16 +116,16 @@ struct Walk {
 };
 
 // Room of find_share.
-template <int kThreads>
+template <int kWarps>
 struct ScanRoom {
-  long long sums[kThreads / 32];
-  long long in_seq;
-  int seq;
+  long long sums[kWarps];
+  long long in_seq[kWarps];
+  int seq[kWarps];
 };
 
 // Sum over the block of a thread's v, and the sum over the threads before it.
-template <int kThreads>
-__device__ inline long long block_scan(long long v, long long* total, ScanRoom<kThreads>* room) {
+template <int kWarps>
+__device__ inline long long block_scan(long long v, long long* total, ScanRoom<kWarps>* room) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   long long incl = v;
 #pragma unroll
@@ -137,7 +138,7 @@ __device__ inline long long block_scan(long long v, long long* total, ScanRoom<k
   __syncthreads();
   long long before = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
+  for (int w = 0; w < kWarps; ++w) {
     if (w < warp) before += room->sums[w];
     all += room->sums[w];
   }
@@ -145,9 +146,10 @@ __device__ inline long long block_scan(long long v, long long* total, ScanRoom<k
   return before + incl - v;
 }
 
-// The block's share: its first place, and how many stages; *per: stages of a whole share.
-template <int SR, int kThreads>
-__device__ inline int find_share(const PagedArgs& a, Walk<SR>* w, int* per, ScanRoom<kThreads>* room) {
+// The warp's share: its first place, and how many stages (0: none); *per: stages of a whole share. Every thread of the block calls.
+template <int SR, int kWarps>
+__device__ inline int find_share(const PagedArgs& a, int warp, Walk<SR>* w, int* per, ScanRoom<kWarps>* room) {
+  constexpr int kThreads = 32 * kWarps;
   const int units = a.kvH * a.HB;
   long long shared_total = 0;
   if (a.RB > 0) shared_total = static_cast<long long>(a.kvH) * a.RB * w->shared_stages(a);
@@ -155,11 +157,34 @@ __device__ inline int find_share(const PagedArgs& a, Walk<SR>* w, int* per, Scan
   const int mine = static_cast<int>(threadIdx.x) < a.B ? own_stages<SR>(a, threadIdx.x) : 0;
   long long sum = mine, total;
   for (int b = static_cast<int>(threadIdx.x) + kThreads; b < a.B; b += kThreads) sum += own_stages<SR>(a, b);
-  const long long before = block_scan<kThreads>(sum, &total, room);
-  const long long all = shared_total + total * units;
-  const long long share = max(1ll, (all + gridDim.x - 1) / gridDim.x);
+  const long long before = block_scan<kWarps>(sum, &total, room);
+  const long long all = shared_total + total * units, shares = static_cast<long long>(gridDim.x) * kWarps;
+  const long long share = max(1ll, (all + shares - 1) / shares);
   *per = static_cast<int>(share);
-  const long long first = share * blockIdx.x, stages = min(share, all - first);
+  const long long first_of_block = share * blockIdx.x * kWarps, end_of_block = min(first_of_block + share * kWarps, all);
+  if (end_of_block > shared_total) {
+    long long base = shared_total;
+    for (int b0 = 0; b0 < a.B && base < end_of_block; b0 += kThreads) {
+      const int b = b0 + static_cast<int>(threadIdx.x);
+      long long n = mine, chunk = total, ahead = before;  // (of the only chunk)
+      if (a.B > kThreads) {
+        if (b0 > 0) n = b < a.B ? own_stages<SR>(a, b) : 0;
+        ahead = block_scan<kWarps>(n, &chunk, room);
+      }
+      const long long at = base + ahead * units;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) {
+        const long long first = first_of_block + share * i;
+        if (first >= at && first < at + n * units) {
+          room->seq[i] = b;
+          room->in_seq[i] = first - at;
+        }
+      }
+      base += chunk * units;
+    }
+  }
+  __syncthreads();
+  const long long first = first_of_block + share * warp, stages = min(share, all - first);
   if (stages <= 0) return 0;
   if (first < shared_total) {
     w->on_shared(a);
@@ -168,24 +193,8 @@ __device__ inline int find_share(const PagedArgs& a, Walk<SR>* w, int* per, Scan
     w->kvh = u / a.RB;
     w->hb = u % a.RB;
   } else {
-    long long base = shared_total;
-    for (int b0 = 0; b0 < a.B && base <= first; b0 += kThreads) {
-      const int b = b0 + static_cast<int>(threadIdx.x);
-      long long n = mine, chunk = total, ahead = before;  // (of the only chunk)
-      if (a.B > kThreads) {
-        if (b0 > 0) n = b < a.B ? own_stages<SR>(a, b) : 0;
-        ahead = block_scan<kThreads>(n, &chunk, room);
-      }
-      const long long at = base + ahead * units;
-      if (first >= at && first < at + n * units) {
-        room->seq = b;
-        room->in_seq = first - at;
-      }
-      base += chunk * units;
-    }
-    __syncthreads();
-    w->on_sequence(a, room->seq);
-    const long long in_seq = room->in_seq;
+    w->on_sequence(a, room->seq[warp]);
+    const long long in_seq = room->in_seq[warp];
     const int u = static_cast<int>(in_seq / w->n);
     w->st = static_cast<int>(in_seq - static_cast<long long>(u) * w->n);
     w->kvh = u / a.HB;
@@ -195,12 +204,12 @@ __device__ inline int find_share(const PagedArgs& a, Walk<SR>* w, int* per, Scan
   return static_cast<int>(stages);
 }
 
-// What the warps that compute have to know of a stage.
+// What a warp has to know of a stage when its copy has landed.
 struct StageInfo {
   int b, kvh, hb, uid;
   int keys;        // of the stage
   unsigned pages;  // bit i: keys 16 i and on are there
-  int first;       // of the block's part of the unit
+  int first;       // of the warp's part of the unit
   int last;        // the same; 2: and the part is the result, the unit being whole and no shared pages ahead of it
 };
 
@@ -228,127 +237,108 @@ __device__ inline void put4<__nv_bfloat16>(__nv_bfloat16* dst, float4 v) {
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack_pair<__nv_bfloat16>(v.x, v.y), pack_pair<__nv_bfloat16>(v.z, v.w));
 }
 
-// The end of the block's part of a unit, by `threads` threads: rows of (m, l) and O in shared memory. (l is 0 where no key was
-// seen, and NaN where one that is not finite was.)
-template <typename T, int D, int RU>
-__device__ inline void put_unit(const PagedArgs& a, const StageInfo& u, const float* m, const float* l, const float* o, int threads) {
-  constexpr int kVec = D / 4;
-  const size_t part = (static_cast<size_t>(blockIdx.x) + u.uid) * a.rs;
-  for (int i = threadIdx.x; i < RU * kVec; i += threads) {
-    const int r = i / kVec, col = i % kVec * 4;
-    int b, h;
-    if (!unit_row<RU>(a, u, r, &b, &h)) continue;
-    const float4 v = *reinterpret_cast<const float4*>(o + r * D + col);
-    if (u.last == 2) {
-      const float inv = 1.f / l[r];
-      const size_t row = static_cast<size_t>(b) * a.H + h;
-      put4(static_cast<T*>(a.out) + row * D + col,
-           l[r] == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-      if (a.lse && col == 0) a.lse[row] = l[r] > 0.f ? m[r] * kLn2 + logf(l[r]) : l[r] == 0.f ? -INFINITY : l[r];
-    } else {
-      *reinterpret_cast<float4*>(a.part_o + (part + r) * D + col) = v;
-      if (col == 0) a.part_ml[part + r] = make_float2(m[r], l[r]);
-    }
-  }
-}
-
-// Shared memory of a block of either kernel: kWarps warps that compute, then the one that copies. A stage's tensor is kBoxes boxes
-// of SR rows of 128 bytes, 16-byte piece c of a row's box at c ^ (row & 7).
-template <typename T, int D, int kWarps_, int SR_, int kRows_, int kExtra>
+// Shared memory of a block of either kernel: the rings of its warps, a stage being K's kBoxes boxes of SR rows of 128 bytes and
+// then V's, 16-byte piece c of a row's box at c ^ (row & 7).
+template <typename T, int D, int SR_, int kRows_, int kQueryBytes>
 struct PagedBlock {
-  static constexpr int kWarps = kWarps_, SR = SR_, RU = kRows_, kThreads = (kWarps + 1) * 32;
+  static constexpr int SR = SR_, RU = kRows_;
+  static constexpr int kWarps = D == 256 ? 2 : 4, kThreads = kWarps * 32;
   static constexpr int kEs = static_cast<int>(sizeof(T));
   static constexpr int kBoxes = D * kEs > 128 ? D * kEs / 128 : 1, kBoxCols = 128 / kEs;
   static constexpr int kTileBytes = SR * kBoxes * 128;  // per tensor
-  static constexpr int kStages = 96 * 1024 / (2 * kTileBytes) < 8 ? 96 * 1024 / (2 * kTileBytes) : 8;
-  static constexpr int kOffMerge = 2 * kStages * kTileBytes;  // O of the warps, summed up
-  static constexpr int kOffExtra = kOffMerge + RU * D * 4;
-  static constexpr int kOffMl = kOffExtra + kExtra;           // m of every warp's rows and of all, then l
-  static constexpr int kOffInfo = (kOffMl + (kWarps + 1) * RU * 8 + 15) & ~15;
-  static constexpr int kOffBar = kOffInfo + kStages * static_cast<int>(sizeof(StageInfo));
-  static constexpr int kOffRoom = kOffBar + (2 * kStages + 1) * 8;
-  static constexpr int kOffFlag = kOffRoom + static_cast<int>(sizeof(ScanRoom<kThreads>));
+  static constexpr int kStages = 96 * 1024 / kWarps / (2 * kTileBytes);
+  static constexpr int kRingBytes = 2 * kStages * kTileBytes;  // of a warp
+  static constexpr int kOffQuery = kWarps * kRingBytes;        // fp32: every warp's query rows
+  static constexpr int kOffInfo = kOffQuery + kWarps * kQueryBytes;
+  static constexpr int kOffBar = kOffInfo + kWarps * kStages * static_cast<int>(sizeof(StageInfo));
+  static constexpr int kOffRoom = kOffBar + kWarps * kStages * 8;
+  static constexpr int kOffFlag = kOffRoom + static_cast<int>(sizeof(ScanRoom<kWarps>));
   static constexpr int kSmemBytes = kOffFlag + 8;
+  static_assert(kTileBytes % 1024 == 0 && kStages >= 3, "the ring");
   static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two blocks to an SM");
 };
 
-__device__ inline bool warp_wait(const PagedArgs& a, unsigned bar, unsigned parity, volatile int* gave_up, int which, int at) {
-  return __all_sync(0xffffffffu, tcgen::mbar_wait(bar, parity, gave_up, a.status, which, at, a.wait_ns)) != 0;
-}
-
-// The warp that copies: `total` stages from the place w on.
+// A warp's ring: copies run kStages stages ahead of what it computes.
 template <typename C>
-__device__ inline void copy_stages(const PagedArgs& a, const CUtensorMap* map_k, const CUtensorMap* map_v, Walk<C::SR> w, int total,
-                                   int per, unsigned char* smem, unsigned base, volatile int* gave_up) {
-  constexpr int SR = C::SR;
-  const int lane = threadIdx.x & 31;
-  const unsigned bar_full = base + C::kOffBar, bar_empty = bar_full + 8 * C::kStages;
-  // a lane's copies: a piece of the stage's rows, a box of one tensor (no more than 32: SR / 16 times kBoxes is at most 8)
-  static_assert(2 * C::kBoxes * (SR / 16) <= 32, "a copy a lane");
-  const int rows = min(1 << a.shift, SR), pieces = SR / rows;
-  const int piece = lane % pieces, box = lane / pieces % C::kBoxes, tensor = lane / pieces / C::kBoxes;
-  // the page of this lane's piece, as the head its rows are in the tensor map; -1 where there is none
-  auto look_up = [&]() {
-    if (piece * rows >= w.left()) return -1;
-    const int at = (w.start + w.st * SR + piece * rows) >> a.shift;
+struct Ring {
+  const PagedArgs& a;
+  const CUtensorMap *map_k, *map_v;
+  unsigned tiles, full;  // shared memory: the ring, its barriers
+  StageInfo* info;
+  volatile int* gave_up;
+  Walk<C::SR> w;         // the next stage to copy
+  int total, per, next = 0, first_st, head;
+
+  // A lane's copies: a piece of the stage's rows, a box of one tensor.
+  static_assert(2 * C::kBoxes * ((C::SR + 15) / 16) <= 32, "a copy a lane");
+  __device__ inline int rows() const { return min(1 << a.shift, C::SR); }
+  // The page of this lane's piece, as the head its rows are in the tensor map; -1 where there is none.
+  __device__ inline int look_up() const {
+    const int piece = static_cast<int>(threadIdx.x & 31) % (C::SR / rows());
+    if (piece * rows() >= w.left()) return -1;
+    const int at = (w.start + w.st * C::SR + piece * rows()) >> a.shift;
     const int* const table = w.b < 0 ? a.shared_pages : a.table + w.b * a.table_stride;
     if (at >= (w.b < 0 ? a.shared_len >> a.shift : a.max_pages)) return -1;
     const int page = table[at];
     return page >= 0 && page < a.num_pages ? page * a.kvH + w.kvh : -1;
-  };
-  int head = look_up(), first_st = w.st;
-  for (int s = 0; s < total; ++s) {
-    const int slot = s % C::kStages, use = s / C::kStages;
+  }
+  __device__ inline void begin() {
+    first_st = w.st;
+    head = look_up();
+    for (int s = 0; s < C::kStages; ++s) copy(s);
+  }
+  // Copies the next stage, if there is one, to a place that is free.
+  __device__ inline void copy(int slot) {
+    if (next >= total) return;
+    const int lane = threadIdx.x & 31, pieces = C::SR / rows();
+    const int piece = lane % pieces, box = lane / pieces % C::kBoxes, tensor = lane / pieces / C::kBoxes;
     if (w.st == 0) {
       first_st = 0;
-      // the block with a unit's first stage says which blocks have parts of it: this one and those that the rest reaches into
-      const int here = min(w.n, total - s);
-      if (lane == 0) a.unit_parts[w.uid] = make_int2(static_cast<int>(blockIdx.x), 1 + (w.n - here + per - 1) / per);
+      // the warp with a unit's first stage says which shares have parts of it: its own and those that the rest reaches into
+      const int here = min(w.n, total - next);
+      if (lane == 0)
+        a.unit_parts[w.uid] = make_int2(static_cast<int>(blockIdx.x * C::kWarps + (threadIdx.x >> 5)), 1 + (w.n - here + per - 1) / per);
     }
-    const int row = (w.start + w.st * SR + piece * rows) & ((1 << a.shift) - 1);
-    const int my_head = head;
-    const unsigned there = __ballot_sync(0xffffffffu, my_head >= 0 && lane < pieces);
-    StageInfo info;
-    info.b = w.b, info.kvh = w.kvh, info.hb = w.hb, info.uid = w.uid;
-    info.keys = min(SR, w.left());
-    info.pages = 0;
-#pragma unroll
-    for (int i = 0; i < SR / 16; ++i) info.pages |= (there >> (i * 16 / rows) & 1u) << i;
-    const bool ends = w.st == w.n - 1;
-    info.first = w.st == first_st;
-    info.last = ends && first_st == 0 && w.b >= 0 && w.start == 0 ? 2 : ends || s == total - 1;
-    // on to the next stage: its page numbers are on their way while this one waits for its place
-    if (s + 1 < total) {
+    const int row = (w.start + w.st * C::SR + piece * rows()) & ((1 << a.shift) - 1);
+    const unsigned there = __ballot_sync(0xffffffffu, head >= 0 && lane < pieces);
+    if (lane == 0) {
+      StageInfo i;
+      i.b = w.b, i.kvh = w.kvh, i.hb = w.hb, i.uid = w.uid;
+      i.keys = min(C::SR, w.left());
+      i.pages = there;
+      if (C::SR > 16 && pieces == 1) i.pages |= there << 1;  // (a page of 32 keys and more)
+      const bool ends = w.st == w.n - 1;
+      i.first = w.st == first_st;
+      i.last = ends && first_st == 0 && w.b >= 0 && w.start == 0 ? 2 : ends || next == total - 1;
+      info[slot] = i;
+      tcgen::mbar_expect_tx(full + 8 * slot, 2 * C::kBoxes * 128 * rows() * __popc(there));
+    }
+    __syncwarp();
+    if (tensor < 2 && head >= 0)
+      tcgen::tma_load_3d(tiles + (2 * slot + tensor) * C::kTileBytes + (box * C::SR + piece * rows()) * 128,
+                         tensor == 0 ? map_k : map_v, full + 8 * slot, box * C::kBoxCols, row, head);
+    if (++next < total) {
       w.next(a);
       head = look_up();
     }
-    if (use >= 1 && !warp_wait(a, bar_empty + 8 * slot, (use + 1) & 1, gave_up, 1, s)) break;
-    if (lane == 0) {
-      *reinterpret_cast<StageInfo*>(smem + C::kOffInfo + slot * sizeof(StageInfo)) = info;
-      tcgen::mbar_expect_tx(bar_full + 8 * slot, 2 * C::kBoxes * 128 * rows * __popc(there));
-    }
-    __syncwarp();
-    if (tensor < 2 && my_head >= 0)
-      tcgen::tma_load_3d(base + (tensor * C::kStages + slot) * C::kTileBytes + (box * SR + piece * rows) * 128,
-                         tensor == 0 ? map_k : map_v, bar_full + 8 * slot, box * C::kBoxCols, row, my_head);
   }
-}
+  // Waits for stage s; false: the warp gives up.
+  __device__ inline bool wait(int s) {
+    return __all_sync(0xffffffffu, tcgen::mbar_wait(full + 8 * (s % C::kStages), (s / C::kStages) & 1, gave_up, a.status, 3, s,
+                                                    a.wait_ns)) != 0;
+  }
+};
 
-// What every block does around its walk. `compute(warp, total, base, smem, gave_up)` runs in the warps that compute.
+// What a block does around its warps' walks; compute(ring, warp) is a warp's.
 template <typename C, typename Compute>
 __device__ inline void paged_block(const PagedArgs& a, const CUtensorMap* map_k, const CUtensorMap* map_v, unsigned char* smem,
                                    Compute compute) {
   const unsigned base = tcgen::smem_u32(smem);
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   volatile int* const gave_up = reinterpret_cast<volatile int*>(smem + C::kOffFlag);
-  const unsigned bars = base + C::kOffBar;
   let_next_start();
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
-      tcgen::mbar_init(bars + 8 * s, 1);                          // full
-      tcgen::mbar_init(bars + 8 * (C::kStages + s), C::kWarps);   // empty
-    }
-    tcgen::mbar_init(bars + 16 * C::kStages, C::kWarps);          // a meeting of the warps that compute
+    for (int s = 0; s < C::kWarps * C::kStages; ++s) tcgen::mbar_init(base + C::kOffBar + 8 * s, 1);
     *gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     tcgen::prefetch_map(map_k);
@@ -357,42 +347,26 @@ __device__ inline void paged_block(const PagedArgs& a, const CUtensorMap* map_k,
   // Behind the kernel of the shared pages, whose blocks let this one begin when all that came before them has completed,
   // nothing waits for that kernel itself but the end: the fold, which waits for this grid, then finds both kernels' parts.
   if (a.shared_ml == nullptr) wait_for_previous();
-  Walk<C::SR> w;
-  int per = 1;
-  int total = find_share<C::SR, C::kThreads>(a, &w, &per, reinterpret_cast<ScanRoom<C::kThreads>*>(smem + C::kOffRoom));
+  Ring<C> ring{a, map_k, map_v, base + warp * C::kRingBytes, base + C::kOffBar + warp * C::kStages * 8,
+               reinterpret_cast<StageInfo*>(smem + C::kOffInfo) + warp * C::kStages, gave_up};
+  ring.total = find_share<C::SR, C::kWarps>(a, warp, &ring.w, &ring.per, reinterpret_cast<ScanRoom<C::kWarps>*>(smem + C::kOffRoom));
   // (behind a launch that gave up nothing is computed; the fold writes nothing then either)
-  if (*reinterpret_cast<volatile int*>(a.status) != 0) total = 0;
-  total = __syncthreads_or(total == 0) ? 0 : total;
-  if (total > 0) {
-    if (warp == C::kWarps) copy_stages<C>(a, map_k, map_v, w, total, per, smem, base, gave_up);
-    else compute(warp, total, base, gave_up);
-    __syncthreads();
-    if (*gave_up) {  // give copies in flight time to land
-      const unsigned long long t0 = tcgen::global_ns();
-      while (tcgen::global_ns() - t0 < 1000000ull) __nanosleep(1000);
-    }
+  if (ring.total > 0 && __shfl_sync(0xffffffffu, *reinterpret_cast<volatile int*>(a.status), 0) == 0) {
+    ring.begin();
+    compute(ring, warp);
+  }
+  __syncthreads();
+  if (*gave_up) {  // give copies in flight time to land
+    const unsigned long long t0 = tcgen::global_ns();
+    while (tcgen::global_ns() - t0 < 1000000ull) __nanosleep(1000);
   }
   if (a.shared_ml != nullptr) wait_for_previous();
 }
 
-// A meeting of the warps that compute; false when some warp gave up.
-template <typename C>
-struct Meeting {
-  unsigned bar;
-  unsigned phase = 0;
-  __device__ inline bool meet(const PagedArgs& a, volatile int* gave_up, int at) {
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) tcgen::mbar_arrive(bar);
-    const bool ok = warp_wait(a, bar, phase, gave_up, 2, at);
-    phase ^= 1;
-    return ok;
-  }
-};
-
 // ---- 16-bit caches ------------------------------------------------------------------
 
 template <typename T, int D>
-using MmaBlock = PagedBlock<T, D, D == 256 ? 2 : 4, D == 256 ? 32 : 64, 16, 0>;
+using MmaBlock = PagedBlock<T, D, D <= 64 ? 32 : 16, 16, 0>;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(MmaBlock<T, D>::kThreads, 2)
@@ -401,18 +375,13 @@ __global__ void __launch_bounds__(MmaBlock<T, D>::kThreads, 2)
   using C = MmaBlock<T, D>;
   constexpr int SR = C::SR, RU = C::RU;
   extern __shared__ __align__(1024) unsigned char smem[];
-  paged_block<C>(a, &map_k, &map_v, smem, [&](int warp, int total, unsigned base, volatile int* gave_up) {
-    float* const merge = reinterpret_cast<float*>(smem + C::kOffMerge);
-    float* const red_m = reinterpret_cast<float*>(smem + C::kOffMl);  // [warps + 1][16]
-    float* const red_l = red_m + (C::kWarps + 1) * 16;
-    const unsigned bar_full = base + C::kOffBar, bar_empty = bar_full + 8 * C::kStages;
-    Meeting<C> all{bar_empty + 8 * C::kStages};
+  paged_block<C>(a, &map_k, &map_v, smem, [&](Ring<C>& ring, int warp) {
     const int lane = threadIdx.x & 31;
     const int g = lane >> 2, tq = lane & 3;  // fragment row (and row + 8), column pair
-    const int mi = lane >> 3, r8 = lane & 7, key0 = warp * 16;
+    const int mi = lane >> 3, r8 = lane & 7;
     // a lane's rows of the ldmatrix tiles, and the swizzled offsets of its pieces c = 2 i + (0 or 1) of a box
-    const unsigned k_row = base + static_cast<unsigned>(key0 + (mi >> 1) * 8 + r8) * 128;
-    const unsigned v_row = base + static_cast<unsigned>(C::kStages * C::kTileBytes + (key0 + (mi & 1) * 8 + r8) * 128);
+    const unsigned k_row = ring.tiles + static_cast<unsigned>((mi >> 1) * 8 + r8) * 128;
+    const unsigned v_row = ring.tiles + static_cast<unsigned>(C::kTileBytes + ((mi & 1) * 8 + r8) * 128);
     unsigned k_off[4], v_off[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -422,10 +391,11 @@ __global__ void __launch_bounds__(MmaBlock<T, D>::kThreads, 2)
     unsigned qa[D / 16][4];
     float o[D / 8][4];
     float m_run[2], l_run[2];
+    const int total = ring.total;
     for (int s = 0; s < total; ++s) {
       const int slot = s % C::kStages;
-      if (!warp_wait(a, bar_full + 8 * slot, (s / C::kStages) & 1, gave_up, 3, s)) return;
-      const StageInfo u = *reinterpret_cast<const StageInfo*>(smem + C::kOffInfo + slot * sizeof(StageInfo));
+      if (!ring.wait(s)) return;
+      const StageInfo u = ring.info[slot];
       if (u.first) {
         // Q as A fragments: reg0 (row g, k 2tq..), reg1 (row g+8, same k), reg2 / reg3 the same at k+8
         int b0, h0, b1, h1;
@@ -444,15 +414,20 @@ __global__ void __launch_bounds__(MmaBlock<T, D>::kThreads, 2)
         m_run[0] = m_run[1] = -INFINITY;
         l_run[0] = l_run[1] = 0.f;  // this lane's share of the row sums
       }
-      const int n_valid = u.keys - key0;  // keys of this warp
-      if (n_valid > 0 && (u.pages >> warp & 1u)) {
-        const unsigned kt = k_row + slot * C::kTileBytes, vt = v_row + slot * C::kTileBytes;
+#pragma unroll 1
+      for (int key0 = 0; key0 < SR; key0 += 16) {
+        const int n_valid = u.keys - key0;  // keys from here on
+        if (n_valid <= 0) break;
+        if (!(u.pages >> (key0 / 16) & 1u)) continue;
+        const unsigned kt = k_row + 2 * slot * C::kTileBytes + key0 * 128, vt = v_row + 2 * slot * C::kTileBytes + key0 * 128;
         if (n_valid < 16) {
           // what a page holds behind the sequence's end has weight 0, but may be anything: out of V's rows with it
-          unsigned char* const v_tile = smem + (C::kStages + slot) * C::kTileBytes;
+          const unsigned v_tile = ring.tiles + (2 * slot + 1) * C::kTileBytes;
           for (int i = lane; i < (16 - n_valid) * C::kBoxes * 8; i += 32)
-            *reinterpret_cast<uint4*>(v_tile + (i / 8 % C::kBoxes * SR + key0 + n_valid + i / 8 / C::kBoxes) * 128 + i % 8 * 16) =
-                make_uint4(0u, 0u, 0u, 0u);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                             v_tile + (i / 8 % C::kBoxes * SR + key0 + n_valid + i / 8 / C::kBoxes) * 128 + i % 8 * 16),
+                         "r"(0)
+                         : "memory");
           __syncwarp();
         }
         // S = Q K^T for 16 keys: s0 = keys 0..7, s1 = keys 8..15
@@ -518,58 +493,32 @@ __global__ void __launch_bounds__(MmaBlock<T, D>::kThreads, 2)
         if (n_valid < 16) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next copy lands behind those zeros
       }
       __syncwarp();
-      if (lane == 0) tcgen::mbar_arrive(bar_empty + 8 * slot);
+      ring.copy(slot);
       if (u.last) {
-        // the lanes of a row, then the warps one after the other
+        const size_t part = (static_cast<size_t>(blockIdx.x) * C::kWarps + warp + u.uid) * a.rs;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 1);
-          l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 2);
-        }
-        if (tq == 0) {
-          red_m[warp * 16 + g] = m_run[0];
-          red_m[warp * 16 + g + 8] = m_run[1];
-          red_l[warp * 16 + g] = l_run[0];
-          red_l[warp * 16 + g + 8] = l_run[1];
-        }
-        if (!all.meet(a, gave_up, s)) return;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float m_all = -INFINITY, l_all = 0.f;
-#pragma unroll
-          for (int w = 0; w < C::kWarps; ++w) m_all = fmaxf(m_all, red_m[w * 16 + g + 8 * i]);
-#pragma unroll
-          for (int w = 0; w < C::kWarps; ++w) {
-            const float mw = red_m[w * 16 + g + 8 * i];
-            l_all += (mw == -INFINITY ? 1.f : ex2(mw - m_all)) * red_l[w * 16 + g + 8 * i];
-          }
-          const float f = m_run[i] == -INFINITY ? 1.f : ex2(m_run[i] - m_all);
-#pragma unroll
-          for (int n = 0; n < D / 8; ++n) {
-            o[n][2 * i] *= f;
-            o[n][2 * i + 1] *= f;
-          }
-          if (warp == 0 && tq == 0) {
-            red_m[C::kWarps * 16 + g + 8 * i] = m_all;
-            red_l[C::kWarps * 16 + g + 8 * i] = l_all;
-          }
-        }
-#pragma unroll 1
-        for (int w = 0; w < C::kWarps; ++w) {
-          if (warp == w) {
+          float l = l_run[i];
+          l += __shfl_xor_sync(0xffffffffu, l, 1);
+          l += __shfl_xor_sync(0xffffffffu, l, 2);
+          const int r = g + 8 * i;
+          int b, h;
+          if (!unit_row<RU>(a, u, r, &b, &h)) continue;
+          if (u.last == 2) {
+            const size_t row = static_cast<size_t>(b) * a.H + h;
+            const float inv = l == 0.f ? 0.f : 1.f / l;  // (no key seen: O is 0 as well)
+            T* const dst = static_cast<T*>(a.out) + row * D + 2 * tq;
 #pragma unroll
             for (int n = 0; n < D / 8; ++n)
+              *reinterpret_cast<unsigned*>(dst + n * 8) = pack_pair<T>(o[n][2 * i] * inv, o[n][2 * i + 1] * inv);
+            if (a.lse && tq == 0) a.lse[row] = l > 0.f ? m_run[i] * kLn2 + logf(l) : l == 0.f ? -INFINITY : l;
+          } else {
+            float* const dst = a.part_o + (part + r) * D + 2 * tq;
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                float2* const x = reinterpret_cast<float2*>(merge + (g + 8 * i) * D + n * 8 + 2 * tq);
-                const float2 y = w == 0 ? make_float2(0.f, 0.f) : *x;
-                *x = make_float2(y.x + o[n][2 * i], y.y + o[n][2 * i + 1]);
-              }
+            for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+            if (tq == 0) a.part_ml[part + r] = make_float2(m_run[i], l);
           }
-          if (!all.meet(a, gave_up, s)) return;
         }
-        put_unit<T, D, RU>(a, u, red_m + C::kWarps * 16, red_l + C::kWarps * 16, merge, C::kWarps * 32);
-        if (!all.meet(a, gave_up, s)) return;
       }
     }
   });
@@ -578,7 +527,7 @@ __global__ void __launch_bounds__(MmaBlock<T, D>::kThreads, 2)
 // ---- fp32 caches --------------------------------------------------------------------
 
 template <int D, int kRows>
-using F32Block = PagedBlock<float, D, 4, D == 256 ? 16 : 32, kRows, kRows * D * 4>;
+using F32Block = PagedBlock<float, D, D == 32 ? 32 : D == 64 ? 16 : 8, kRows, kRows * D * 4>;
 
 template <int D, int kRows>
 __global__ void __launch_bounds__(F32Block<D, kRows>::kThreads, 2)
@@ -586,35 +535,31 @@ __global__ void __launch_bounds__(F32Block<D, kRows>::kThreads, 2)
                      const __grid_constant__ PagedArgs a) {
   using C = F32Block<D, kRows>;
   constexpr int SR = C::SR, RU = C::RU, kVec = D / 4;
-  constexpr int kKeys = SR / 4;                       // of a warp and stage
-  constexpr int kParts = 32 / kKeys;                  // lanes that share out a key's row
-  constexpr int kCols = kVec < 32 ? kVec : 32;        // lanes side by side on a row of V
+  constexpr int kKeys = 8, kParts = 4;                   // keys at a time, lanes that share out a key's row
+  constexpr int kCols = kVec < 32 ? kVec : 32;           // lanes side by side on a row of V
   constexpr int kAt = 32 / kCols, kEach = kVec / kCols;  // rows of V at a time, 16-byte pieces of one a lane
   extern __shared__ __align__(1024) unsigned char smem[];
-  paged_block<C>(a, &map_k, &map_v, smem, [&](int warp, int total, unsigned base, volatile int* gave_up) {
-    float* const merge = reinterpret_cast<float*>(smem + C::kOffMerge);
-    const float4* const q_s = reinterpret_cast<const float4*>(smem + C::kOffExtra);  // [row][D / 4]
-    float* const red_m = reinterpret_cast<float*>(smem + C::kOffMl);                 // [warps + 1][RU]
-    float* const red_l = red_m + (C::kWarps + 1) * RU;
-    const unsigned bar_full = base + C::kOffBar, bar_empty = bar_full + 8 * C::kStages;
-    Meeting<C> all{bar_empty + 8 * C::kStages};
+  paged_block<C>(a, &map_k, &map_v, smem, [&](Ring<C>& ring, int warp) {
+    float4* const q_s = reinterpret_cast<float4*>(smem + C::kOffQuery) + warp * (RU * kVec);  // [row][D / 4]
+    const unsigned char* const tiles = smem + warp * C::kRingBytes;
     const int lane = threadIdx.x & 31;
     const int key = lane / kParts, part = lane % kParts;  // scores
     const int col = lane % kCols, sub = lane / kCols;     // sum over V
-    const int key0 = warp * kKeys;
     float4 o[RU][kEach];
     float m_run[RU], l_run[RU];
+    const int total = ring.total;
     for (int s = 0; s < total; ++s) {
       const int slot = s % C::kStages;
-      if (!warp_wait(a, bar_full + 8 * slot, (s / C::kStages) & 1, gave_up, 3, s)) return;
-      const StageInfo u = *reinterpret_cast<const StageInfo*>(smem + C::kOffInfo + slot * sizeof(StageInfo));
+      if (!ring.wait(s)) return;
+      const StageInfo u = ring.info[slot];
       if (u.first) {
-        for (int i = threadIdx.x; i < RU * kVec; i += C::kWarps * 32) {
+        __syncwarp();
+        for (int i = lane; i < RU * kVec; i += 32) {
           int b, h;
           float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
           if (unit_row<RU>(a, u, i / kVec, &b, &h))
             x = static_cast<const float4*>(a.q)[(static_cast<size_t>(b) * a.H + h) * kVec + i % kVec];
-          reinterpret_cast<float4*>(smem + C::kOffExtra)[i] = x;
+          q_s[i] = x;
         }
 #pragma unroll
         for (int r = 0; r < RU; ++r) {
@@ -623,37 +568,37 @@ __global__ void __launch_bounds__(F32Block<D, kRows>::kThreads, 2)
 #pragma unroll
           for (int i = 0; i < kEach; ++i) o[r][i] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        if (!all.meet(a, gave_up, s)) return;
+        __syncwarp();
       }
-      const int n_valid = u.keys - key0;
-      if (n_valid > 0 && (u.pages >> (key0 / 16) & 1u)) {
-        const unsigned char* const kt = smem + slot * C::kTileBytes + (key0 + key) * 128;
-        const unsigned char* const vt = smem + (C::kStages + slot) * C::kTileBytes + key0 * 128;
+#pragma unroll 1
+      for (int key0 = 0; key0 < SR; key0 += kKeys) {
+        const int n_valid = u.keys - key0;
+        if (n_valid <= 0) break;
+        if (!(u.pages >> (key0 / 16) & 1u)) continue;
+        const unsigned char* const kt = tiles + 2 * slot * C::kTileBytes + (key0 + key) * 128;
+        const unsigned char* const vt = tiles + (2 * slot + 1) * C::kTileBytes + key0 * 128;
         float sc[RU];
 #pragma unroll
         for (int r = 0; r < RU; ++r) sc[r] = 0.f;
-        // A lane's pieces: every other one of a box, so that the two keys of eight neighbouring lanes, a bank apart by their
-        // swizzle, do not meet; with eight lanes to a key they are neighbours.
+        // A lane's pieces: every other one of a box, so that the two keys of eight neighbouring lanes, whose pieces the
+        // swizzle exchanges, do not meet in a bank.
 #pragma unroll 4
         for (int j = 0; j < kVec / kParts; ++j) {
-          const int c = kParts == 4 ? (j >> 1) * 8 + 2 * part + (j & 1) : j * kParts + part;
-          const float4 x = *reinterpret_cast<const float4*>(kt + c / 8 * (SR * 128) + ((c % 8) ^ ((key0 + key) & 7)) * 16);
+          const int c = (j >> 1) * 8 + 2 * part + (j & 1);
+          const float4 x = *reinterpret_cast<const float4*>(kt + c / 8 * (SR * 128) + ((c % 8) ^ key) * 16);
 #pragma unroll
           for (int r = 0; r < RU; ++r) {
             const float4 y = q_s[r * kVec + c];
             sc[r] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, sc[r]))));
           }
         }
+        float mx[RU];
+        bool moved = false;
 #pragma unroll
         for (int r = 0; r < RU; ++r) {
 #pragma unroll
           for (int i = 1; i < kParts; i *= 2) sc[r] += __shfl_xor_sync(0xffffffffu, sc[r], i);
           sc[r] = key < n_valid ? sc[r] * a.scale_log2 : -INFINITY;
-        }
-        float mx[RU];
-        bool moved = false;
-#pragma unroll
-        for (int r = 0; r < RU; ++r) {
           mx[r] = sc[r];
 #pragma unroll
           for (int i = kParts; i < 32; i *= 2) mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], i));
@@ -685,7 +630,7 @@ __global__ void __launch_bounds__(F32Block<D, kRows>::kThreads, 2)
 #pragma unroll
             for (int e = 0; e < kEach; ++e) {
               const int c = e * kCols + col;
-              const float4 x = *reinterpret_cast<const float4*>(vt + (c / 8 * SR + row) * 128 + ((c % 8) ^ ((key0 + row) & 7)) * 16);
+              const float4 x = *reinterpret_cast<const float4*>(vt + (c / 8 * SR + row) * 128 + ((c % 8) ^ row) * 16);
 #pragma unroll
               for (int r = 0; r < RU; ++r) {
                 o[r][e].x = fmaf(p[r], x.x, o[r][e].x);
@@ -698,13 +643,14 @@ __global__ void __launch_bounds__(F32Block<D, kRows>::kThreads, 2)
         }
       }
       __syncwarp();
-      if (lane == 0) tcgen::mbar_arrive(bar_empty + 8 * slot);
+      ring.copy(slot);
       if (u.last) {
-        // the lanes of a row, then the warps one after the other
+        const size_t at = (static_cast<size_t>(blockIdx.x) * C::kWarps + warp + u.uid) * a.rs;
 #pragma unroll
         for (int r = 0; r < RU; ++r) {
+          float l = l_run[r];
 #pragma unroll
-          for (int i = kParts; i < 32; i *= 2) l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], i);
+          for (int i = kParts; i < 32; i *= 2) l += __shfl_xor_sync(0xffffffffu, l, i);
 #pragma unroll
           for (int e = 0; e < kEach; ++e)
 #pragma unroll
@@ -714,46 +660,18 @@ __global__ void __launch_bounds__(F32Block<D, kRows>::kThreads, 2)
               o[r][e].z += __shfl_xor_sync(0xffffffffu, o[r][e].z, i);
               o[r][e].w += __shfl_xor_sync(0xffffffffu, o[r][e].w, i);
             }
-          if (lane == 0) {
-            red_m[warp * RU + r] = m_run[r];
-            red_l[warp * RU + r] = l_run[r];
-          }
+          int b, h;
+          if (!unit_row<RU>(a, u, r, &b, &h) || sub != 0) continue;
+          const bool result = u.last == 2;
+          const size_t row = static_cast<size_t>(b) * a.H + h;
+          const float f = !result ? 1.f : l == 0.f ? 0.f : 1.f / l;  // (no key seen: O is 0 as well)
+          float4* const dst = reinterpret_cast<float4*>(result ? static_cast<float*>(a.out) + row * D : a.part_o + (at + r) * D);
+#pragma unroll
+          for (int e = 0; e < kEach; ++e)
+            dst[e * kCols + col] = make_float4(o[r][e].x * f, o[r][e].y * f, o[r][e].z * f, o[r][e].w * f);
+          if (lane == 0 && !result) a.part_ml[at + r] = make_float2(m_run[r], l);
+          if (lane == 0 && result && a.lse) a.lse[row] = l > 0.f ? m_run[r] * kLn2 + logf(l) : l == 0.f ? -INFINITY : l;
         }
-        if (!all.meet(a, gave_up, s)) return;
-#pragma unroll
-        for (int r = 0; r < RU; ++r) {
-          float m_all = -INFINITY, l_all = 0.f;
-#pragma unroll
-          for (int w = 0; w < C::kWarps; ++w) m_all = fmaxf(m_all, red_m[w * RU + r]);
-#pragma unroll
-          for (int w = 0; w < C::kWarps; ++w) {
-            const float mw = red_m[w * RU + r];
-            l_all += (mw == -INFINITY ? 1.f : ex2(mw - m_all)) * red_l[w * RU + r];
-          }
-          const float f = m_run[r] == -INFINITY ? 1.f : ex2(m_run[r] - m_all);
-#pragma unroll
-          for (int e = 0; e < kEach; ++e) o[r][e] = make_float4(o[r][e].x * f, o[r][e].y * f, o[r][e].z * f, o[r][e].w * f);
-          if (threadIdx.x == 0) {
-            red_m[C::kWarps * RU + r] = m_all;
-            red_l[C::kWarps * RU + r] = l_all;
-          }
-        }
-#pragma unroll 1
-        for (int w = 0; w < C::kWarps; ++w) {
-          if (warp == w && sub == 0) {
-#pragma unroll
-            for (int r = 0; r < RU; ++r)
-#pragma unroll
-              for (int e = 0; e < kEach; ++e) {
-                float4* const x = reinterpret_cast<float4*>(merge) + r * kVec + e * kCols + col;
-                const float4 y = w == 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *x;
-                *x = make_float4(y.x + o[r][e].x, y.y + o[r][e].y, y.z + o[r][e].z, y.w + o[r][e].w);
-              }
-          }
-          if (!all.meet(a, gave_up, s)) return;
-        }
-        put_unit<float, D, RU>(a, u, red_m + C::kWarps * RU, red_l + C::kWarps * RU, merge, C::kWarps * 32);
-        if (!all.meet(a, gave_up, s)) return;
       }
     }
   });
@@ -761,10 +679,9 @@ __global__ void __launch_bounds__(F32Block<D, kRows>::kThreads, 2)
 
 // ---- fold ---------------------------------------------------------------------------
 
-// Parts of the rows that no block finished, and rows without keys. A row has D / 4 threads, four columns each, times kSlices, which
+// Parts of the rows that no warp finished, and rows without keys. A row has D / 4 threads, four columns each, times kSlices, which
 // take every kSlices-th part; a thread asks for eight parts at a time.
-constexpr int kFoldThreads = 256;
-template <typename T, int D, int RU, int kSlices>
+template <typename T, int D, int RU, int kFoldThreads, int kSlices>
 __global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const __grid_constant__ PagedArgs a) {
   constexpr int kVec = D / 4, kRowsPer = kFoldThreads / kVec / kSlices, kBatch = 8;
   __shared__ float4 acc_of[kSlices > 1 ? kFoldThreads : 1];
@@ -802,7 +719,7 @@ __global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const __grid_c
       pre_n = pre.y;
     }
   }
-  const bool done = lost || (own_n == 1 && start == 0);  // by the block that had the unit
+  const bool done = lost || (own_n == 1 && start == 0);  // by the warp that had the unit
   const int parts = mine && !done ? own_n + pre_n : 0;
   float m_all = -INFINITY, l_all = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -877,10 +794,10 @@ constexpr int kBlocksPerSm = 2;  // of both kernels
 
 int fp32_rows(int G) { return G <= 1 ? 1 : G <= 2 ? 2 : G <= 4 ? 4 : 8; }
 
-// How a call runs, and its room: which blocks have parts of a unit, and (m, l) and O of every part. A block leaves at most one
-// part of a unit, and block c's of unit u is part c + u: both only grow along the list, so no two meet.
+// How a call runs, and its room: which shares have parts of a unit, and (m, l) and O of every part. A share leaves at most one
+// part of a unit, and share c's of unit u is part c + u: both only grow along the list, so no two meet.
 struct PagedPlan {
-  int RU, SR, HB, RB, blocks;
+  int RU, SR, HB, RB, warps, blocks;  // (warps of a block)
   int rs;       // rows of a part
   double most;  // stages that there can be
   bool tc;      // shared pages by the tensor-core kernel
@@ -894,7 +811,8 @@ PagedPlan make_plan(const ra_paged_kv& c, int heads, int shared_len) {
   const bool f32 = c.dtype == RA_F32;
   const long long rows_shared = shared_len > 0 ? static_cast<long long>(c.batch) * G : 0;
   p.RU = f32 ? fp32_rows(static_cast<int>(std::max<long long>(std::min<long long>(rows_shared, 8), G))) : 16;
-  p.SR = f32 ? (c.head_dim == 256 ? 16 : 32) : c.head_dim == 256 ? 32 : 64;
+  p.SR = f32 ? (c.head_dim == 32 ? 32 : c.head_dim == 64 ? 16 : 8) : c.head_dim <= 64 ? 32 : 16;
+  p.warps = c.head_dim == 256 ? 2 : 4;
   p.tc = !f32 && rows_shared > 0 && plan_shared_prefix(c.batch, heads, c.kv_heads, c.head_dim, shared_len, &p.shared);
   p.HB = (G + p.RU - 1) / p.RU;
   p.RB = p.tc ? 0 : static_cast<int>((rows_shared + p.RU - 1) / p.RU);
@@ -904,10 +822,10 @@ PagedPlan make_plan(const ra_paged_kv& c, int heads, int shared_len) {
   p.most = static_cast<double>(c.kv_heads) * (static_cast<double>(c.batch) * p.HB * ((room + p.SR - 1) / p.SR) +
                                               static_cast<double>(p.RB) * ((shared_len + p.SR - 1) / p.SR));
   const int wave = kBlocksPerSm * sm_count();
-  p.blocks = p.most < wave ? static_cast<int>(p.most) : wave;
+  p.blocks = p.most < static_cast<double>(wave) * p.warps ? (static_cast<int>(p.most) + p.warps - 1) / p.warps : wave;
   p.rs = p.RB > 0 ? p.RU : std::min(p.RU, G);
   auto whole = [](size_t n) { return (n + 127) & ~static_cast<size_t>(127); };
-  const size_t rows = (units + p.blocks) * p.rs, shared_rows = p.tc ? shared_part_rows(p.shared, c.kv_heads) : 0;
+  const size_t rows = (units + static_cast<size_t>(p.blocks) * p.warps) * p.rs, shared_rows = p.tc ? shared_part_rows(p.shared, c.kv_heads) : 0;
   p.unit_bytes = whole(units * sizeof(int2));
   p.ml_bytes = whole(rows * sizeof(float2));
   p.o_bytes = whole(rows * c.head_dim * sizeof(float));
@@ -929,19 +847,21 @@ int launch_main(const CUtensorMap& k, const CUtensorMap& v, int blocks, const Pa
   return RA_OK;
 }
 
+// Threads of the fold that share out a row's parts: all of a large block where there is a row an SM and less, since the shares
+// of a whole wave may then belong to one row; eight where there are a few; one elsewhere.
 template <typename T, int D, int RU>
 int launch_fold(const PagedArgs& a, cudaStream_t stream) {
-  const long long rows = static_cast<long long>(a.B) * a.H;
-  constexpr int kPer = kFoldThreads / (D / 4), kMany = kPer < 8 ? kPer : 8;
-  // few rows: their parts are shared out, since the blocks of a wave may all have parts of the same row
-  if (rows <= static_cast<long long>(sm_count()) * kPer) {
-    RAB_CUDA(launch_overlapped(paged_fold_kernel<T, D, RU, kMany>, dim3(static_cast<unsigned>((rows * kMany + kPer - 1) / kPer)),
-                               dim3(kFoldThreads), 0, stream, a));
-  } else {
-    RAB_CUDA(launch_overlapped(paged_fold_kernel<T, D, RU, 1>, dim3(static_cast<unsigned>((rows + kPer - 1) / kPer)),
-                               dim3(kFoldThreads), 0, stream, a));
-  }
-  return RA_OK;
+  const long long rows = static_cast<long long>(a.B) * a.H, sms = sm_count();
+  auto go = [&](auto threads, auto slices) -> int {
+    constexpr int kThreads = decltype(threads)::value, kSlices = decltype(slices)::value, kPer = kThreads / (D / 4) / kSlices;
+    RAB_CUDA(launch_overlapped(paged_fold_kernel<T, D, RU, kThreads, kSlices>, dim3(static_cast<unsigned>((rows + kPer - 1) / kPer)),
+                               dim3(kThreads), 0, stream, a));
+    return RA_OK;
+  };
+  constexpr int kSome = 256 / (D / 4) < 8 ? 256 / (D / 4) : 8, kAll = 1024 / (D / 4) < 32 ? 1024 / (D / 4) : 32;
+  if (rows <= sms) return go(std::integral_constant<int, 32 * (D / 4) < 1024 ? 32 * (D / 4) : 1024>(), std::integral_constant<int, kAll>());
+  if (rows <= 8 * sms) return go(std::integral_constant<int, 256>(), std::integral_constant<int, kSome>());
+  return go(std::integral_constant<int, 256>(), std::integral_constant<int, 1>());
 }
 
 template <typename T, int D, int RU>
@@ -1018,7 +938,7 @@ int ra_paged_decode(const ra_paged_kv* cache, const void* q, int heads, const in
   const ra_paged_kv c = without_pages(*cache, &shared_len);
   const PagedPlan p = make_plan(c, heads, shared_len);
   // (a share is counted in 32 bits; tables that name a page over and over could ask for more)
-  RAB_REQUIRE(p.most < 2147483648.0 * std::max(p.blocks, 1), RA_ERR_INVALID, "paged_decode: too many keys");
+  RAB_REQUIRE(p.most < 2147483648.0 * std::max(p.blocks * p.warps, 1), RA_ERR_INVALID, "paged_decode: too many keys");
   RAB_REQUIRE(workspace && workspace_bytes >= p.bytes && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, RA_ERR_OVERFLOW,
               "paged_decode: workspace too small or not 16-byte aligned");
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
