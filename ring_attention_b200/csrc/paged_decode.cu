@@ -39,6 +39,8 @@ using tcgen::kLog2e;
 
 struct PagedArgs {
   const void* q;
+  const void* k;
+  const void* v;
   void* out;
   float* lse;  // or NULL
   const int* table;
@@ -237,19 +239,21 @@ __device__ inline void put4<__nv_bfloat16>(__nv_bfloat16* dst, float4 v) {
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack_pair<__nv_bfloat16>(v.x, v.y), pack_pair<__nv_bfloat16>(v.z, v.w));
 }
 
-// Shared memory of a block of either kernel: the rings of its warps, a stage being K's kBoxes boxes of SR rows of 128 bytes and
-// then V's, 16-byte piece c of a row's box at c ^ (row & 7).
-template <typename T, int D, int SR_, int kRows_, int kQueryBytes>
+// Shared memory of a block of either kernel: the rings of its warps, a stage being SR rows of K and then of V. 16 bits: a tensor's
+// kBoxes boxes of 128 bytes of every row, by tensor maps, 16-byte piece c of a row's box at c ^ (row & 7). fp32: whole rows, one
+// after the other as in the page, by plain bulk copies (boxes of 8 rows and 128 bytes kept TMA busy: 16384 rows of D128 67 us).
+template <typename T, int D, int SR_, int kRows_, int kExtraBytes>
 struct PagedBlock {
   static constexpr int SR = SR_, RU = kRows_;
   static constexpr int kWarps = D == 256 ? 2 : 4, kThreads = kWarps * 32;
-  static constexpr int kEs = static_cast<int>(sizeof(T));
-  static constexpr int kBoxes = D * kEs > 128 ? D * kEs / 128 : 1, kBoxCols = 128 / kEs;
-  static constexpr int kTileBytes = SR * kBoxes * 128;  // per tensor
+  static constexpr bool kBulk = sizeof(T) == 4;
+  static constexpr int kBoxes = kBulk || D <= 64 ? 1 : D / 64;
+  static constexpr int kRowBytes = kBulk ? D * 4 : kBoxes * 128;  // in shared memory
+  static constexpr int kTileBytes = SR * kRowBytes;               // per tensor
   static constexpr int kStages = 96 * 1024 / kWarps / (2 * kTileBytes);
   static constexpr int kRingBytes = 2 * kStages * kTileBytes;  // of a warp
-  static constexpr int kOffQuery = kWarps * kRingBytes;        // fp32: every warp's query rows
-  static constexpr int kOffInfo = kOffQuery + kWarps * kQueryBytes;
+  static constexpr int kOffExtra = kWarps * kRingBytes;        // fp32: every warp's weights and factors
+  static constexpr int kOffInfo = kOffExtra + kWarps * kExtraBytes;
   static constexpr int kOffBar = kOffInfo + kWarps * kStages * static_cast<int>(sizeof(StageInfo));
   static constexpr int kOffRoom = kOffBar + kWarps * kStages * 8;
   static constexpr int kOffFlag = kOffRoom + static_cast<int>(sizeof(ScanRoom<kWarps>));
@@ -311,12 +315,19 @@ struct Ring {
       i.first = w.st == first_st;
       i.last = ends && first_st == 0 && w.b >= 0 && w.start == 0 ? 2 : ends || next == total - 1;
       info[slot] = i;
-      tcgen::mbar_expect_tx(full + 8 * slot, 2 * C::kBoxes * 128 * rows() * __popc(there));
+      tcgen::mbar_expect_tx(full + 8 * slot, 2 * C::kRowBytes * rows() * __popc(there));
     }
     __syncwarp();
-    if (tensor < 2 && head >= 0)
+    if constexpr (C::kBulk) {
+      if (tensor < 2 && head >= 0)
+        tcgen::bulk_load(tiles + (2 * slot + tensor) * C::kTileBytes + piece * rows() * C::kRowBytes,
+                         static_cast<const unsigned char*>(tensor == 0 ? a.k : a.v) +
+                             ((static_cast<size_t>(head) << a.shift) + row) * C::kRowBytes,
+                         C::kRowBytes * rows(), full + 8 * slot);
+    } else if (tensor < 2 && head >= 0) {
       tcgen::tma_load_3d(tiles + (2 * slot + tensor) * C::kTileBytes + (box * C::SR + piece * rows()) * 128,
-                         tensor == 0 ? map_k : map_v, full + 8 * slot, box * C::kBoxCols, row, head);
+                         tensor == 0 ? map_k : map_v, full + 8 * slot, box * 64, row, head);
+    }
     if (++next < total) {
       w.next(a);
       head = look_up();
@@ -341,8 +352,10 @@ __device__ inline void paged_block(const PagedArgs& a, const CUtensorMap* map_k,
     for (int s = 0; s < C::kWarps * C::kStages; ++s) tcgen::mbar_init(base + C::kOffBar + 8 * s, 1);
     *gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    tcgen::prefetch_map(map_k);
-    tcgen::prefetch_map(map_v);
+    if constexpr (!C::kBulk) {
+      tcgen::prefetch_map(map_k);
+      tcgen::prefetch_map(map_v);
+    }
   }
   // Behind the kernel of the shared pages, whose blocks let this one begin when all that came before them has completed,
   // nothing waits for that kernel itself but the end: the fold, which waits for this grid, then finds both kernels' parts.
@@ -526,117 +539,156 @@ __global__ void __launch_bounds__(MmaBlock<T, D>::kThreads, 2)
 
 // ---- fp32 caches --------------------------------------------------------------------
 
+// kParts lanes share out a key's row and have their pieces of all query rows in registers. A step's partial sums, of RU rows for
+// 32 / kParts keys, go through one butterfly that halves the rows of a lane at each exchange, so a lane ends with one row's score of
+// one key, and keeps that row's maximum and sum. The weights go through shared memory to the lanes that have the columns of V.
 template <int D, int kRows>
-using F32Block = PagedBlock<float, D, D == 32 ? 32 : D == 64 ? 16 : 8, kRows, kRows * D * 4>;
+struct F32Cfg {
+  static constexpr int kWant = kRows == 1 ? 4 : 2 * kRows;
+  static constexpr int kParts = kWant < D / 4 ? kWant : D / 4;
+  static constexpr int kExtraBytes = (8 * 2 + 2) * kRows * 4;  // weights of 8 keys, each twice, and a factor a row, twice
+  using Block = PagedBlock<float, D, D == 32 ? 32 : D == 64 ? 16 : 8, kRows, (kExtraBytes + 15) & ~15>;
+};
 
 template <int D, int kRows>
-__global__ void __launch_bounds__(F32Block<D, kRows>::kThreads, 2)
-    paged_f32_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                     const __grid_constant__ PagedArgs a) {
-  using C = F32Block<D, kRows>;
+__global__ void __launch_bounds__(F32Cfg<D, kRows>::Block::kThreads, 2) paged_f32_kernel(const __grid_constant__ PagedArgs a) {
+  using C = typename F32Cfg<D, kRows>::Block;
+  using tcgen::ffma2;
   constexpr int SR = C::SR, RU = C::RU, kVec = D / 4;
-  constexpr int kKeys = 8, kParts = 4;                   // keys at a time, lanes that share out a key's row
+  constexpr int kKeys = 8, kParts = F32Cfg<D, kRows>::kParts;
+  constexpr int kAtOnce = 32 / kParts, kSteps = kKeys / kAtOnce, kPieces = kVec / kParts;
   constexpr int kCols = kVec < 32 ? kVec : 32;           // lanes side by side on a row of V
   constexpr int kAt = 32 / kCols, kEach = kVec / kCols;  // rows of V at a time, 16-byte pieces of one a lane
   extern __shared__ __align__(1024) unsigned char smem[];
-  paged_block<C>(a, &map_k, &map_v, smem, [&](Ring<C>& ring, int warp) {
-    float4* const q_s = reinterpret_cast<float4*>(smem + C::kOffQuery) + warp * (RU * kVec);  // [row][D / 4]
+  paged_block<C>(a, nullptr, nullptr, smem, [&](Ring<C>& ring, int warp) {
+    float2* const p_s = reinterpret_cast<float2*>(smem + C::kOffExtra + warp * ((F32Cfg<D, kRows>::kExtraBytes + 15) & ~15));  // [key][row]
+    float2* const f_s = p_s + kKeys * RU;
     const unsigned char* const tiles = smem + warp * C::kRingBytes;
     const int lane = threadIdx.x & 31;
-    const int key = lane / kParts, part = lane % kParts;  // scores
-    const int col = lane % kCols, sub = lane / kCols;     // sum over V
-    float4 o[RU][kEach];
-    float m_run[RU], l_run[RU];
+    const int part = lane % kParts, key_at = lane / kParts;  // scores
+    const int col = lane % kCols, sub = lane / kCols;        // sum over V
+    // the row whose scores the butterfly leaves here
+    int my_row = 0;
+#pragma unroll
+    for (int d = 1, n = RU; d < kParts; d *= 2)
+      if (n > 1) {
+        n /= 2;
+        if (lane & d) my_row += n;
+      }
+    // Pieces of a lane: every kParts-th. With four lanes to a key, eight neighbouring lanes have two keys, whose rows begin in the same
+    // bank, so those of odd keys take the other half of each group of eight pieces first.
+    auto piece = [&](int j) { return (j * kParts + part) ^ (kParts == 4 ? (key_at & 1) * 4 : 0); };
+    float4 q[RU][kPieces];
+    float2 o[RU][kEach][2];
+    float m_run = -INFINITY, l_run = 0.f;
     const int total = ring.total;
     for (int s = 0; s < total; ++s) {
       const int slot = s % C::kStages;
       if (!ring.wait(s)) return;
       const StageInfo u = ring.info[slot];
       if (u.first) {
-        __syncwarp();
-        for (int i = lane; i < RU * kVec; i += 32) {
-          int b, h;
-          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (unit_row<RU>(a, u, i / kVec, &b, &h))
-            x = static_cast<const float4*>(a.q)[(static_cast<size_t>(b) * a.H + h) * kVec + i % kVec];
-          q_s[i] = x;
-        }
 #pragma unroll
         for (int r = 0; r < RU; ++r) {
-          m_run[r] = -INFINITY;
-          l_run[r] = 0.f;
+          int b, h;
+          const bool is = unit_row<RU>(a, u, r, &b, &h);
+          const float4* const src = static_cast<const float4*>(a.q) + (is ? static_cast<size_t>(b) * a.H + h : 0) * kVec;
 #pragma unroll
-          for (int i = 0; i < kEach; ++i) o[r][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int j = 0; j < kPieces; ++j) q[r][j] = is ? src[piece(j)] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) o[r][e][0] = o[r][e][1] = make_float2(0.f, 0.f);
         }
-        __syncwarp();
+        m_run = -INFINITY;
+        l_run = 0.f;
       }
 #pragma unroll 1
       for (int key0 = 0; key0 < SR; key0 += kKeys) {
         const int n_valid = u.keys - key0;
         if (n_valid <= 0) break;
         if (!(u.pages >> (key0 / 16) & 1u)) continue;
-        const unsigned char* const kt = tiles + 2 * slot * C::kTileBytes + (key0 + key) * 128;
-        const unsigned char* const vt = tiles + (2 * slot + 1) * C::kTileBytes + key0 * 128;
-        float sc[RU];
+        const unsigned char* const kt = tiles + 2 * slot * C::kTileBytes + key0 * C::kRowBytes;
+        const unsigned char* const vt = tiles + (2 * slot + 1) * C::kTileBytes + key0 * C::kRowBytes;
+        float sc[kSteps];
 #pragma unroll
-        for (int r = 0; r < RU; ++r) sc[r] = 0.f;
-        // A lane's pieces: every other one of a box, so that the two keys of eight neighbouring lanes, whose pieces the
-        // swizzle exchanges, do not meet in a bank.
-#pragma unroll 4
-        for (int j = 0; j < kVec / kParts; ++j) {
-          const int c = (j >> 1) * 8 + 2 * part + (j & 1);
-          const float4 x = *reinterpret_cast<const float4*>(kt + c / 8 * (SR * 128) + ((c % 8) ^ key) * 16);
+        for (int st = 0; st < kSteps; ++st) {
+          const float4* const row = reinterpret_cast<const float4*>(kt + (st * kAtOnce + key_at) * C::kRowBytes);
+          float2 acc[RU];
+#pragma unroll
+          for (int r = 0; r < RU; ++r) acc[r] = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int j = 0; j < kPieces; ++j) {
+            const float4 x = row[piece(j)];
+#pragma unroll
+            for (int r = 0; r < RU; ++r) {
+              acc[r] = ffma2(make_float2(x.x, x.y), make_float2(q[r][j].x, q[r][j].y), acc[r]);
+              acc[r] = ffma2(make_float2(x.z, x.w), make_float2(q[r][j].z, q[r][j].w), acc[r]);
+            }
+          }
+          float v[RU];
+#pragma unroll
+          for (int r = 0; r < RU; ++r) v[r] = acc[r].x + acc[r].y;
+#pragma unroll
+          for (int d = 1, n = RU; d < kParts; d *= 2) {
+            if (n > 1) {
+              n /= 2;
+              const bool upper = (lane & d) != 0;
+#pragma unroll
+              for (int r = 0; r < RU / 2; ++r) {
+                if (r >= n) break;
+                const float keep = upper ? v[r + n] : v[r], give = upper ? v[r] : v[r + n];
+                v[r] = keep + __shfl_xor_sync(0xffffffffu, give, d);
+              }
+            } else {
+              v[0] += __shfl_xor_sync(0xffffffffu, v[0], d);
+            }
+          }
+          sc[st] = st * kAtOnce + key_at < n_valid ? v[0] * a.scale_log2 : -INFINITY;
+        }
+        // this lane's row: maximum over the stage's keys
+        float mx = sc[0];
+#pragma unroll
+        for (int st = 1; st < kSteps; ++st) mx = fmaxf(mx, sc[st]);
+#pragma unroll
+        for (int d = kParts; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+        if (__any_sync(0xffffffffu, mx > m_run)) {
+          const float mn = fmaxf(m_run, mx);
+          const float f = m_run == -INFINITY ? 0.f : ex2(m_run - mn);
+          l_run = m_run == -INFINITY ? l_run : l_run * f;  // (0, or NaN to keep)
+          m_run = mn;
+          __syncwarp();
+          if (key_at == 0) f_s[my_row] = make_float2(f, f);
+          __syncwarp();
 #pragma unroll
           for (int r = 0; r < RU; ++r) {
-            const float4 y = q_s[r * kVec + c];
-            sc[r] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, sc[r]))));
+            const float2 g = f_s[r];
+#pragma unroll
+            for (int e = 0; e < kEach; ++e)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) o[r][e][i] = make_float2(o[r][e][i].x * g.x, o[r][e][i].y * g.x);
           }
         }
-        float mx[RU];
-        bool moved = false;
+        const float ms = m_run == -INFINITY ? 0.f : m_run;
+        __syncwarp();  // the weights of the keys before have been read
 #pragma unroll
-        for (int r = 0; r < RU; ++r) {
-#pragma unroll
-          for (int i = 1; i < kParts; i *= 2) sc[r] += __shfl_xor_sync(0xffffffffu, sc[r], i);
-          sc[r] = key < n_valid ? sc[r] * a.scale_log2 : -INFINITY;
-          mx[r] = sc[r];
-#pragma unroll
-          for (int i = kParts; i < 32; i *= 2) mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], i));
-          moved = moved || mx[r] > m_run[r];
+        for (int st = 0; st < kSteps; ++st) {
+          const float p = ex2(sc[st] - ms);
+          l_run += p;
+          p_s[(st * kAtOnce + key_at) * RU + my_row] = make_float2(p, p);
         }
-        if (moved) {  // (the same in all lanes)
-#pragma unroll
-          for (int r = 0; r < RU; ++r) {
-            const float mn = fmaxf(m_run[r], mx[r]);
-            const float f = m_run[r] == -INFINITY ? 0.f : ex2(m_run[r] - mn);
-            l_run[r] = m_run[r] == -INFINITY ? l_run[r] : l_run[r] * f;
-            m_run[r] = mn;
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) o[r][i] = make_float4(o[r][i].x * f, o[r][i].y * f, o[r][i].z * f, o[r][i].w * f);
-          }
-        }
-#pragma unroll
-        for (int r = 0; r < RU; ++r) {
-          sc[r] = ex2(sc[r] - (m_run[r] == -INFINITY ? 0.f : m_run[r]));
-          l_run[r] += sc[r];  // of this lane's key
-        }
+        __syncwarp();
 #pragma unroll
         for (int i = 0; i < kKeys / kAt; ++i) {
           const int row = i * kAt + sub;
-          float p[RU];
-#pragma unroll
-          for (int r = 0; r < RU; ++r) p[r] = __shfl_sync(0xffffffffu, sc[r], row * kParts);
           if (row < n_valid) {  // (rows behind the end may hold anything)
+            float4 x[kEach];
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-              const int c = e * kCols + col;
-              const float4 x = *reinterpret_cast<const float4*>(vt + (c / 8 * SR + row) * 128 + ((c % 8) ^ row) * 16);
+            for (int e = 0; e < kEach; ++e) x[e] = reinterpret_cast<const float4*>(vt + row * C::kRowBytes)[e * kCols + col];
 #pragma unroll
-              for (int r = 0; r < RU; ++r) {
-                o[r][e].x = fmaf(p[r], x.x, o[r][e].x);
-                o[r][e].y = fmaf(p[r], x.y, o[r][e].y);
-                o[r][e].z = fmaf(p[r], x.z, o[r][e].z);
-                o[r][e].w = fmaf(p[r], x.w, o[r][e].w);
+            for (int r = 0; r < RU; ++r) {
+              const float2 p = p_s[row * RU + r];
+#pragma unroll
+              for (int e = 0; e < kEach; ++e) {
+                o[r][e][0] = ffma2(p, make_float2(x[e].x, x[e].y), o[r][e][0]);
+                o[r][e][1] = ffma2(p, make_float2(x[e].z, x[e].w), o[r][e][1]);
               }
             }
           }
@@ -646,31 +698,35 @@ __global__ void __launch_bounds__(F32Block<D, kRows>::kThreads, 2)
       ring.copy(slot);
       if (u.last) {
         const size_t at = (static_cast<size_t>(blockIdx.x) * C::kWarps + warp + u.uid) * a.rs;
+        float l_of = l_run;
+#pragma unroll
+        for (int d = kParts; d < 32; d *= 2) l_of += __shfl_xor_sync(0xffffffffu, l_of, d);
+        __syncwarp();
+        if (key_at == 0) f_s[my_row] = make_float2(m_run, l_of);
+        __syncwarp();
 #pragma unroll
         for (int r = 0; r < RU; ++r) {
-          float l = l_run[r];
-#pragma unroll
-          for (int i = kParts; i < 32; i *= 2) l += __shfl_xor_sync(0xffffffffu, l, i);
 #pragma unroll
           for (int e = 0; e < kEach; ++e)
 #pragma unroll
-            for (int i = kCols; i < 32; i *= 2) {
-              o[r][e].x += __shfl_xor_sync(0xffffffffu, o[r][e].x, i);
-              o[r][e].y += __shfl_xor_sync(0xffffffffu, o[r][e].y, i);
-              o[r][e].z += __shfl_xor_sync(0xffffffffu, o[r][e].z, i);
-              o[r][e].w += __shfl_xor_sync(0xffffffffu, o[r][e].w, i);
-            }
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int d = kCols; d < 32; d *= 2) {
+                o[r][e][i].x += __shfl_xor_sync(0xffffffffu, o[r][e][i].x, d);
+                o[r][e][i].y += __shfl_xor_sync(0xffffffffu, o[r][e][i].y, d);
+              }
           int b, h;
           if (!unit_row<RU>(a, u, r, &b, &h) || sub != 0) continue;
+          const float2 ml = f_s[r];
           const bool result = u.last == 2;
           const size_t row = static_cast<size_t>(b) * a.H + h;
-          const float f = !result ? 1.f : l == 0.f ? 0.f : 1.f / l;  // (no key seen: O is 0 as well)
+          const float f = !result ? 1.f : ml.y == 0.f ? 0.f : 1.f / ml.y;  // (no key seen: O is 0 as well)
           float4* const dst = reinterpret_cast<float4*>(result ? static_cast<float*>(a.out) + row * D : a.part_o + (at + r) * D);
 #pragma unroll
           for (int e = 0; e < kEach; ++e)
-            dst[e * kCols + col] = make_float4(o[r][e].x * f, o[r][e].y * f, o[r][e].z * f, o[r][e].w * f);
-          if (lane == 0 && !result) a.part_ml[at + r] = make_float2(m_run[r], l);
-          if (lane == 0 && result && a.lse) a.lse[row] = l > 0.f ? m_run[r] * kLn2 + logf(l) : l == 0.f ? -INFINITY : l;
+            dst[e * kCols + col] = make_float4(o[r][e][0].x * f, o[r][e][0].y * f, o[r][e][1].x * f, o[r][e][1].y * f);
+          if (lane == 0 && !result) a.part_ml[at + r] = ml;
+          if (lane == 0 && result && a.lse) a.lse[row] = ml.y > 0.f ? ml.x * kLn2 + logf(ml.y) : ml.y == 0.f ? -INFINITY : ml.y;
         }
       }
     }
@@ -679,15 +735,17 @@ __global__ void __launch_bounds__(F32Block<D, kRows>::kThreads, 2)
 
 // ---- fold ---------------------------------------------------------------------------
 
-// Parts of the rows that no warp finished, and rows without keys. A row has D / 4 threads, four columns each, times kSlices, which
-// take every kSlices-th part; a thread asks for eight parts at a time.
-template <typename T, int D, int RU, int kFoldThreads, int kSlices>
+// Parts of the rows that no warp finished, and rows without keys. A row's kCols columns have kCols / 4 threads, four columns each,
+// times kSlices, which take every kSlices-th part; a thread asks for eight parts at a time.
+template <typename T, int D, int RU, int kFoldThreads, int kSlices, int kCols>
 __global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const __grid_constant__ PagedArgs a) {
-  constexpr int kVec = D / 4, kRowsPer = kFoldThreads / kVec / kSlices, kBatch = 8;
-  __shared__ float4 acc_of[kSlices > 1 ? kFoldThreads : 1];
-  __shared__ float2 ml_of[kSlices > 1 ? kFoldThreads / kVec : 1];
+  constexpr int kVec = kCols / 4, kRowsPer = kFoldThreads / kVec / kSlices, kBatch = 8;
+  // slices that sit in one warp meet by shuffles, the others (kGroups of a row) through shared memory
+  constexpr int kInWarp = kSlices < 32 / kVec ? kSlices : kVec < 32 ? 32 / kVec : 1, kGroups = kSlices / kInWarp;
+  __shared__ float4 acc_of[kGroups > 1 ? kFoldThreads / kInWarp : 1];
+  __shared__ float2 ml_of[kGroups > 1 ? kFoldThreads / kVec / kInWarp : 1];
   let_next_start();
-  const int col = threadIdx.x % kVec, lane_row = threadIdx.x / kVec, slice = lane_row % kSlices;
+  const int col = static_cast<int>(blockIdx.y) * kVec + threadIdx.x % kVec, lane_row = threadIdx.x / kVec, slice = lane_row % kSlices;
   const int row = static_cast<int>(blockIdx.x) * kRowsPer + lane_row / kSlices;
   const bool mine = row < a.B * a.H;
   const int b = mine ? row / a.H : 0, h = mine ? row - b * a.H : 0, kvh = h % a.kvH, g = h / a.kvH;
@@ -756,27 +814,35 @@ __global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const __grid_c
       acc.w += f * o[j].w;
     }
   }
-  if constexpr (kSlices > 1) {
-    acc_of[threadIdx.x] = acc;
-    if (col == 0) ml_of[lane_row] = make_float2(m_all, l_all);
+  auto join = [&](float m, float l, float4 o) {  // of another slice
+    const float m_new = fmaxf(m_all, m);
+    const float f0 = m_all > -INFINITY ? ex2(m_all - m_new) : 1.f, f1 = m > -INFINITY ? ex2(m - m_new) : 1.f;
+    m_all = m_new;
+    l_all = f0 * l_all + f1 * l;
+    acc = make_float4(f0 * acc.x + f1 * o.x, f0 * acc.y + f1 * o.y, f0 * acc.z + f1 * o.z, f0 * acc.w + f1 * o.w);
+  };
+#pragma unroll
+  for (int d = kVec; d < kVec * kInWarp; d *= 2) {
+    const float m = __shfl_xor_sync(0xffffffffu, m_all, d), l = __shfl_xor_sync(0xffffffffu, l_all, d);
+    float4 o;
+    o.x = __shfl_xor_sync(0xffffffffu, acc.x, d);
+    o.y = __shfl_xor_sync(0xffffffffu, acc.y, d);
+    o.z = __shfl_xor_sync(0xffffffffu, acc.z, d);
+    o.w = __shfl_xor_sync(0xffffffffu, acc.w, d);
+    join(m, l, o);
+  }
+  if constexpr (kGroups > 1) {
+    const int at = threadIdx.x % kVec, group = lane_row / kInWarp;  // (a row's groups lie one after the other)
+    if (slice % kInWarp == 0) {
+      acc_of[group * kVec + at] = acc;
+      if (at == 0) ml_of[group] = make_float2(m_all, l_all);
+    }
     __syncthreads();
     if (slice == 0) {
-      const float2 first = make_float2(m_all, l_all);
-#pragma unroll
-      for (int i = 1; i < kSlices; ++i) m_all = fmaxf(m_all, ml_of[lane_row + i].x);
-      const float f0 = first.x > -INFINITY ? ex2(first.x - m_all) : 1.f;
-      l_all = f0 * first.y;
-      acc = make_float4(f0 * acc.x, f0 * acc.y, f0 * acc.z, f0 * acc.w);
-#pragma unroll
-      for (int i = 1; i < kSlices; ++i) {
-        const float2 ml = ml_of[lane_row + i];
-        const float4 o = acc_of[threadIdx.x + i * kVec];
-        const float f = ml.x > -INFINITY ? ex2(ml.x - m_all) : 1.f;
-        l_all += f * ml.y;
-        acc.x += f * o.x;
-        acc.y += f * o.y;
-        acc.z += f * o.z;
-        acc.w += f * o.w;
+#pragma unroll 8
+      for (int i = 1; i < kGroups; ++i) {
+        const float2 ml = ml_of[group + i];
+        join(ml.x, ml.y, acc_of[(group + i) * kVec + at]);
       }
     }
   }
@@ -834,8 +900,8 @@ PagedPlan make_plan(const ra_paged_kv& c, int heads, int shared_len) {
   return p;
 }
 
-template <void (*kern)(CUtensorMap, CUtensorMap, PagedArgs), typename C>
-int launch_main(const CUtensorMap& k, const CUtensorMap& v, int blocks, const PagedArgs& a, cudaStream_t stream) {
+template <auto kern, typename C, typename... Args>
+int launch_main(int blocks, cudaStream_t stream, const Args&... args) {
   static std::atomic<unsigned long long> smem_set{0};  // once per device and instantiation
   int dev = 0;
   RAB_CUDA(cudaGetDevice(&dev));
@@ -843,41 +909,43 @@ int launch_main(const CUtensorMap& k, const CUtensorMap& v, int blocks, const Pa
     RAB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
     if (dev >= 0 && dev < 64) smem_set.fetch_or(1ull << dev, std::memory_order_release);
   }
-  RAB_CUDA(launch_overlapped(kern, dim3(static_cast<unsigned>(blocks)), dim3(C::kThreads), C::kSmemBytes, stream, k, v, a));
+  RAB_CUDA(launch_overlapped(kern, dim3(static_cast<unsigned>(blocks)), dim3(C::kThreads), C::kSmemBytes, stream, args...));
   return RA_OK;
 }
 
-// Threads of the fold that share out a row's parts: all of a large block where there is a row an SM and less, since the shares
-// of a whole wave may then belong to one row; eight where there are a few; one elsewhere.
+// Threads of the fold that share out a row's parts. With few rows the shares of a whole wave may belong to one of them: then 128
+// threads share out a row's parts for 32 columns; eight where there are more rows, one where there are many.
 template <typename T, int D, int RU>
 int launch_fold(const PagedArgs& a, cudaStream_t stream) {
   const long long rows = static_cast<long long>(a.B) * a.H, sms = sm_count();
-  auto go = [&](auto threads, auto slices) -> int {
-    constexpr int kThreads = decltype(threads)::value, kSlices = decltype(slices)::value, kPer = kThreads / (D / 4) / kSlices;
-    RAB_CUDA(launch_overlapped(paged_fold_kernel<T, D, RU, kThreads, kSlices>, dim3(static_cast<unsigned>((rows + kPer - 1) / kPer)),
-                               dim3(kThreads), 0, stream, a));
+  auto go = [&](auto threads, auto slices, auto cols) -> int {
+    constexpr int kThreads = decltype(threads)::value, kSlices = decltype(slices)::value, kCols = decltype(cols)::value;
+    constexpr int kPer = kThreads / (kCols / 4) / kSlices;
+    RAB_CUDA(launch_overlapped(paged_fold_kernel<T, D, RU, kThreads, kSlices, kCols>,
+                               dim3(static_cast<unsigned>((rows + kPer - 1) / kPer), D / kCols), dim3(kThreads), 0, stream, a));
     return RA_OK;
   };
-  constexpr int kSome = 256 / (D / 4) < 8 ? 256 / (D / 4) : 8, kAll = 1024 / (D / 4) < 32 ? 1024 / (D / 4) : 32;
-  if (rows <= sms) return go(std::integral_constant<int, 32 * (D / 4) < 1024 ? 32 * (D / 4) : 1024>(), std::integral_constant<int, kAll>());
-  if (rows <= 8 * sms) return go(std::integral_constant<int, 256>(), std::integral_constant<int, kSome>());
-  return go(std::integral_constant<int, 256>(), std::integral_constant<int, 1>());
+  using std::integral_constant;
+  constexpr int kSome = 256 / (D / 4) < 8 ? 256 / (D / 4) : 8;
+  if (rows * (D / 32) <= 2 * sms) return go(integral_constant<int, 1024>(), integral_constant<int, 128>(), integral_constant<int, 32>());
+  if (rows <= 8 * sms) return go(integral_constant<int, 256>(), integral_constant<int, kSome>(), integral_constant<int, D>());
+  return go(integral_constant<int, 256>(), integral_constant<int, 1>(), integral_constant<int, D>());
 }
 
 template <typename T, int D, int RU>
 int launch_rows(const ra_paged_kv& c, const PagedArgs& a, const PagedPlan& p, cudaStream_t stream) {
-  if (p.blocks > 0) {
+  int rc = RA_OK;
+  if constexpr (sizeof(T) == 4) {
+    if (p.blocks > 0) rc = launch_main<paged_f32_kernel<D, RU>, typename F32Cfg<D, RU>::Block>(p.blocks, stream, a);
+  } else if (p.blocks > 0) {
     CUtensorMap k, v;
     const long long heads = static_cast<long long>(a.num_pages) * a.kvH, stride = static_cast<long long>(c.page_size) * D;
     const int box = std::min(c.page_size, p.SR);
-    int rc = tcgen::make_map(&k, c.dtype, c.k, D, c.page_size, heads, stride, box);
+    rc = tcgen::make_map(&k, c.dtype, c.k, D, c.page_size, heads, stride, box);
     if (rc == RA_OK) rc = tcgen::make_map(&v, c.dtype, c.v, D, c.page_size, heads, stride, box);
-    if (rc == RA_OK) {
-      if constexpr (sizeof(T) == 4) rc = launch_main<paged_f32_kernel<D, RU>, F32Block<D, RU>>(k, v, p.blocks, a, stream);
-      else rc = launch_main<paged_mma_kernel<T, D>, MmaBlock<T, D>>(k, v, p.blocks, a, stream);
-    }
-    if (rc != RA_OK) return rc;
+    if (rc == RA_OK) rc = launch_main<paged_mma_kernel<T, D>, MmaBlock<T, D>>(p.blocks, stream, k, v, a);
   }
+  if (rc != RA_OK) return rc;
   return launch_fold<T, D, RU>(a, stream);
 }
 
@@ -945,6 +1013,8 @@ int ra_paged_decode(const ra_paged_kv* cache, const void* q, int heads, const in
   unsigned char* const ws = static_cast<unsigned char*>(workspace);
   PagedArgs a;
   a.q = q;
+  a.k = c.k;
+  a.v = c.v;
   a.out = out;
   a.lse = lse;
   a.table = c.page_table;
