@@ -4,11 +4,12 @@
 //   y = R_p (x r w),  r = (mean(x^2) + eps)^-1/2,  R_p turns pair i by p f_i
 //   backward, with g = R_-p dy:  dw = sum over rows of g x r,  dx = r (g w - x r^2 mean(g w x))
 //
-// All of it is bound by memory: a row comes in once and goes out once. A lane holds 16 bytes of a row (32 of an fp32 row of
-// 256), so 4 to 32 lanes share a row and a warp takes several heads of one token at a time. cos and sin of the token's position
-// are worked out once for all heads that the warp takes, from an angle in fixed point (see ra_rope), and multiplied by the
-// weights ahead of the rows: a row then costs a sum of squares and two multiply-adds an element. With pairs half a row apart the
-// partner's elements come by shuffles of the raw words, with neighbouring pairs they are the lane's own.
+// All of it is bound by memory: a row comes in once and goes out once. A lane holds two 16-byte pieces of a row, in such a place
+// that the elements it turns into one another are its own: with pairs half a row apart, a piece of either half. So 2 to 32
+// lanes share a row, a warp takes several heads of one token at a time, and nothing crosses lanes but the sum of squares. cos and
+// sin of the token's position are worked out once for all heads that the warp takes, from an angle in fixed point (see ra_rope),
+// and multiplied by the weights ahead of the rows: a row then costs a sum of squares and three multiply-adds an element, two
+// elements an instruction.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -20,14 +21,13 @@ namespace rab {
 namespace {
 
 constexpr int kWarps = 8;
+constexpr int kBackwardBlocks = 2;  // of the backward pass, to an SM
 
-// E elements of a row to a lane, L lanes to a row, R rows to a warp.
-template <typename T, int D>
+// Two pieces of P elements (kBytes) of a row to a lane, L lanes to a row, R rows to a warp.
+template <typename T, int D, int kBytes>
 struct RowCfg {
-  static constexpr int E = D * static_cast<int>(sizeof(T)) > 512 ? D / 32 : 16 / static_cast<int>(sizeof(T));
-  static constexpr int L = D / E;
-  static constexpr int R = 32 / L;
-  static constexpr int kWords = E * static_cast<int>(sizeof(T)) / 4;  // 32-bit words of a lane
+  static constexpr int W = kBytes / 4, P = kBytes / static_cast<int>(sizeof(T)), E = 2 * P;
+  static constexpr int L = D / E, R = 32 / L;
 };
 
 template <typename T>
@@ -40,19 +40,29 @@ template <>
 __device__ inline float2 unpack2<__nv_bfloat16>(unsigned u) {
   return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
-template <typename T, int E>
-__device__ inline void unpack(const unsigned* u, float (&x)[E]) {
-  if constexpr (sizeof(T) == 4) {
+template <typename T, int P, int W>
+__device__ inline void unpack(const unsigned (&u)[W], float2 (&x)[P / 2]) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) x[i] = __uint_as_float(u[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < E / 2; ++i) {
-      const float2 f = unpack2<T>(u[i]);
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
+  for (int i = 0; i < P / 2; ++i) {
+    if constexpr (sizeof(T) == 4) x[i] = make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+    else x[i] = unpack2<T>(u[i]);
   }
+}
+// two elements an instruction
+__device__ inline float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(*reinterpret_cast<unsigned long long*>(&d))
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return d;
+}
+__device__ inline float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(*reinterpret_cast<unsigned long long*>(&d))
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)),
+        "l"(*reinterpret_cast<unsigned long long*>(&c)));
+  return d;
 }
 template <typename T>
 __device__ inline unsigned pack2(float a, float b);
@@ -66,26 +76,24 @@ __device__ inline unsigned pack2<__nv_bfloat16>(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const unsigned*>(&h);
 }
-template <typename T, int E>
-__device__ inline void pack(const float (&x)[E], unsigned* u) {
-  if constexpr (sizeof(T) == 4) {
+template <typename T, int P, int W>
+__device__ inline void pack(const float2 (&x)[P / 2], unsigned (&u)[W]) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) u[i] = __float_as_uint(x[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < E / 2; ++i) u[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
+  for (int i = 0; i < P / 2; ++i) {
+    if constexpr (sizeof(T) == 4) u[2 * i] = __float_as_uint(x[i].x), u[2 * i + 1] = __float_as_uint(x[i].y);
+    else u[i] = pack2<T>(x[i].x, x[i].y);
   }
 }
 
-// A lane's words of a row: 16 bytes at a time, or (`vec` false: some row is not 16-byte aligned) an element at a time.
+// A piece of a row: at once, or (`vec` false: some row is not 16-byte aligned) an element at a time.
 template <typename T, int W>
-__device__ inline void load_words(const T* p, bool vec, unsigned (&u)[W]) {
-  if (vec) {
-#pragma unroll
-    for (int i = 0; i < W / 4; ++i) {
-      const uint4 v = *reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned*>(p) + 4 * i);
-      u[4 * i] = v.x, u[4 * i + 1] = v.y, u[4 * i + 2] = v.z, u[4 * i + 3] = v.w;
-    }
+__device__ inline void load_piece(const T* p, bool vec, unsigned (&u)[W]) {
+  if (vec && W == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    u[0] = v.x, u[1] = v.y, u[W - 2] = v.z, u[W - 1] = v.w;
+  } else if (vec) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    u[0] = v.x, u[1] = v.y;
   } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int i = 0; i < W; ++i) u[i] = __float_as_uint(p[i]);
@@ -96,12 +104,11 @@ __device__ inline void load_words(const T* p, bool vec, unsigned (&u)[W]) {
   }
 }
 template <typename T, int W>
-__device__ inline void store_words(T* p, bool vec, const unsigned (&u)[W]) {
-  if (vec) {
-#pragma unroll
-    for (int i = 0; i < W / 4; ++i)
-      *reinterpret_cast<uint4*>(reinterpret_cast<unsigned*>(p) + 4 * i) =
-          make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+__device__ inline void store_piece(T* p, bool vec, const unsigned (&u)[W]) {
+  if (vec && W == 4) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[W - 2], u[W - 1]);
+  } else if (vec) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
   } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int i = 0; i < W; ++i) p[i] = __uint_as_float(u[i]);
@@ -115,6 +122,12 @@ __device__ inline void store_words(T* p, bool vec, const unsigned (&u)[W]) {
   }
 }
 
+// Bytes of a piece. The backward pass has a lane's share of the weights' gradients in registers beside two rows, and takes half as
+// much of a 16-bit row.
+constexpr int kForwardBytes = 16;
+template <typename T>
+constexpr int kBackwardBytes = sizeof(T) == 2 ? 8 : 16;
+
 struct Rows {
   char* data;
   long long batch, head, row;  // strides in elements
@@ -124,9 +137,9 @@ struct Rows {
 struct Args {
   Rows in[3], dy[2], out[3];  // q, k, v (v and a cache's k_out, v_out: see paged below)
   int heads[3];               // 0: that side is absent
-  int B, S;
+  unsigned S;
   const void* w[2];
-  int w_f32;
+  int w_f32, w_vec;  // fp32 or of the rows' type; both 16-byte aligned
   float eps;
   int rot_dim;  // 0: no rotation
   PosMap map;
@@ -143,78 +156,93 @@ struct Args {
   unsigned long long turns[RA_ROPE_MAX_PAIRS];
 };
 
-__device__ inline float weight_at(const void* w, int w_f32, int i, float) { return static_cast<const float*>(w)[i]; }
-__device__ inline float weight_at(const void* w, int w_f32, int i, __half) {
-  return w_f32 ? static_cast<const float*>(w)[i] : __half2float(static_cast<const __half*>(w)[i]);
-}
-__device__ inline float weight_at(const void* w, int w_f32, int i, __nv_bfloat16) {
-  return w_f32 ? static_cast<const float*>(w)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]);
+// P weights from element `at` on.
+template <typename T, int P>
+__device__ inline void load_weights(const void* w, int w_f32, int vec, int at, float2 (&x)[P / 2]) {
+  if (sizeof(T) == 2 && w_f32) {
+    unsigned u[4];
+#pragma unroll
+    for (int i = 0; i < P / 4; ++i) {
+      load_piece<float, 4>(static_cast<const float*>(w) + at + 4 * i, vec, u);
+      x[2 * i] = make_float2(__uint_as_float(u[0]), __uint_as_float(u[1]));
+      x[2 * i + 1] = make_float2(__uint_as_float(u[2]), __uint_as_float(u[3]));
+    }
+  } else {
+    unsigned u[P * sizeof(T) / 4];
+    load_piece<T>(static_cast<const T*>(w) + at, vec, u);
+    unpack<T, P>(u, x);
+  }
 }
 
 __device__ inline long long row_position(const Args& a, int b, int s) {
   if (a.positions) return a.positions[b * a.pos_batch + s];
   if (a.lens) return static_cast<long long>(a.lens[b]) + s;
-  const int seg = s / a.map.seg_len;
+  const int seg = static_cast<int>(static_cast<unsigned>(s) / static_cast<unsigned>(a.map.seg_len));
   return a.map.base[seg] + static_cast<long long>(s - seg * a.map.seg_len) * a.pos_stride;
 }
 
-// The place of a lane's elements in the rotation: its partner's lane, and (cos, signed sin) of its elements, so that
-// y[e] = x[e] c[e] + partner[e] s[e].
-template <typename T, int D, bool kInter>
+// A lane's two pieces of a row and how they turn: y[q] = x[q] (cos) + other(x)[q] (signed sin), q = 0, 1, where other exchanges
+// what turns into one another: the pieces, or (kInter) neighbours. Behind rot_dim nothing turns: cos 1, sin 0, and nothing other,
+// whatever the elements hold.
+template <typename T, int D, bool kInter, int kBytes>
 struct Turn {
-  using C = RowCfg<T, D>;
-  static constexpr int E = C::E;
-  int partner;  // lane; its own where nothing turns
+  using C = RowCfg<T, D, kBytes>;
+  static constexpr int P = C::P;
+  int at[2];   // first element of each piece
   bool turns;
-  float c[E], s[E];
+  float2 c[P / 2], s[P / 2];  // of the lane's P pairs
   __device__ inline void place(const Args& a, int lane) {
-    const int at = lane % C::L * E, half = a.rot_dim / 2;
-    turns = at < a.rot_dim;
-    partner = kInter || !turns ? lane : at < half ? lane + half / E : lane - half / E;
+    const int l = lane % C::L;
+    turns = l * C::E < a.rot_dim;
+    at[0] = !kInter && turns ? l * P : l * C::E;
+    at[1] = at[0] + (!kInter && turns ? a.rot_dim / 2 : P);
   }
-  __device__ inline void angles(const Args& a, int lane, long long pos) {
-    const int at = lane % C::L * E, half = a.rot_dim / 2;
+  __device__ inline void angles(const unsigned long long* turns_of, int lane, long long pos) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) c[e] = 1.f, s[e] = 0.f;
+    for (int e = 0; e < P / 2; ++e) c[e] = make_float2(1.f, 1.f), s[e] = make_float2(0.f, 0.f);
     if (!turns) return;
     // (the angle in half turns, from the upper word of its place in the turn: off by 2^-25 of a half turn at most)
     auto angle = [&](int pair, float* si, float* co) {
-      const unsigned long long t = static_cast<unsigned long long>(pos) * a.turns[pair];
+      const unsigned long long t = static_cast<unsigned long long>(pos) * turns_of[pair];
       sincospif(static_cast<float>(static_cast<int>(t >> 32)) * 4.656612873077393e-10f, si, co);
     };
-    if constexpr (kInter) {
+    const int pair = lane % C::L * P;
 #pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        float si, co;
-        angle((at + e) / 2, &si, &co);
-        c[e] = c[e + 1] = co;
-        s[e] = -si;
-        s[e + 1] = si;
-      }
-    } else {
-      const int first = at < half ? at : at - half;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        float si, co;
-        angle(first + e, &si, &co);
-        c[e] = co;
-        s[e] = at < half ? -si : si;
-      }
+    for (int e = 0; e < P / 2; ++e) {
+      angle(pair + 2 * e, &s[e].x, &c[e].x);
+      angle(pair + 2 * e + 1, &s[e].y, &c[e].y);
     }
   }
-  // The partner's elements of a row whose words are u and whose elements are x (every lane of the warp calls).
-  __device__ inline void other(const unsigned (&u)[C::kWords], const float (&x)[E], float (&xp)[E]) const {
-    if constexpr (kInter) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) xp[e] = x[e ^ 1];
-    } else {
-      unsigned up[C::kWords];
-#pragma unroll
-      for (int i = 0; i < C::kWords; ++i) up[i] = __shfl_sync(0xffffffffu, u[i], partner);
-      unpack<T, E>(up, xp);
-    }
+  // cos and signed sin of element pair e of piece q
+  __device__ inline float2 cos_of(int q, int e) const {
+    if constexpr (!kInter) return c[e];
+    const float v = e % 2 ? c[q * (P / 4) + e / 2].y : c[q * (P / 4) + e / 2].x;
+    return make_float2(v, v);
+  }
+  __device__ inline float2 sin_back(int q, int e) const {  // of the turn back
+    if constexpr (!kInter) return q == 0 ? s[e] : make_float2(-s[e].x, -s[e].y);
+    const float v = e % 2 ? s[q * (P / 4) + e / 2].y : s[q * (P / 4) + e / 2].x;
+    return make_float2(v, -v);
+  }
+  __device__ inline float2 sin_of(int q, int e) const {
+    if constexpr (!kInter) return q == 0 ? make_float2(-s[e].x, -s[e].y) : s[e];
+    const float v = e % 2 ? s[q * (P / 4) + e / 2].y : s[q * (P / 4) + e / 2].x;
+    return make_float2(-v, v);
+  }
+  // (kAll: all of the row turns)
+  template <bool kAll>
+  __device__ inline float2 other(const float2 (&x)[2][P / 2], int q, int e) const {
+    const float2 o = kInter ? make_float2(x[q][e].y, x[q][e].x) : x[1 - q][e];
+    return kAll || turns ? o : make_float2(0.f, 0.f);
   }
 };
+
+// The rotation's table into shared memory (from the launch's parameters, where lanes that ask for different entries wait for one
+// another).
+__device__ inline void load_turns(const Args& a, unsigned long long* turns_of) {
+  for (int i = threadIdx.x; i < a.rot_dim / 2; i += kWarps * 32) turns_of[i] = a.turns[i];
+  __syncthreads();
+}
 
 template <int L>
 __device__ inline float row_sum(float v) {
@@ -223,163 +251,240 @@ __device__ inline float row_sum(float v) {
   return v;
 }
 
-// A warp takes `per` groups of R rows of one token, from the list of q's groups, then k's, then v's.
+// A warp has the rows of kAhead groups on their way; two blocks of eight warps to an SM leave a thread 128 registers. us a pass
+// (32768 tokens of 40 heads of 128, bf16): 117, with three groups 124, three blocks and two groups 122, 8-byte pieces 122.
+// A warp takes `per` groups of R rows of one of the `total` tokens, from the list of q's groups, then k's, then v's.
 template <typename T, int D, bool kInter, bool kPaged>
-__global__ void __launch_bounds__(kWarps * 32) norm_rope_kernel(const __grid_constant__ Args a, long long total, int per) {
-  using C = RowCfg<T, D>;
-  constexpr int E = C::E, W = C::kWords, kAhead = 4;
-  const int lane = threadIdx.x & 31, sub = lane / C::L, at = lane % C::L * E;
-  const long long id = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+__global__ void __launch_bounds__(kWarps * 32, 2) norm_rope_kernel(const __grid_constant__ Args a, unsigned total, int per) {
+  using C = RowCfg<T, D, kForwardBytes>;
+  constexpr int P = C::P, kAhead = 4;
+  const int lane = threadIdx.x & 31, sub = lane / C::L;
+  __shared__ unsigned long long turns_of[RA_ROPE_MAX_PAIRS];
+  const unsigned token = blockIdx.x * kWarps + (threadIdx.x >> 5);
   let_next_start();
+  load_turns(a, turns_of);
   wait_for_previous();
-  if (id >= total) return;
-  const long long tokens = static_cast<long long>(a.B) * a.S;
-  const int chunk = static_cast<int>(id / tokens);
-  const long long token = id - chunk * tokens;
-  const int b = static_cast<int>(token / a.S), t = static_cast<int>(token - static_cast<long long>(b) * a.S);
+  if (token >= total) return;
+  const int b = static_cast<int>(token / a.S), t = static_cast<int>(token - static_cast<unsigned>(b) * a.S);
   long long place = -1;  // paged: row of the cache's first head that takes the token's K and V
   if constexpr (kPaged) {
     if (a.counts && t >= a.counts[b]) return;
     place = paged_row(a.table + b * a.table_stride, a.max_pages, a.num_pages, a.page_shift, a.heads[1],
                       static_cast<long long>(a.lens[b]) + t);
   }
-  Turn<T, D, kInter> turn;
+  Turn<T, D, kInter, kForwardBytes> turn;
   turn.place(a, lane);
-  turn.angles(a, lane, a.rot_dim ? row_position(a, b, t) : 0);
-  const int beg = chunk * per, end = beg + per;
+  const long long pos = a.rot_dim ? row_position(a, b, t) : 0;
+  const int beg = static_cast<int>(blockIdx.y) * per, end = beg + per;
   int first = 0;  // group of a side's first row
+  bool turned = false;
 #pragma unroll
   for (int side = 0; side < (kPaged ? 3 : 2); ++side) {
     const int heads = a.heads[side], groups = (heads + C::R - 1) / C::R;
     const int lo = max(beg - first, 0), hi = min(end - first, groups);
     first += groups;
-    if (lo >= hi) continue;
-    const Rows in = a.in[side], out = a.out[side];
     const bool to_cache = kPaged && side > 0;
-    if (to_cache && place < 0) continue;
-    const T* src = reinterpret_cast<const T*>(in.data) + b * in.batch + t * in.row + at;
-    T* dst = reinterpret_cast<T*>(out.data) + (to_cache ? place * D : b * out.batch + t * out.row) + at;
+    if (lo >= hi || (to_cache && place < 0)) continue;
+    const Rows in = a.in[side], out = a.out[side];
     const long long out_head = to_cache ? static_cast<long long>(D) << a.page_shift : out.head;
-    const bool norm = side < 2 && a.w[side < 2 ? side : 0] != nullptr;
-    // factors of the element and of its partner, weights included
-    float fx[E], fp[E];
-    if (side < 2) {
-      const int p_at = kInter ? at : turn.partner % C::L * E;
+    int h = lo * C::R + sub;
+    const T* src = reinterpret_cast<const T*>(in.data) + b * in.batch + t * in.row;
+    T* dst = reinterpret_cast<T*>(out.data) + (to_cache ? place * D : b * out.batch + t * out.row) + h * out_head;
+    unsigned u[kAhead][2][C::W];
+    auto load = [&](int g) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        fx[e] = turn.c[e] * (norm ? weight_at(a.w[side], a.w_f32, at + e, T()) : 1.f);
-        fp[e] = turn.s[e] * (norm ? weight_at(a.w[side], a.w_f32, p_at + (kInter ? e ^ 1 : e), T()) : 1.f);
-      }
-    }
-    for (int g = lo; g < hi; g += kAhead) {
-      unsigned u[kAhead][W];
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int h = (g + i) * C::R + sub;
-#pragma unroll
-        for (int j = 0; j < W; ++j) u[i][j] = 0;
-        if (g + i < hi && h < heads) load_words<T, W>(src + h * in.head, in.vec, u[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
+      for (int i = 0; i < kAhead; ++i) {  // (rows behind the last one are the last one once more)
         if (g + i >= hi) break;
-        const int h = (g + i) * C::R + sub;
-        if (side < 2) {
-          float x[E], xp[E], y[E];
-          unpack<T, E>(u[i], x);
-          float r = 1.f;
-          if (norm) {
-            float sum = 0.f;
+        const T* const row = src + min((g + i) * C::R + sub, heads - 1) * in.head;
 #pragma unroll
-            for (int e = 0; e < E; ++e) sum = fmaf(x[e], x[e], sum);
-            r = rsqrtf(row_sum<C::L>(sum) * (1.f / D) + a.eps);
-          }
-          turn.other(u[i], x, xp);
-#pragma unroll
-          for (int e = 0; e < E; ++e) y[e] = r * (turn.turns ? fmaf(x[e], fx[e], xp[e] * fp[e]) : x[e] * fx[e]);
-          pack<T, E>(y, u[i]);
-        }
-        if (h < heads) store_words<T, W>(dst + h * out_head, out.vec, u[i]);
+        for (int q = 0; q < 2; ++q) load_piece<T, C::W>(row + turn.at[q], in.vec, u[i][q]);
       }
+    };
+    load(lo);  // (on their way while the angles are worked out)
+    // factors of a lane's elements and of those that turn into them, weights included
+    float2 fx[2][P / 2], fp[2][P / 2];
+    const bool norm = side < 2 && a.w[side < 2 ? side : 0] != nullptr;
+    if (side < 2) {
+      if (!turned && a.rot_dim) turn.angles(turns_of, lane, pos);
+      if (!turned && !a.rot_dim) {
+#pragma unroll
+        for (int e = 0; e < P / 2; ++e) turn.c[e] = make_float2(1.f, 1.f), turn.s[e] = make_float2(0.f, 0.f);
+      }
+      turned = true;
+      float2 w[2][P / 2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+#pragma unroll
+        for (int e = 0; e < P / 2; ++e) w[q][e] = make_float2(1.f, 1.f);
+        if (norm) load_weights<T, P>(a.w[side], a.w_f32, a.w_vec, turn.at[q], w[q]);
+      }
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int e = 0; e < P / 2; ++e) {
+          fx[q][e] = mul2(turn.cos_of(q, e), w[q][e]);
+          fp[q][e] = mul2(turn.sin_of(q, e), turn.template other<false>(w, q, e));
+        }
     }
+    auto rows = [&](auto all) {
+      constexpr bool kAll = decltype(all)::value;
+      for (int g = lo; g < hi; g += kAhead) {
+        if (g > lo) load(g);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          if (g + i >= hi) break;
+          if (side < 2) {
+            float2 x[2][P / 2], y[P / 2];
+            unpack<T, P>(u[i][0], x[0]);
+            unpack<T, P>(u[i][1], x[1]);
+            float r = 1.f;
+            if (norm) {
+              float2 sum = mul2(x[0][0], x[0][0]), more = mul2(x[1][0], x[1][0]);
+#pragma unroll
+              for (int e = 1; e < P / 2; ++e) {
+                sum = fma2(x[0][e], x[0][e], sum);
+                more = fma2(x[1][e], x[1][e], more);
+              }
+              r = rsqrtf(row_sum<C::L>((sum.x + sum.y) + (more.x + more.y)) * (1.f / D) + a.eps);
+            }
+            const float2 r2 = make_float2(r, r);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+#pragma unroll
+              for (int e = 0; e < P / 2; ++e)
+                y[e] = mul2(r2, fma2(x[q][e], fx[q][e], mul2(turn.template other<kAll>(x, q, e), fp[q][e])));
+              pack<T, P>(y, u[i][q]);
+            }
+          }
+          if (h < heads) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) store_piece<T, C::W>(dst + turn.at[q], out.vec, u[i][q]);
+          }
+          h += C::R;
+          dst += C::R * out_head;
+        }
+      }
+    };
+    if (a.rot_dim == D) rows(std::true_type());
+    else rows(std::false_type());
   }
 }
 
 // The backward pass: a warp walks over tokens, all heads of each, and keeps its share of the weights' gradients; the block's
 // sums go to its place in the workspace, in an order that does not depend on timing.
 template <typename T, int D, bool kInter>
-__global__ void __launch_bounds__(kWarps * 32) norm_rope_backward_kernel(const __grid_constant__ Args a) {
-  using C = RowCfg<T, D>;
-  constexpr int E = C::E, W = C::kWords, kAhead = 2;
+__global__ void __launch_bounds__(kWarps * 32, kBackwardBlocks) norm_rope_backward_kernel(const __grid_constant__ Args a, unsigned tokens) {
+  using C = RowCfg<T, D, kBackwardBytes<T>>;
+  constexpr int P = C::P, kAhead = sizeof(T) == 2 ? 4 : 3;
   __shared__ float sums[kWarps][2][D];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / C::L, at = lane % C::L * E;
+  __shared__ unsigned long long turns_of[RA_ROPE_MAX_PAIRS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / C::L;
   let_next_start();
+  load_turns(a, turns_of);
   wait_for_previous();
-  const long long tokens = static_cast<long long>(a.B) * a.S;
-  Turn<T, D, kInter> turn;
+  Turn<T, D, kInter, kBackwardBytes<T>> turn;
   turn.place(a, lane);
-  float dw[2][E];
+  float2 dw[2][2][P / 2];
 #pragma unroll
-  for (int e = 0; e < E; ++e) dw[0][e] = dw[1][e] = 0.f;
-  for (long long token = static_cast<long long>(blockIdx.x) * kWarps + warp; token < tokens;
-       token += static_cast<long long>(gridDim.x) * kWarps) {
-    const int b = static_cast<int>(token / a.S), t = static_cast<int>(token - static_cast<long long>(b) * a.S);
-    turn.angles(a, lane, a.rot_dim ? row_position(a, b, t) : 0);
+  for (int side = 0; side < 2; ++side)
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int e = 0; e < P / 2; ++e) dw[side][q][e] = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int e = 0; e < P / 2; ++e) turn.c[e] = make_float2(1.f, 1.f), turn.s[e] = make_float2(0.f, 0.f);
+  for (unsigned token = blockIdx.x * kWarps + warp; token < tokens; token += gridDim.x * kWarps) {
+    const int b = static_cast<int>(token / a.S), t = static_cast<int>(token - static_cast<unsigned>(b) * a.S);
+    const long long pos = a.rot_dim ? row_position(a, b, t) : 0;
+    bool turned = a.rot_dim == 0;
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
       const int heads = a.heads[side], groups = (heads + C::R - 1) / C::R;
       if (heads == 0) continue;
       const Rows in = a.in[side], dy = a.dy[side], out = a.out[side];
       const bool norm = a.w[side] != nullptr;
-      const T* src = reinterpret_cast<const T*>(in.data) + (norm ? b * in.batch + t * in.row + at : 0);
-      const T* grad = reinterpret_cast<const T*>(dy.data) + b * dy.batch + t * dy.row + at;
-      T* dst = reinterpret_cast<T*>(out.data) + b * out.batch + t * out.row + at;
-      float w[E];
+      const T* src = reinterpret_cast<const T*>(in.data) + (norm ? b * in.batch + t * in.row : 0);
+      const T* grad = reinterpret_cast<const T*>(dy.data) + b * dy.batch + t * dy.row;
+      T* dst = reinterpret_cast<T*>(out.data) + b * out.batch + t * out.row;
+      unsigned ux[kAhead][2][C::W], ug[kAhead][2][C::W];
+      auto load = [&](int g) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) w[e] = norm ? weight_at(a.w[side], a.w_f32, at + e, T()) : 1.f;
-      for (int g = 0; g < groups; g += kAhead) {
-        unsigned ux[kAhead][W], ug[kAhead][W];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          const int h = (g + i) * C::R + sub;
-#pragma unroll
-          for (int j = 0; j < W; ++j) ux[i][j] = ug[i][j] = 0;
-          if (h < heads) {
-            load_words<T, W>(grad + h * dy.head, dy.vec, ug[i]);
-            if (norm) load_words<T, W>(src + h * in.head, in.vec, ux[i]);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
+        for (int i = 0; i < kAhead; ++i) {  // (rows behind the last one are the last one once more)
           if (g + i >= groups) break;
-          const int h = (g + i) * C::R + sub;
-          float x[E], y[E], gr[E];
-          unpack<T, E>(ug[i], y);
-          turn.other(ug[i], y, gr);
+          const int h = min((g + i) * C::R + sub, heads - 1);
 #pragma unroll
-          for (int e = 0; e < E; ++e) gr[e] = turn.turns ? fmaf(y[e], turn.c[e], -gr[e] * turn.s[e]) : y[e];
-          if (norm) {
-            unpack<T, E>(ux[i], x);
-            float sq = 0.f, dot = 0.f;
+          for (int q = 0; q < 2; ++q) {
+            load_piece<T, C::W>(grad + h * dy.head + turn.at[q], dy.vec, ug[i][q]);
+            if (norm) load_piece<T, C::W>(src + h * in.head + turn.at[q], in.vec, ux[i][q]);
+          }
+        }
+      };
+      load(0);  // (on their way while the angles are worked out)
+      float2 w[2][P / 2];
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-              sq = fmaf(x[e], x[e], sq);
-              dot = fmaf(gr[e] * w[e], x[e], dot);
+      for (int q = 0; q < 2; ++q) {
+#pragma unroll
+        for (int e = 0; e < P / 2; ++e) w[q][e] = make_float2(1.f, 1.f);
+        if (norm) load_weights<T, P>(a.w[side], a.w_f32, a.w_vec, turn.at[q], w[q]);
+      }
+      if (!turned) turn.angles(turns_of, lane, pos);
+      turned = true;
+      auto rows = [&](auto all) {
+        constexpr bool kAll = decltype(all)::value;
+        for (int g = 0; g < groups; g += kAhead) {
+          if (g > 0) load(g);
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) {
+            if (g + i >= groups) break;
+            const int h = (g + i) * C::R + sub;
+            float2 y[2][P / 2], gr[2][P / 2];
+            unpack<T, P>(ug[i][0], y[0]);
+            unpack<T, P>(ug[i][1], y[1]);
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+              for (int e = 0; e < P / 2; ++e)  // (the other way round)
+                gr[q][e] = fma2(y[q][e], turn.cos_of(q, e), mul2(turn.template other<kAll>(y, q, e), turn.sin_back(q, e)));
+            if (norm) {
+              float2 x[2][P / 2], gw[2][P / 2], sq2[2], dot2[2];
+              unpack<T, P>(ux[i][0], x[0]);
+              unpack<T, P>(ux[i][1], x[1]);
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+#pragma unroll
+                for (int e = 0; e < P / 2; ++e) {
+                  gw[q][e] = mul2(gr[q][e], w[q][e]);
+                  sq2[q] = e == 0 ? mul2(x[q][e], x[q][e]) : fma2(x[q][e], x[q][e], sq2[q]);
+                  dot2[q] = e == 0 ? mul2(gw[q][e], x[q][e]) : fma2(gw[q][e], x[q][e], dot2[q]);
+                }
+              }
+              const float sq = row_sum<C::L>((sq2[0].x + sq2[0].y) + (sq2[1].x + sq2[1].y));
+              const float dot = row_sum<C::L>((dot2[0].x + dot2[0].y) + (dot2[1].x + dot2[1].y));
+              const float r = rsqrtf(sq * (1.f / D) + a.eps);
+              const float back = -dot * (1.f / D) * r * r;
+              const float2 r2 = make_float2(r, r), back2 = make_float2(back, back);
+              const bool counts = h < heads;
+#pragma unroll
+              for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int e = 0; e < P / 2; ++e) {
+                  if (counts) dw[side][q][e] = fma2(gr[q][e], mul2(x[q][e], r2), dw[side][q][e]);
+                  gr[q][e] = mul2(r2, fma2(x[q][e], back2, gw[q][e]));
+                }
             }
-            sq = row_sum<C::L>(sq);
-            dot = row_sum<C::L>(dot);
-            const float r = rsqrtf(sq * (1.f / D) + a.eps);
-            const float back = dot * (1.f / D) * r * r;
+            if (h < heads) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-              dw[side][e] = fmaf(gr[e], x[e] * r, dw[side][e]);
-              gr[e] = r * (gr[e] * w[e] - x[e] * back);
+              for (int q = 0; q < 2; ++q) {
+                unsigned v[C::W];
+                pack<T, P>(gr[q], v);
+                store_piece<T, C::W>(dst + h * out.head + turn.at[q], out.vec, v);
+              }
             }
           }
-          pack<T, E>(gr, ug[i]);
-          if (h < heads) store_words<T, W>(dst + h * out.head, out.vec, ug[i]);
         }
-      }
+      };
+      if (a.rot_dim == D) rows(std::true_type());
+      else rows(std::false_type());
     }
   }
   if (a.part == nullptr) return;
@@ -387,11 +492,11 @@ __global__ void __launch_bounds__(kWarps * 32) norm_rope_backward_kernel(const _
 #pragma unroll
   for (int side = 0; side < 2; ++side)
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      float v = dw[side][e];
+    for (int e = 0; e < 2 * P; ++e) {
+      float v = e % 2 ? dw[side][e / P][e % P / 2].y : dw[side][e / P][e % P / 2].x;
 #pragma unroll
       for (int i = C::L; i < 32; i *= 2) v += __shfl_xor_sync(0xffffffffu, v, i);
-      if (sub == 0) sums[warp][side][at + e] = v;
+      if (sub == 0) sums[warp][side][turn.at[e / P] + e % P] = v;
     }
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * D; i += kWarps * 32) {
@@ -423,8 +528,6 @@ __global__ void __launch_bounds__(256) weight_grad_kernel(const float* part, int
 
 // ---- host side ----------------------------------------------------------------------
 
-constexpr int kBackwardPerSm = 4;  // blocks of the backward pass on an SM
-
 bool aligned_rows(const ra_rows& r, int es, int batch, int heads, int rows) {
   unsigned long long all = reinterpret_cast<uintptr_t>(r.data);
   if (batch > 1) all |= static_cast<unsigned long long>(r.batch_stride) * es;
@@ -446,7 +549,7 @@ int common_args(Args* a, int* inter, const char* what, int dtype, int batch, int
   RAB_REQUIRE(head_dim == 32 || head_dim == 64 || head_dim == 128 || head_dim == 256, RA_ERR_UNSUPPORTED,
               "%s: unsupported head_dim=%d (supported: 32, 64, 128, 256)", what, head_dim);
   std::memset(a, 0, sizeof(*a));
-  a->B = batch;
+  RAB_REQUIRE(static_cast<long long>(batch) * seq < (1ll << 31), RA_ERR_INVALID, "%s: too many tokens", what);
   a->S = seq;
   a->map = affine_posmap(0, seq);
   a->pos_stride = 1;
@@ -458,6 +561,7 @@ int common_args(Args* a, int* inter, const char* what, int dtype, int batch, int
   a->w[0] = how->q_weight;
   a->w[1] = how->k_weight;
   a->w_f32 = how->weight_dtype == RA_F32;
+  a->w_vec = ((reinterpret_cast<uintptr_t>(how->q_weight) | reinterpret_cast<uintptr_t>(how->k_weight)) & 15u) == 0;
   a->eps = how->eps;
   if (!how->rope) return RA_OK;
   const int rot = how->rope->rot_dim;
@@ -508,18 +612,15 @@ int groups_per_warp(long long tokens, int groups) {
 }
 
 template <bool kPaged>
-int launch_forward(int dtype, int head_dim, int inter, const Args& a, cudaStream_t stream) {
+int launch_forward(int dtype, int head_dim, int inter, const Args& a, unsigned tokens, cudaStream_t stream) {
   return dispatch(dtype, head_dim, inter, [&](auto t, auto d, auto i) -> int {
-    using C = RowCfg<decltype(t), d()>;
+    using C = RowCfg<decltype(t), d(), kForwardBytes>;
     int groups = 0;
     for (int side = 0; side < 3; ++side) groups += (a.heads[side] + C::R - 1) / C::R;
-    const long long tokens = static_cast<long long>(a.B) * a.S;
     if (tokens == 0 || groups == 0) return RA_OK;
     const int per = groups_per_warp(tokens, groups);
-    const long long total = tokens * ((groups + per - 1) / per), blocks = (total + kWarps - 1) / kWarps;
-    RAB_REQUIRE(blocks < (1ll << 31), RA_ERR_INVALID, "norm and rotation: too many rows");
-    RAB_CUDA(launch_overlapped(norm_rope_kernel<decltype(t), d(), i(), kPaged>, dim3(static_cast<unsigned>(blocks)),
-                               dim3(kWarps * 32), 0, stream, a, total, per));
+    RAB_CUDA(launch_overlapped(norm_rope_kernel<decltype(t), d(), i(), kPaged>,
+                               dim3((tokens + kWarps - 1) / kWarps, (groups + per - 1) / per), dim3(kWarps * 32), 0, stream, a, tokens, per));
     return RA_OK;
   });
 }
@@ -588,14 +689,14 @@ int ra_qk_norm_rope(int dtype, const ra_rows* q, const ra_rows* k, const ra_rows
     RAB_REQUIRE(empty || (in[side]->data && out[side]->data), RA_ERR_INVALID, "qk_norm_rope: null argument");
     a.heads[side] = heads[side];
     const int es = dtype == RA_F32 ? 4 : 2;
-    a.in[side] = make_rows(*in[side], es, a.B, heads[side], a.S);
-    a.out[side] = make_rows(*out[side], es, a.B, heads[side], a.S);
+    a.in[side] = make_rows(*in[side], es, shape->batch, heads[side], a.S);
+    a.out[side] = make_rows(*out[side], es, shape->batch, heads[side], a.S);
   }
-  return launch_forward<false>(dtype, shape->head_dim, inter, a, static_cast<cudaStream_t>(stream));
+  return launch_forward<false>(dtype, shape->head_dim, inter, a, static_cast<unsigned>(shape->batch) * a.S, static_cast<cudaStream_t>(stream));
 }
 
 size_t ra_qk_norm_rope_backward_workspace_bytes(int head_dim) {
-  return head_dim > 0 ? static_cast<size_t>(kBackwardPerSm) * sm_count() * 2 * head_dim * sizeof(float) : 0;
+  return head_dim > 0 ? static_cast<size_t>(kBackwardBlocks) * sm_count() * 2 * head_dim * sizeof(float) : 0;
 }
 
 int ra_qk_norm_rope_backward(int dtype, const ra_rows* q, const ra_rows* k, const ra_rows* dq_out, const ra_rows* dk_out,
@@ -624,21 +725,20 @@ int ra_qk_norm_rope_backward(int dtype, const ra_rows* q, const ra_rows* k, cons
                 "%s: null argument", what);
     a.heads[side] = heads[side];
     const int es = dtype == RA_F32 ? 4 : 2;
-    if (a.w[side]) a.in[side] = make_rows(*in[side], es, a.B, heads[side], a.S);
-    a.dy[side] = make_rows(*grad[side], es, a.B, heads[side], a.S);
-    a.out[side] = make_rows(*out[side], es, a.B, heads[side], a.S);
+    if (a.w[side]) a.in[side] = make_rows(*in[side], es, shape->batch, heads[side], a.S);
+    a.dy[side] = make_rows(*grad[side], es, shape->batch, heads[side], a.S);
+    a.out[side] = make_rows(*out[side], es, shape->batch, heads[side], a.S);
   }
   const bool want = dq_weight || dk_weight;
   RAB_REQUIRE(!want || (workspace && workspace_bytes >= ra_qk_norm_rope_backward_workspace_bytes(shape->head_dim)),
               RA_ERR_OVERFLOW, "%s: workspace too small", what);
-  const long long tokens = static_cast<long long>(a.B) * a.S;
-  const long long need = (tokens + kWarps - 1) / kWarps;
-  const int blocks = static_cast<int>(std::min<long long>(need, static_cast<long long>(kBackwardPerSm) * sm_count()));
+  const unsigned tokens = static_cast<unsigned>(shape->batch) * a.S;
+  const int blocks = static_cast<int>(std::min<unsigned>((tokens + kWarps - 1) / kWarps, kBackwardBlocks * sm_count()));
   a.part = want ? static_cast<float*>(workspace) : nullptr;
   if (blocks > 0) {
     const int rc2 = dispatch(dtype, shape->head_dim, inter, [&](auto t, auto d, auto i) -> int {
       RAB_CUDA(launch_overlapped(norm_rope_backward_kernel<decltype(t), d(), i()>, dim3(static_cast<unsigned>(blocks)),
-                                 dim3(kWarps * 32), 0, stream, a));
+                                 dim3(kWarps * 32), 0, stream, a, tokens));
       return RA_OK;
     });
     if (rc2 != RA_OK) return rc2;
@@ -664,18 +764,18 @@ int ra_paged_append(const ra_paged_kv* cache, const ra_rows* k, const ra_rows* v
   if (rc == RA_OK) rc = check_paged(*cache, what);
   if (rc != RA_OK) return rc;
   RAB_REQUIRE(!q == !q_out && (!q || heads > 0), RA_ERR_INVALID, "%s: queries without a result, or a result without queries", what);
-  if (a.B == 0 || a.S == 0) return RA_OK;
+  if (cache->batch == 0 || rows == 0) return RA_OK;
   RAB_REQUIRE(k->data && v->data && (!q || (q->data && q_out->data)), RA_ERR_INVALID, "%s: null argument", what);
   const int es = cache->dtype == RA_F32 ? 4 : 2;
   a.heads[1] = a.heads[2] = cache->kv_heads;
-  a.in[1] = make_rows(*k, es, a.B, cache->kv_heads, a.S);
-  a.in[2] = make_rows(*v, es, a.B, cache->kv_heads, a.S);
+  a.in[1] = make_rows(*k, es, cache->batch, cache->kv_heads, rows);
+  a.in[2] = make_rows(*v, es, cache->batch, cache->kv_heads, rows);
   a.out[1] = {static_cast<char*>(cache->k), 0, 0, 0, 1};
   a.out[2] = {static_cast<char*>(cache->v), 0, 0, 0, 1};
   if (q) {
     a.heads[0] = heads;
-    a.in[0] = make_rows(*q, es, a.B, heads, a.S);
-    a.out[0] = make_rows(*q_out, es, a.B, heads, a.S);
+    a.in[0] = make_rows(*q, es, cache->batch, heads, rows);
+    a.out[0] = make_rows(*q_out, es, cache->batch, heads, rows);
   }
   a.lens = cache->lens;
   a.counts = counts;
@@ -684,7 +784,7 @@ int ra_paged_append(const ra_paged_kv* cache, const ra_rows* k, const ra_rows* v
   a.num_pages = cache->num_pages;
   a.max_pages = cache->max_pages;
   a.page_shift = page_shift(cache->page_size);
-  return launch_forward<true>(cache->dtype, cache->head_dim, inter, a, static_cast<cudaStream_t>(stream));
+  return launch_forward<true>(cache->dtype, cache->head_dim, inter, a, static_cast<unsigned>(cache->batch) * a.S, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
