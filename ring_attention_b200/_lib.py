@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libring_attention_b200.so")
@@ -215,6 +216,26 @@ _SIG = {
 }
 
 _lib = None
+
+# Argument structures as bytes (struct.Struct in native layout), which a call of a few microseconds builds faster than ctypes
+# structures.
+PACK_ROWS = struct.Struct("@Pqqq").pack
+PACK_NORM_ROPE = struct.Struct("@PPifPPiPq").pack
+PACK_PAGED_KV = struct.Struct("@iiiiiPPiiqPP").pack
+PACK_SHAPE = struct.Struct("@iiiiii").pack
+_packed = {}
+
+
+def packed(name):
+    """The function ``name`` of the library with addresses or bytes in the place of pointers to structures."""
+    fn = _packed.get(name)
+    if fn is None:
+        fn = lib()[name]
+        res, args = _SIG[name]
+        fn.restype = res
+        fn.argtypes = [_P if a in (_ROWS, C.POINTER(PagedKV), C.POINTER(NormRope), C.POINTER(Shape)) else a for a in args]
+        _packed[name] = fn
+    return fn
 
 
 def lib():

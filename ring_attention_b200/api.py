@@ -15,7 +15,8 @@ import torch
 
 from . import _lib
 from ._lib import (RA_BF16, RA_F16, RA_F32, RA_STEP_CAUSAL, RA_STEP_FINALIZE, RA_STEP_FORCE_SIMT,
-                   RA_STEP_FRESH, NormRope, PagedKV, RingConfig, RingResult, Rope, Rows, SegMap, Shape, check, lib)
+                   RA_STEP_FRESH, PACK_NORM_ROPE, PACK_PAGED_KV, PACK_ROWS, PACK_SHAPE, RingConfig, RingResult, Rope, SegMap,
+                   Shape, check, lib, packed)
 
 _DT = {torch.float32: RA_F32, torch.float16: RA_F16, torch.bfloat16: RA_BF16}
 
@@ -493,40 +494,38 @@ def _rows(t, shape, dtype, out=False):
     sb, sh, ss, sd = t.stride()
     if sd != 1:
         raise ValueError("the elements of a row must be contiguous")
-    if out and (sb == 0 and shape[0] > 1 or sh == 0 and shape[1] > 1 or ss == 0 and shape[2] > 1):
+    if out and not (sb and sh and ss) and (sb == 0 and shape[0] > 1 or sh == 0 and shape[1] > 1 or ss == 0 and shape[2] > 1):
         raise ValueError("rows of a result must not share memory")
-    return Rows(t.data_ptr(), sb, sh, ss)
+    return PACK_ROWS(t.data_ptr(), sb, sh, ss)
 
 
 def _int32(t, shape, name):
-    if t.dtype != torch.int32 or t.shape != shape or shape[-1] > 1 and t.stride(-1) != 1:
+    if t.dtype != torch.int32 or t.shape != shape or t.stride(-1) != 1 and shape[-1] > 1:
         raise ValueError(f"{name}: expected an int32 tensor of {tuple(shape)} with contiguous rows")
     return t.data_ptr()
 
 
 def _norm_rope(dtype, B, S, D, q_weight, k_weight, eps, rope, segmap, pos_stride, positions):
     """ra_norm_rope of the arguments that the functions below share."""
-    h = NormRope(eps=eps, pos_stride=pos_stride)
-    w_dtype = None
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is None:
-            continue
-        if w.shape != (D,) or w.stride(0) != 1 or w.dtype not in (dtype, torch.float32) or w_dtype not in (None, w.dtype):
-            raise ValueError(f"{name}: expected {D} contiguous elements, of the rows' dtype or fp32, alike for Q and K")
-        w_dtype = w.dtype
-        setattr(h, name, w.data_ptr())
-    if w_dtype is not None:
-        h.weight_dtype = _DT[w_dtype]
+    w = q_weight if q_weight is not None else k_weight
+    w_dtype = 0
+    if w is not None:
+        for x in (q_weight, k_weight):
+            if x is not None and (x.shape != (D,) or x.stride(0) != 1 or x.dtype != w.dtype):
+                raise ValueError(f"weights: expected {D} contiguous elements, of the rows' dtype or fp32, alike for Q and K")
+        if w.dtype != dtype and w.dtype != torch.float32:
+            raise ValueError(f"weights: expected {D} contiguous elements, of the rows' dtype or fp32, alike for Q and K")
+        w_dtype = _DT[w.dtype]
+    at, of_batch, where = 0, 0, 0
     if rope is not None:
-        h.rope = C.pointer(rope)
         if positions is not None:
             if positions.dim() == 1:
                 positions = positions.unsqueeze(0).expand(B, -1)
-            h.positions = _int32(positions, (B, S), "positions")
-            h.pos_batch_stride = positions.stride(0)
+            at, of_batch = _int32(positions, (B, S), "positions"), positions.stride(0)
         elif segmap is not None:
-            h.segmap = C.pointer(segmap)
-    return h
+            where = C.addressof(segmap)
+    return PACK_NORM_ROPE(q_weight.data_ptr() if q_weight is not None else 0, k_weight.data_ptr() if k_weight is not None else 0,
+                          w_dtype, eps, C.addressof(rope) if rope is not None else 0, where, pos_stride, at, of_batch)
 
 
 def qk_norm_rope(q, k, q_out, k_out, *, q_weight=None, k_weight=None, eps=1e-6, rope=None, segmap=None, pos_stride=1,
@@ -535,21 +534,21 @@ def qk_norm_rope(q, k, q_out, k_out, *, q_weight=None, k_weight=None, eps=1e-6, 
     q_weight)``, ``k_out`` likewise; without a weight no norm, without ``rope`` (a ``Rope``) no rotation. q is (batch, heads,
     seq, head_dim) and k (batch, kv_heads, seq, head_dim), with any strides but contiguous rows, so a transposed view of a
     projection's token-major output goes in as it is; either may be None with its result. Results may be the inputs.
-    Row i is at position ``segmap`` / ``pos_stride`` say (``RingPartition.step_maps``), at ``positions`` ((batch, seq) or (seq,),
-    int32), or at i."""
+    Row i is at the position that ``segmap`` and ``pos_stride`` say (``RingPartition.step_maps``), at ``positions`` ((batch,
+    seq) or (seq,), int32), or at i."""
     one = q if q is not None else k
     if one is None or (q is None) != (q_out is None) or (k is None) != (k_out is None):
         raise ValueError("qk_norm_rope: rows without a result, or a result without rows")
     B, _, S, D = one.shape
     dt = one.dtype
-    H, kvH = (t.shape[1] if t is not None else 0 for t in (q, k))
+    H, kvH = q.shape[1] if q is not None else 0, k.shape[1] if k is not None else 0
     _on_device(q, k, q_out, k_out, q_weight, k_weight, positions)
     if rope is not None and segmap is None and positions is None:
         segmap = SegMap.make([0], S)
     how = _norm_rope(dt, B, S, D, q_weight, k_weight, eps, rope, segmap, pos_stride, positions)
     qs, ks = (B, H, S, D), (B, kvH, S, D)
-    check(lib().ra_qk_norm_rope(_dtype(one), _rows(q, qs, dt), _rows(k, ks, dt), _rows(q_out, qs, dt, True),
-                                _rows(k_out, ks, dt, True), Shape(B, H or 1, S, S, D, kvH), how, _stream()))
+    check(packed("ra_qk_norm_rope")(_dtype(one), _rows(q, qs, dt), _rows(k, ks, dt), _rows(q_out, qs, dt, True),
+                                    _rows(k_out, ks, dt, True), PACK_SHAPE(B, H or 1, S, S, D, kvH), how, _stream()))
 
 
 def qk_norm_rope_backward(q, k, dq_out, dk_out, dq, dk, *, dq_weight=None, dk_weight=None, q_weight=None, k_weight=None,
@@ -562,7 +561,7 @@ def qk_norm_rope_backward(q, k, dq_out, dk_out, dq, dk, *, dq_weight=None, dk_we
         raise ValueError("qk_norm_rope_backward: a gradient of the result without one of the rows, or the other way round")
     B, _, S, D = one.shape
     dt = one.dtype
-    H, kvH = (t.shape[1] if t is not None else 0 for t in (dq_out, dk_out))
+    H, kvH = dq_out.shape[1] if dq_out is not None else 0, dk_out.shape[1] if dk_out is not None else 0
     _on_device(q, k, dq_out, dk_out, dq, dk, dq_weight, dk_weight, q_weight, k_weight, positions, workspace)
     if rope is not None and segmap is None and positions is None:
         segmap = SegMap.make([0], S)
@@ -574,26 +573,26 @@ def qk_norm_rope_backward(q, k, dq_out, dk_out, dq, dk, *, dq_weight=None, dk_we
                 raise ValueError(f"gradients of weights are {D} contiguous elements in fp32")
             need = lib().ra_qk_norm_rope_backward_workspace_bytes(D)
     if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=one.device)
+        workspace = one.new_empty(need, dtype=torch.uint8)
     qs, ks = (B, H, S, D), (B, kvH, S, D)
-    check(lib().ra_qk_norm_rope_backward(
-        _dtype(one), _rows(q if q_weight is not None else None, qs, dt), _rows(k if k_weight is not None else None, ks, dt),
-        _rows(dq_out, qs, dt), _rows(dk_out, ks, dt), _rows(dq, qs, dt, True), _rows(dk, ks, dt, True), _ptr(dq_weight),
-        _ptr(dk_weight), Shape(B, H or 1, S, S, D, kvH), how, _ptr(workspace) if need else None,
+    check(packed("ra_qk_norm_rope_backward")(
+        _dtype(one), _rows(q, qs, dt) if q_weight is not None else None, _rows(k, ks, dt) if k_weight is not None else None,
+        _rows(dq_out, qs, dt), _rows(dk_out, ks, dt), _rows(dq, qs, dt, True), _rows(dk, ks, dt, True),
+        dq_weight.data_ptr() if dq_weight is not None else None, dk_weight.data_ptr() if dk_weight is not None else None,
+        PACK_SHAPE(B, H or 1, S, S, D, kvH), how, _ptr(workspace) if need else None,
         workspace.numel() * workspace.element_size() if need else 0, _stream()))
 
 
 def _paged_kv(k_pages, v_pages, page_table, lens):
-    """ra_paged_kv of the tensors (see ``paged_append``)."""
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or \
+    """(ra_paged_kv, kv heads, page size, head_dim, batch) of the tensors (see ``paged_append``)."""
+    shape, (B, most) = k_pages.shape, page_table.shape
+    if len(shape) != 4 or shape != v_pages.shape or k_pages.dtype != v_pages.dtype or \
             not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         raise ValueError("k_pages and v_pages: expected contiguous (num_pages, kv_heads, page_size, head_dim) tensors alike")
-    n, kvH, page, D = k_pages.shape
-    if page_table.dim() != 2:
-        raise ValueError("page_table: expected (batch, max_pages)")
-    B, most = page_table.shape
-    return PagedKV(_dtype(k_pages), n, kvH, page, D, k_pages.data_ptr(), v_pages.data_ptr(), B, most, page_table.stride(0),
-                   _int32(page_table, (B, most), "page_table"), _int32(lens, (B,), "lens"))
+    n, kvH, page, D = shape
+    return PACK_PAGED_KV(_dtype(k_pages), n, kvH, page, D, k_pages.data_ptr(), v_pages.data_ptr(), B, most,
+                         page_table.stride(0), _int32(page_table, (B, most), "page_table"),
+                         _int32(lens, (B,), "lens")), kvH, page, D, B
 
 
 def paged_append(k, v, k_pages, v_pages, page_table, lens, *, counts=None, rope=None, positions=None, k_weight=None, q=None,
@@ -607,8 +606,8 @@ def paged_append(k, v, k_pages, v_pages, page_table, lens, *, counts=None, rope=
     B, kvH, T, D = k.shape
     dt = k_pages.dtype
     _on_device(k, v, k_pages, v_pages, page_table, lens, counts, positions, k_weight, q, q_out, q_weight)
-    cache = _paged_kv(k_pages, v_pages, page_table, lens)
-    if (B, kvH, D) != (page_table.shape[0], cache.kv_heads, cache.head_dim):
+    cache, c_heads, _, c_dim, c_batch = _paged_kv(k_pages, v_pages, page_table, lens)
+    if B != c_batch or kvH != c_heads or D != c_dim:
         raise ValueError("paged_append: k does not fit the cache")
     if (q is None) != (q_out is None):
         raise ValueError("paged_append: queries without a result, or a result without queries")
@@ -617,9 +616,9 @@ def paged_append(k, v, k_pages, v_pages, page_table, lens, *, counts=None, rope=
         how = _norm_rope(dt, B, T, D, q_weight, k_weight, eps, rope, None, 1, positions)
     H = q.shape[1] if q is not None else 0
     ks, qs = (B, kvH, T, D), (B, H, T, D)
-    check(lib().ra_paged_append(cache, _rows(k, ks, dt), _rows(v, ks, dt), T,
-                                _int32(counts, (B,), "counts") if counts is not None else None, _rows(q, qs, dt),
-                                _rows(q_out, qs, dt, True), H, how, _stream()))
+    check(packed("ra_paged_append")(cache, _rows(k, ks, dt), _rows(v, ks, dt), T,
+                                    _int32(counts, (B,), "counts") if counts is not None else None, _rows(q, qs, dt),
+                                    _rows(q_out, qs, dt, True), H, how, _stream()))
 
 
 def paged_decode(q, k_pages, v_pages, page_table, lens, out, *, lse=None, shared_pages=None, workspace=None):
@@ -628,17 +627,19 @@ def paged_decode(q, k_pages, v_pages, page_table, lens, out, *, lse=None, shared
     ((batch, heads), fp32) gets the log-sum-exp. A sequence without rows gives zeros and -inf. ``shared_pages`` (int32):
     the pages that every sequence with at least that many rows begins with; they are read once for all of them."""
     _on_device(q, k_pages, v_pages, page_table, lens, out, lse, shared_pages, workspace)
-    cache = _paged_kv(k_pages, v_pages, page_table, lens)
-    if q.dim() != 3 or q.dtype != k_pages.dtype or (q.shape[0], q.shape[2]) != (page_table.shape[0], cache.head_dim):
+    cache, _, page, D, B = _paged_kv(k_pages, v_pages, page_table, lens)
+    shape = q.shape
+    if len(shape) != 3 or q.dtype != k_pages.dtype or shape[0] != B or shape[2] != D:
         raise ValueError("paged_decode: q does not fit the cache")
-    if out.shape != q.shape or out.dtype != q.dtype or \
-            lse is not None and (lse.shape != q.shape[:2] or lse.dtype != torch.float32):
+    H = shape[1]
+    if out.shape != shape or out.dtype != q.dtype or \
+            lse is not None and (lse.shape != (B, H) or lse.dtype != torch.float32):
         raise ValueError("paged_decode: out is like q, lse (batch, heads) in fp32")
-    H, shared_len, pages = q.shape[1], 0, None
+    shared_len, pages = 0, None
     if shared_pages is not None:
-        shared_len = shared_pages.numel() * cache.page_size
-        pages = _int32(shared_pages, (shared_pages.numel(),), "shared_pages")
+        n = shared_pages.numel()
+        shared_len, pages = n * page, _int32(shared_pages, (n,), "shared_pages")
     if workspace is None:
-        workspace = torch.empty(lib().ra_paged_decode_workspace_bytes(cache, H, shared_len), dtype=torch.uint8, device=q.device)
-    check(lib().ra_paged_decode(cache, _ptr(q), H, pages, shared_len, _ptr(out), _ptr(lse), _ptr(workspace),
-                                workspace.numel() * workspace.element_size(), _stream()))
+        workspace = q.new_empty(packed("ra_paged_decode_workspace_bytes")(cache, H, shared_len), dtype=torch.uint8)
+    check(packed("ra_paged_decode")(cache, _ptr(q), H, pages, shared_len, _ptr(out), _ptr(lse), _ptr(workspace),
+                                    workspace.numel() * workspace.element_size(), _stream()))

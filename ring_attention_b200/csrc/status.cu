@@ -1,5 +1,7 @@
 // Thread-local error text, the library version and the per-device status word that
 // bounded device-side waits report into.
+#include <atomic>
+
 #include "common.cuh"
 
 namespace rab {
@@ -69,9 +71,15 @@ int status_after_sync() {
 }
 
 int sm_count() {
+  static std::atomic<int> of_device[64];  // asked once: the question is asked several times a call
   int dev = 0, v = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+  if (cudaGetDevice(&dev) != cudaSuccess) {
     cudaGetLastError();
+    return 148;
+  }
+  if (dev >= 0 && dev < 64 && (v = of_device[dev].load(std::memory_order_relaxed)) > 0) return v;
+  if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) cudaGetLastError();
+  if (v > 0 && dev >= 0 && dev < 64) of_device[dev].store(v, std::memory_order_relaxed);
   return v > 0 ? v : 148;
 }
 

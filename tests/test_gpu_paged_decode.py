@@ -7,6 +7,7 @@ import torch
 from norm_rope_ref import check, default_freqs, forward, rounded
 from paged_ref import table_of, want
 from ring_attention_b200 import api
+from ring_attention_b200._lib import PagedKV
 
 pytestmark = pytest.mark.gpu
 
@@ -236,7 +237,9 @@ def test_the_same_bits_twice_and_on_two_streams_at_once():
 def test_caller_workspace_of_just_the_size(dtype):
     lens = np.array([300, 20, 77])
     p = problem(13, dtype, 3, 8, 2, 64, 16, lens, 1)
-    cache = api._paged_kv(gpu(p[1], dtype), gpu(p[2], dtype), i32(p[3]), i32(lens))
+    pages = gpu(p[1], dtype)
+    n, kvH, page, D = pages.shape
+    cache = PagedKV(api._DT[dtype], n, kvH, page, D, pages.data_ptr(), pages.data_ptr(), 3, p[3].shape[1], p[3].shape[1], 1, 1)
     need = api.lib().ra_paged_decode_workspace_bytes(cache, 8, 16)
     room = torch.full((need + 256,), 0xFF, dtype=torch.uint8, device="cuda")
     compare(dtype, *p[:4], lens, p[4], run(dtype, *p[:4], lens, p[4], workspace=room[:need]))

@@ -220,6 +220,12 @@ def test_structures_are_those_of_the_header(tmp_path):
     got = [int(x) for x in subprocess.run([str(tmp_path / "sizes")], capture_output=True, check=True).stdout.split()]
     want = [C.sizeof(s) for s in names.values()] + [getattr(s, f[0]).offset for s in names.values() for f in s._fields_]
     assert got == want
+    # and the packed forms of the same
+    c = PagedKV(1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12)
+    assert _lib.PACK_PAGED_KV(1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12) == bytes(c)
+    assert _lib.PACK_ROWS(1, 2, 3, 4) == bytes(Rows(1, 2, 3, 4)) and _lib.PACK_SHAPE(*range(6)) == bytes(Shape(*range(6)))
+    h = NormRope(1, 2, 3, 0.5, None, None, 4, 5, 6)
+    assert _lib.PACK_NORM_ROPE(1, 2, 3, 0.5, 0, 0, 4, 5, 6) == bytes(h)
 
 
 @pytest.mark.parametrize("interleaved", [False, True])
