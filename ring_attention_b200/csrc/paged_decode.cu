@@ -13,7 +13,9 @@
 // page and 128 bytes of its rows a lane, 128-byte swizzle) into a ring of its own, 192 KB for the warps of an SM. Where a unit
 // ends and the next one's queries come, and where it waits for a copy, the others of the SM run on. us a pass, four sequences of
 // 131072 to 262144 rows (H32/kvH8 D128 fp16) and 256 of 300 to 600: 16-byte cp.async of all threads and a barrier a stage
-// 854; a copying warp to four that meet where a unit ends 502 and 103; so 499 and 80.
+// 854 and more than 120; a copying warp to four that meet where a unit ends 502 and 103; so 500 and 89. A place of the ring is
+// filled again a stage after it was read, so that two stages are on their way and not three: with three the memory
+// is the slower for it (528 and 94).
 //
 // 16-bit caches: both products on mma.sync m16n8k16, the unit's rows as its M rows, as in decode_mma_kernel (decode.cu). fp32:
 // plain multiply-adds, four lanes to a key for the scores, four columns a lane for the sum over V.
@@ -245,7 +247,8 @@ __device__ inline void put4<__nv_bfloat16>(__nv_bfloat16* dst, float4 v) {
 template <typename T, int D, int SR_, int kRows_, int kExtraBytes>
 struct PagedBlock {
   static constexpr int SR = SR_, RU = kRows_;
-  static constexpr int kWarps = D == 256 ? 2 : 4, kThreads = kWarps * 32;
+  static constexpr bool kMany = D == 32 && sizeof(T) == 2;  // a row is 64 bytes: more warps for its instructions
+  static constexpr int kWarps = D == 256 ? 2 : kMany ? 8 : 4, kThreads = kWarps * 32;
   static constexpr bool kBulk = sizeof(T) == 4;
   static constexpr int kBoxes = kBulk || D <= 64 ? 1 : D / 64;
   static constexpr int kRowBytes = kBulk ? D * 4 : kBoxes * 128;  // in shared memory
@@ -262,7 +265,7 @@ struct PagedBlock {
   static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two blocks to an SM");
 };
 
-// A warp's ring: copies run kStages stages ahead of what it computes.
+// A warp's ring: copies run kStages - 1 stages ahead of what it computes.
 template <typename C>
 struct Ring {
   const PagedArgs& a;
@@ -271,31 +274,46 @@ struct Ring {
   StageInfo* info;
   volatile int* gave_up;
   Walk<C::SR> w;         // the next stage to copy
-  int total, per, next = 0, first_st, head;
+  int total, per, next = 0, first_st;
+  int head[C::kStages];  // this lane's page of the next stages, as far as they are looked up (see look_up)
 
-  // A lane's copies: a piece of the stage's rows, a box of one tensor.
-  static_assert(2 * C::kBoxes * ((C::SR + 15) / 16) <= 32, "a copy a lane");
-  __device__ inline int rows() const { return min(1 << a.shift, C::SR); }
+  // A lane's copies: a piece of the stage's rows (two where a stage takes 32 and a page has 16), a box of one tensor.
+  static_assert(C::SR <= 32 && 2 * C::kBoxes * ((C::SR + 15) / 16) <= 32, "a copy a lane");
+  __device__ inline bool halved() const { return C::SR == 32 && a.shift == 4; }
+  __device__ inline int rows() const { return halved() ? 16 : C::SR; }
   // The page of this lane's piece, as the head its rows are in the tensor map; -1 where there is none.
-  __device__ inline int look_up() const {
-    const int piece = static_cast<int>(threadIdx.x & 31) % (C::SR / rows());
-    if (piece * rows() >= w.left()) return -1;
-    const int at = (w.start + w.st * C::SR + piece * rows()) >> a.shift;
+  __device__ inline int look_up(const Walk<C::SR>& w) const {
+    const int first = halved() ? static_cast<int>(threadIdx.x & 1) * 16 : 0;  // row of the piece
+    if (first >= w.left()) return -1;
+    const int at = (w.start + w.st * C::SR + first) >> a.shift;
     const int* const table = w.b < 0 ? a.shared_pages : a.table + w.b * a.table_stride;
     if (at >= (w.b < 0 ? a.shared_len >> a.shift : a.max_pages)) return -1;
     const int page = table[at];
     return page >= 0 && page < a.num_pages ? page * a.kvH + w.kvh : -1;
   }
+  // Looks the first stages up together, so that their copies do not wait for one another's page numbers, and copies them.
   __device__ inline void begin() {
     first_st = w.st;
-    head = look_up();
-    for (int s = 0; s < C::kStages; ++s) copy(s);
+    Walk<C::SR> ahead = w;
+#pragma unroll
+    for (int s = 0; s < C::kStages; ++s) {
+      head[s] = s < total ? look_up(ahead) : -1;
+      if (s + 1 < total) ahead.next(a);
+    }
+#pragma unroll
+    for (int s = 0; s < C::kStages; ++s) copy(s, head[s]);
+    if (next < total) head[0] = look_up(w);
   }
-  // Copies the next stage, if there is one, to a place that is free.
-  __device__ inline void copy(int slot) {
+  // Copies the next stage, if there is one, to a place that is free, and looks the one behind it up.
+  __device__ inline void copy_next(int slot) {
     if (next >= total) return;
-    const int lane = threadIdx.x & 31, pieces = C::SR / rows();
-    const int piece = lane % pieces, box = lane / pieces % C::kBoxes, tensor = lane / pieces / C::kBoxes;
+    copy(slot, head[0]);
+    if (next < total) head[0] = look_up(w);
+  }
+  __device__ inline void copy(int slot, int head) {
+    if (next >= total) return;
+    const int lane = threadIdx.x & 31, pieces = halved() ? 2 : 1, at = halved() ? lane >> 1 : lane;
+    const int first = halved() ? (lane & 1) * 16 : 0, box = at % C::kBoxes, tensor = at / C::kBoxes;
     if (w.st == 0) {
       first_st = 0;
       // the warp with a unit's first stage says which shares have parts of it: its own and those that the rest reaches into
@@ -303,7 +321,7 @@ struct Ring {
       if (lane == 0)
         a.unit_parts[w.uid] = make_int2(static_cast<int>(blockIdx.x * C::kWarps + (threadIdx.x >> 5)), 1 + (w.n - here + per - 1) / per);
     }
-    const int row = (w.start + w.st * C::SR + piece * rows()) & ((1 << a.shift) - 1);
+    const int row = (w.start + w.st * C::SR + first) & ((1 << a.shift) - 1);
     const unsigned there = __ballot_sync(0xffffffffu, head >= 0 && lane < pieces);
     if (lane == 0) {
       StageInfo i;
@@ -320,18 +338,15 @@ struct Ring {
     __syncwarp();
     if constexpr (C::kBulk) {
       if (tensor < 2 && head >= 0)
-        tcgen::bulk_load(tiles + (2 * slot + tensor) * C::kTileBytes + piece * rows() * C::kRowBytes,
+        tcgen::bulk_load(tiles + (2 * slot + tensor) * C::kTileBytes + first * C::kRowBytes,
                          static_cast<const unsigned char*>(tensor == 0 ? a.k : a.v) +
                              ((static_cast<size_t>(head) << a.shift) + row) * C::kRowBytes,
                          C::kRowBytes * rows(), full + 8 * slot);
     } else if (tensor < 2 && head >= 0) {
-      tcgen::tma_load_3d(tiles + (2 * slot + tensor) * C::kTileBytes + (box * C::SR + piece * rows()) * 128,
+      tcgen::tma_load_3d(tiles + (2 * slot + tensor) * C::kTileBytes + (box * C::SR + first) * 128,
                          tensor == 0 ? map_k : map_v, full + 8 * slot, box * 64, row, head);
     }
-    if (++next < total) {
-      w.next(a);
-      head = look_up();
-    }
+    if (++next < total) w.next(a);
   }
   // Waits for stage s; false: the warp gives up.
   __device__ inline bool wait(int s) {
@@ -379,7 +394,7 @@ __device__ inline void paged_block(const PagedArgs& a, const CUtensorMap* map_k,
 // ---- 16-bit caches ------------------------------------------------------------------
 
 template <typename T, int D>
-using MmaBlock = PagedBlock<T, D, D <= 64 ? 32 : 16, 16, 0>;
+using MmaBlock = PagedBlock<T, D, D == 64 ? 32 : 16, 16, 0>;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(MmaBlock<T, D>::kThreads, 2)
@@ -407,9 +422,8 @@ __global__ void __launch_bounds__(MmaBlock<T, D>::kThreads, 2)
     const int total = ring.total;
     for (int s = 0; s < total; ++s) {
       const int slot = s % C::kStages;
-      if (!ring.wait(s)) return;
       const StageInfo u = ring.info[slot];
-      if (u.first) {
+      if (u.first) {  // (while the copy is on its way)
         // Q as A fragments: reg0 (row g, k 2tq..), reg1 (row g+8, same k), reg2 / reg3 the same at k+8
         int b0, h0, b1, h1;
         const bool is0 = unit_row<RU>(a, u, g, &b0, &h0), is1 = unit_row<RU>(a, u, g + 8, &b1, &h1);
@@ -427,6 +441,7 @@ __global__ void __launch_bounds__(MmaBlock<T, D>::kThreads, 2)
         m_run[0] = m_run[1] = -INFINITY;
         l_run[0] = l_run[1] = 0.f;  // this lane's share of the row sums
       }
+      if (!ring.wait(s)) return;
 #pragma unroll 1
       for (int key0 = 0; key0 < SR; key0 += 16) {
         const int n_valid = u.keys - key0;  // keys from here on
@@ -506,7 +521,7 @@ __global__ void __launch_bounds__(MmaBlock<T, D>::kThreads, 2)
         if (n_valid < 16) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next copy lands behind those zeros
       }
       __syncwarp();
-      ring.copy(slot);
+      if (s > 0) ring.copy_next((s - 1) % C::kStages);
       if (u.last) {
         const size_t part = (static_cast<size_t>(blockIdx.x) * C::kWarps + warp + u.uid) * a.rs;
 #pragma unroll
@@ -584,9 +599,8 @@ __global__ void __launch_bounds__(F32Cfg<D, kRows>::Block::kThreads, 2) paged_f3
     const int total = ring.total;
     for (int s = 0; s < total; ++s) {
       const int slot = s % C::kStages;
-      if (!ring.wait(s)) return;
       const StageInfo u = ring.info[slot];
-      if (u.first) {
+      if (u.first) {  // (while the copy is on its way)
 #pragma unroll
         for (int r = 0; r < RU; ++r) {
           int b, h;
@@ -600,6 +614,7 @@ __global__ void __launch_bounds__(F32Cfg<D, kRows>::Block::kThreads, 2) paged_f3
         m_run = -INFINITY;
         l_run = 0.f;
       }
+      if (!ring.wait(s)) return;
 #pragma unroll 1
       for (int key0 = 0; key0 < SR; key0 += kKeys) {
         const int n_valid = u.keys - key0;
@@ -695,7 +710,7 @@ __global__ void __launch_bounds__(F32Cfg<D, kRows>::Block::kThreads, 2) paged_f3
         }
       }
       __syncwarp();
-      ring.copy(slot);
+      if (s > 0) ring.copy_next((s - 1) % C::kStages);
       if (u.last) {
         const size_t at = (static_cast<size_t>(blockIdx.x) * C::kWarps + warp + u.uid) * a.rs;
         float l_of = l_run;
@@ -877,8 +892,8 @@ PagedPlan make_plan(const ra_paged_kv& c, int heads, int shared_len) {
   const bool f32 = c.dtype == RA_F32;
   const long long rows_shared = shared_len > 0 ? static_cast<long long>(c.batch) * G : 0;
   p.RU = f32 ? fp32_rows(static_cast<int>(std::max<long long>(std::min<long long>(rows_shared, 8), G))) : 16;
-  p.SR = f32 ? (c.head_dim == 32 ? 32 : c.head_dim == 64 ? 16 : 8) : c.head_dim <= 64 ? 32 : 16;
-  p.warps = c.head_dim == 256 ? 2 : 4;
+  p.SR = f32 ? (c.head_dim == 32 ? 32 : c.head_dim == 64 ? 16 : 8) : c.head_dim == 64 ? 32 : 16;
+  p.warps = c.head_dim == 256 ? 2 : c.head_dim == 32 && !f32 ? 8 : 4;
   p.tc = !f32 && rows_shared > 0 && plan_shared_prefix(c.batch, heads, c.kv_heads, c.head_dim, shared_len, &p.shared);
   p.HB = (G + p.RU - 1) / p.RU;
   p.RB = p.tc ? 0 : static_cast<int>((rows_shared + p.RU - 1) / p.RU);
@@ -926,9 +941,13 @@ int launch_fold(const PagedArgs& a, cudaStream_t stream) {
     return RA_OK;
   };
   using std::integral_constant;
-  constexpr int kSome = 256 / (D / 4) < 8 ? 256 / (D / 4) : 8;
   if (rows * (D / 32) <= 2 * sms) return go(integral_constant<int, 1024>(), integral_constant<int, 128>(), integral_constant<int, 32>());
-  if (rows <= 8 * sms) return go(integral_constant<int, 256>(), integral_constant<int, kSome>(), integral_constant<int, D>());
+  // as many slices as leave the threads of all rows room on the SMs at once
+  constexpr int kMost = 256 / (D / 4);
+  const long long room = sms * 768 / (rows * (D / 4));
+  if (kMost >= 8 && room >= 8) return go(integral_constant<int, 256>(), integral_constant<int, kMost >= 8 ? 8 : 1>(), integral_constant<int, D>());
+  if (room >= 4) return go(integral_constant<int, 256>(), integral_constant<int, 4>(), integral_constant<int, D>());
+  if (room >= 2) return go(integral_constant<int, 256>(), integral_constant<int, 2>(), integral_constant<int, D>());
   return go(integral_constant<int, 256>(), integral_constant<int, 1>(), integral_constant<int, D>());
 }
 
