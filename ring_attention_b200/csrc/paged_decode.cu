@@ -226,21 +226,6 @@ __device__ inline bool unit_row(const PagedArgs& a, const StageInfo& u, int r, i
   return *b < a.B && *h < a.H;
 }
 
-template <typename T>
-__device__ inline void put4(T* dst, float4 v);
-template <>
-__device__ inline void put4<float>(float* dst, float4 v) {
-  *reinterpret_cast<float4*>(dst) = v;
-}
-template <>
-__device__ inline void put4<__half>(__half* dst, float4 v) {
-  *reinterpret_cast<uint2*>(dst) = make_uint2(pack_pair<__half>(v.x, v.y), pack_pair<__half>(v.z, v.w));
-}
-template <>
-__device__ inline void put4<__nv_bfloat16>(__nv_bfloat16* dst, float4 v) {
-  *reinterpret_cast<uint2*>(dst) = make_uint2(pack_pair<__nv_bfloat16>(v.x, v.y), pack_pair<__nv_bfloat16>(v.z, v.w));
-}
-
 // Shared memory of a block of either kernel: the rings of its warps, a stage being SR rows of K and then of V. 16 bits: a tensor's
 // kBoxes boxes of 128 bytes of every row, by tensor maps, 16-byte piece c of a row's box at c ^ (row & 7). fp32: whole rows, one
 // after the other as in the page, by plain bulk copies (boxes of 8 rows and 128 bytes kept TMA busy: 16384 rows of D128 67 us).
@@ -750,22 +735,51 @@ __global__ void __launch_bounds__(F32Cfg<D, kRows>::Block::kThreads, 2) paged_f3
 
 // ---- fold ---------------------------------------------------------------------------
 
-// Parts of the rows that no warp finished, and rows without keys. A row's kCols columns have kCols / 4 threads, four columns each,
-// times kSlices, which take every kSlices-th part; a thread asks for eight parts at a time.
+struct Acc8 {  // eight columns of a row
+  float4 lo, hi;
+};
+__device__ inline Acc8 scaled(float f, const Acc8& a) {
+  return {make_float4(f * a.lo.x, f * a.lo.y, f * a.lo.z, f * a.lo.w), make_float4(f * a.hi.x, f * a.hi.y, f * a.hi.z, f * a.hi.w)};
+}
+__device__ inline void add_scaled(Acc8& s, float f, const Acc8& a) {
+  s.lo.x = fmaf(f, a.lo.x, s.lo.x), s.lo.y = fmaf(f, a.lo.y, s.lo.y), s.lo.z = fmaf(f, a.lo.z, s.lo.z), s.lo.w = fmaf(f, a.lo.w, s.lo.w);
+  s.hi.x = fmaf(f, a.hi.x, s.hi.x), s.hi.y = fmaf(f, a.hi.y, s.hi.y), s.hi.z = fmaf(f, a.hi.z, s.hi.z), s.hi.w = fmaf(f, a.hi.w, s.hi.w);
+}
+__device__ inline float4 shfl4(float4 v, int d) {
+  return make_float4(__shfl_xor_sync(0xffffffffu, v.x, d), __shfl_xor_sync(0xffffffffu, v.y, d), __shfl_xor_sync(0xffffffffu, v.z, d),
+                     __shfl_xor_sync(0xffffffffu, v.w, d));
+}
+
+// Parts of the rows that no warp finished, and rows without keys. A row's kCols columns have kCols / 8 threads, eight columns each,
+// times kSlices, which take every kSlices-th part; a thread asks for eight parts at a time, or, where there are many rows, for four.
 template <typename T, int D, int RU, int kFoldThreads, int kSlices, int kCols>
 __global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const __grid_constant__ PagedArgs a) {
-  constexpr int kVec = kCols / 4, kRowsPer = kFoldThreads / kVec / kSlices, kBatch = 8;
+  constexpr int kVec = kCols / 8, kRowsPer = kFoldThreads / kVec / kSlices, kBatch = kSlices >= 8 ? 8 : 4;
   // slices that sit in one warp meet by shuffles, the others (kGroups of a row) through shared memory
-  constexpr int kInWarp = kSlices < 32 / kVec ? kSlices : kVec < 32 ? 32 / kVec : 1, kGroups = kSlices / kInWarp;
-  __shared__ float4 acc_of[kGroups > 1 ? kFoldThreads / kInWarp : 1];
-  __shared__ float2 ml_of[kGroups > 1 ? kFoldThreads / kVec / kInWarp : 1];
+  constexpr int kInWarp = kSlices < 32 / kVec ? kSlices : 32 / kVec, kGroups = kSlices / kInWarp;
+  __shared__ Acc8 acc_of[kGroups > 1 ? kFoldThreads / kInWarp : 1];
+  __shared__ float m_of[kGroups > 1 ? kFoldThreads / kVec / kInWarp : 1], l_of[kGroups > 1 ? kFoldThreads / kVec / kInWarp : 1];
   let_next_start();
-  const int col = static_cast<int>(blockIdx.y) * kVec + threadIdx.x % kVec, lane_row = threadIdx.x / kVec, slice = lane_row % kSlices;
+  const int col = (static_cast<int>(blockIdx.y) * kVec + threadIdx.x % kVec) * 8, lane_row = threadIdx.x / kVec, slice = lane_row % kSlices;
   const int row = static_cast<int>(blockIdx.x) * kRowsPer + lane_row / kSlices;
   const bool mine = row < a.B * a.H;
   const int b = mine ? row / a.H : 0, h = mine ? row - b * a.H : 0, kvh = h % a.kvH, g = h / a.kvH;
   const int own_uid = a.kvH * a.RB + (b * a.kvH + kvh) * a.HB + g / RU;
   const int of_all = b * a.G + g, shared_uid = a.RB > 0 ? kvh * a.RB + of_all / RU : own_uid;
+  // the row's first part of the shared pages, and how far the next one is
+  int pre_n = 0;
+  long long pre_lo = 0, pre_step = a.rs;
+  const float2* pre_ml = a.part_ml;
+  const float* pre_o = a.part_o;
+  if (a.shared_ml) {
+    const SharedPlan& s = a.shared;
+    const int tile = s.pack > 1 ? g / s.pack : b / 128 * a.G + g, at = s.pack > 1 ? g % s.pack * a.B + b : b % 128;
+    pre_step = s.tiles_per_block * 128;
+    pre_lo = (static_cast<long long>(kvh) * s.blocks + tile / s.tiles_per_block) * s.shares * pre_step + tile % s.tiles_per_block * 128 + at;
+    pre_n = s.shares;
+    pre_ml = a.shared_ml;
+    pre_o = a.shared_o;
+  }
   wait_for_previous();
   const bool lost = *reinterpret_cast<const volatile int*>(a.status) != 0;  // some wait ran out: the rows stay as they are
   const int2 own = a.unit_parts[own_uid], pre = a.unit_parts[shared_uid];
@@ -773,42 +787,29 @@ __global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const __grid_c
   if (mine) own_keys(a, b, &start, &end);
   const int own_n = end > start ? own.y : 0;
   const long long own_lo = (static_cast<long long>(own.x) + own_uid) * a.rs + g % RU;
-  int pre_n = 0;
-  long long pre_lo = 0, pre_step = a.rs;
-  const float2* pre_ml = a.part_ml;
-  const float* pre_o = a.part_o;
-  if (start > 0) {
-    if (a.shared_ml) {
-      const SharedPlan& s = a.shared;
-      const int tile = s.pack > 1 ? g / s.pack : b / 128 * a.G + g, at = s.pack > 1 ? g % s.pack * a.B + b : b % 128;
-      pre_step = s.tiles_per_block * 128;
-      pre_lo = (static_cast<long long>(kvh) * s.blocks + tile / s.tiles_per_block) * s.shares * pre_step +
-               tile % s.tiles_per_block * 128 + at;
-      pre_n = s.shares;
-      pre_ml = a.shared_ml;
-      pre_o = a.shared_o;
-    } else {
-      pre_lo = (static_cast<long long>(pre.x) + shared_uid) * a.rs + of_all % RU;
-      pre_n = pre.y;
-    }
+  if (!a.shared_ml) {
+    pre_lo = (static_cast<long long>(pre.x) + shared_uid) * a.rs + of_all % RU;
+    pre_n = pre.y;
   }
+  if (start == 0) pre_n = 0;
   const bool done = lost || (own_n == 1 && start == 0);  // by the warp that had the unit
   const int parts = mine && !done ? own_n + pre_n : 0;
   float m_all = -INFINITY, l_all = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  Acc8 acc = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
   for (int i0 = slice; i0 < parts; i0 += kSlices * kBatch) {
     float2 ml[kBatch];
-    float4 o[kBatch];
+    Acc8 o[kBatch];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       const int i = i0 + j * kSlices;
       ml[j] = make_float2(-INFINITY, 0.f);
-      o[j] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (i < parts) {
         const bool is_pre = i < pre_n;
         const long long at = is_pre ? pre_lo + i * pre_step : own_lo + static_cast<long long>(i - pre_n) * a.rs;
         ml[j] = (is_pre ? pre_ml : a.part_ml)[at];
-        o[j] = *reinterpret_cast<const float4*>((is_pre ? pre_o : a.part_o) + at * D + col * 4);
+        const float4* const src = reinterpret_cast<const float4*>((is_pre ? pre_o : a.part_o) + at * D + col);
+        o[j].lo = src[0];
+        o[j].hi = src[1];
       }
     }
     float m_new = m_all;
@@ -816,56 +817,72 @@ __global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const __grid_c
     for (int j = 0; j < kBatch; ++j) m_new = fmaxf(m_new, ml[j].x);
     const float f_old = m_all == -INFINITY ? 1.f : ex2(m_all - m_new);
     l_all *= f_old;
-    acc = make_float4(acc.x * f_old, acc.y * f_old, acc.z * f_old, acc.w * f_old);
+    acc = scaled(f_old, acc);
     m_all = m_new;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       if (ml[j].y == 0.f) continue;  // saw nothing, and may have left no O
       const float f = ml[j].x > -INFINITY ? ex2(ml[j].x - m_all) : 1.f;
       l_all += f * ml[j].y;
-      acc.x += f * o[j].x;
-      acc.y += f * o[j].y;
-      acc.z += f * o[j].z;
-      acc.w += f * o[j].w;
+      add_scaled(acc, f, o[j]);
     }
   }
-  auto join = [&](float m, float l, float4 o) {  // of another slice
-    const float m_new = fmaxf(m_all, m);
-    const float f0 = m_all > -INFINITY ? ex2(m_all - m_new) : 1.f, f1 = m > -INFINITY ? ex2(m - m_new) : 1.f;
-    m_all = m_new;
-    l_all = f0 * l_all + f1 * l;
-    acc = make_float4(f0 * acc.x + f1 * o.x, f0 * acc.y + f1 * o.y, f0 * acc.z + f1 * o.z, f0 * acc.w + f1 * o.w);
-  };
+  // the slices of a row: the largest m of all, then plain sums
+  T* const out = static_cast<T*>(a.out) + static_cast<size_t>(row) * D;
+  if constexpr (kSlices > 1) {
+    float m_row = m_all;
 #pragma unroll
-  for (int d = kVec; d < kVec * kInWarp; d *= 2) {
-    const float m = __shfl_xor_sync(0xffffffffu, m_all, d), l = __shfl_xor_sync(0xffffffffu, l_all, d);
-    float4 o;
-    o.x = __shfl_xor_sync(0xffffffffu, acc.x, d);
-    o.y = __shfl_xor_sync(0xffffffffu, acc.y, d);
-    o.z = __shfl_xor_sync(0xffffffffu, acc.z, d);
-    o.w = __shfl_xor_sync(0xffffffffu, acc.w, d);
-    join(m, l, o);
-  }
-  if constexpr (kGroups > 1) {
-    const int at = threadIdx.x % kVec, group = lane_row / kInWarp;  // (a row's groups lie one after the other)
-    if (slice % kInWarp == 0) {
-      acc_of[group * kVec + at] = acc;
-      if (at == 0) ml_of[group] = make_float2(m_all, l_all);
-    }
-    __syncthreads();
-    if (slice == 0) {
+    for (int d = kVec; d < kVec * kInWarp; d *= 2) m_row = fmaxf(m_row, __shfl_xor_sync(0xffffffffu, m_row, d));
+    const int group = lane_row / kInWarp, first_group = lane_row / kSlices * kGroups;  // (a row's groups lie one after the other)
+    if constexpr (kGroups > 1) {
+      if (threadIdx.x % (kVec * kInWarp) == 0) m_of[group] = m_row;
+      __syncthreads();
 #pragma unroll 8
-      for (int i = 1; i < kGroups; ++i) {
-        const float2 ml = ml_of[group + i];
-        join(ml.x, ml.y, acc_of[(group + i) * kVec + at]);
+      for (int k = 0; k < kGroups; ++k) m_row = fmaxf(m_row, m_of[first_group + k]);
+    }
+    const float f = m_all > -INFINITY ? ex2(m_all - m_row) : 1.f;
+    m_all = m_row;
+    l_all *= f;
+    acc = scaled(f, acc);
+#pragma unroll
+    for (int d = kVec; d < kVec * kInWarp; d *= 2) {
+      l_all += __shfl_xor_sync(0xffffffffu, l_all, d);
+      add_scaled(acc, 1.f, {shfl4(acc.lo, d), shfl4(acc.hi, d)});
+    }
+    if constexpr (kGroups > 1) {
+      const int at = threadIdx.x % kVec;
+      if (slice % kInWarp == 0) {
+        acc_of[group * kVec + at] = acc;
+        if (at == 0) l_of[group] = l_all;
       }
+      __syncthreads();
+      if (!mine || done) return;
+      l_all = 0.f;
+#pragma unroll 8
+      for (int k = 0; k < kGroups; ++k) l_all += l_of[first_group + k];
+      const bool any = l_all != 0.f;  // (NaN counts)
+      const float inv = any ? 1.f / l_all : 0.f;
+      const int mine_of = threadIdx.x % (kVec * kSlices);  // the row's threads take a column at a time
+      for (int c = mine_of; c < kCols; c += kVec * kSlices) {
+        float sum = 0.f;
+#pragma unroll 8
+        for (int k = 0; k < kGroups; ++k) sum += reinterpret_cast<const float*>(acc_of)[(first_group + k) * kCols + c];
+        out[static_cast<int>(blockIdx.y) * kCols + c] = static_cast<T>(any ? sum * inv : 0.f);
+      }
+      if (a.lse && blockIdx.y == 0 && mine_of == 0) a.lse[row] = l_all > 0.f ? m_all * kLn2 + logf(l_all) : any ? l_all : -INFINITY;
+      return;
     }
   }
   if (!mine || done || slice != 0) return;
   const bool any = l_all != 0.f;  // (NaN counts)
-  const float inv = 1.f / l_all;
-  put4(static_cast<T*>(a.out) + static_cast<size_t>(row) * D + col * 4,
-       any ? make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f));
+  acc = any ? scaled(1.f / l_all, acc) : Acc8{make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(out + col)[0] = acc.lo;
+    reinterpret_cast<float4*>(out + col)[1] = acc.hi;
+  } else {
+    *reinterpret_cast<uint4*>(out + col) = make_uint4(pack_pair<T>(acc.lo.x, acc.lo.y), pack_pair<T>(acc.lo.z, acc.lo.w),
+                                                      pack_pair<T>(acc.hi.x, acc.hi.y), pack_pair<T>(acc.hi.z, acc.hi.w));
+  }
   if (a.lse && col == 0) a.lse[row] = l_all > 0.f ? m_all * kLn2 + logf(l_all) : any ? l_all : -INFINITY;
 }
 
@@ -929,23 +946,21 @@ int launch_main(int blocks, cudaStream_t stream, const Args&... args) {
 }
 
 // Threads of the fold that share out a row's parts. With few rows the shares of a whole wave may belong to one of them: then 128
-// threads share out a row's parts for 32 columns; eight where there are more rows, one where there are many.
+// threads share out a row's parts for 32 columns; elsewhere as many as leave the threads of all rows room on the SMs at once.
 template <typename T, int D, int RU>
 int launch_fold(const PagedArgs& a, cudaStream_t stream) {
   const long long rows = static_cast<long long>(a.B) * a.H, sms = sm_count();
   auto go = [&](auto threads, auto slices, auto cols) -> int {
     constexpr int kThreads = decltype(threads)::value, kSlices = decltype(slices)::value, kCols = decltype(cols)::value;
-    constexpr int kPer = kThreads / (kCols / 4) / kSlices;
+    constexpr int kPer = kThreads / (kCols / 8) / kSlices;
     RAB_CUDA(launch_overlapped(paged_fold_kernel<T, D, RU, kThreads, kSlices, kCols>,
                                dim3(static_cast<unsigned>((rows + kPer - 1) / kPer), D / kCols), dim3(kThreads), 0, stream, a));
     return RA_OK;
   };
   using std::integral_constant;
-  if (rows * (D / 32) <= 2 * sms) return go(integral_constant<int, 1024>(), integral_constant<int, 128>(), integral_constant<int, 32>());
-  // as many slices as leave the threads of all rows room on the SMs at once
-  constexpr int kMost = 256 / (D / 4);
-  const long long room = sms * 768 / (rows * (D / 4));
-  if (kMost >= 8 && room >= 8) return go(integral_constant<int, 256>(), integral_constant<int, kMost >= 8 ? 8 : 1>(), integral_constant<int, D>());
+  if (rows * (D / 32) <= 2 * sms) return go(integral_constant<int, 512>(), integral_constant<int, 128>(), integral_constant<int, 32>());
+  const long long room = sms * 768 / (rows * (D / 8));
+  if (room >= 8) return go(integral_constant<int, 256>(), integral_constant<int, 8>(), integral_constant<int, D>());
   if (room >= 4) return go(integral_constant<int, 256>(), integral_constant<int, 4>(), integral_constant<int, D>());
   if (room >= 2) return go(integral_constant<int, 256>(), integral_constant<int, 2>(), integral_constant<int, D>());
   return go(integral_constant<int, 256>(), integral_constant<int, 1>(), integral_constant<int, D>());
