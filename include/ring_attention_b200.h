@@ -353,8 +353,8 @@ typedef struct ra_norm_rope {
 
 /* Norms of queries and keys for each head with the position rotation in the same pass: q -> q_out (shape->heads heads) and
  * k -> k_out (kv heads), shape->seq_q = shape->seq_k rows each; q and q_out, or k and k_out, may be NULL. Sums, norms and angles
- * are held in 32 bits and each result is rounded once to dtype. An output is its input (same address and strides) or shares no
- * memory with any row that the call reads. head_dim 32, 64, 128 or 256. */
+ * are held in 32 bits and each result is rounded once to dtype (so the squares of a row have to add up in fp32's range). An
+ * output is its input (same address and strides) or shares no memory with any row that the call reads. head_dim 32, 64, 128 or 256. */
 RA_API int ra_qk_norm_rope(int dtype, const ra_rows* q, const ra_rows* k, const ra_rows* q_out, const ra_rows* k_out,
                            const ra_shape* shape, const ra_norm_rope* how, ra_stream stream);
 
@@ -362,7 +362,7 @@ RA_API int ra_qk_norm_rope(int dtype, const ra_rows* q, const ra_rows* k, const 
  * (rounded once to dtype) and dq_weight, dk_weight of the weights (fp32, head_dim each, overwritten; NULL: not wanted). q and k
  * are needed where there is a weight and may be NULL elsewhere, with the whole side absent if its gradient is. dq may be dq_out
  * or q, dk likewise. The weights' gradients are summed in a fixed order, so the same call gives the same bits.
- * `workspace`: ra_qk_norm_rope_backward_workspace_bytes(head_dim) bytes (needed where a weight's gradient is wanted). */
+ * `workspace`: ra_qk_norm_rope_backward_workspace_bytes(head_dim) bytes, 16-byte aligned (needed where a weight's gradient is wanted). */
 RA_API size_t ra_qk_norm_rope_backward_workspace_bytes(int head_dim);
 RA_API int ra_qk_norm_rope_backward(int dtype, const ra_rows* q, const ra_rows* k, const ra_rows* dq_out,
                                     const ra_rows* dk_out, const ra_rows* dq, const ra_rows* dk, float* dq_weight,
@@ -401,7 +401,9 @@ RA_API int ra_paged_append(const ra_paged_kv* cache, const ra_rows* k, const ra_
  * as ra_attention_decode_step does, and the result once. 16-byte aligned q and out; heads 1 to 4096.
  * shared_pages: the pages of the first shared_len rows (a multiple of page_size; 0: none) of every sequence that has at least
  * that many, as a long common prompt has them. They are read once for all sequences instead of once for each; the tables still
- * have an entry for them, which sequences with fewer rows use.
+ * have an entry for them, which sequences with fewer rows use. shared_len is at most 2^30.
+ * When a device-side wait runs out (ra_device_status tells), rows of out and lse that are not finished yet stay as they are, as
+ * do all rows of later calls until the word is read.
  * `workspace`: ra_paged_decode_workspace_bytes(...) bytes, 16-byte aligned, of this call's launches alone. Lengths, tables
  * and pages are read by the launches: a captured call follows them. */
 RA_API size_t ra_paged_decode_workspace_bytes(const ra_paged_kv* cache, int heads, int shared_len);

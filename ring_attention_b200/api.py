@@ -639,6 +639,8 @@ def paged_decode(q, k_pages, v_pages, page_table, lens, out, *, lse=None, shared
     if shared_pages is not None:
         n = shared_pages.numel()
         shared_len, pages = n * page, _int32(shared_pages, (n,), "shared_pages")
+        if shared_len > 1 << 30:
+            raise ValueError("paged_decode: more than 2^30 shared rows")
     if workspace is None:
         workspace = q.new_empty(packed("ra_paged_decode_workspace_bytes")(cache, H, shared_len), dtype=torch.uint8)
     check(packed("ra_paged_decode")(cache, _ptr(q), H, pages, shared_len, _ptr(out), _ptr(lse), _ptr(workspace),

@@ -540,6 +540,11 @@ Rows make_rows(const ra_rows& r, int es, int batch, int heads, int rows) {
   return {static_cast<char*>(r.data), r.batch_stride, r.head_stride, r.row_stride, aligned_rows(r, es, batch, heads, rows)};
 }
 
+// Rows are read an element at a time where they are not 16-byte aligned, so that elements have to be.
+bool whole_elements(const ra_rows* r, int dtype) {
+  return !r || (reinterpret_cast<uintptr_t>(r->data) & (dtype == RA_F32 ? 3u : 1u)) == 0;
+}
+
 // What the three entry points check alike; fills everything of `a` but rows and pages. `segments`: positions may come from
 // how->segmap.
 int common_args(Args* a, int* inter, const char* what, int dtype, int batch, int seq, int head_dim, const ra_norm_rope* how,
@@ -561,6 +566,9 @@ int common_args(Args* a, int* inter, const char* what, int dtype, int batch, int
   a->w[0] = how->q_weight;
   a->w[1] = how->k_weight;
   a->w_f32 = how->weight_dtype == RA_F32;
+  RAB_REQUIRE(((reinterpret_cast<uintptr_t>(how->q_weight) | reinterpret_cast<uintptr_t>(how->k_weight)) & (a->w_f32 ? 3u : 1u)) == 0 &&
+                  (reinterpret_cast<uintptr_t>(how->positions) & 3u) == 0,
+              RA_ERR_INVALID, "%s: weights or positions are not aligned to their elements", what);
   a->w_vec = ((reinterpret_cast<uintptr_t>(how->q_weight) | reinterpret_cast<uintptr_t>(how->k_weight)) & 15u) == 0;
   a->eps = how->eps;
   if (!how->rope) return RA_OK;
@@ -687,6 +695,8 @@ int ra_qk_norm_rope(int dtype, const ra_rows* q, const ra_rows* k, const ra_rows
     if (!in[side]) continue;
     RAB_REQUIRE(heads[side] > 0, RA_ERR_INVALID, "qk_norm_rope: bad heads");
     RAB_REQUIRE(empty || (in[side]->data && out[side]->data), RA_ERR_INVALID, "qk_norm_rope: null argument");
+    RAB_REQUIRE(whole_elements(in[side], dtype) && whole_elements(out[side], dtype), RA_ERR_INVALID,
+                "qk_norm_rope: rows are not aligned to their elements");
     a.heads[side] = heads[side];
     const int es = dtype == RA_F32 ? 4 : 2;
     a.in[side] = make_rows(*in[side], es, shape->batch, heads[side], a.S);
@@ -723,6 +733,9 @@ int ra_qk_norm_rope_backward(int dtype, const ra_rows* q, const ra_rows* k, cons
     RAB_REQUIRE(!a.w[side] || in[side], RA_ERR_INVALID, "%s: the norm's gradient needs the rows", what);
     RAB_REQUIRE(empty || (grad[side]->data && out[side]->data && (!a.w[side] || in[side]->data)), RA_ERR_INVALID,
                 "%s: null argument", what);
+    RAB_REQUIRE(whole_elements(in[side], dtype) && whole_elements(grad[side], dtype) && whole_elements(out[side], dtype) &&
+                    (reinterpret_cast<uintptr_t>(dw[side]) & 3u) == 0,
+                RA_ERR_INVALID, "%s: rows or gradients are not aligned to their elements", what);
     a.heads[side] = heads[side];
     const int es = dtype == RA_F32 ? 4 : 2;
     if (a.w[side]) a.in[side] = make_rows(*in[side], es, shape->batch, heads[side], a.S);
@@ -730,8 +743,9 @@ int ra_qk_norm_rope_backward(int dtype, const ra_rows* q, const ra_rows* k, cons
     a.out[side] = make_rows(*out[side], es, shape->batch, heads[side], a.S);
   }
   const bool want = dq_weight || dk_weight;
-  RAB_REQUIRE(!want || (workspace && workspace_bytes >= ra_qk_norm_rope_backward_workspace_bytes(shape->head_dim)),
-              RA_ERR_OVERFLOW, "%s: workspace too small", what);
+  RAB_REQUIRE(!want || (workspace && workspace_bytes >= ra_qk_norm_rope_backward_workspace_bytes(shape->head_dim) &&
+                        (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0),
+              RA_ERR_OVERFLOW, "%s: workspace too small or not 16-byte aligned", what);
   const unsigned tokens = static_cast<unsigned>(shape->batch) * a.S;
   const int blocks = static_cast<int>(std::min<unsigned>((tokens + kWarps - 1) / kWarps, kBackwardBlocks * sm_count()));
   a.part = want ? static_cast<float*>(workspace) : nullptr;
@@ -766,6 +780,9 @@ int ra_paged_append(const ra_paged_kv* cache, const ra_rows* k, const ra_rows* v
   RAB_REQUIRE(!q == !q_out && (!q || heads > 0), RA_ERR_INVALID, "%s: queries without a result, or a result without queries", what);
   if (cache->batch == 0 || rows == 0) return RA_OK;
   RAB_REQUIRE(k->data && v->data && (!q || (q->data && q_out->data)), RA_ERR_INVALID, "%s: null argument", what);
+  RAB_REQUIRE(whole_elements(k, cache->dtype) && whole_elements(v, cache->dtype) && whole_elements(q, cache->dtype) &&
+                  whole_elements(q_out, cache->dtype) && (reinterpret_cast<uintptr_t>(counts) & 3u) == 0,
+              RA_ERR_INVALID, "%s: rows or counts are not aligned to their elements", what);
   const int es = cache->dtype == RA_F32 ? 4 : 2;
   a.heads[1] = a.heads[2] = cache->kv_heads;
   a.in[1] = make_rows(*k, es, cache->batch, cache->kv_heads, rows);

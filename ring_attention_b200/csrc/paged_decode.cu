@@ -1005,6 +1005,7 @@ int check_decode(const ra_paged_kv& c, int heads, const int* shared_pages, int s
   RAB_REQUIRE(static_cast<long long>(c.num_pages) * c.kv_heads < (1ll << 31) - 1, RA_ERR_INVALID, "%s: too many pages", what);
   RAB_REQUIRE(shared_len >= 0 && shared_len % c.page_size == 0 && (shared_len == 0 || shared_pages), RA_ERR_INVALID,
               "%s: shared pages are whole: shared_len=%d, page_size=%d", what, shared_len, c.page_size);
+  RAB_REQUIRE(shared_len <= 1 << 30, RA_ERR_INVALID, "%s: shared_len=%d is above 2^30", what, shared_len);
   return RA_OK;
 }
 
@@ -1037,6 +1038,8 @@ int ra_paged_decode(const ra_paged_kv* cache, const void* q, int heads, const in
   RAB_REQUIRE(q && out, RA_ERR_INVALID, "paged_decode: null argument");
   RAB_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0, RA_ERR_INVALID,
               "paged_decode: q and out must be 16-byte aligned");
+  RAB_REQUIRE(((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(shared_pages)) & 3u) == 0, RA_ERR_INVALID,
+              "paged_decode: lse or shared_pages is not aligned to its elements");
   const ra_paged_kv c = without_pages(*cache, &shared_len);
   const PagedPlan p = make_plan(c, heads, shared_len);
   // (a share is counted in 32 bits; tables that name a page over and over could ask for more)

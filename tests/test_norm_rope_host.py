@@ -112,6 +112,13 @@ def test_norm_rope_refusals():
     bad = SegMap.make([0], 8)
     bad.n_seg = 17
     refused(call(h=how(rope=C.pointer(rope), segmap=C.pointer(bad))), 1, "n_seg")
+    # what is not aligned to its elements
+    refused(call(q=rows(P + 1)), 1, "aligned")
+    refused(call(ko=rows(P + 1)), 1, "aligned")
+    refused(call(dtype=0, k=rows(P + 2)), 1, "aligned")
+    refused(call(h=how(q_weight=P + 2, weight_dtype=0)), 1, "aligned")
+    refused(call(h=how(k_weight=P + 1, weight_dtype=1)), 1, "aligned")
+    refused(call(h=how(rope=C.pointer(rope), positions=P + 2)), 1, "aligned")
     # nothing to do
     assert call(s=Shape(0, 4, 8, 8, 64, 2)) == 0
     assert call(q=rows(None), qo=rows(None), s=Shape(2, 4, 0, 0, 64, 2)) == 0
@@ -137,6 +144,11 @@ def test_norm_rope_backward_refusals():
     refused(call(h=w, dwq=P), 6, "workspace")
     refused(call(h=w, dwk=P, ws=P, n=need - 1), 6, "workspace")
     refused(call(q=None, dyq=None, dq=None, h=w, dwq=P, ws=P, n=need), 1, "weight that there is not")
+    refused(call(h=w, dwk=P, ws=P + 4, n=need), 6, "aligned")
+    refused(call(h=w, dwk=P + 2, ws=P, n=need), 1, "aligned")
+    refused(call(h=w, q=rows(P + 1)), 1, "aligned")
+    refused(call(dq=rows(P + 1)), 1, "aligned")
+    refused(call(dtype=0, dyk=rows(P + 2)), 1, "aligned")
     assert call(s=Shape(2, 4, 0, 0, 64, 2)) == 0
 
 
@@ -172,6 +184,12 @@ def test_append_refusals():
     refused(call(q=rows()), 1, "queries")
     refused(call(q=rows(), qo=rows(), heads=0), 1, "queries")
     refused(call(h=how(rope=C.pointer(Rope.make(128)))), 1, "rot_dim")
+    refused(call(k=rows(P + 1)), 1, "aligned")
+    refused(call(c=paged(dtype=0), v=rows(P + 2)), 1, "aligned")
+    refused(call(q=rows(), qo=rows(P + 1), heads=2), 1, "aligned")
+    refused(call(c=paged(lens=P + 2)), 1, "aligned")
+    refused(call(c=paged(page_table=P + 1)), 1, "aligned")
+    refused(L.ra_paged_append(paged(), rows(), rows(), 1, P + 2, None, None, 0, None, None), 1, "aligned")
     assert call(n=0) == 0 and call(c=paged(batch=0)) == 0
 
 
@@ -197,6 +215,10 @@ def test_decode_refusals():
     refused(call(heads=1), 1, "heads")
     refused(call(heads=4097), 1, "heads")
     refused(call(c=paged(batch=1 << 23)), 1, "rows")
+    refused(call(pages=P + 2, n=16), 1, "aligned")
+    refused(L.ra_paged_decode(paged(), P, 4, None, 0, P, P + 2, P, 1 << 40, None), 1, "aligned")
+    refused(call(pages=P, n=(1 << 30) + 16), 1, "2^30")
+    assert L.ra_paged_decode_workspace_bytes(paged(), 4, 2 ** 31 - 16) == 0
     refused(call(n=16), 1, "shared")
     refused(call(pages=P, n=17), 1, "whole")
     refused(call(pages=P, n=-16), 1, "whole")
