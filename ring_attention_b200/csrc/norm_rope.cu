@@ -776,6 +776,7 @@ int ra_paged_append(const ra_paged_kv* cache, const ra_rows* k, const ra_rows* v
   int inter = 0;
   int rc = common_args(&a, &inter, what, cache->dtype, cache->batch, rows, cache->head_dim, how, false);
   if (rc == RA_OK) rc = check_paged(*cache, what);
+  if (rc == RA_OK) rc = check_lists(*cache, what);
   if (rc != RA_OK) return rc;
   RAB_REQUIRE(!q == !q_out && (!q || heads > 0), RA_ERR_INVALID, "%s: queries without a result, or a result without queries", what);
   if (cache->batch == 0 || rows == 0) return RA_OK;

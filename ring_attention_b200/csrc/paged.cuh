@@ -29,9 +29,14 @@ inline int check_paged(const ra_paged_kv& c, const char* what) {
   RAB_REQUIRE(((reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) & 15u) == 0, RA_ERR_INVALID,
               "%s: the pages must be 16-byte aligned", what);
   RAB_REQUIRE(c.batch == 0 || (c.lens && (c.page_table || c.max_pages == 0)), RA_ERR_INVALID, "%s: null argument", what);
+  RAB_REQUIRE(c.batch <= 1 || c.table_stride >= 0, RA_ERR_INVALID, "%s: bad stride of the page table", what);
+  return RA_OK;
+}
+
+// (of a call that reads them; the size of a workspace does not depend on where they are)
+inline int check_lists(const ra_paged_kv& c, const char* what) {
   RAB_REQUIRE(((reinterpret_cast<uintptr_t>(c.lens) | reinterpret_cast<uintptr_t>(c.page_table)) & 3u) == 0, RA_ERR_INVALID,
               "%s: lens or page_table is not aligned to its elements", what);
-  RAB_REQUIRE(c.batch <= 1 || c.table_stride >= 0, RA_ERR_INVALID, "%s: bad stride of the page table", what);
   return RA_OK;
 }
 

@@ -66,6 +66,7 @@ struct PagedArgs {
   float* shared_o;
   int* status;
   unsigned long long wait_ns;
+  int missing;  // (test hook: bytes that every stage waits for in vain; 0: none)
 };
 
 // Keys [start, end) of a sequence that its own table holds: behind the shared pages if it has all of them.
@@ -318,7 +319,7 @@ struct Ring {
       i.first = w.st == first_st;
       i.last = ends && first_st == 0 && w.b >= 0 && w.start == 0 ? 2 : ends || next == total - 1;
       info[slot] = i;
-      tcgen::mbar_expect_tx(full + 8 * slot, 2 * C::kRowBytes * rows() * __popc(there));
+      tcgen::mbar_expect_tx(full + 8 * slot, 2 * C::kRowBytes * rows() * __popc(there) + a.missing);
     }
     __syncwarp();
     if constexpr (C::kBulk) {
@@ -359,7 +360,9 @@ __device__ inline void paged_block(const PagedArgs& a, const CUtensorMap* map_k,
   }
   // Behind the kernel of the shared pages, whose blocks let this one begin when all that came before them has completed,
   // nothing waits for that kernel itself but the end: the fold, which waits for this grid, then finds both kernels' parts.
+  // (The fence stands for the wait's other half: no line that this SM holds from before is read as if it were new.)
   if (a.shared_ml == nullptr) wait_for_previous();
+  else __threadfence();
   Ring<C> ring{a, map_k, map_v, base + warp * C::kRingBytes, base + C::kOffBar + warp * C::kStages * 8,
                reinterpret_cast<StageInfo*>(smem + C::kOffInfo) + warp * C::kStages, gave_up};
   ring.total = find_share<C::SR, C::kWarps>(a, warp, &ring.w, &ring.per, reinterpret_cast<ScanRoom<C::kWarps>*>(smem + C::kOffRoom));
@@ -1033,6 +1036,7 @@ int ra_paged_decode(const ra_paged_kv* cache, const void* q, int heads, const in
                     float* lse, void* workspace, size_t workspace_bytes, ra_stream stream_) {
   RAB_REQUIRE(cache != nullptr, RA_ERR_INVALID, "paged_decode: null argument");
   int rc = check_decode(*cache, heads, shared_pages, shared_len);
+  if (rc == RA_OK) rc = check_lists(*cache, "paged_decode");
   if (rc != RA_OK) return rc;
   if (cache->batch == 0) return RA_OK;
   RAB_REQUIRE(q && out, RA_ERR_INVALID, "paged_decode: null argument");
@@ -1079,6 +1083,7 @@ int ra_paged_decode(const ra_paged_kv* cache, const void* q, int heads, const in
   a.status = device_status_ptr();
   RAB_REQUIRE(a.status != nullptr, RA_ERR_CUDA, "paged_decode: no device status word");
   a.wait_ns = tcgen::tc_wait_limit_ns();
+  a.missing = tcgen::tc_stall_after() >= 0 ? 16 : 0;
   if (p.tc) {
     a.shared_ml = reinterpret_cast<float2*>(ws + p.unit_bytes + p.ml_bytes + p.o_bytes);
     a.shared_o = reinterpret_cast<float*>(ws + p.unit_bytes + p.ml_bytes + p.o_bytes + p.shared_ml_bytes);

@@ -283,6 +283,72 @@ def test_norm_rotation_append_and_decode_together(dtype):
                 table, at + 1, (), (out, lse))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_chain_of_steps_with_shared_pages(dtype):
+    """Steps enqueued one behind the other, each of which writes the queries, rows and lengths that the next one reads, with
+    nothing waiting between them: the same bits as step by step."""
+    B, H, kvH, D, page, steps = 6, 8, 2, 128, 32, 30
+    rng = np.random.default_rng(15)
+    shared = np.arange(5)
+    table = np.concatenate([np.tile(shared, (B, 1)), 5 + np.arange(B * 3).reshape(B, 3)], 1)
+    rope = api.Rope.make(D)
+    start = 5 * page + np.array([0, 1, 31, 32, 40, 60])
+    new = [gpu(rng.standard_normal((steps, B, h, 1, D)), dtype) for h in (H, kvH, kvH)]
+    pages = [gpu(rng.standard_normal((5 + 3 * B, kvH, page, D)), dtype) for _ in range(2)]
+    dt, ds = i32(table), i32(shared)
+
+    def chain(wait):
+        k_pages, v_pages = (x.clone() for x in pages)
+        lens, q = i32(start), torch.empty(B, H, 1, D, dtype=dtype, device="cuda")
+        outs = torch.empty(steps, B, H, D, dtype=dtype, device="cuda")
+        for i in range(steps):
+            api.paged_append(new[1][i], new[2][i], k_pages, v_pages, dt, lens, rope=rope, q=new[0][i], q_out=q)
+            lens += 1
+            wait()
+            api.paged_decode(q[:, :, 0], k_pages, v_pages, dt, lens, outs[i], shared_pages=ds)
+            wait()
+        return outs
+
+    slow = chain(torch.cuda.synchronize)
+    for _ in range(3):
+        assert torch.equal(slow, chain(lambda: None))
+
+
+def test_more_sequences_than_the_shared_pages_have_blocks_for():
+    """A batch whose rows on the shared pages are too many for the tensor-core kernel's list of blocks."""
+    B = 5200
+    lens = 16 + np.arange(B) % 5
+    lens[::7] = 15
+    p = problem(16, torch.float16, B, 8, 1, 32, 16, lens, 1)
+    compare(torch.float16, *p[:4], lens, p[4], run(torch.float16, *p[:4], lens, p[4]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n_shared", [0, 40])
+def test_a_wait_that_runs_out_is_reported_and_leaves_the_rows(dtype, n_shared):
+    lens = [40000, 30000]
+    q, k, v, table, shared = problem(17, dtype, 2, 4, 2, 64, 64, np.array(lens), n_shared)
+    args = gpu(q, dtype), gpu(k, dtype), gpu(v, dtype), i32(table), i32(lens)
+    out, lse = torch.full(q.shape, 7, dtype=dtype, device="cuda"), torch.full(q.shape[:2], 7.0, device="cuda")
+    kw = dict(lse=lse, shared_pages=i32(shared) if n_shared else None)
+    L = api.lib()
+    assert api.device_status()[0] == 0
+    L.ra_debug_set_wait_limit_ns(5_000_000)
+    L.ra_debug_stall_producer_after(1)  # keys that never come
+    try:
+        api.paged_decode(*args, out, **kw)
+        torch.cuda.synchronize()
+    finally:
+        L.ra_debug_stall_producer_after(-1)
+        L.ra_debug_set_wait_limit_ns(0)
+    api.paged_decode(*args, out, **kw)  # behind it nothing is computed until the word is read
+    torch.cuda.synchronize()
+    assert (out == 7).all() and (lse == 7).all()
+    assert api.device_status()[0] == 5 and api.device_status()[0] == 0
+    api.paged_decode(*args, out, **kw)
+    compare(dtype, q, k, v, table, lens, shared, (out, lse))
+
+
 def test_decode_wrapper_refusals():
     q = torch.zeros(2, 4, 64, device="cuda")
     p, o = torch.zeros(3, 2, 16, 64, device="cuda"), torch.empty_like(q)
