@@ -371,7 +371,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) norm_rope_kernel(const __grid_
 }
 
 // The backward pass: a warp walks over tokens, all heads of each, and keeps its share of the weights' gradients; the block's
-// sums go to its place in the workspace, in an order that does not depend on timing.
+// sums go to its place in the workspace, in an order that does not depend on timing. us a pass (32768 tokens of 32 heads of 128,
+// bf16; 123 at the copy's rate): 186, where some 217 instructions and two sums over 16 lanes for two rows, of 16 warps an SM, fill 56 %
+// of the issue slots; 16-byte pieces 217, a second set of registers for loads ahead 216, rows through a ring in shared memory 184,
+// which costs fp32 (253) 40 more.
 template <typename T, int D, bool kInter>
 __global__ void __launch_bounds__(kWarps * 32, kBackwardBlocks) norm_rope_backward_kernel(const __grid_constant__ Args a, unsigned tokens) {
   using C = RowCfg<T, D, kBackwardBytes<T>>;
@@ -612,7 +615,8 @@ int dispatch(int dtype, int head_dim, int inter, F f) {
 }
 
 // How many groups of rows a warp takes of a token: all of them where there are tokens enough to fill the SMs with warps, since
-// the angles are then worked out once a token, fewer where there are not.
+// the angles are then worked out once a token, fewer where there are not (16 tokens of 40 heads 6.0 us with all, 2.9 so; 64 into
+// a cache 7.4 and 3.9; 500 tokens, where the rule changes, 6.6 and 6.9).
 int groups_per_warp(long long tokens, int groups) {
   const long long warps = 16ll * sm_count();
   const long long chunks = tokens >= warps ? 1 : (warps + tokens - 1) / tokens;

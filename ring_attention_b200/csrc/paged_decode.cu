@@ -228,8 +228,12 @@ __device__ inline bool unit_row(const PagedArgs& a, const StageInfo& u, int r, i
 }
 
 // Shared memory of a block of either kernel: the rings of its warps, a stage being SR rows of K and then of V. 16 bits: a tensor's
-// kBoxes boxes of 128 bytes of every row, by tensor maps, 16-byte piece c of a row's box at c ^ (row & 7). fp32: whole rows, one
+// kBoxes boxes of 128 bytes of every row, by tensor maps, 16-byte piece c of a row's box at c ^ (row & 7) (rows of 64 bytes: one
+// box of those, c ^ (row / 2 & 3)). fp32: whole rows, one
 // after the other as in the page, by plain bulk copies (boxes of 8 rows and 128 bytes kept TMA busy: 16384 rows of D128 67 us).
+// The shorter a row, the more of them a stage and the more warps, for the instructions around a stage: us a pass, four sequences of
+// 131072 to 262144 rows (H32/kvH8 fp16), head_dim 64 in stages of 16 / 32 rows 324 / 254; head_dim 32 in stages of 16 rows that fill
+// 128 bytes each, four / eight warps 294 / 178, of 32 rows of 64 bytes, eight warps, 138.
 template <typename T, int D, int SR_, int kRows_, int kExtraBytes>
 struct PagedBlock {
   static constexpr int SR = SR_, RU = kRows_;
@@ -237,7 +241,8 @@ struct PagedBlock {
   static constexpr int kWarps = D == 256 ? 2 : kMany ? 8 : 4, kThreads = kWarps * 32;
   static constexpr bool kBulk = sizeof(T) == 4;
   static constexpr int kBoxes = kBulk || D <= 64 ? 1 : D / 64;
-  static constexpr int kRowBytes = kBulk ? D * 4 : kBoxes * 128;  // in shared memory
+  static constexpr int kBoxBytes = D == 32 && !kBulk ? 64 : 128;
+  static constexpr int kRowBytes = kBulk ? D * 4 : kBoxes * kBoxBytes;  // in shared memory
   static constexpr int kTileBytes = SR * kRowBytes;               // per tensor
   static constexpr int kStages = 96 * 1024 / kWarps / (2 * kTileBytes);
   static constexpr int kRingBytes = 2 * kStages * kTileBytes;  // of a warp
@@ -329,7 +334,7 @@ struct Ring {
                              ((static_cast<size_t>(head) << a.shift) + row) * C::kRowBytes,
                          C::kRowBytes * rows(), full + 8 * slot);
     } else if (tensor < 2 && head >= 0) {
-      tcgen::tma_load_3d(tiles + (2 * slot + tensor) * C::kTileBytes + (box * C::SR + first) * 128,
+      tcgen::tma_load_3d(tiles + (2 * slot + tensor) * C::kTileBytes + (box * C::SR + first) * C::kBoxBytes,
                          tensor == 0 ? map_k : map_v, full + 8 * slot, box * 64, row, head);
     }
     if (++next < total) w.next(a);
@@ -382,27 +387,29 @@ __device__ inline void paged_block(const PagedArgs& a, const CUtensorMap* map_k,
 // ---- 16-bit caches ------------------------------------------------------------------
 
 template <typename T, int D>
-using MmaBlock = PagedBlock<T, D, D == 64 ? 32 : 16, 16, 0>;
+using MmaBlock = PagedBlock<T, D, D <= 64 ? 32 : 16, 16, 0>;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(MmaBlock<T, D>::kThreads, 2)
     paged_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                      const __grid_constant__ PagedArgs a) {
   using C = MmaBlock<T, D>;
-  constexpr int SR = C::SR, RU = C::RU;
+  constexpr int SR = C::SR, RU = C::RU, kBoxBytes = C::kBoxBytes, kBoxPieces = kBoxBytes / 16;
   extern __shared__ __align__(1024) unsigned char smem[];
   paged_block<C>(a, &map_k, &map_v, smem, [&](Ring<C>& ring, int warp) {
     const int lane = threadIdx.x & 31;
     const int g = lane >> 2, tq = lane & 3;  // fragment row (and row + 8), column pair
     const int mi = lane >> 3, r8 = lane & 7;
     // a lane's rows of the ldmatrix tiles, and the swizzled offsets of its pieces c = 2 i + (0 or 1) of a box
-    const unsigned k_row = ring.tiles + static_cast<unsigned>((mi >> 1) * 8 + r8) * 128;
-    const unsigned v_row = ring.tiles + static_cast<unsigned>(C::kTileBytes + ((mi & 1) * 8 + r8) * 128);
-    unsigned k_off[4], v_off[4];
+    const unsigned k_row = ring.tiles + static_cast<unsigned>((mi >> 1) * 8 + r8) * kBoxBytes;
+    const unsigned v_row = ring.tiles + static_cast<unsigned>(C::kTileBytes + ((mi & 1) * 8 + r8) * kBoxBytes);
+    constexpr int kSteps = kBoxPieces / 2;  // of 16 columns in a box
+    const int turn = kBoxBytes == 64 ? r8 >> 1 : r8;
+    unsigned k_off[kSteps], v_off[kSteps];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      k_off[i] = ((2 * i + (mi & 1)) ^ r8) << 4;
-      v_off[i] = ((2 * i + (mi >> 1)) ^ r8) << 4;
+    for (int i = 0; i < kSteps; ++i) {
+      k_off[i] = ((2 * i + (mi & 1)) ^ turn) << 4;
+      v_off[i] = ((2 * i + (mi >> 1)) ^ turn) << 4;
     }
     unsigned qa[D / 16][4];
     float o[D / 8][4];
@@ -435,13 +442,13 @@ __global__ void __launch_bounds__(MmaBlock<T, D>::kThreads, 2)
         const int n_valid = u.keys - key0;  // keys from here on
         if (n_valid <= 0) break;
         if (!(u.pages >> (key0 / 16) & 1u)) continue;
-        const unsigned kt = k_row + 2 * slot * C::kTileBytes + key0 * 128, vt = v_row + 2 * slot * C::kTileBytes + key0 * 128;
+        const unsigned kt = k_row + 2 * slot * C::kTileBytes + key0 * kBoxBytes, vt = v_row + 2 * slot * C::kTileBytes + key0 * kBoxBytes;
         if (n_valid < 16) {
           // what a page holds behind the sequence's end has weight 0, but may be anything: out of V's rows with it
           const unsigned v_tile = ring.tiles + (2 * slot + 1) * C::kTileBytes;
-          for (int i = lane; i < (16 - n_valid) * C::kBoxes * 8; i += 32)
+          for (int i = lane; i < (16 - n_valid) * C::kBoxes * kBoxPieces; i += 32)
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
-                             v_tile + (i / 8 % C::kBoxes * SR + key0 + n_valid + i / 8 / C::kBoxes) * 128 + i % 8 * 16),
+                             v_tile + (i / kBoxPieces % C::kBoxes * SR + key0 + n_valid + i / kBoxPieces / C::kBoxes) * kBoxBytes + i % kBoxPieces * 16),
                          "r"(0)
                          : "memory");
           __syncwarp();
@@ -451,7 +458,7 @@ __global__ void __launch_bounds__(MmaBlock<T, D>::kThreads, 2)
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
           unsigned kb[4];
-          ldmatrix_x4(kb, kt + ks / 4 * (SR * 128) + k_off[ks % 4]);
+          ldmatrix_x4(kb, kt + ks / kSteps * (SR * kBoxBytes) + k_off[ks % kSteps]);
           mma16816<T>(s0, qa[ks], kb[0], kb[1]);
           mma16816<T>(s1, qa[ks], kb[2], kb[3]);
         }
@@ -502,7 +509,7 @@ __global__ void __launch_bounds__(MmaBlock<T, D>::kThreads, 2)
 #pragma unroll
         for (int c2 = 0; c2 < D / 16; ++c2) {
           unsigned vb[4];
-          ldmatrix_x4_trans(vb, vt + c2 / 4 * (SR * 128) + v_off[c2 % 4]);
+          ldmatrix_x4_trans(vb, vt + c2 / kSteps * (SR * kBoxBytes) + v_off[c2 % kSteps]);
           mma16816<T>(o[2 * c2], pa, vb[0], vb[1]);
           mma16816<T>(o[2 * c2 + 1], pa, vb[2], vb[3]);
         }
@@ -901,7 +908,7 @@ struct PagedPlan {
   int RU, SR, HB, RB, warps, blocks;  // (warps of a block)
   int rs;       // rows of a part
   double most;  // stages that there can be
-  bool tc;      // shared pages by the tensor-core kernel
+  bool tc;      // shared pages by the tensor-core kernel (32 sequences on 32768 rows, H32/kvH8 D128: 323 us without, 57 with it)
   SharedPlan shared;
   size_t unit_bytes, ml_bytes, o_bytes, shared_ml_bytes, bytes;
 };
@@ -912,7 +919,7 @@ PagedPlan make_plan(const ra_paged_kv& c, int heads, int shared_len) {
   const bool f32 = c.dtype == RA_F32;
   const long long rows_shared = shared_len > 0 ? static_cast<long long>(c.batch) * G : 0;
   p.RU = f32 ? fp32_rows(static_cast<int>(std::max<long long>(std::min<long long>(rows_shared, 8), G))) : 16;
-  p.SR = f32 ? (c.head_dim == 32 ? 32 : c.head_dim == 64 ? 16 : 8) : c.head_dim == 64 ? 32 : 16;
+  p.SR = f32 ? (c.head_dim == 32 ? 32 : c.head_dim == 64 ? 16 : 8) : c.head_dim <= 64 ? 32 : 16;
   p.warps = c.head_dim == 256 ? 2 : c.head_dim == 32 && !f32 ? 8 : 4;
   p.tc = !f32 && rows_shared > 0 && plan_shared_prefix(c.batch, heads, c.kv_heads, c.head_dim, shared_len, &p.shared);
   p.HB = (G + p.RU - 1) / p.RU;
@@ -949,7 +956,9 @@ int launch_main(int blocks, cudaStream_t stream, const Args&... args) {
 }
 
 // Threads of the fold that share out a row's parts. With few rows the shares of a whole wave may belong to one of them: then 128
-// threads share out a row's parts for 32 columns; elsewhere as many as leave the threads of all rows room on the SMs at once.
+// threads share out a row's parts for 32 columns (8 rows, 262144 keys: 58 us without, 33 with); elsewhere as many as leave the
+// threads of all rows room on the SMs at once (one for all / as many: 168 rows of 1531 keys 16.5 / 8.5 us, 1024 rows behind 32768
+// shared ones 58.3 / 53.6, fp32, 192 rows of 16384 keys 104 / 87).
 template <typename T, int D, int RU>
 int launch_fold(const PagedArgs& a, cudaStream_t stream) {
   const long long rows = static_cast<long long>(a.B) * a.H, sms = sm_count();
@@ -978,8 +987,8 @@ int launch_rows(const ra_paged_kv& c, const PagedArgs& a, const PagedPlan& p, cu
     CUtensorMap k, v;
     const long long heads = static_cast<long long>(a.num_pages) * a.kvH, stride = static_cast<long long>(c.page_size) * D;
     const int box = std::min(c.page_size, p.SR);
-    rc = tcgen::make_map(&k, c.dtype, c.k, D, c.page_size, heads, stride, box);
-    if (rc == RA_OK) rc = tcgen::make_map(&v, c.dtype, c.v, D, c.page_size, heads, stride, box);
+    rc = tcgen::make_map(&k, c.dtype, c.k, D, c.page_size, heads, stride, box, MmaBlock<T, D>::kBoxBytes);
+    if (rc == RA_OK) rc = tcgen::make_map(&v, c.dtype, c.v, D, c.page_size, heads, stride, box, MmaBlock<T, D>::kBoxBytes);
     if (rc == RA_OK) rc = launch_main<paged_mma_kernel<T, D>, MmaBlock<T, D>>(p.blocks, stream, k, v, a);
   }
   if (rc != RA_OK) return rc;

@@ -13,14 +13,15 @@
 //   blocks per KV head the grid is turned so that all query blocks of the heads sharing one KV
 //   head run before the next KV head (see launch_cfg).
 //
-// Six forms of the same kernel, tested against each other: P in tensor memory (default) or staged
+// Seven forms of the same kernel, tested against each other: P in tensor memory (default) or staged
 // through shared memory (RA_STEP_P_IN_SMEM); cluster pairs (RA_STEP_CTA_PAIR, head_dim 128 / 256):
 // tcgen05.mma.cta_group::2 with M = 256 over the two blocks of a cluster, each block loading half of
 // every K and V tile; the key split (chosen by shape, pick_key_split): 2 to 8 blocks of a cluster
 // share the key tiles of one query block and merge their states (merge_key_split); the fold (chosen by
-// shape, fold_rows): a block's two query tiles are a head's light and heavy ones instead of neighbours; and
+// shape, fold_rows): a block's two query tiles are a head's light and heavy ones instead of neighbours;
 // the spread form (chosen by shape where the caller gives a workspace, plan_spread): the key tiles of all query tiles in equal
-// shares over the SMs, whose partial states a second kernel folds, and heads with few rows in one query tile.
+// shares over the SMs, whose partial states a second kernel folds, and heads with few rows in one query tile; and that form on the
+// pages that a decode batch shares (launch_shared_prefix), with the sequences as the query rows.
 //
 // Roles inside a block (384 threads)
 //   warp 0        TMA producer: Q tiles once, then K_j, V_j, K_j+1, ... into a shared-memory
@@ -1633,7 +1634,9 @@ bool step_tc_supported(int dtype, const StepArgs& a) {
 }
 
 // Shares of a query block's key tiles, for the least time of the last block: a block costs its tiles and kBlock of prologue and
-// end. As many as fill the SMs once, or twice where more query blocks than SMs want it.
+// end. As many as fill the SMs once, or twice where more query blocks than SMs want it. (Fewer, so that SMs are left to the kernel of
+// the sequences' own rows, gain nothing: 256 sequences on 16384 shared rows and up to 616 more, H32/kvH8 D128, four shares 145 us,
+// three 156, two 193.)
 bool plan_shared_prefix(int B, int H, int kvH, int D, int shared_len, SharedPlan* plan) {
   if (H % kvH != 0) return false;
   const int group = H / kvH, kTiles = D == 256 ? 1 : 2;

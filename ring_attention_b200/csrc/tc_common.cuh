@@ -789,9 +789,9 @@ inline EncodeTiledFn encode_fn() {
 // (D, rows, heads) tensor of 16-bit (RA_F16 / RA_BF16) or 32-bit (RA_F32) elements, box = one
 // 128-byte row piece (64 or 32 elements) x box_rows rows x 1, 128B swizzle. With a box wider than
 // the tensor (head_dim 32 in 16 bits) the upper elements of every row are out of bounds and
-// arrive as zeros, which is exactly a head_dim 64 tile whose upper half is zero.
+// arrive as zeros, which is exactly a head_dim 64 tile whose upper half is zero. box_bytes 64: half as wide, 64B swizzle.
 inline int make_map(CUtensorMap* map, int dtype, const void* base, int D, long long rows,
-                    long long heads, long long head_stride_elems, int box_rows = 128) {
+                    long long heads, long long head_stride_elems, int box_rows = 128, int box_bytes = 128) {
   EncodeTiledFn fn = encode_fn();
   RAB_REQUIRE(fn != nullptr, RA_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   const cuuint64_t es = dtype == RA_F32 ? 4 : 2;
@@ -799,13 +799,13 @@ inline int make_map(CUtensorMap* map, int dtype, const void* base, int D, long l
                               static_cast<cuuint64_t>(heads)};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(D) * es,
                                  static_cast<cuuint64_t>(head_stride_elems) * es};
-  const cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / es), static_cast<cuuint32_t>(box_rows), 1};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_bytes / es), static_cast<cuuint32_t>(box_rows), 1};
   const cuuint32_t estr[3] = {1, 1, 1};
   const CUtensorMapDataType type = dtype == RA_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : dtype == RA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const CUresult r = fn(map, type, 3, const_cast<void*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   RAB_REQUIRE(r == CUDA_SUCCESS, RA_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d",
               static_cast<int>(r));
