@@ -478,18 +478,19 @@ class Ring:
 
 
 def _on_device(*tensors):
-    """Refuses tensors that the kernels of the current device cannot read on its current stream."""
+    """The current device; refuses tensors that its kernels cannot read on its current stream."""
     dev = _current_device()
     for t in tensors:
         if t is not None and t.get_device() != dev:
             raise ValueError("expected tensors of the current CUDA device")
+    return dev
 
 
 def _rows(t, shape, dtype, out=False):
     """ra_rows of a (batch, heads, seq, head_dim) tensor with strides of its own and contiguous elements of a row."""
     if t is None:
         return None
-    if t.shape != shape or t.dtype != dtype:
+    if t.shape != shape or t.dtype is not dtype:
         raise ValueError(f"expected a tensor of {tuple(shape)} in {dtype}, got {tuple(t.shape)} in {t.dtype}")
     sb, sh, ss, sd = t.stride()
     if sd != 1:
@@ -499,8 +500,11 @@ def _rows(t, shape, dtype, out=False):
     return PACK_ROWS(t.data_ptr(), sb, sh, ss)
 
 
+_INT32 = torch.int32
+
+
 def _int32(t, shape, name):
-    if t.dtype != torch.int32 or t.shape != shape or t.stride(-1) != 1 and shape[-1] > 1:
+    if t.dtype is not _INT32 or t.shape != shape or not t.is_contiguous() and t.stride(-1) != 1 and shape[-1] > 1:
         raise ValueError(f"{name}: expected an int32 tensor of {tuple(shape)} with contiguous rows")
     return t.data_ptr()
 
@@ -542,13 +546,13 @@ def qk_norm_rope(q, k, q_out, k_out, *, q_weight=None, k_weight=None, eps=1e-6, 
     B, _, S, D = one.shape
     dt = one.dtype
     H, kvH = q.shape[1] if q is not None else 0, k.shape[1] if k is not None else 0
-    _on_device(q, k, q_out, k_out, q_weight, k_weight, positions)
+    dev = _on_device(q, k, q_out, k_out, q_weight, k_weight, positions)
     if rope is not None and segmap is None and positions is None:
         segmap = SegMap.make([0], S)
     how = _norm_rope(dt, B, S, D, q_weight, k_weight, eps, rope, segmap, pos_stride, positions)
     qs, ks = (B, H, S, D), (B, kvH, S, D)
     check(packed("ra_qk_norm_rope")(_dtype(one), _rows(q, qs, dt), _rows(k, ks, dt), _rows(q_out, qs, dt, True),
-                                    _rows(k_out, ks, dt, True), PACK_SHAPE(B, H or 1, S, S, D, kvH), how, _stream()))
+                                    _rows(k_out, ks, dt, True), PACK_SHAPE(B, H or 1, S, S, D, kvH), how, _raw_stream(dev)))
 
 
 def qk_norm_rope_backward(q, k, dq_out, dk_out, dq, dk, *, dq_weight=None, dk_weight=None, q_weight=None, k_weight=None,
@@ -562,7 +566,7 @@ def qk_norm_rope_backward(q, k, dq_out, dk_out, dq, dk, *, dq_weight=None, dk_we
     B, _, S, D = one.shape
     dt = one.dtype
     H, kvH = dq_out.shape[1] if dq_out is not None else 0, dk_out.shape[1] if dk_out is not None else 0
-    _on_device(q, k, dq_out, dk_out, dq, dk, dq_weight, dk_weight, q_weight, k_weight, positions, workspace)
+    dev = _on_device(q, k, dq_out, dk_out, dq, dk, dq_weight, dk_weight, q_weight, k_weight, positions, workspace)
     if rope is not None and segmap is None and positions is None:
         segmap = SegMap.make([0], S)
     how = _norm_rope(dt, B, S, D, q_weight, k_weight, eps, rope, segmap, pos_stride, positions)
@@ -571,7 +575,7 @@ def qk_norm_rope_backward(q, k, dq_out, dk_out, dq, dk, *, dq_weight=None, dk_we
         if w is not None:
             if w.shape != (D,) or w.dtype != torch.float32 or w.stride(0) != 1:
                 raise ValueError(f"gradients of weights are {D} contiguous elements in fp32")
-            need = lib().ra_qk_norm_rope_backward_workspace_bytes(D)
+            need = need or packed("ra_qk_norm_rope_backward_workspace_bytes")(D)
     if need and workspace is None:
         workspace = one.new_empty(need, dtype=torch.uint8)
     qs, ks = (B, H, S, D), (B, kvH, S, D)
@@ -580,7 +584,7 @@ def qk_norm_rope_backward(q, k, dq_out, dk_out, dq, dk, *, dq_weight=None, dk_we
         _rows(dq_out, qs, dt), _rows(dk_out, ks, dt), _rows(dq, qs, dt, True), _rows(dk, ks, dt, True),
         dq_weight.data_ptr() if dq_weight is not None else None, dk_weight.data_ptr() if dk_weight is not None else None,
         PACK_SHAPE(B, H or 1, S, S, D, kvH), how, _ptr(workspace) if need else None,
-        workspace.numel() * workspace.element_size() if need else 0, _stream()))
+        workspace.nbytes if need else 0, _raw_stream(dev)))
 
 
 def _paged_kv(k_pages, v_pages, page_table, lens):
@@ -605,7 +609,7 @@ def paged_append(k, v, k_pages, v_pages, page_table, lens, *, counts=None, rope=
     the same tokens go to q_out in the same launch. ``lens`` (int32) stays as it is: the caller adds the counts."""
     B, kvH, T, D = k.shape
     dt = k_pages.dtype
-    _on_device(k, v, k_pages, v_pages, page_table, lens, counts, positions, k_weight, q, q_out, q_weight)
+    dev = _on_device(k, v, k_pages, v_pages, page_table, lens, counts, positions, k_weight, q, q_out, q_weight)
     cache, c_heads, _, c_dim, c_batch = _paged_kv(k_pages, v_pages, page_table, lens)
     if B != c_batch or kvH != c_heads or D != c_dim:
         raise ValueError("paged_append: k does not fit the cache")
@@ -618,7 +622,7 @@ def paged_append(k, v, k_pages, v_pages, page_table, lens, *, counts=None, rope=
     ks, qs = (B, kvH, T, D), (B, H, T, D)
     check(packed("ra_paged_append")(cache, _rows(k, ks, dt), _rows(v, ks, dt), T,
                                     _int32(counts, (B,), "counts") if counts is not None else None, _rows(q, qs, dt),
-                                    _rows(q_out, qs, dt, True), H, how, _stream()))
+                                    _rows(q_out, qs, dt, True), H, how, _raw_stream(dev)))
 
 
 def paged_decode(q, k_pages, v_pages, page_table, lens, out, *, lse=None, shared_pages=None, workspace=None):
@@ -626,7 +630,7 @@ def paged_decode(q, k_pages, v_pages, page_table, lens, out, *, lse=None, shared
     head_dim) in the cache's dtype, query head h reads KV head h % kv_heads, sequence b sees its first lens[b] rows. ``lse``
     ((batch, heads), fp32) gets the log-sum-exp. A sequence without rows gives zeros and -inf. ``shared_pages`` (int32):
     the pages that every sequence with at least that many rows begins with; they are read once for all of them."""
-    _on_device(q, k_pages, v_pages, page_table, lens, out, lse, shared_pages, workspace)
+    dev = _on_device(q, k_pages, v_pages, page_table, lens, out, lse, shared_pages, workspace)
     cache, _, page, D, B = _paged_kv(k_pages, v_pages, page_table, lens)
     shape = q.shape
     if len(shape) != 3 or q.dtype != k_pages.dtype or shape[0] != B or shape[2] != D:
@@ -644,4 +648,4 @@ def paged_decode(q, k_pages, v_pages, page_table, lens, out, *, lse=None, shared
     if workspace is None:
         workspace = q.new_empty(packed("ra_paged_decode_workspace_bytes")(cache, H, shared_len), dtype=torch.uint8)
     check(packed("ra_paged_decode")(cache, _ptr(q), H, pages, shared_len, _ptr(out), _ptr(lse), _ptr(workspace),
-                                    workspace.numel() * workspace.element_size(), _stream()))
+                                    workspace.nbytes, _raw_stream(dev)))
