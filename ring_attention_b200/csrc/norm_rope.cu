@@ -6,10 +6,12 @@
 //
 // All of it is bound by memory: a row comes in once and goes out once. A lane holds two 16-byte pieces of a row, in such a place
 // that the elements it turns into one another are its own: with pairs half a row apart, a piece of either half. So 2 to 32
-// lanes share a row, a warp takes several heads of one token at a time, and nothing crosses lanes but the sum of squares. cos and
-// sin of the token's position are worked out once for all heads that the warp takes, from an angle in fixed point (see ra_rope),
-// and multiplied by the weights ahead of the rows: a row then costs a sum of squares and three multiply-adds an element, two
-// elements an instruction.
+// lanes share a row and nothing crosses lanes but the sum of squares. The row groups of a warp take a token each, one head after the
+// other: cos and sin of a token are worked out once for all heads that the warp takes, no lane is idle whatever the heads' number, and
+// the rows of a head lie side by side. (With the warp's row groups on heads of one token, each had its angles over again: us a pass, 32768
+// tokens of 40 heads of 128 in bf16 117, so 109; 804858 tokens of four heads of 32, backward, 967 and 182.) The angles come from
+// fixed point (see ra_rope) and are multiplied by the weights ahead of the rows: a row then costs a sum of squares and three
+// multiply-adds an element, two elements an instruction.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -251,51 +253,59 @@ __device__ inline float row_sum(float v) {
   return v;
 }
 
-// A warp has the rows of kAhead groups on their way; two blocks of eight warps to an SM leave a thread 128 registers. us a pass
-// (32768 tokens of 40 heads of 128, bf16): 117, with three groups 124, three blocks and two groups 122, 8-byte pieces 122.
-// A warp takes `per` groups of R rows of one of the `total` tokens, from the list of q's groups, then k's, then v's.
+// A warp has the rows of kAhead heads on their way; two blocks of eight warps to an SM leave a thread 128 registers. us a pass
+// (32768 tokens of 40 heads of 128, bf16; by one token a warp): 117, with three heads 124, three blocks and two heads 122, 8-byte pieces
+// 122.
+// A warp takes R of the `total` tokens, a row's lanes one of them, and `per` heads of each, from the list of q's heads, then k's,
+// then v's.
 template <typename T, int D, bool kInter, bool kPaged>
 __global__ void __launch_bounds__(kWarps * 32, 2) norm_rope_kernel(const __grid_constant__ Args a, unsigned total, int per) {
   using C = RowCfg<T, D, kForwardBytes>;
   constexpr int P = C::P, kAhead = 4;
   const int lane = threadIdx.x & 31, sub = lane / C::L;
   __shared__ unsigned long long turns_of[RA_ROPE_MAX_PAIRS];
-  const unsigned token = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const unsigned token0 = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * C::R;
   let_next_start();
   load_turns(a, turns_of);
   wait_for_previous();
-  if (token >= total) return;
-  const int b = static_cast<int>(token / a.S), t = static_cast<int>(token - static_cast<unsigned>(b) * a.S);
+  if (token0 >= total) return;
+  const bool there = token0 + sub < total;  // (lanes without a token read the last one's rows, and store nothing)
+  const unsigned token = min(token0 + sub, total - 1);
+  int b = static_cast<int>(token / a.S), t = static_cast<int>(token - static_cast<unsigned>(b) * a.S);
+  bool mine = there;
   long long place = -1;  // paged: row of the cache's first head that takes the token's K and V
   if constexpr (kPaged) {
-    if (a.counts && t >= a.counts[b]) return;
-    place = paged_row(a.table + b * a.table_stride, a.max_pages, a.num_pages, a.page_shift, a.heads[1],
-                      static_cast<long long>(a.lens[b]) + t);
+    if (a.counts) mine = mine && t < a.counts[b];
+    const unsigned some = __ballot_sync(0xffffffffu, mine);
+    if (some == 0) return;
+    // (rows behind a count are not read either)
+    const int from = __ffs(static_cast<int>(some)) - 1, b_from = __shfl_sync(0xffffffffu, b, from), t_from = __shfl_sync(0xffffffffu, t, from);
+    if (!mine) b = b_from, t = t_from;
+    else place = paged_row(a.table + b * a.table_stride, a.max_pages, a.num_pages, a.page_shift, a.heads[1],
+                           static_cast<long long>(a.lens[b]) + t);
   }
   Turn<T, D, kInter, kForwardBytes> turn;
   turn.place(a, lane);
   const long long pos = a.rot_dim ? row_position(a, b, t) : 0;
   const int beg = static_cast<int>(blockIdx.y) * per, end = beg + per;
-  int first = 0;  // group of a side's first row
+  int first = 0;  // place of a side's first head in the list
   bool turned = false;
 #pragma unroll
   for (int side = 0; side < (kPaged ? 3 : 2); ++side) {
-    const int heads = a.heads[side], groups = (heads + C::R - 1) / C::R;
-    const int lo = max(beg - first, 0), hi = min(end - first, groups);
-    first += groups;
-    const bool to_cache = kPaged && side > 0;
-    if (lo >= hi || (to_cache && place < 0)) continue;
+    const int lo = max(beg - first, 0), hi = min(end - first, a.heads[side]);
+    first += a.heads[side];
+    if (lo >= hi) continue;
+    const bool to_cache = kPaged && side > 0, store = to_cache ? place >= 0 : mine;
     const Rows in = a.in[side], out = a.out[side];
     const long long out_head = to_cache ? static_cast<long long>(D) << a.page_shift : out.head;
-    int h = lo * C::R + sub;
     const T* src = reinterpret_cast<const T*>(in.data) + b * in.batch + t * in.row;
-    T* dst = reinterpret_cast<T*>(out.data) + (to_cache ? place * D : b * out.batch + t * out.row) + h * out_head;
+    T* dst = reinterpret_cast<T*>(out.data) + (to_cache ? place * D : b * out.batch + t * out.row) + lo * out_head;
     unsigned u[kAhead][2][C::W];
     auto load = [&](int g) {
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {  // (rows behind the last one are the last one once more)
+      for (int i = 0; i < kAhead; ++i) {
         if (g + i >= hi) break;
-        const T* const row = src + min((g + i) * C::R + sub, heads - 1) * in.head;
+        const T* const row = src + (g + i) * in.head;
 #pragma unroll
         for (int q = 0; q < 2; ++q) load_piece<T, C::W>(row + turn.at[q], in.vec, u[i][q]);
       }
@@ -356,12 +366,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) norm_rope_kernel(const __grid_
               pack<T, P>(y, u[i][q]);
             }
           }
-          if (h < heads) {
+          if (store) {
 #pragma unroll
             for (int q = 0; q < 2; ++q) store_piece<T, C::W>(dst + turn.at[q], out.vec, u[i][q]);
           }
-          h += C::R;
-          dst += C::R * out_head;
+          dst += out_head;
         }
       }
     };
@@ -370,13 +379,13 @@ __global__ void __launch_bounds__(kWarps * 32, 2) norm_rope_kernel(const __grid_
   }
 }
 
-// The backward pass: a warp walks over tokens, all heads of each, and keeps its share of the weights' gradients; the block's
+// The backward pass: a warp walks over units of R tokens and `per` heads of each, `chunks` units to the same tokens, and keeps its share of the weights' gradients; the block's
 // sums go to its place in the workspace, in an order that does not depend on timing. us a pass (32768 tokens of 32 heads of 128,
-// bf16; 123 at the copy's rate): 186, where some 217 instructions and two sums over 16 lanes for two rows, of 16 warps an SM, fill 56 %
-// of the issue slots; 16-byte pieces 217, a second set of registers for loads ahead 216, rows through a ring in shared memory 184,
-// which costs fp32 (253) 40 more.
+// bf16; 123 at the copy's rate): 167, with three heads on their way 174, six 181 (spills), 16-byte pieces 227, three blocks of two heads
+// 229 (both spill); by one token a warp 186, and so with rows through a ring in shared memory 184, which cost fp32 (254) 40 more.
 template <typename T, int D, bool kInter>
-__global__ void __launch_bounds__(kWarps * 32, kBackwardBlocks) norm_rope_backward_kernel(const __grid_constant__ Args a, unsigned tokens) {
+__global__ void __launch_bounds__(kWarps * 32, kBackwardBlocks) norm_rope_backward_kernel(const __grid_constant__ Args a, unsigned tokens, unsigned units,
+                                                                                                 unsigned chunks, int per) {
   using C = RowCfg<T, D, kBackwardBytes<T>>;
   constexpr int P = C::P, kAhead = sizeof(T) == 2 ? 4 : 3;
   __shared__ float sums[kWarps][2][D];
@@ -396,14 +405,20 @@ __global__ void __launch_bounds__(kWarps * 32, kBackwardBlocks) norm_rope_backwa
       for (int e = 0; e < P / 2; ++e) dw[side][q][e] = make_float2(0.f, 0.f);
 #pragma unroll
   for (int e = 0; e < P / 2; ++e) turn.c[e] = make_float2(1.f, 1.f), turn.s[e] = make_float2(0.f, 0.f);
-  for (unsigned token = blockIdx.x * kWarps + warp; token < tokens; token += gridDim.x * kWarps) {
+  for (unsigned unit = blockIdx.x * kWarps + warp; unit < units; unit += gridDim.x * kWarps) {
+    const unsigned of_tokens = unit / chunks, token0 = of_tokens * C::R;
+    const int beg = static_cast<int>(unit - of_tokens * chunks) * per, end = beg + per;
+    const bool mine = token0 + sub < tokens;  // (lanes without a token read the last one's rows, store and sum nothing)
+    const unsigned token = min(token0 + sub, tokens - 1);
     const int b = static_cast<int>(token / a.S), t = static_cast<int>(token - static_cast<unsigned>(b) * a.S);
     const long long pos = a.rot_dim ? row_position(a, b, t) : 0;
     bool turned = a.rot_dim == 0;
+    int first = 0;  // place of a side's first head in the list of q's heads, then k's
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
-      const int heads = a.heads[side], groups = (heads + C::R - 1) / C::R;
-      if (heads == 0) continue;
+      const int lo = max(beg - first, 0), hi = min(end - first, a.heads[side]);
+      first += a.heads[side];
+      if (lo >= hi) continue;
       const Rows in = a.in[side], dy = a.dy[side], out = a.out[side];
       const bool norm = a.w[side] != nullptr;
       const T* src = reinterpret_cast<const T*>(in.data) + (norm ? b * in.batch + t * in.row : 0);
@@ -412,9 +427,9 @@ __global__ void __launch_bounds__(kWarps * 32, kBackwardBlocks) norm_rope_backwa
       unsigned ux[kAhead][2][C::W], ug[kAhead][2][C::W];
       auto load = [&](int g) {
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {  // (rows behind the last one are the last one once more)
-          if (g + i >= groups) break;
-          const int h = min((g + i) * C::R + sub, heads - 1);
+        for (int i = 0; i < kAhead; ++i) {
+          const int h = g + i;
+          if (h >= hi) break;
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             load_piece<T, C::W>(grad + h * dy.head + turn.at[q], dy.vec, ug[i][q]);
@@ -422,7 +437,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBackwardBlocks) norm_rope_backwa
           }
         }
       };
-      load(0);  // (on their way while the angles are worked out)
+      load(lo);  // (on their way while the angles are worked out)
       float2 w[2][P / 2];
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
@@ -434,12 +449,12 @@ __global__ void __launch_bounds__(kWarps * 32, kBackwardBlocks) norm_rope_backwa
       turned = true;
       auto rows = [&](auto all) {
         constexpr bool kAll = decltype(all)::value;
-        for (int g = 0; g < groups; g += kAhead) {
-          if (g > 0) load(g);
+        for (int g = lo; g < hi; g += kAhead) {
+          if (g > lo) load(g);
 #pragma unroll
           for (int i = 0; i < kAhead; ++i) {
-            if (g + i >= groups) break;
-            const int h = (g + i) * C::R + sub;
+            const int h = g + i;
+            if (h >= hi) break;
             float2 y[2][P / 2], gr[2][P / 2];
             unpack<T, P>(ug[i][0], y[0]);
             unpack<T, P>(ug[i][1], y[1]);
@@ -466,16 +481,15 @@ __global__ void __launch_bounds__(kWarps * 32, kBackwardBlocks) norm_rope_backwa
               const float r = rsqrtf(sq * (1.f / D) + a.eps);
               const float back = -dot * (1.f / D) * r * r;
               const float2 r2 = make_float2(r, r), back2 = make_float2(back, back);
-              const bool counts = h < heads;
 #pragma unroll
               for (int q = 0; q < 2; ++q)
 #pragma unroll
                 for (int e = 0; e < P / 2; ++e) {
-                  if (counts) dw[side][q][e] = fma2(gr[q][e], mul2(x[q][e], r2), dw[side][q][e]);
+                  if (mine) dw[side][q][e] = fma2(gr[q][e], mul2(x[q][e], r2), dw[side][q][e]);
                   gr[q][e] = mul2(r2, fma2(x[q][e], back2, gw[q][e]));
                 }
             }
-            if (h < heads) {
+            if (mine) {
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
                 unsigned v[C::W];
@@ -614,25 +628,35 @@ int dispatch(int dtype, int head_dim, int inter, F f) {
   return by_dim(__nv_bfloat16());
 }
 
-// How many groups of rows a warp takes of a token: all of them where there are tokens enough to fill the SMs with warps, since
-// the angles are then worked out once a token, fewer where there are not (16 tokens of 40 heads 6.0 us with all, 2.9 so; 64 into
-// a cache 7.4 and 3.9; 500 tokens, where the rule changes, 6.6 and 6.9).
-int groups_per_warp(long long tokens, int groups) {
+// How many heads of its tokens a warp takes, of `heads`, where `groups` warps have the tokens: for the least time of as many rounds
+// as the warps that the SMs hold at once need, where a warp costs its heads' rows and kAngles rows for its tokens' angles. us: 32768
+// tokens of 40 heads with 40 / 20 (so) / 10 heads a warp 113 / 109 / 120; 500 tokens with 1 / 2 / 3 (so) 8.4 / 6.7 / 5.0; backward of
+// 2 x 1531 tokens of 16 heads of 64 in fp32 with 1 / 3 / 6 (so) 18.0 / 13.8 / 13.3.
+int heads_per_warp(long long groups, int heads) {
+  constexpr int kAngles = 4;
   const long long warps = 16ll * sm_count();
-  const long long chunks = tokens >= warps ? 1 : (warps + tokens - 1) / tokens;
-  return static_cast<int>((groups + chunks - 1) / chunks);
+  if (groups * heads <= warps) return 1;
+  const int most = static_cast<int>(std::min<long long>(heads, 2 * warps / groups + 2));
+  int best = heads;
+  long long least = -1;
+  for (int chunks = 1; chunks <= most; ++chunks) {
+    const int per = (heads + chunks - 1) / chunks;
+    const long long cost = (groups * ((heads + per - 1) / per) + warps - 1) / warps * (kAngles + per);
+    if (least < 0 || cost < least) least = cost, best = per;
+  }
+  return best;
 }
 
 template <bool kPaged>
 int launch_forward(int dtype, int head_dim, int inter, const Args& a, unsigned tokens, cudaStream_t stream) {
   return dispatch(dtype, head_dim, inter, [&](auto t, auto d, auto i) -> int {
     using C = RowCfg<decltype(t), d(), kForwardBytes>;
-    int groups = 0;
-    for (int side = 0; side < 3; ++side) groups += (a.heads[side] + C::R - 1) / C::R;
-    if (tokens == 0 || groups == 0) return RA_OK;
-    const int per = groups_per_warp(tokens, groups);
+    const int heads = a.heads[0] + a.heads[1] + a.heads[2];
+    if (tokens == 0 || heads == 0) return RA_OK;
+    const unsigned groups = (tokens + C::R - 1) / C::R;
+    const int per = heads_per_warp(groups, heads);
     RAB_CUDA(launch_overlapped(norm_rope_kernel<decltype(t), d(), i(), kPaged>,
-                               dim3((tokens + kWarps - 1) / kWarps, (groups + per - 1) / per), dim3(kWarps * 32), 0, stream, a, tokens, per));
+                               dim3((groups + kWarps - 1) / kWarps, static_cast<unsigned>((heads + per - 1) / per)), dim3(kWarps * 32), 0, stream, a, tokens, per));
     return RA_OK;
   });
 }
@@ -751,12 +775,18 @@ int ra_qk_norm_rope_backward(int dtype, const ra_rows* q, const ra_rows* k, cons
                         (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0),
               RA_ERR_OVERFLOW, "%s: workspace too small or not 16-byte aligned", what);
   const unsigned tokens = static_cast<unsigned>(shape->batch) * a.S;
-  const int blocks = static_cast<int>(std::min<unsigned>((tokens + kWarps - 1) / kWarps, kBackwardBlocks * sm_count()));
   a.part = want ? static_cast<float*>(workspace) : nullptr;
-  if (blocks > 0) {
+  int blocks = 0;
+  if (tokens > 0 && a.heads[0] + a.heads[1] > 0) {
     const int rc2 = dispatch(dtype, shape->head_dim, inter, [&](auto t, auto d, auto i) -> int {
+      using C = RowCfg<decltype(t), d(), kBackwardBytes<decltype(t)>>;
+      const int all = a.heads[0] + a.heads[1];
+      const unsigned groups = (tokens + C::R - 1) / C::R;
+      const int per = heads_per_warp(groups, all);
+      const unsigned chunks = static_cast<unsigned>((all + per - 1) / per), units = groups * chunks;
+      blocks = static_cast<int>(std::min<unsigned>((units + kWarps - 1) / kWarps, kBackwardBlocks * sm_count()));
       RAB_CUDA(launch_overlapped(norm_rope_backward_kernel<decltype(t), d(), i()>, dim3(static_cast<unsigned>(blocks)),
-                                 dim3(kWarps * 32), 0, stream, a, tokens));
+                                 dim3(kWarps * 32), 0, stream, a, tokens, units, chunks, per));
       return RA_OK;
     });
     if (rc2 != RA_OK) return rc2;
