@@ -279,7 +279,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) norm_rope_kernel(const __grid_
     const unsigned some = __ballot_sync(0xffffffffu, mine);
     if (some == 0) return;
     // (rows behind a count are not read either)
-    const int from = __ffs(static_cast<int>(some)) - 1, b_from = __shfl_sync(0xffffffffu, b, from), t_from = __shfl_sync(0xffffffffu, t, from);
+    const int from = __ffs(static_cast<int>(some)) - 1;
+    const int b_from = __shfl_sync(0xffffffffu, b, from), t_from = __shfl_sync(0xffffffffu, t, from);
     if (!mine) b = b_from, t = t_from;
     else place = paged_row(a.table + b * a.table_stride, a.max_pages, a.num_pages, a.page_shift, a.heads[1],
                            static_cast<long long>(a.lens[b]) + t);
@@ -379,13 +380,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2) norm_rope_kernel(const __grid_
   }
 }
 
-// The backward pass: a warp walks over units of R tokens and `per` heads of each, `chunks` units to the same tokens, and keeps its share of the weights' gradients; the block's
-// sums go to its place in the workspace, in an order that does not depend on timing. us a pass (32768 tokens of 32 heads of 128,
-// bf16; 123 at the copy's rate): 167, with three heads on their way 174, six 181 (spills), 16-byte pieces 227, three blocks of two heads
-// 229 (both spill); by one token a warp 186, and so with rows through a ring in shared memory 184, which cost fp32 (254) 40 more.
+// The backward pass: a warp walks over units of R tokens and `per` heads of each, `chunks` units to the same tokens, and keeps its
+// share of the weights' gradients; the block's sums go to its place in the workspace, in an order that does not depend on timing.
+// us a pass (32768 tokens of 32 heads of 128, bf16; 123 at the copy's rate): 167, with three heads on their way 174, six 181 (spills),
+// 16-byte pieces 227, three blocks of two heads 229 (both spill); by one token a warp 186, and so with rows through a ring in shared
+// memory 184, which cost fp32 (254) 40 more.
 template <typename T, int D, bool kInter>
-__global__ void __launch_bounds__(kWarps * 32, kBackwardBlocks) norm_rope_backward_kernel(const __grid_constant__ Args a, unsigned tokens, unsigned units,
-                                                                                                 unsigned chunks, int per) {
+__global__ void __launch_bounds__(kWarps * 32, kBackwardBlocks)
+    norm_rope_backward_kernel(const __grid_constant__ Args a, unsigned tokens, unsigned units, unsigned chunks, int per) {
   using C = RowCfg<T, D, kBackwardBytes<T>>;
   constexpr int P = C::P, kAhead = sizeof(T) == 2 ? 4 : 3;
   __shared__ float sums[kWarps][2][D];

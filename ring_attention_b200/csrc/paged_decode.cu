@@ -554,7 +554,8 @@ __global__ void __launch_bounds__(MmaBlock<T, D>::kThreads, 2)
 // one key, and keeps that row's maximum and sum. The weights go through shared memory to the lanes that have the columns of V.
 template <int D, int kRows>
 struct F32Cfg {
-  static constexpr int kWant = kRows == 1 ? 4 : 2 * kRows;
+  // (eight rows: half the exchanges with eight lanes to a key, as far as the registers go: 64 heads on 8, 16384 rows of 128 87 -> 85 us)
+  static constexpr int kWant = kRows == 1 ? 4 : kRows == 8 && D <= 128 ? 8 : 2 * kRows;
   static constexpr int kParts = kWant < D / 4 ? kWant : D / 4;
   static constexpr int kExtraBytes = (8 * 2 + 2) * kRows * 4;  // weights of 8 keys, each twice, and a factor a row, twice
   using Block = PagedBlock<float, D, D == 32 ? 32 : D == 64 ? 16 : 8, kRows, (kExtraBytes + 15) & ~15>;
