@@ -401,8 +401,9 @@ RA_API int ra_paged_append(const ra_paged_kv* cache, const ra_rows* k, const ra_
  * that sees no key gives zeros and -inf. Sums are held in 32 bits; 16-bit caches round the weights of the sum over V to their type,
  * as ra_attention_decode_step does, and the result once. 16-byte aligned q and out; heads 1 to 4096.
  * shared_pages: the pages of the first shared_len rows (a multiple of page_size; 0: none) of every sequence that has at least
- * that many, as a long common prompt has them. They are read once for all sequences instead of once for each; the tables still
- * have an entry for them, which sequences with fewer rows use. shared_len is at most 2^30.
+ * that many, as a long common prompt has them. They are read once for all sequences instead of once for each (but where a small
+ * 16-bit batch is faster with each sequence reading them for itself); the tables still have an entry for them, which sequences
+ * with fewer rows use. shared_len is at most 2^30.
  * When a device-side wait runs out (ra_device_status tells), rows of out and lse that are not finished yet stay as they are, as
  * do all rows of later calls until the word is read.
  * `workspace`: ra_paged_decode_workspace_bytes(...) bytes, 16-byte aligned, of this call's launches alone. Lengths, tables

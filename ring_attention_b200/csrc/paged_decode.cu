@@ -49,7 +49,8 @@ struct PagedArgs {
   long long table_stride;
   const int* lens;
   const int* shared_pages;
-  int shared_len;  // rows in shared pages
+  int shared_len;  // rows in shared pages that are read once for the batch
+  int listed_len;  // or rows that a sequence which has all of them reads from shared_pages instead of its table
   int num_pages, max_pages, shift;
   int B, H, kvH;
   int G;   // heads of a KV head, at most
@@ -89,16 +90,19 @@ struct Walk {
   int b, kvh, hb;  // b = -1: on the shared pages
   int st, n;       // stage of the unit and how many it has
   int start, end;  // its keys
+  int listed;      // so many pages from the list of shared pages
   __device__ inline int shared_stages(const PagedArgs& a) const { return (a.shared_len + SR - 1) / SR; }
   __device__ inline void on_shared(const PagedArgs& a) {
     b = -1;
     start = 0;
     end = a.shared_len;
+    listed = a.shared_len >> a.shift;
     n = shared_stages(a);
   }
   __device__ inline void on_sequence(const PagedArgs& a, int seq) {
     b = seq;
     own_keys(a, b, &start, &end);
+    listed = end >= a.listed_len ? a.listed_len >> a.shift : 0;
     n = static_cast<int>((static_cast<long long>(end) - start + SR - 1) / SR);
   }
   __device__ inline void number(const PagedArgs& a) { uid = b < 0 ? kvh * a.RB + hb : a.kvH * a.RB + (b * a.kvH + kvh) * a.HB + hb; }
@@ -277,9 +281,8 @@ struct Ring {
     const int first = halved() ? static_cast<int>(threadIdx.x & 1) * 16 : 0;  // row of the piece
     if (first >= w.left()) return -1;
     const int at = (w.start + w.st * C::SR + first) >> a.shift;
-    const int* const table = w.b < 0 ? a.shared_pages : a.table + w.b * a.table_stride;
-    if (at >= (w.b < 0 ? a.shared_len >> a.shift : a.max_pages)) return -1;
-    const int page = table[at];
+    if (at >= w.listed && (w.b < 0 || at >= a.max_pages)) return -1;
+    const int page = at < w.listed ? a.shared_pages[at] : a.table[w.b * a.table_stride + at];
     return page >= 0 && page < a.num_pages ? page * a.kvH + w.kvh : -1;
   }
   // Looks the first stages up together, so that their copies do not wait for one another's page numbers, and copies them.
@@ -909,15 +912,24 @@ struct PagedPlan {
   int RU, SR, HB, RB, warps, blocks;  // (warps of a block)
   int rs;       // rows of a part
   double most;  // stages that there can be
+  bool listed;  // shared pages by every sequence for itself, the batch being small
   bool tc;      // shared pages by the tensor-core kernel (32 sequences on 32768 rows, H32/kvH8 D128: 323 us without, 57 with it)
   SharedPlan shared;
   size_t unit_bytes, ml_bytes, o_bytes, shared_ml_bytes, bytes;
 };
 
+// 16 bits: where the batch would read no more than this over again, every sequence reads the shared pages for itself, out of the L2
+// but for the first, and the call has one kernel less in its chain. us on the device, by every sequence / once: H32/kvH8 D128, 2 sequences
+// on 2048 shared rows (8 MB over again) 12.5 / 15.9, on 4096 (17 MB) 14.9 / 17.7, 64 on 64 (17 MB) 12.3 / 16.0, 32 on 256 (33 MB) 13.8 /
+// 13.2; 200 on 512, H16/kvH4 D32 (52 MB) 21.7 / 17.5.
+constexpr double kListedBytes = 28e6;
+
 PagedPlan make_plan(const ra_paged_kv& c, int heads, int shared_len) {
   PagedPlan p = {};
   const int G = (heads + c.kv_heads - 1) / c.kv_heads;
   const bool f32 = c.dtype == RA_F32;
+  p.listed = !f32 && shared_len > 0 && 4.0 * (c.batch - 1) * shared_len * c.kv_heads * c.head_dim <= kListedBytes;
+  if (p.listed) shared_len = 0;
   const long long rows_shared = shared_len > 0 ? static_cast<long long>(c.batch) * G : 0;
   p.RU = f32 ? fp32_rows(static_cast<int>(std::max<long long>(std::min<long long>(rows_shared, 8), G))) : 16;
   p.SR = f32 ? (c.head_dim == 32 ? 32 : c.head_dim == 64 ? 16 : 8) : c.head_dim <= 64 ? 32 : 16;
@@ -1072,7 +1084,8 @@ int ra_paged_decode(const ra_paged_kv* cache, const void* q, int heads, const in
   a.table_stride = c.table_stride;
   a.lens = c.lens;
   a.shared_pages = shared_pages;
-  a.shared_len = shared_len;
+  a.shared_len = p.listed ? 0 : shared_len;
+  a.listed_len = p.listed ? shared_len : 0;
   a.num_pages = c.num_pages;
   a.max_pages = c.max_pages;
   a.shift = page_shift(c.page_size);

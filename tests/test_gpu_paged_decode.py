@@ -284,17 +284,79 @@ def test_norm_rotation_append_and_decode_together(dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-def test_a_chain_of_steps_with_shared_pages(dtype):
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("B,H,kvH,page,n_shared,lens", [
+    (7, 12, 6, 16, 430, [6880, 6881, 7000, 0, 6879, 9000, 6900]), (130, 6, 2, 64, 15, [960 + i % 70 for i in range(130)]),
+    (40, 15, 3, 32, 66, [2112 + 3 * i - 2112 * (i % 9 == 4) for i in range(40)]), (20, 2, 1, 256, 51, [13056 + 20 * i for i in range(20)]),
+    (33, 5, 2, 128, 30, [3840 + i for i in range(33)])])
+def test_shared_pages_of_large_batches_against_64_bits(dtype, D, B, H, kvH, page, n_shared, lens):
+    """Batches that read the shared pages once for all, which small ones in 16 bits do not."""
+    p = problem(B + D, dtype, B, H, kvH, D, page, np.array(lens), n_shared, bad=D in (64, 256))
+    compare(dtype, *p[:4], lens, p[4], run(dtype, *p[:4], lens, p[4]))
+
+
+def test_what_is_not_finite_in_the_pages_of_a_large_batch():
+    dtype, lens, n_shared = torch.float16, [20100, 20033, 20090, 19999], 1250
+    q, k, v, table, shared = problem(10, dtype, 4, 4, 2, 64, 16, np.array(lens), n_shared)
+    q = rounded(np.abs(q) + 0.25, dtype)
+    k[table[2, 20080 // 16], 0, 0] = np.nan
+    k[shared[7], 1, 3] = np.nan
+    table[3, 7] = table[3, 8]  # (the last sequence is shorter than the shared pages: its own table counts)
+    out, lse = run(dtype, q, k, v, table, lens, shared)
+    hit = np.zeros((4, 4), bool)
+    hit[2, 0::2] = True
+    hit[:3, 1::2] = True
+    assert np.array_equal(out.isnan().any(-1).cpu().numpy(), hit) and np.array_equal(lse.isnan().cpu().numpy(), hit)
+    assert out[torch.from_numpy(~hit).cuda()].isfinite().all()
+
+
+def test_captured_calls_of_a_large_batch_follow_lengths():
+    dtype, B, H, kvH, D, page = torch.bfloat16, 5, 8, 2, 128, 16
+    lens = np.array([7500, 77, 0, 7360, 7700])
+    q, k, v, table, shared = problem(11, dtype, B, H, kvH, D, page, lens, 460)
+    dq, dk, dv, dt, dl, ds = gpu(q, dtype), gpu(k, dtype), gpu(v, dtype), i32(table), i32(lens), i32(shared)
+    out, lse = torch.empty_like(dq), torch.empty(B, H, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        api.paged_decode(dq, dk, dv, dt, dl, out, lse=lse, shared_pages=ds)
+    for now in (lens, np.array([7359, 1, 0, 0, 7360]), lens):
+        dl.copy_(i32(now))
+        g.replay()
+        compare(dtype, q, k, v, table, now, shared, (out, lse))
+
+
+def test_large_batches_on_two_streams_at_once():
+    dtype, lens = torch.bfloat16, np.array([6000, 5100, 5500, 1])
+    p = problem(12, dtype, 4, 16, 4, 128, 64, lens, 79)
+    q, k, v = (gpu(x, dtype) for x in p[:3])
+    t, n, s = i32(p[3]), i32(lens), i32(p[4])
+    first = torch.empty_like(q)
+    api.paged_decode(q, k, v, t, n, first, shared_pages=s)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[torch.empty_like(q) for _ in range(8)] for _ in streams]
+    for i in range(8):
+        for st, o in zip(streams, outs):
+            with torch.cuda.stream(st):
+                api.paged_decode(q, k, v, t, n, o[i], shared_pages=s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(first, x) for o in outs for x in o)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n_shared", [5, 190])
+def test_a_chain_of_steps_with_shared_pages(dtype, n_shared):
     """Steps enqueued one behind the other, each of which writes the queries, rows and lengths that the next one reads, with
     nothing waiting between them: the same bits as step by step."""
     B, H, kvH, D, page, steps = 6, 8, 2, 128, 32, 30
     rng = np.random.default_rng(15)
-    shared = np.arange(5)
-    table = np.concatenate([np.tile(shared, (B, 1)), 5 + np.arange(B * 3).reshape(B, 3)], 1)
+    shared = np.arange(n_shared)
+    table = np.concatenate([np.tile(shared, (B, 1)), n_shared + np.arange(B * 3).reshape(B, 3)], 1)
     rope = api.Rope.make(D)
-    start = 5 * page + np.array([0, 1, 31, 32, 40, 60])
+    start = n_shared * page + np.array([0, 1, 31, 32, 40, 60])
     new = [gpu(rng.standard_normal((steps, B, h, 1, D)), dtype) for h in (H, kvH, kvH)]
-    pages = [gpu(rng.standard_normal((5 + 3 * B, kvH, page, D)), dtype) for _ in range(2)]
+    pages = [gpu(rng.standard_normal((n_shared + 3 * B, kvH, page, D)), dtype) for _ in range(2)]
     dt, ds = i32(table), i32(shared)
 
     def chain(wait):
@@ -314,19 +376,20 @@ def test_a_chain_of_steps_with_shared_pages(dtype):
         assert torch.equal(slow, chain(lambda: None))
 
 
-def test_more_sequences_than_the_shared_pages_have_blocks_for():
+@pytest.mark.parametrize("n_shared", [1, 3])
+def test_more_sequences_than_the_shared_pages_have_blocks_for(n_shared):
     """A batch whose rows on the shared pages are too many for the tensor-core kernel's list of blocks."""
     B = 5200
-    lens = 16 + np.arange(B) % 5
+    lens = 16 * n_shared + np.arange(B) % 5
     lens[::7] = 15
-    p = problem(16, torch.float16, B, 8, 1, 32, 16, lens, 1)
+    p = problem(16, torch.float16, B, 8, 1, 32, 16, lens, n_shared)
     compare(torch.float16, *p[:4], lens, p[4], run(torch.float16, *p[:4], lens, p[4]))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("n_shared", [0, 40])
+@pytest.mark.parametrize("n_shared", [0, 40, 960])
 def test_a_wait_that_runs_out_is_reported_and_leaves_the_rows(dtype, n_shared):
-    lens = [40000, 30000]
+    lens = [40000, 30000] if n_shared < 960 else [62000, 61500]
     q, k, v, table, shared = problem(17, dtype, 2, 4, 2, 64, 64, np.array(lens), n_shared)
     args = gpu(q, dtype), gpu(k, dtype), gpu(v, dtype), i32(table), i32(lens)
     out, lse = torch.full(q.shape, 7, dtype=dtype, device="cuda"), torch.full(q.shape[:2], 7.0, device="cuda")
