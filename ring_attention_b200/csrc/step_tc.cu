@@ -1171,7 +1171,9 @@ __global__ void __launch_bounds__((TcCfg<D, kPInTmem, kPair, kSplit, kFold>::kTh
       RowStore<DR>::run(
           lane, a.part_o, part0, __ballot_sync(0xffffffffu, row_valid),
           s_q + w * C::kTileBytes + (warp & 3) * RowStore<DR>::kStageBytes, t_o, n_tiles > 0 && w < live, true, wait_o, [&]() {
-            const bool have = row_valid && n_tiles > 0 && m_ref > -INFINITY;
+            bool have = row_valid && n_tiles > 0 && m_ref > -INFINITY;
+            // (scores of NaN alone set no reference: a decode row that saw them is NaN and not one without keys)
+            if constexpr (kPaged) have = have || (row_valid && n_tiles > 0 && l_run != l_run);
             a.part_ml[part0 + lane] = make_float2(have ? m_ref : -INFINITY, have ? l_run : 0.f);
             return RowOut{have, have, 0.f, 1.f, 1.f};
           });

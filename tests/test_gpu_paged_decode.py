@@ -310,6 +310,24 @@ def test_what_is_not_finite_in_the_pages_of_a_large_batch():
     assert out[torch.from_numpy(~hit).cuda()].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,n_shared", [(32, 2500), (64, 1250), (128, 625), (256, 320)])
+def test_rows_and_shared_pages_of_nothing_but_nan(dtype, D, n_shared):
+    """A query of NaN, of a sequence with no rows but the shared ones and of one with more, gives NaN and not what a row without
+    keys gives; so do shared pages whose every key of a KV head is NaN, so that no share of them has a score."""
+    P = 16 * n_shared
+    lens = [P, P + 33, P + 90, P - 1]
+    q, k, v, table, shared = problem(18, dtype, 4, 4, 2, D, 16, np.array(lens), n_shared)
+    q[:2, 1] = np.nan
+    k[shared, 0] = np.nan
+    out, lse = run(dtype, q, k, v, table, lens, shared)
+    hit = np.zeros((4, 4), bool)
+    hit[:2, 1] = True
+    hit[:, 0::2] = True
+    assert np.array_equal(out.isnan().any(-1).cpu().numpy(), hit) and np.array_equal(lse.isnan().cpu().numpy(), hit)
+    assert out[torch.from_numpy(hit).cuda()].isnan().all()
+    assert out[torch.from_numpy(~hit).cuda()].isfinite().all()
+
 def test_captured_calls_of_a_large_batch_follow_lengths():
     dtype, B, H, kvH, D, page = torch.bfloat16, 5, 8, 2, 128, 16
     lens = np.array([7500, 77, 0, 7360, 7700])
