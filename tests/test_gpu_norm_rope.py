@@ -68,6 +68,34 @@ def test_forward_and_backward(dtype, D, rot, interleaved, norm, B, H, kvH, S):
             check(dw, want, err, torch.float32, "dw")
 
 
+@pytest.mark.parametrize("dtype,D,rot,interleaved,S,w_dtype", [
+    (torch.bfloat16, 128, 128, False, 2001, torch.bfloat16), (torch.float32, 128, 96, False, 2001, torch.float32),
+    (torch.float16, 32, 32, True, 6667, torch.float32), (torch.bfloat16, 64, 32, True, 3335, torch.float32),
+    (torch.bfloat16, 256, 256, False, 1003, torch.float32), (torch.float32, 256, 64, True, 1003, torch.float32)])
+def test_walks_over_many_tokens_and_heads(dtype, D, rot, interleaved, S, w_dtype):
+    """So many tokens that a warp takes more heads than it has on their way at once, and in the backward pass several units one
+    after the other; 13 and 4 heads are no multiple of what it takes, so that some have heads of both sides; the last
+    warp has lanes without a token."""
+    B, H, kvH = 3, 13, 4
+    rope, freqs = api.Rope.make(rot, interleaved=interleaved), default_freqs(rot)
+    q, k = inputs(1, B, H, S, D, dtype), inputs(2, B, kvH, S, D, dtype, 0.6)
+    wq, wk = weight(3, D, w_dtype), weight(4, D, w_dtype)
+    pos = np.broadcast_to(np.arange(S) * 3 + 7, (B, 1, S))
+    how = dict(q_weight=gpu(wq, w_dtype), k_weight=gpu(wk, w_dtype), eps=1e-5, rope=rope, segmap=api.SegMap.make([7], S), pos_stride=3)
+    dq, dk = token_major(q, dtype), gpu(k, dtype)
+    q_out, k_out = (torch.full((B, h, S, D), float("nan"), dtype=dtype, device="cuda") for h in (H, kvH))
+    api.qk_norm_rope(dq, dk, q_out, k_out, **how)
+    for got, x, w in ((q_out, q, wq), (k_out, k, wk)):
+        check(got, *forward(x, w, pos, rot, interleaved, freqs, np.float32(1e-5)), dtype, "forward")
+    gq, gk = inputs(5, B, H, S, D, dtype), inputs(6, B, kvH, S, D, dtype)
+    rq, rk = torch.full_like(q_out, float("nan")), torch.full_like(k_out, float("nan"))
+    dwq, dwk = (torch.full((D,), float("nan"), device="cuda") for _ in range(2))
+    api.qk_norm_rope_backward(dq, dk, gpu(gq, dtype), token_major(gk, dtype), rq, rk, dq_weight=dwq, dk_weight=dwk, **how)
+    for got, dw, x, w, g, h in ((rq, dwq, q, wq, gq, H), (rk, dwk, k, wk, gk, kvH)):
+        dx, dx_err, want, err = backward(x, w, g, pos, rot, interleaved, freqs, np.float32(1e-5), chain_of(B, S, h))
+        check(got, dx, dx_err, dtype, "dx")
+        check(dw, want, err, torch.float32, "dw")
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("layout,cp,n_splits", [(0, 2, 2), (1, 2, 2), (1, 4, 4), (2, 4, 2)])
 def test_positions_of_a_rings_shards(dtype, layout, cp, n_splits):
