@@ -368,9 +368,16 @@ __device__ inline void paged_block(const PagedArgs& a, const CUtensorMap* map_k,
   }
   // Behind the kernel of the shared pages, whose blocks let this one begin when all that came before them has completed,
   // nothing waits for that kernel itself but the end: the fold, which waits for this grid, then finds both kernels' parts.
-  // (The fence stands for the wait's other half: no line that this SM holds from before is read as if it were new.)
-  if (a.shared_ml == nullptr) wait_for_previous();
-  else __threadfence();
+  // A grid that begins early is promised nothing about memory, so fences stand for the wait's other half: that kernel's threads
+  // have one between their wait and the signal, these have one behind it, and one more for the copies, which read what plain
+  // stores wrote (an append's rows). us a pass in a graph, 256 sequences behind 16384 rows and 32 behind 32768 (H32/kvH8 D128 bf16): so
+  // 146.7 and 54.2, waiting here 154.4 and 54.5, without the fences 146.5 and 53.9.
+  if (a.shared_ml == nullptr) {
+    wait_for_previous();
+  } else {
+    __threadfence();
+    asm volatile("fence.proxy.async.global;" ::: "memory");
+  }
   Ring<C> ring{a, map_k, map_v, base + warp * C::kRingBytes, base + C::kOffBar + warp * C::kStages * 8,
                reinterpret_cast<StageInfo*>(smem + C::kOffInfo) + warp * C::kStages, gave_up};
   ring.total = find_share<C::SR, C::kWarps>(a, warp, &ring.w, &ring.per, reinterpret_cast<ScanRoom<C::kWarps>*>(smem + C::kOffRoom));

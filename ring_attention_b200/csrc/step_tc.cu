@@ -413,8 +413,12 @@ __global__ void __launch_bounds__((TcCfg<D, kPInTmem, kPair, kSplit, kFold>::kTh
   // Everything so far touched no memory but the status word. A word that is set says to leave; one that is not may
   // yet be set by a launch before this one, so the producer reads it again.
   wait_for_previous();
-  // (what follows may begin when every block is here, and need not wait for what came before: see paged_decode.cu)
-  if constexpr (kPaged) let_next_start();
+  // What follows may begin when every block is here, and need not wait for what came before, which the fence hands on: see
+  // paged_block in paged_decode.cu.
+  if constexpr (kPaged) {
+    __threadfence();
+    let_next_start();
+  }
   if (leave) {
     if (warp == 1)
       asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem_base) : "memory");

@@ -394,6 +394,55 @@ def test_a_chain_of_steps_with_shared_pages(dtype, n_shared):
         assert torch.equal(slow, chain(lambda: None))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,n_shared", [(64, 400), (128, 5), (128, 190)])
+def test_append_and_decode_with_nothing_between_their_launches(dtype, D, n_shared):
+    """Steps whose decode comes directly behind the append that writes its queries and rows, and the next step's append directly
+    behind the decode that reads them: the same bits as step by step, enqueued and from a graph. (Lengths of all steps are there
+    before the first, so that no launch of the caller's stands between.)"""
+    B, H, kvH, page, steps = 6, 8, 2, 32, 40
+    rng = np.random.default_rng(19)
+    shared = np.arange(n_shared)
+    table = np.concatenate([np.tile(shared, (B, 1)), n_shared + np.arange(B * 4).reshape(B, 4)], 1)
+    rope = api.Rope.make(D)
+    start = n_shared * page + np.array([0, 1, 31, 32, 40, 60])
+    lens = [i32(start + i) for i in range(steps + 1)]
+    new = [gpu(rng.standard_normal((steps, B, h, 1, D)), dtype) for h in (H, kvH, kvH)]
+    pages = [gpu(rng.standard_normal((n_shared + 4 * B, kvH, page, D)), dtype) for _ in range(2)]
+    k_pages, v_pages = (x.clone() for x in pages)
+    q, outs = torch.empty(B, H, 1, D, dtype=dtype, device="cuda"), torch.empty(steps, B, H, D, dtype=dtype, device="cuda")
+    dt, ds = i32(table), i32(shared)
+
+    def begin():
+        for x, y in zip((k_pages, v_pages), pages):
+            x.copy_(y)
+        q.zero_()
+        outs.zero_()
+
+    def chain(wait=lambda: None):
+        for i in range(steps):
+            api.paged_append(new[1][i], new[2][i], k_pages, v_pages, dt, lens[i], rope=rope, q=new[0][i], q_out=q)
+            wait()
+            api.paged_decode(q[:, :, 0], k_pages, v_pages, dt, lens[i + 1], outs[i], shared_pages=ds)
+            wait()
+
+    begin()
+    chain(torch.cuda.synchronize)
+    slow = outs.clone()
+    assert not (slow == 0).all(-1).any()
+    for _ in range(5):
+        begin()
+        chain()
+        assert torch.equal(slow, outs)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        chain()
+    for _ in range(5):
+        begin()
+        g.replay()
+        assert torch.equal(slow, outs)
+
 @pytest.mark.parametrize("n_shared", [1, 3])
 def test_more_sequences_than_the_shared_pages_have_blocks_for(n_shared):
     """A batch whose rows on the shared pages are too many for the tensor-core kernel's list of blocks."""
