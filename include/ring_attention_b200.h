@@ -411,6 +411,9 @@ RA_API int ra_paged_append(const ra_paged_kv* cache, const ra_rows* k, const ra_
 RA_API size_t ra_paged_decode_workspace_bytes(const ra_paged_kv* cache, int heads, int shared_len);
 RA_API int ra_paged_decode(const ra_paged_kv* cache, const void* q, int heads, const int* shared_pages, int shared_len,
                            void* out, float* lse, void* workspace, size_t workspace_bytes, ra_stream stream);
+/* How such a call reads the shared pages (shared_len rows in all): 0 there are none, 1 each sequence for itself, 2 once for all by
+ * the decode kernel, 3 once by the tensor-core kernel; -1 for arguments that the call refuses. Host only; for tests. */
+RA_API int ra_debug_paged_route(const ra_paged_kv* cache, int heads, int shared_len);
 
 /* ---------------------------------------------------------------- partition ---- */
 

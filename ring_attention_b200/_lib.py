@@ -212,6 +212,7 @@ _SIG = {
     "ra_paged_decode_workspace_bytes": (C.c_size_t, [C.POINTER(PagedKV), C.c_int, C.c_int]),
     "ra_paged_decode": (C.c_int, [C.POINTER(PagedKV), _P, C.c_int, _P, C.c_int, _P, _P, _P, C.c_size_t, _P]),
     "ra_debug_paged_row": (C.c_longlong, [C.POINTER(C.c_int), C.c_int, C.c_int, C.c_int, C.c_int, C.c_longlong]),
+    "ra_debug_paged_route": (C.c_int, [C.POINTER(PagedKV), C.c_int, C.c_int]),
     "ra_debug_append_route": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
 }
 

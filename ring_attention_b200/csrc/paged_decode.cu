@@ -1061,6 +1061,14 @@ size_t ra_paged_decode_workspace_bytes(const ra_paged_kv* cache, int heads, int 
   return make_plan(c, heads, shared_len).bytes;
 }
 
+int ra_debug_paged_route(const ra_paged_kv* cache, int heads, int shared_len) {
+  int none = 0;
+  if (!cache || check_decode(*cache, heads, &none, shared_len) != RA_OK) return -1;
+  const ra_paged_kv c = without_pages(*cache, &shared_len);
+  const PagedPlan p = make_plan(c, heads, shared_len);
+  return shared_len == 0 ? 0 : p.listed ? 1 : p.tc ? 3 : 2;
+}
+
 int ra_paged_decode(const ra_paged_kv* cache, const void* q, int heads, const int* shared_pages, int shared_len, void* out,
                     float* lse, void* workspace, size_t workspace_bytes, ra_stream stream_) {
   RAB_REQUIRE(cache != nullptr, RA_ERR_INVALID, "paged_decode: null argument");

@@ -454,6 +454,19 @@ def test_more_sequences_than_the_shared_pages_have_blocks_for(n_shared):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,n_shared", [(5200, 1), (1000, 1), (5200, 2)])
+def test_one_shared_page_of_many_sequences(dtype, B, n_shared):
+    """A page or two that many sequences read once for all: by the tensor-core kernel, and, where it has too few blocks for their
+    rows, by the units that the others have."""
+    H, kvH, D, page = 8, 1, 128, 16 if B > 1000 else 256
+    lens = page * n_shared + np.arange(B) % 5
+    lens[::7] = page - 1
+    p = problem(20, dtype, B, H, kvH, D, page, lens, n_shared)
+    cache = PagedKV(api._DT[dtype], len(p[1]), kvH, page, D, 0x1000, 0x1000, B, p[3].shape[1], p[3].shape[1], 0x1000, 0x1000)
+    assert api.lib().ra_debug_paged_route(cache, H, n_shared * page) == (2 if B > 1000 or dtype == torch.float32 else 3)
+    compare(dtype, *p[:4], lens, p[4], run(dtype, *p[:4], lens, p[4]))
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n_shared", [0, 40, 960])
 def test_a_wait_that_runs_out_is_reported_and_leaves_the_rows(dtype, n_shared):
     lens = [40000, 30000] if n_shared < 960 else [62000, 61500]

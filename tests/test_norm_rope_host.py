@@ -231,6 +231,25 @@ def test_decode_refusals():
     assert call(c=paged(batch=0)) == 0
 
 
+@pytest.mark.parametrize("route,dtype,B,H,kvH,D,page,n_shared", [
+    (0, 1, 4, 4, 2, 64, 16, 0), (0, 0, 4, 4, 2, 64, 16, 0),
+    # each sequence for itself: 16 bits and little to read over again
+    (1, 1, 7, 6, 6, 32, 16, 9), (1, 2, 33, 16, 2, 256, 256, 1), (1, 1, 8, 24, 6, 64, 16, 128), (1, 1, 5200, 8, 1, 32, 16, 1),
+    # fp32; heads that are no multiple of the cache's; rows of more query blocks than the tensor-core kernel's list has
+    (2, 0, 7, 6, 6, 32, 16, 9), (2, 0, 256, 32, 8, 128, 16, 1024), (2, 1, 33, 5, 2, 128, 128, 30), (2, 1, 5200, 8, 1, 32, 16, 3),
+    (2, 1, 5200, 8, 1, 128, 16, 1), (2, 2, 5200, 8, 1, 128, 16, 1),
+    # one page and many, on the tensor core
+    (3, 1, 1000, 8, 1, 128, 256, 1), (3, 2, 32, 32, 8, 128, 64, 512), (3, 2, 256, 32, 8, 128, 16, 1024), (3, 1, 4, 4, 2, 64, 16, 1250),
+    (3, 2, 6, 8, 2, 128, 32, 190), (3, 1, 5, 8, 2, 128, 16, 460), (3, 2, 4, 16, 4, 128, 64, 79)])
+def test_which_way_shared_pages_are_read(route, dtype, B, H, kvH, D, page, n_shared):
+    """The ways that the GPU tests mean to take, so that another threshold does not take them elsewhere unseen."""
+    c = PagedKV(dtype, 10, kvH, page, D, P, P, B, 4, 4, P, P)
+    assert lib().ra_debug_paged_route(c, H, n_shared * page) == route
+    assert lib().ra_debug_paged_route(c, H, n_shared * page + 1) == -1 and lib().ra_debug_paged_route(None, H, 0) == -1
+    c.num_pages = 0
+    assert lib().ra_debug_paged_route(c, H, n_shared * page) == 0
+
+
 def test_structures_are_those_of_the_header(tmp_path):
     """Sizes and offsets of the fields as a C compiler lays them out."""
     names = {"ra_rope": Rope, "ra_rows": Rows, "ra_norm_rope": NormRope, "ra_paged_kv": PagedKV}
