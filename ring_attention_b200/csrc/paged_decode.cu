@@ -231,6 +231,12 @@ __device__ inline bool unit_row(const PagedArgs& a, const StageInfo& u, int r, i
   return *b < a.B && *h < a.H;
 }
 
+// What the kernels are built with and the host sizes the workspace by: keys of a stage, warps of a block, and rows of a unit in 16
+// bits (fp32: see fp32_rows).
+constexpr int stage_keys(bool f32, int D) { return f32 ? (D == 32 ? 32 : D == 64 ? 16 : 8) : D <= 64 ? 32 : 16; }
+constexpr int block_warps(bool f32, int D) { return D == 256 ? 2 : D == 32 && !f32 ? 8 : 4; }  // (64 bytes a row: more, for its instructions)
+constexpr int kMmaRows = 16;
+
 // Shared memory of a block of either kernel: the rings of its warps, a stage being SR rows of K and then of V. 16 bits: a tensor's
 // kBoxes boxes of 128 bytes of every row, by tensor maps, 16-byte piece c of a row's box at c ^ (row & 7) (rows of 64 bytes: one
 // box of those, c ^ (row / 2 & 3)). fp32: whole rows, one
@@ -238,12 +244,11 @@ __device__ inline bool unit_row(const PagedArgs& a, const StageInfo& u, int r, i
 // The shorter a row, the more of them a stage and the more warps, for the instructions around a stage: us a pass, four sequences of
 // 131072 to 262144 rows (H32/kvH8 fp16), head_dim 64 in stages of 16 / 32 rows 324 / 254; head_dim 32 in stages of 16 rows that fill
 // 128 bytes each, four / eight warps 294 / 178, of 32 rows of 64 bytes, eight warps, 138.
-template <typename T, int D, int SR_, int kRows_, int kExtraBytes>
+template <typename T, int D, int kRows_, int kExtraBytes>
 struct PagedBlock {
-  static constexpr int SR = SR_, RU = kRows_;
-  static constexpr bool kMany = D == 32 && sizeof(T) == 2;  // a row is 64 bytes: more warps for its instructions
-  static constexpr int kWarps = D == 256 ? 2 : kMany ? 8 : 4, kThreads = kWarps * 32;
   static constexpr bool kBulk = sizeof(T) == 4;
+  static constexpr int SR = stage_keys(kBulk, D), RU = kRows_;
+  static constexpr int kWarps = block_warps(kBulk, D), kThreads = kWarps * 32;
   static constexpr int kBoxes = kBulk || D <= 64 ? 1 : D / 64;
   static constexpr int kBoxBytes = D == 32 && !kBulk ? 64 : 128;
   static constexpr int kRowBytes = kBulk ? D * 4 : kBoxes * kBoxBytes;  // in shared memory
@@ -397,7 +402,7 @@ __device__ inline void paged_block(const PagedArgs& a, const CUtensorMap* map_k,
 // ---- 16-bit caches ------------------------------------------------------------------
 
 template <typename T, int D>
-using MmaBlock = PagedBlock<T, D, D <= 64 ? 32 : 16, 16, 0>;
+using MmaBlock = PagedBlock<T, D, kMmaRows, 0>;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(MmaBlock<T, D>::kThreads, 2)
@@ -568,7 +573,7 @@ struct F32Cfg {
   static constexpr int kWant = kRows == 1 ? 4 : kRows == 8 && D <= 128 ? 8 : 2 * kRows;
   static constexpr int kParts = kWant < D / 4 ? kWant : D / 4;
   static constexpr int kExtraBytes = (8 * 2 + 2) * kRows * 4;  // weights of 8 keys, each twice, and a factor a row, twice
-  using Block = PagedBlock<float, D, D == 32 ? 32 : D == 64 ? 16 : 8, kRows, (kExtraBytes + 15) & ~15>;
+  using Block = PagedBlock<float, D, kRows, (kExtraBytes + 15) & ~15>;
 };
 
 template <int D, int kRows>
@@ -938,9 +943,9 @@ PagedPlan make_plan(const ra_paged_kv& c, int heads, int shared_len) {
   p.listed = !f32 && shared_len > 0 && 4.0 * (c.batch - 1) * shared_len * c.kv_heads * c.head_dim <= kListedBytes;
   if (p.listed) shared_len = 0;
   const long long rows_shared = shared_len > 0 ? static_cast<long long>(c.batch) * G : 0;
-  p.RU = f32 ? fp32_rows(static_cast<int>(std::max<long long>(std::min<long long>(rows_shared, 8), G))) : 16;
-  p.SR = f32 ? (c.head_dim == 32 ? 32 : c.head_dim == 64 ? 16 : 8) : c.head_dim <= 64 ? 32 : 16;
-  p.warps = c.head_dim == 256 ? 2 : c.head_dim == 32 && !f32 ? 8 : 4;
+  p.RU = f32 ? fp32_rows(static_cast<int>(std::max<long long>(std::min<long long>(rows_shared, 8), G))) : kMmaRows;
+  p.SR = stage_keys(f32, c.head_dim);
+  p.warps = block_warps(f32, c.head_dim);
   p.tc = !f32 && rows_shared > 0 && plan_shared_prefix(c.batch, heads, c.kv_heads, c.head_dim, shared_len, &p.shared);
   p.HB = (G + p.RU - 1) / p.RU;
   p.RB = p.tc ? 0 : static_cast<int>((rows_shared + p.RU - 1) / p.RU);
@@ -1017,8 +1022,8 @@ int launch_rows(const ra_paged_kv& c, const PagedArgs& a, const PagedPlan& p, cu
 
 template <int D>
 int launch_head_dim(const ra_paged_kv& c, const PagedArgs& a, const PagedPlan& p, cudaStream_t stream) {
-  if (c.dtype == RA_F16) return launch_rows<__half, D, 16>(c, a, p, stream);
-  if (c.dtype == RA_BF16) return launch_rows<__nv_bfloat16, D, 16>(c, a, p, stream);
+  if (c.dtype == RA_F16) return launch_rows<__half, D, kMmaRows>(c, a, p, stream);
+  if (c.dtype == RA_BF16) return launch_rows<__nv_bfloat16, D, kMmaRows>(c, a, p, stream);
   if (p.RU == 1) return launch_rows<float, D, 1>(c, a, p, stream);
   if (p.RU == 2) return launch_rows<float, D, 2>(c, a, p, stream);
   if (p.RU == 4) return launch_rows<float, D, 4>(c, a, p, stream);

@@ -1645,7 +1645,8 @@ bool step_tc_supported(int dtype, const StepArgs& a) {
 // three 156, two 193.)
 bool plan_shared_prefix(int B, int H, int kvH, int D, int shared_len, SharedPlan* plan) {
   if (H % kvH != 0) return false;
-  const int group = H / kvH, kTiles = D == 256 ? 1 : 2;
+  // (as launch_paged runs it)
+  const int group = H / kvH, kTiles = D == 256 ? TcCfg<256, true>::kTiles : D == 128 ? TcCfg<128, true>::kTiles : TcCfg<64, true>::kTiles;
   plan->pack = 2 * B <= kBM ? std::min(group, kBM / B) : 1;
   const long long tiles = plan->pack > 1 ? (group + plan->pack - 1) / plan->pack : static_cast<long long>(group) * ((B + kBM - 1) / kBM);
   const long long blocks = (tiles + kTiles - 1) / kTiles;
