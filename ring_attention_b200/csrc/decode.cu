@@ -56,6 +56,18 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kStages = 4;
 constexpr int kMaxSplits = 128;
 
+__device__ inline void cp_async16(void* smem_dst, const void* gsrc, int src_bytes) {
+  const unsigned d = static_cast<unsigned>(__cvta_generic_to_shared(smem_dst));
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(gsrc),
+               "r"(src_bytes)
+               : "memory");
+}
+__device__ inline void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ inline void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // Unpack one 16-byte piece into floats.
 template <typename T>
 struct Piece;

@@ -1,22 +1,9 @@
-// Warp-level building blocks of the decode kernels: 16-byte asynchronous copies into shared memory and the m16n8k16
-// products of 16-bit operands.
+// Warp-level building blocks of the decode kernels: the m16n8k16 products of 16-bit operands.
 #pragma once
 
 #include "common.cuh"
 
 namespace rab {
-
-__device__ inline void cp_async16(void* smem_dst, const void* gsrc, int src_bytes) {
-  const unsigned d = static_cast<unsigned>(__cvta_generic_to_shared(smem_dst));
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(gsrc),
-               "r"(src_bytes)
-               : "memory");
-}
-__device__ inline void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ inline void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 
 template <typename T>
 __device__ inline void mma16816(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1);
