@@ -559,7 +559,8 @@ def qk_norm_rope_backward(q, k, dq_out, dk_out, dq, dk, *, dq_weight=None, dk_we
                           eps=1e-6, rope=None, segmap=None, pos_stride=1, positions=None, workspace=None):
     """The gradients of ``qk_norm_rope`` with the same keywords: from its inputs q and k (needed where there is a weight) and
     the gradients dq_out, dk_out of its results into dq, dk (which may be dq_out, dk_out) and, where wanted, dq_weight,
-    dk_weight (fp32, head_dim; overwritten, summed over all rows in a fixed order)."""
+    dk_weight (fp32, head_dim; overwritten, summed over all rows in a fixed order). A side whose gradient is None, with that of
+    its rows, has none worked out; its rows and weight may be there all the same."""
     one = dq_out if dq_out is not None else dk_out
     if one is None or (dq is None) != (dq_out is None) or (dk is None) != (dk_out is None):
         raise ValueError("qk_norm_rope_backward: a gradient of the result without one of the rows, or the other way round")
@@ -580,7 +581,8 @@ def qk_norm_rope_backward(q, k, dq_out, dk_out, dq, dk, *, dq_weight=None, dk_we
         workspace = one.new_empty(need, dtype=torch.uint8)
     qs, ks = (B, H, S, D), (B, kvH, S, D)
     check(packed("ra_qk_norm_rope_backward")(
-        _dtype(one), _rows(q, qs, dt) if q_weight is not None else None, _rows(k, ks, dt) if k_weight is not None else None,
+        _dtype(one), _rows(q, qs, dt) if q_weight is not None and H else None,
+        _rows(k, ks, dt) if k_weight is not None and kvH else None,
         _rows(dq_out, qs, dt), _rows(dk_out, ks, dt), _rows(dq, qs, dt, True), _rows(dk, ks, dt, True),
         dq_weight.data_ptr() if dq_weight is not None else None, dk_weight.data_ptr() if dk_weight is not None else None,
         PACK_SHAPE(B, H or 1, S, S, D, kvH), how, _ptr(workspace) if need else None,

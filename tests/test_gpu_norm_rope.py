@@ -201,6 +201,25 @@ def test_broadcast_rows_and_one_side_alone():
     check(dw, want, err, torch.float32)
 
 
+def test_gradients_of_one_side_with_the_rows_of_both():
+    """One of q and k needs no gradient: its rows and weight go in as in the forward call and change nothing."""
+    B, H, kvH, S, D = 2, 6, 2, 9, 64
+    q, k = torch.randn(B, H, S, D, device="cuda"), torch.randn(B, kvH, S, D, device="cuda")
+    w, rope = {n + "_weight": 1 + torch.rand(D, device="cuda") for n in "qk"}, api.Rope.make(D)
+    for x, n in ((q, "q"), (k, "k")):
+        dy = torch.randn_like(x)
+        got = []
+        for both in (False, True):
+            dx, dw = torch.empty_like(x), torch.empty(D, device="cuda")
+            rows = (q, k) if both else (q, None) if n == "q" else (None, k)
+            args = (dy, None, dx, None) if n == "q" else (None, dy, None, dx)
+            how = w if both else {n + "_weight": w[n + "_weight"]}
+            api.qk_norm_rope_backward(*rows, *args, **{f"d{n}_weight": dw}, **how, rope=rope)
+            got.append((dx, dw))
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+    with pytest.raises(ValueError):
+        api.qk_norm_rope_backward(q, k, None, None, None, None, **w, rope=rope)
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_fp32_weights_of_16_bit_rows(dtype):
     B, H, S, D = 2, 4, 6, 128
