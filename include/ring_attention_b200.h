@@ -83,7 +83,7 @@ RA_API int ra_device_status(int out[4]);
  * switch that makes that kernel's TMA producer stop after `items` K/V tiles (negative = off),
  * so that a test can watch a wait run out: the kernel returns, ra_device_status reports
  * RA_ERR_DEVICE_WAIT, nothing is accessed out of bounds. Both hold for ra_paged_decode too, which then misses a part of
- * every copy. Process-wide; not for production use. */
+ * every copy (with 0 items it computes nothing, as behind a wait that ran out). Process-wide; not for production use. */
 RA_API void ra_debug_set_wait_limit_ns(unsigned long long ns);
 RA_API void ra_debug_stall_producer_after(int items);
 /* Block order of the tcgen05 step kernel: -1 = chosen by shape (default), 0 = (batch, head)

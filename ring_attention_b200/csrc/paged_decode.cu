@@ -67,7 +67,8 @@ struct PagedArgs {
   float* shared_o;
   int* status;
   unsigned long long wait_ns;
-  int missing;  // (test hook: bytes that every stage waits for in vain; 0: none)
+  int shares;   // that the stages are dealt in
+  int missing;  // (test hook: bytes that every stage waits for in vain; 0: none; -1: no warp does anything)
 };
 
 // Keys [start, end) of a sequence that its own table holds: behind the shared pages if it has all of them.
@@ -387,7 +388,7 @@ __device__ inline void paged_block(const PagedArgs& a, const CUtensorMap* map_k,
                reinterpret_cast<StageInfo*>(smem + C::kOffInfo) + warp * C::kStages, gave_up};
   ring.total = find_share<C::SR, C::kWarps>(a, warp, &ring.w, &ring.per, reinterpret_cast<ScanRoom<C::kWarps>*>(smem + C::kOffRoom));
   // (behind a launch that gave up nothing is computed; the fold writes nothing then either)
-  if (ring.total > 0 && __shfl_sync(0xffffffffu, *reinterpret_cast<volatile int*>(a.status), 0) == 0) {
+  if (ring.total > 0 && a.missing >= 0 && __shfl_sync(0xffffffffu, *reinterpret_cast<volatile int*>(a.status), 0) == 0) {
     ring.begin();
     compute(ring, warp);
   }
@@ -807,10 +808,14 @@ __global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const __grid_c
     pre_o = a.shared_o;
   }
   wait_for_previous();
-  const bool lost = *reinterpret_cast<const volatile int*>(a.status) != 0;  // some wait ran out: the rows stay as they are
+  bool lost = *reinterpret_cast<const volatile int*>(a.status) != 0;  // some wait ran out: the rows stay as they are
   const int2 own = a.unit_parts[own_uid], pre = a.unit_parts[shared_uid];
   int start = 0, end = 0;
   if (mine) own_keys(a, b, &start, &end);
+  // So they do where no warp of this call has said which parts there are: the word was set when the warps looked at it, and another
+  // thread of the host has read and cleared it since. What the workspace holds in that place may be anything.
+  auto said = [&](const int2& p) { return p.x >= 0 && p.y > 0 && p.y <= a.shares - p.x; };
+  if ((end > start && !said(own)) || (start > 0 && !a.shared_ml && !said(pre))) lost = true;
   const int own_n = end > start ? own.y : 0;
   const long long own_lo = (static_cast<long long>(own.x) + own_uid) * a.rs + g % RU;
   if (!a.shared_ml) {
@@ -1126,7 +1131,9 @@ int ra_paged_decode(const ra_paged_kv* cache, const void* q, int heads, const in
   a.status = device_status_ptr();
   RAB_REQUIRE(a.status != nullptr, RA_ERR_CUDA, "paged_decode: no device status word");
   a.wait_ns = tcgen::tc_wait_limit_ns();
-  a.missing = tcgen::tc_stall_after() >= 0 ? 16 : 0;
+  a.shares = p.blocks * p.warps;
+  const int stall = tcgen::tc_stall_after();
+  a.missing = stall > 0 ? 16 : stall == 0 ? -1 : 0;
   if (p.tc) {
     a.shared_ml = reinterpret_cast<float2*>(ws + p.unit_bytes + p.ml_bytes + p.o_bytes);
     a.shared_o = reinterpret_cast<float*>(ws + p.unit_bytes + p.ml_bytes + p.o_bytes + p.shared_ml_bytes);

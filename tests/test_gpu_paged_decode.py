@@ -492,6 +492,30 @@ def test_a_wait_that_runs_out_is_reported_and_leaves_the_rows(dtype, n_shared):
     compare(dtype, q, k, v, table, lens, shared, (out, lse))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n_shared", [0, 3])
+@pytest.mark.parametrize("fill", [0x00, 0x01, 0x7F, 0x80, 0xFF])
+def test_parts_that_no_warp_has_left(dtype, n_shared, fill):
+    """Where no warp computed anything (a status word that was set when they looked, and cleared since), what a workspace happens
+    to hold is no list of parts: the rows stay, but for those that have no keys."""
+    lens = np.array([700, 48, 0, 300, 17])
+    q, k, v, table, shared = problem(21, dtype, 5, 8, 2, 64, 16, lens, n_shared)
+    args = gpu(q, dtype), gpu(k, dtype), gpu(v, dtype), i32(table), i32(lens)
+    out, lse = torch.full(q.shape, 7, dtype=dtype, device="cuda"), torch.full(q.shape[:2], 7.0, device="cuda")
+    kw = dict(lse=lse, shared_pages=i32(shared) if n_shared else None, workspace=torch.full((1 << 23,), fill, dtype=torch.uint8, device="cuda"))
+    L = api.lib()
+    L.ra_debug_stall_producer_after(0)
+    try:
+        api.paged_decode(*args, out, **kw)
+        torch.cuda.synchronize()
+    finally:
+        L.ra_debug_stall_producer_after(-1)
+    assert api.device_status()[0] == 0
+    there = torch.tensor(lens > 0, device="cuda")
+    assert (out[there] == 7).all() and (lse[there] == 7).all() and (out[~there] == 0).all() and (lse[~there] == -float("inf")).all()
+    api.paged_decode(*args, out, **kw)
+    compare(dtype, q, k, v, table, lens, shared, (out, lse))
+
 def test_decode_wrapper_refusals():
     q = torch.zeros(2, 4, 64, device="cuda")
     p, o = torch.zeros(3, 2, 16, 64, device="cuda"), torch.empty_like(q)
