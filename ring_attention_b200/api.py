@@ -629,9 +629,12 @@ def paged_append(k, v, k_pages, v_pages, page_table, lens, *, counts=None, rope=
 
 def paged_decode(q, k_pages, v_pages, page_table, lens, out, *, lse=None, shared_pages=None, workspace=None):
     """Decode attention of one query row a sequence over a paged KV cache (see ``paged_append``): q and out are (batch, heads,
-    head_dim) in the cache's dtype, query head h reads KV head h % kv_heads, sequence b sees its first lens[b] rows. ``lse``
-    ((batch, heads), fp32) gets the log-sum-exp. A sequence without rows gives zeros and -inf. ``shared_pages`` (int32):
-    the pages that every sequence with at least that many rows begins with; they are read once for all of them."""
+    head_dim) in the cache's dtype, heads from kv_heads to 4096, query head h reads KV head h % kv_heads, sequence b sees its
+    first lens[b] rows. ``lse`` ((batch, heads), fp32) gets the log-sum-exp. A sequence without rows gives zeros and -inf. Sums and
+    the softmax are held in 32 bits; 16-bit caches round the weights to their type for the sum over V, as the decode step does.
+    ``shared_pages`` (int32): the pages that every sequence with at least that many rows begins with; they are read once for all
+    of them, but by each for itself where a small 16-bit batch is faster so. In fp32 that saves reads and no arithmetic: with
+    eight or more heads to a KV head, or a few hundred shared rows, a call without it can be the faster one."""
     dev = _on_device(q, k_pages, v_pages, page_table, lens, out, lse, shared_pages, workspace)
     cache, _, page, D, B = _paged_kv(k_pages, v_pages, page_table, lens)
     shape = q.shape

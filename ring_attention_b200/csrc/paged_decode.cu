@@ -18,10 +18,12 @@
 // is the slower for it (528 and 94).
 //
 // 16-bit caches: both products on mma.sync m16n8k16, the unit's rows as its M rows, as in decode_mma_kernel (decode.cu). fp32:
-// plain multiply-adds, four lanes to a key for the scores, four columns a lane for the sum over V.
+// plain multiply-adds, 4 to 16 lanes to a key for the scores (see F32Cfg), four columns a lane (head_dim 256: eight) for the sum over V.
 //
 // Every wait on a barrier is bounded, as in the step kernels: when one runs out the warp records it in the device status word
 // and leaves, and the fold leaves every row that it would have written as it is.
+//
+// Times in this file are of launches one behind the other in a CUDA graph; calls of less than some 15 us wait for the host otherwise.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -516,7 +518,9 @@ __global__ void __launch_bounds__(MmaBlock<T, D>::kThreads, 2)
         }
         l_run[0] += (p[0] + p[1]) + (p[2] + p[3]);
         l_run[1] += (p[4] + p[5]) + (p[6] + p[7]);
-        // P as the A fragment of the second product, rounded to the cache's type as the products want it
+        // P as the A fragment of the second product, rounded to the cache's type as the products want it (l above is not): with the
+        // rounding of the result that makes 1.2 to 1.4 times the distance from 64 bits that the latter alone makes. In fp16 a weight
+        // of less than 2^-25 of the largest so far counts in l alone.
         unsigned pa[4];
         pa[0] = pack_pair<T>(p[0], p[1]);
         pa[1] = pack_pair<T>(p[4], p[5]);
