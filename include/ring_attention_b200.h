@@ -416,6 +416,40 @@ RA_API int ra_paged_decode(const ra_paged_kv* cache, const void* q, int heads, c
  * the decode kernel, 3 once by the tensor-core kernel; -1 for arguments that the call refuses. Host only; for tests. */
 RA_API int ra_debug_paged_route(const ra_paged_kv* cache, int heads, int shared_len);
 
+/* Rows of sequences out of a paged cache, one sequence's behind the other's, as ra_packed_attention reads them: row i of k_out and
+ * v_out ((rows, kv_heads, head_dim) of the cache's dtype; batch_stride is not used), for ends[b] <= i < ends[b + 1], gets row
+ * start[b] + i - ends[b] of sequence b (`ends`: device, batch + 1, rising; `start`: device, batch; NULL: 0). A row that the cache does not hold
+ * is zeros; rows before ends[0] and from ends[batch] on stay as they are. cache->lens is not read and may be NULL. */
+RA_API int ra_paged_read(const ra_paged_kv* cache, const int* ends, const int* start, const ra_rows* k_out, const ra_rows* v_out,
+                         int rows, ra_stream stream);
+
+/* ------------------------------------------------- paged KV cache in 4 bits ---- */
+
+/* The same cache with rows in 4 bits: cache->k and cache->v are (num_pages, kv_heads) pieces of page_size * head_dim * 9 / 16 bytes, 16-byte
+ * aligned, and cache->dtype (RA_F16 or RA_BF16) is that of the rows that come and go. 16 elements of a row share a scale in e4m3, the
+ * nearest to their largest magnitude / 6 in units of k_scale or v_scale (powers of two from 2^-30 to 2^30, the same in every call on the
+ * cache), 448 at most; an element is the nearest of 0, 1/2, 1, 3/2, 2, 3, 4, 6 (with its sign) times its scale, the even code of two equally near ones
+ * (e2m1). So a scale of 1 serves rows whose largest elements are between about 0.1 and 2688. Sixteen elements with a NaN among them are
+ * all NaN, an infinity is the largest number. In a piece the codes of its page_size rows come first, two to a byte, element 2 i in the lower half of byte
+ * i, with bytes [16 c, 16 c + 16) of row j at 16 (c ^ t), t = (4 (j & 1) | (j & 2)) & (head_dim / 32 - 1); then, a byte each, the rows' scales. */
+
+/* ra_paged_append to such a cache: a row is worked out and rounded to its dtype as there, and its 4 bits are of that. */
+RA_API int ra_paged_append_4bit(const ra_paged_kv* cache, float k_scale, float v_scale, const ra_rows* k, const ra_rows* v, int rows,
+                                const int* counts, const ra_rows* q, const ra_rows* q_out, int heads, const ra_norm_rope* how,
+                                ra_stream stream);
+
+/* ra_paged_read out of such a cache: the values as they are held, rounded once to dtype where a factor takes them out of its range. */
+RA_API int ra_paged_read_4bit(const ra_paged_kv* cache, float k_scale, float v_scale, const int* ends, const int* start,
+                              const ra_rows* k_out, const ra_rows* v_out, int rows, ra_stream stream);
+
+/* ra_paged_decode over such a cache, without shared pages. q and out are of cache->dtype. The cached values enter both products
+ * exactly; the queries do but for elements less than 2^-14 of their row's largest, which lose less than 2^-25 of that; the weights of the sum
+ * over V are rounded to fp16, and the result once. A wait that ran out is treated as there.
+ * `workspace`: ra_paged_decode_4bit_workspace_bytes(...) bytes, 16-byte aligned, of this call's launches alone. */
+RA_API size_t ra_paged_decode_4bit_workspace_bytes(const ra_paged_kv* cache, int heads);
+RA_API int ra_paged_decode_4bit(const ra_paged_kv* cache, float k_scale, float v_scale, const void* q, int heads, void* out, float* lse,
+                                void* workspace, size_t workspace_bytes, ra_stream stream);
+
 /* ---------------------------------------------------------------- partition ---- */
 
 /* Index maps of RingPartition (src/ring_partition.hpp:11-75, src/ring_partition.cpp:41-108).

@@ -601,6 +601,22 @@ def _paged_kv(k_pages, v_pages, page_table, lens):
                          _int32(lens, (B,), "lens")), kvH, page, D, B
 
 
+def _append(name, dt, c_heads, c_dim, c_batch, k, v, counts, rope, positions, k_weight, q, q_out, q_weight, eps):
+    """What the appending calls pass on alike, from k to ra_norm_rope; dt is the rows' dtype."""
+    B, kvH, T, D = k.shape
+    if B != c_batch or kvH != c_heads or D != c_dim:
+        raise ValueError(f"{name}: k does not fit the cache")
+    if (q is None) != (q_out is None):
+        raise ValueError(f"{name}: queries without a result, or a result without queries")
+    how = None
+    if rope is not None or k_weight is not None or q_weight is not None:
+        how = _norm_rope(dt, B, T, D, q_weight, k_weight, eps, rope, None, 1, positions)
+    H = q.shape[1] if q is not None else 0
+    ks, qs = (B, kvH, T, D), (B, H, T, D)
+    return (_rows(k, ks, dt), _rows(v, ks, dt), T, _int32(counts, (B,), "counts") if counts is not None else None, _rows(q, qs, dt),
+            _rows(q_out, qs, dt, True), H, how)
+
+
 def paged_append(k, v, k_pages, v_pages, page_table, lens, *, counts=None, rope=None, positions=None, k_weight=None, q=None,
                  q_out=None, q_weight=None, eps=1e-6):
     """Appends rows to a paged KV cache, K normed and rotated on the way (see ``qk_norm_rope``; row t at position lens[b] + t
@@ -609,22 +625,10 @@ def paged_append(k, v, k_pages, v_pages, page_table, lens, *, counts=None, rope=
     would go there are dropped). k and v are (batch, kv_heads, rows, head_dim) with any strides but contiguous rows; row t of
     the first counts[b] (int32; None: all) becomes row lens[b] + t. With q ((batch, heads, rows, head_dim)) the queries of
     the same tokens go to q_out in the same launch. ``lens`` (int32) stays as it is: the caller adds the counts."""
-    B, kvH, T, D = k.shape
-    dt = k_pages.dtype
     dev = _on_device(k, v, k_pages, v_pages, page_table, lens, counts, positions, k_weight, q, q_out, q_weight)
     cache, c_heads, _, c_dim, c_batch = _paged_kv(k_pages, v_pages, page_table, lens)
-    if B != c_batch or kvH != c_heads or D != c_dim:
-        raise ValueError("paged_append: k does not fit the cache")
-    if (q is None) != (q_out is None):
-        raise ValueError("paged_append: queries without a result, or a result without queries")
-    how = None
-    if rope is not None or k_weight is not None or q_weight is not None:
-        how = _norm_rope(dt, B, T, D, q_weight, k_weight, eps, rope, None, 1, positions)
-    H = q.shape[1] if q is not None else 0
-    ks, qs = (B, kvH, T, D), (B, H, T, D)
-    check(packed("ra_paged_append")(cache, _rows(k, ks, dt), _rows(v, ks, dt), T,
-                                    _int32(counts, (B,), "counts") if counts is not None else None, _rows(q, qs, dt),
-                                    _rows(q_out, qs, dt, True), H, how, _raw_stream(dev)))
+    check(packed("ra_paged_append")(cache, *_append("paged_append", k_pages.dtype, c_heads, c_dim, c_batch, k, v, counts, rope,
+                                                    positions, k_weight, q, q_out, q_weight, eps), _raw_stream(dev)))
 
 
 def paged_decode(q, k_pages, v_pages, page_table, lens, out, *, lse=None, shared_pages=None, workspace=None):
@@ -654,3 +658,103 @@ def paged_decode(q, k_pages, v_pages, page_table, lens, out, *, lse=None, shared
         workspace = q.new_empty(packed("ra_paged_decode_workspace_bytes")(cache, H, shared_len), dtype=torch.uint8)
     check(packed("ra_paged_decode")(cache, _ptr(q), H, pages, shared_len, _ptr(out), _ptr(lse), _ptr(workspace),
                                     workspace.nbytes, _raw_stream(dev)))
+
+
+def _packed_rows(t, shape, dtype, out=False):
+    """ra_rows of a (rows, heads, head_dim) tensor with strides of its own and contiguous elements of a row."""
+    if t.shape != shape or t.dtype is not dtype:
+        raise ValueError(f"expected a tensor of {tuple(shape)} in {dtype}, got {tuple(t.shape)} in {t.dtype}")
+    sr, sh, sd = t.stride()
+    if sd != 1:
+        raise ValueError("the elements of a row must be contiguous")
+    if out and (sr == 0 and shape[0] > 1 or sh == 0 and shape[1] > 1):
+        raise ValueError("rows of a result must not share memory")
+    return PACK_ROWS(t.data_ptr(), 0, sh, sr)
+
+
+def paged_read(k_pages, v_pages, page_table, ends, k_out, v_out, *, start=None):
+    """Rows of sequences out of a paged KV cache (see ``paged_append``), one sequence's behind the other's, as ``packed_attention``
+    reads them: rows ends[b] to ends[b + 1] of k_out and v_out ((rows, kv_heads, head_dim), contiguous rows) get rows
+    start[b] and on (None: 0) of sequence b. ``ends`` ((batch + 1,), int32) rises; rows of the results that belong to no sequence stay as
+    they are, and those that the cache does not hold are zeros."""
+    dev = _on_device(k_pages, v_pages, page_table, ends, start, k_out, v_out)
+    B = page_table.shape[0]
+    at = _int32(ends, (B + 1,), "ends")
+    cache, kvH, _, D, _ = _paged_kv(k_pages, v_pages, page_table, ends[:B])
+    shape = (k_out.shape[0], kvH, D)
+    check(packed("ra_paged_read")(cache, at, _int32(start, (B,), "start") if start is not None else None,
+                                  _packed_rows(k_out, shape, k_pages.dtype, True), _packed_rows(v_out, shape, k_pages.dtype, True),
+                                  shape[0], _raw_stream(dev)))
+
+
+# ---- the paged cache in 4 bits -------------------------------------------------------------------
+
+
+def pages_4bit(num_pages, kv_heads, page_size, head_dim, device="cuda"):
+    """Empty pages of K or V for ``paged_append_4bit``: (num_pages, kv_heads, page_size * head_dim * 9 / 16) bytes."""
+    return torch.zeros((num_pages, kv_heads, page_size * head_dim * 9 // 16), dtype=torch.uint8, device=device)
+
+
+def _paged_4bit(k_pages, v_pages, page_table, lens, head_dim, dtype):
+    """(ra_paged_kv, kv heads, batch) of a cache in 4 bits whose rows have head_dim elements and come and go in dtype."""
+    shape, (B, most) = k_pages.shape, page_table.shape
+    if len(shape) != 3 or shape != v_pages.shape or k_pages.dtype != torch.uint8 or v_pages.dtype != torch.uint8 or \
+            not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise ValueError("k_pages and v_pages: expected contiguous uint8 (num_pages, kv_heads, page_size * head_dim * 9 / 16) tensors alike")
+    n, kvH, size = shape
+    page, rest = divmod(16 * size, 9 * head_dim) if head_dim > 0 else (0, 1)
+    if rest:
+        raise ValueError("the pages do not hold whole rows of the head_dim")
+    return PACK_PAGED_KV(_dtype_of_4bit(dtype), n, kvH, page, head_dim, k_pages.data_ptr(), v_pages.data_ptr(), B, most,
+                         page_table.stride(0), _int32(page_table, (B, most), "page_table"), _int32(lens, (B,), "lens")), kvH, B
+
+
+def _dtype_of_4bit(dtype):
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
+        raise ValueError(f"a cache in 4 bits takes rows in fp16 or bf16, got {dtype}")
+    return _DT[dtype]
+
+
+def paged_append_4bit(k, v, k_pages, v_pages, page_table, lens, *, k_scale=1.0, v_scale=1.0, counts=None, rope=None, positions=None,
+                      k_weight=None, q=None, q_out=None, q_weight=None, eps=1e-6):
+    """``paged_append`` to a cache in 4 bits: k_pages and v_pages are those of ``pages_4bit``, k and v fp16 or bf16. 16 elements of a row
+    share a scale in e4m3 (their largest magnitude / 6), an element is held as one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (with a sign) times it.
+    Scales are in units of k_scale and v_scale, powers of two that every call on the cache is given alike: 1 serves rows whose largest
+    elements are between about 0.1 and 2688. What is held is the nearest to the row as ``paged_append`` would store it."""
+    dev = _on_device(k, v, k_pages, v_pages, page_table, lens, counts, positions, k_weight, q, q_out, q_weight)
+    D = k.shape[3]
+    cache, kvH, B = _paged_4bit(k_pages, v_pages, page_table, lens, D, k.dtype)
+    check(packed("ra_paged_append_4bit")(cache, k_scale, v_scale,
+                                         *_append("paged_append_4bit", k.dtype, kvH, D, B, k, v, counts, rope, positions, k_weight, q,
+                                                  q_out, q_weight, eps), _raw_stream(dev)))
+
+
+def paged_read_4bit(k_pages, v_pages, page_table, ends, k_out, v_out, *, start=None, k_scale=1.0, v_scale=1.0):
+    """``paged_read`` out of a cache in 4 bits (see ``paged_append_4bit``): the values that the cache holds, in fp16 or bf16."""
+    dev = _on_device(k_pages, v_pages, page_table, ends, start, k_out, v_out)
+    B = page_table.shape[0]
+    at = _int32(ends, (B + 1,), "ends")
+    rows, kvH, D = k_out.shape
+    cache, c_heads, _ = _paged_4bit(k_pages, v_pages, page_table, ends[:B], D, k_out.dtype)
+    shape = (rows, c_heads, D)
+    check(packed("ra_paged_read_4bit")(cache, k_scale, v_scale, at, _int32(start, (B,), "start") if start is not None else None,
+                                       _packed_rows(k_out, shape, k_out.dtype, True), _packed_rows(v_out, shape, k_out.dtype, True),
+                                       rows, _raw_stream(dev)))
+
+
+def paged_decode_4bit(q, k_pages, v_pages, page_table, lens, out, *, k_scale=1.0, v_scale=1.0, lse=None, workspace=None):
+    """``paged_decode`` over a cache in 4 bits (see ``paged_append_4bit``), without shared pages: q and out are (batch, heads,
+    head_dim) in fp16 or bf16. The values that the cache holds enter exactly; the weights of the sum over V are rounded to fp16."""
+    dev = _on_device(q, k_pages, v_pages, page_table, lens, out, lse, workspace)
+    shape = q.shape
+    if len(shape) != 3 or shape[0] != page_table.shape[0]:
+        raise ValueError("paged_decode_4bit: q does not fit the cache")
+    B, H, D = shape
+    cache, _, _ = _paged_4bit(k_pages, v_pages, page_table, lens, D, q.dtype)
+    if out.shape != shape or out.dtype != q.dtype or \
+            lse is not None and (lse.shape != (B, H) or lse.dtype != torch.float32):
+        raise ValueError("paged_decode_4bit: out is like q, lse (batch, heads) in fp32")
+    if workspace is None:
+        workspace = q.new_empty(packed("ra_paged_decode_4bit_workspace_bytes")(cache, H), dtype=torch.uint8)
+    check(packed("ra_paged_decode_4bit")(cache, k_scale, v_scale, _ptr(q), H, _ptr(out), _ptr(lse), _ptr(workspace),
+                                         workspace.nbytes, _raw_stream(dev)))

@@ -40,4 +40,13 @@ inline int check_lists(const ra_paged_kv& c, const char* what) {
   return RA_OK;
 }
 
+// Rows in 4 bits (see ra_paged_append_4bit): of a (page, KV head) first the codes of all rows, half a byte an element, then their
+// scales, a byte to 16 elements. Piece c of 16 bytes of row j's codes is at c ^ four_turn(j, head_dim): so the decode kernel reads them
+// out of shared memory, where they lie as in the page, without bank conflicts (rows of 64 and 128 bytes would meet).
+__host__ __device__ constexpr int four_turn(int row, int head_dim) {
+  return ((row & 1) * 4 | (row & 2)) & (head_dim / 32 - 1);
+}
+__host__ __device__ constexpr int four_row_bytes(int head_dim) { return head_dim / 2 + head_dim / 16; }
+int check_paged_4bit(const ra_paged_kv& c, float k_scale, float v_scale, const char* what);
+
 }  // namespace rab

@@ -1,0 +1,703 @@
+// Decode attention (one query row a sequence) against a paged KV cache whose rows are held in 4 bits, and rows of a paged cache
+// of any kind read back out of it.
+//
+// A row x of K or V is held as 16 elements to a block: a scale s in e4m3 (3 bits of fraction, up to 448), and for each element a
+// code c in e2m1, one of 0, 1/2, 1, 3/2, 2, 3, 4, 6 and a sign; the element's value is c s f, f a power of two for the whole of K or
+// of V. c s has at most 5 significant bits, so it is exact in fp16 (2^-10 to 2688) and the products below see the cached values as
+// they are. A row is 9/16 of its elements' number in bytes.
+//
+//   out[b, h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(q . k_j / sqrt(D)),  j < lens[b],  KV head h % kv_heads
+//
+// The walk is that of paged_decode.cu (paged_walk.cuh). What is different is that a byte of the cache brings two elements and so four
+// times the instructions of a 16-bit one: besides the copy the issue slots bound it. So nothing is moved for the tensor core's sake: both
+// products have the cached operand as the A of mma.sync m16n8k16 (16 keys by 16 columns of K, 16 columns by 16 keys of V), eight
+// query heads as its N, and each lane makes its part of A in registers from the bytes of its own rows: the order of the columns
+// in a contraction is free, so a lane takes 16 columns of K that lie side by side, and 16 of V. A code pair becomes two fp16 by one
+// conversion and their scales one multiplication.
+#include "paged_walk.cuh"
+
+namespace rab {
+
+namespace {
+
+// ---- decode -------------------------------------------------------------------------
+
+struct FourArgs {
+  PagedArgs p;
+  float k_factor, v_factor;
+};
+
+template <int D, int NB>
+struct FourBlock {
+  static constexpr bool kBulk = true, kFour = true;
+  static constexpr int SR = 32, RU = 8 * NB;
+  // accumulators and queries: (D / 4 + D / 8) NB registers
+  static constexpr int kWarps = D * NB <= 128 ? 8 : 4, kThreads = kWarps * 32;
+  static constexpr int kBoxes = 1;
+  static constexpr int kCodeBytes = D / 2, kScaleBytes = D / 16, kRowBytes = kCodeBytes + kScaleBytes;
+  static constexpr int kTileBytes = SR * kRowBytes;  // per tensor: codes, then scales
+  static constexpr int kStages = 110 * 1024 / kWarps / (2 * kTileBytes) < 8 ? 110 * 1024 / kWarps / (2 * kTileBytes) : 8;
+  static constexpr int kRingBytes = 2 * kStages * kTileBytes;
+  static constexpr int kOffInfo = (kWarps * kRingBytes + 15) & ~15;
+  static constexpr int kOffBar = kOffInfo + kWarps * kStages * static_cast<int>(sizeof(StageInfo));
+  static constexpr int kOffRoom = (kOffBar + kWarps * kStages * 8 + 15) & ~15;
+  static constexpr int kOffFlag = kOffRoom + static_cast<int>(sizeof(ScanRoom<kWarps>));
+  static constexpr int kSmemBytes = kOffFlag + 8;
+  static_assert(kTileBytes % 16 == 0 && kStages >= 3 && sizeof(StageInfo) % 4 == 0, "the ring");
+  static_assert((kWarps * kStages * sizeof(StageInfo)) % 8 == 0, "the barriers");
+  static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two blocks to an SM");
+};
+
+// The eight codes of a word as fp16 pairs, neighbours together.
+__device__ inline void codes_to_half(unsigned w, unsigned (&h)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
+// Two scales as fp16.
+__device__ inline unsigned scales_to_half(unsigned short s) {
+  unsigned h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(s));
+  return h;
+}
+__device__ inline unsigned mul_half2(unsigned a, unsigned b) {
+  unsigned d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// An 8 x 8 matrix of 16-bit elements over the warp, transposed.
+__device__ inline unsigned transposed(unsigned a) {
+  unsigned d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+template <typename T>
+__device__ inline float element(const T* p) {
+  return static_cast<float>(*p);
+}
+
+// Words of shared memory, N of them.
+template <int N>
+__device__ inline void load_words(unsigned addr, unsigned* w) {
+  if constexpr (N == 4)
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr) : "memory");
+  else if constexpr (N == 2)
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr) : "memory");
+  else
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr) : "memory");
+}
+__device__ inline unsigned load_u16(unsigned addr) {
+  unsigned short v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ inline unsigned load_u8(unsigned addr) {
+  unsigned v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Where the products' places are. Lane (g, j) of a fragment has its rows g and g + 8 and its columns 2 j, 2 j + 1, 2 j + 8, 2 j + 9.
+// Key at place p of 16: p ^ (p >> 2 & 1), so that the keys 2 j differ in the rest by four, as do the keys g of half a warp: with the
+// pieces' places in a page (four_turn) no two lanes of an access meet in a bank.
+// K: columns of step s, lane j: from k_column on, two and two. V: columns of tile i, lane g: v_column of its row g, and v_other
+// behind it that of its row g + 8.
+__device__ inline int key_at(int place) { return place ^ (place >> 2 & 1); }
+template <int D>
+struct FourCols {
+  static constexpr int kRun = D >= 128 ? 32 : D / 4;  // columns of K that a lane has side by side
+  static constexpr int kVCols = D / 8;                // of V
+  static constexpr int v_other = D / 16;
+  __device__ static int k_column(int s, int j) { return D >= 128 ? s / 8 * 128 + 32 * j + s % 8 * 4 : kRun * j + 4 * s; }
+  __device__ static int v_column(int i, int g) { return kVCols * g + i; }
+};
+
+template <typename T, int D, int NB>
+__global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kernel(const __grid_constant__ FourArgs args) {
+  using C = FourBlock<D, NB>;
+  using Cols = FourCols<D>;
+  constexpr int RU = C::RU, kSteps = D / 16, kTiles = D / 16;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const PagedArgs& a = args.p;
+  paged_block<C>(a, nullptr, nullptr, smem, [&](Ring<C>& ring, int warp) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
+    const int key_g = key_at(g), key_0 = key_at(2 * j), key_1 = key_at(2 * j + 1);
+    const int turn_g = four_turn(key_g, D), turn_0 = four_turn(key_0, D), turn_1 = four_turn(key_1, D);
+    constexpr int kKWords = Cols::kRun / 8, kKPieces = D == 256 ? 2 : 1;
+    constexpr int kVWords = D >= 64 ? D / 64 : 1;
+    // offsets of a lane's bytes in a tile of 16 keys, codes and scales (the turn of a key and of the key 8 behind it are the same)
+    unsigned k_at[kKPieces], v_at[2];
+#pragma unroll
+    for (int p = 0; p < kKPieces; ++p)
+      k_at[p] = key_g * C::kCodeBytes + (D >= 128 ? ((j + 4 * p) ^ turn_g) * 16 : j * (D / 8));
+    const int v_byte = g * (D / 16);
+    v_at[0] = key_0 * C::kCodeBytes + ((v_byte / 16) ^ turn_0) * 16 + v_byte % 16;
+    v_at[1] = key_1 * C::kCodeBytes + ((v_byte / 16) ^ turn_1) * 16 + v_byte % 16;
+    unsigned qb[NB][kSteps][2];
+    float o[NB][kTiles][4];
+    float m_run[NB][2], l_run[NB][2], factor[NB][2];  // of heads 2 j and 2 j + 1 of the eight
+    const int total = ring.total;
+    for (int s = 0; s < total; ++s) {
+      const int slot = s % C::kStages;
+      const StageInfo u = ring.info[slot];
+      if (u.first) {  // (while the copy is on its way)
+        // Q as B fragments, fp16: a row is brought to a largest magnitude of 1 to 2 by a power of two, which leaves all of it
+        // that counts: fp16 rows and bf16 ones lose nothing above 2^-14 of their largest element, and below it less than 2^-25 of that.
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          int b, h;
+          const bool is = unit_row<RU>(a, u, nb * 8 + g, &b, &h);
+          const T* const src = static_cast<const T*>(a.q) + (is ? static_cast<size_t>(b) * a.H + h : 0) * D;
+          float most = 0.f;
+#pragma unroll
+          for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(is ? element(src + Cols::k_column(st, j) + e) : 0.f));
+          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+          // 2^-e by the exponent's bits (rows of zeros, of what is below 2^-100 or not finite: as they are)
+          const int e = static_cast<int>(__float_as_uint(most) >> 23) - 127;
+          const bool plain = e < -100 || e > 127;
+          const float down = plain ? 1.f : __uint_as_float(static_cast<unsigned>(127 - (e > 126 ? 126 : e)) << 23);
+          const float up = plain ? 1.f : 1.f / down;
+#pragma unroll
+          for (int st = 0; st < kSteps; ++st) {
+            const T* const x = src + Cols::k_column(st, j);
+            qb[nb][st][0] = is ? pack_pair<__half>(element(x) * down, element(x + 1) * down) : 0u;
+            qb[nb][st][1] = is ? pack_pair<__half>(element(x + 2) * down, element(x + 3) * down) : 0u;
+          }
+          const float f = up * args.k_factor * a.scale_log2;
+          factor[nb][0] = __shfl_sync(0xffffffffu, f, 8 * j);
+          factor[nb][1] = __shfl_sync(0xffffffffu, f, 8 * j + 4);
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i) o[nb][i][0] = o[nb][i][1] = o[nb][i][2] = o[nb][i][3] = 0.f;
+          m_run[nb][0] = m_run[nb][1] = -INFINITY;
+          l_run[nb][0] = l_run[nb][1] = 0.f;  // this lane's share of the sums
+        }
+      }
+      if (!ring.wait(s)) return;
+      const unsigned k_tile = ring.tiles + 2 * slot * C::kTileBytes, v_tile = k_tile + C::kTileBytes;
+#pragma unroll 1
+      for (int key0 = 0; key0 < C::SR; key0 += 16) {
+        const int n_valid = u.keys - key0;  // keys from here on
+        if (n_valid <= 0) break;
+        if (!(u.pages >> (key0 / 16) & 1u)) continue;
+        // S^T = K Q^T: keys g and g + 8 of the tile, heads 2 j and 2 j + 1
+        float sc[NB][4];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
+        const unsigned k_codes = k_tile + key0 * C::kCodeBytes;
+        const unsigned k_scales = k_tile + C::SR * C::kCodeBytes + (key0 + key_g) * C::kScaleBytes;
+#pragma unroll
+        for (int p = 0; p < kKPieces; ++p) {
+          unsigned w[2][kKWords];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) load_words<kKWords>(k_codes + r * 8 * C::kCodeBytes + k_at[p], w[r]);
+          // scales of the lane's blocks, two to a piece of 32 columns
+          unsigned sk[2][2];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const unsigned at = k_scales + r * 8 * C::kScaleBytes;
+            if constexpr (D >= 128) {
+              const unsigned both = scales_to_half(static_cast<unsigned short>(load_u16(at + 8 * p + 2 * j)));
+              sk[r][0] = __byte_perm(both, both, 0x1010);
+              sk[r][1] = __byte_perm(both, both, 0x3232);
+            } else {
+              const unsigned one = load_u8(at + (D == 64 ? j : j / 2));
+              sk[r][0] = sk[r][1] = scales_to_half(static_cast<unsigned short>(one | one << 8));
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < kKWords; ++i) {
+            unsigned h[2][4];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              codes_to_half(w[r][i], h[r]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) h[r][e] = mul_half2(h[r][e], sk[r][i / 2]);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const unsigned ka[4] = {h[0][2 * e], h[1][2 * e], h[0][2 * e + 1], h[1][2 * e + 1]};
+              const int st = p * 8 + 2 * i + e;
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) mma16816<__half>(sc[nb], ka, qb[nb][st][0], qb[nb][st][1]);
+            }
+          }
+        }
+        const bool in0 = key_g < n_valid, in1 = key_g + 8 < n_valid;
+        bool more = false;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[nb][i] = (i < 2 ? in0 : in1) ? sc[nb][i] * factor[nb][i & 1] : -INFINITY;
+          more = more || fmaxf(sc[nb][0], sc[nb][2]) > m_run[nb][0] || fmaxf(sc[nb][1], sc[nb][3]) > m_run[nb][1];
+        }
+        if (__any_sync(0xffffffffu, more)) {  // rare after the first stages
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            float f[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float mx = fmaxf(sc[nb][c], sc[nb][2 + c]);
+#pragma unroll
+              for (int d = 4; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+              const float mn = fmaxf(m_run[nb][c], mx);
+              f[c] = m_run[nb][c] == -INFINITY ? 0.f : ex2(m_run[nb][c] - mn);
+              l_run[nb][c] = m_run[nb][c] == -INFINITY ? l_run[nb][c] : l_run[nb][c] * f[c];  // (0, or NaN to keep)
+              m_run[nb][c] = mn;
+            }
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+              o[nb][i][0] *= f[0];
+              o[nb][i][1] *= f[1];
+              o[nb][i][2] *= f[0];
+              o[nb][i][3] *= f[1];
+            }
+          }
+        }
+        // P^T as the B fragments of the second product, rounded to fp16 (l is not): 2^-12 of a weight
+        unsigned pb[NB][2];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          float p[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float m = m_run[nb][i & 1];
+            p[i] = ex2(sc[nb][i] - (m == -INFINITY ? 0.f : m));
+          }
+          l_run[nb][0] += p[0] + p[2];
+          l_run[nb][1] += p[1] + p[3];
+          pb[nb][0] = transposed(pack_pair<__half>(p[0], p[1]));
+          pb[nb][1] = transposed(pack_pair<__half>(p[2], p[3]));
+        }
+        // O^T += V^T P^T
+        const unsigned v_codes = v_tile + key0 * C::kCodeBytes;
+        const unsigned v_scales = v_tile + C::SR * C::kCodeBytes + key0 * C::kScaleBytes;
+        unsigned va[2][2][kTiles];  // [keys 2 j.., 2 j + 8..][rows g, g + 8][tile]: pairs of keys
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          unsigned w[2][kVWords];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const unsigned at = v_codes + r * 8 * C::kCodeBytes + v_at[e];
+            if constexpr (D >= 64) load_words<kVWords>(at, w[e]);
+            else w[e][0] = load_u16(at);
+          }
+          // the scales of the two keys, of the block of row g and of that of row g + 8 (head_dim 256: the next block); 0 for
+          // keys that are not the sequence's, whose bytes may be anything
+          unsigned sv[2];
+          {
+            const bool is0 = key_0 + 8 * r < n_valid, is1 = key_1 + 8 * r < n_valid;
+            const unsigned at0 = v_scales + (key_0 + 8 * r) * C::kScaleBytes, at1 = v_scales + (key_1 + 8 * r) * C::kScaleBytes;
+            if constexpr (D == 256) {
+              const unsigned s0 = is0 ? load_u16(at0 + 2 * g) : 0u, s1 = is1 ? load_u16(at1 + 2 * g) : 0u;
+              const unsigned both = __byte_perm(s0, s1, 0x5140);  // (s0.lo, s1.lo, s0.hi, s1.hi)
+              sv[0] = scales_to_half(static_cast<unsigned short>(both));
+              sv[1] = scales_to_half(static_cast<unsigned short>(both >> 16));
+            } else {
+              constexpr int kLanes = 128 / D;  // lanes to a block
+              const unsigned s0 = is0 ? load_u8(at0 + g / kLanes) : 0u, s1 = is1 ? load_u8(at1 + g / kLanes) : 0u;
+              sv[0] = sv[1] = scales_to_half(static_cast<unsigned short>(s0 | s1 << 8));
+            }
+          }
+          // the codes of the two keys change places so that those of a column lie in a byte
+          unsigned h[kVWords][2][4];
+#pragma unroll
+          for (int i = 0; i < kVWords; ++i) {
+            const unsigned even = (w[0][i] & 0x0f0f0f0fu) | ((w[1][i] << 4) & 0xf0f0f0f0u);
+            const unsigned odd = ((w[0][i] >> 4) & 0x0f0f0f0fu) | (w[1][i] & 0xf0f0f0f0u);
+            codes_to_half(even, h[i][0]);
+            codes_to_half(odd, h[i][1]);
+          }
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int col = i + x * Cols::v_other;  // of the lane's
+              va[r][x][i] = mul_half2(h[col / 8][col % 2][col % 8 / 2], sv[x]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+          const unsigned av[4] = {va[0][0][i], va[0][1][i], va[1][0][i], va[1][1][i]};
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) mma16816<__half>(o[nb][i], av, pb[nb][0], pb[nb][1]);
+        }
+      }
+      __syncwarp();
+      if (s > 0) ring.copy_next((s - 1) % C::kStages);
+      if (u.last) {
+        const size_t part = (static_cast<size_t>(blockIdx.x) * C::kWarps + warp + u.uid) * a.rs;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float l = l_run[nb][c];
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) l += __shfl_xor_sync(0xffffffffu, l, d);
+            const int r = nb * 8 + 2 * j + c;
+            int b, h;
+            if (!unit_row<RU>(a, u, r, &b, &h)) continue;
+            const bool result = u.last == 2;
+            const float f = !result ? args.v_factor : l == 0.f ? 0.f : args.v_factor / l;  // (no key seen: O is 0 as well)
+            constexpr int kEach = D / 16;  // columns side by side of row g, as many of row g + 8 behind them
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int col = Cols::v_column(0, g) + x * Cols::v_other;
+              if (result) {
+                T* const dst = static_cast<T*>(a.out) + (static_cast<size_t>(b) * a.H + h) * D + col;
+#pragma unroll
+                for (int i = 0; i < kEach; i += 2)
+                  *reinterpret_cast<unsigned*>(dst + i) = pack_pair<T>(o[nb][i][2 * x + c] * f, o[nb][i + 1][2 * x + c] * f);
+              } else {
+                float* const dst = a.part_o + (part + r) * D + col;
+#pragma unroll
+                for (int i = 0; i < kEach; i += 2)
+                  *reinterpret_cast<float2*>(dst + i) = make_float2(o[nb][i][2 * x + c] * f, o[nb][i + 1][2 * x + c] * f);
+              }
+            }
+            if (g == 0) {
+              if (!result) a.part_ml[part + r] = make_float2(m_run[nb][c], l);
+              else if (a.lse)
+                a.lse[static_cast<size_t>(b) * a.H + h] = l > 0.f ? m_run[nb][c] * kLn2 + logf(l) : l == 0.f ? -INFINITY : l;
+            }
+          }
+      }
+    }
+  });
+}
+
+// ---- rows back out of a cache --------------------------------------------------------
+
+struct ReadRows {
+  char* data;
+  long long row, head;  // strides in elements
+};
+struct ReadArgs {
+  const char* pages[2];  // k, v
+  ReadRows out[2];
+  const int* table;
+  long long table_stride;
+  const int* ends;   // sequence b's rows are rows ends[b] to ends[b + 1] of the results
+  const int* start;  // the first of them in the cache (NULL: 0)
+  int rows, num_pages, max_pages, shift, B, kvH;
+  int vec;           // every row of the results is 16-byte aligned
+  float factor[2];
+};
+
+// A block has kTokens rows of the results: it finds out whose they are and where, and copies them for all heads, 16 bytes of a row a
+// thread, or (4 bits) one block of 16 elements. Bound by memory: a row comes in once and goes out once.
+constexpr int kReadThreads = 256, kReadTokens = 8;
+template <typename T, int D, bool kFour>
+__global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const __grid_constant__ ReadArgs a) {
+  constexpr int kEach = kFour ? 16 : 16 / static_cast<int>(sizeof(T)), kPieces = D / kEach, kOf = kReadTokens * kPieces;
+  constexpr int kWords = kEach * static_cast<int>(sizeof(T)) / 4, kAhead = 4;
+  __shared__ long long place_of[kReadTokens];
+  let_next_start();
+  wait_for_previous();
+  const int token0 = static_cast<int>(blockIdx.x) * kReadTokens;
+  if (threadIdx.x < kReadTokens) {
+    const int i = token0 + static_cast<int>(threadIdx.x);
+    long long place = -2;  // a row of the results that is no sequence's stays as it is
+    if (i < a.rows && i >= a.ends[0] && i < a.ends[a.B]) {
+      int lo = 0, hi = a.B;  // ends[lo] <= i < ends[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (a.ends[mid] <= i) lo = mid;
+        else hi = mid;
+      }
+      place = paged_row(a.table + lo * a.table_stride, a.max_pages, a.num_pages, a.shift, a.kvH,
+                        static_cast<long long>(a.start ? a.start[lo] : 0) + (i - a.ends[lo]));
+    }
+    place_of[threadIdx.x] = place;
+  }
+  __syncthreads();
+  const int total = 2 * a.kvH * kOf;
+  for (int i0 = threadIdx.x; i0 < total; i0 += kAhead * kReadThreads) {
+    unsigned u[kAhead][kFour ? 3 : kWords];
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) {
+      const int i = i0 + n * kReadThreads;
+      if (i >= total) break;
+      const int side_head = i / kOf, token = i % kOf / kPieces, piece = i % kPieces;
+      const int side = side_head >= a.kvH, head = side_head - side * a.kvH;
+      const long long place = place_of[token];
+#pragma unroll
+      for (int w = 0; w < (kFour ? 3 : kWords); ++w) u[n][w] = 0u;  // a row that there is not is zeros
+      if (place < 0) continue;
+      if constexpr (kFour) {
+        const int row = static_cast<int>(place) & ((1 << a.shift) - 1);
+        const char* const page = a.pages[side] + (((place >> a.shift) + head) << a.shift) * four_row_bytes(D);
+        const uint2 c = *reinterpret_cast<const uint2*>(page + row * (D / 2) + ((piece / 2) ^ four_turn(row, D)) * 16 + piece % 2 * 8);
+        u[n][0] = c.x, u[n][1] = c.y;
+        u[n][2] = static_cast<unsigned char>(page[(D / 2 << a.shift) + row * (D / 16) + piece]);
+      } else {
+        const uint4 v = *reinterpret_cast<const uint4*>(
+            a.pages[side] + ((place + (static_cast<long long>(head) << a.shift)) * D + piece * kEach) * sizeof(T));
+        u[n][0] = v.x, u[n][1] = v.y, u[n][2] = v.z, u[n][3] = v.w;
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) {
+      const int i = i0 + n * kReadThreads;
+      if (i >= total) break;
+      const int side_head = i / kOf, token = i % kOf / kPieces, piece = i % kPieces;
+      const int side = side_head >= a.kvH, head = side_head - side * a.kvH;
+      if (place_of[token] == -2) continue;
+      const ReadRows out = a.out[side];
+      T* const dst = reinterpret_cast<T*>(out.data) + (token0 + token) * out.row + head * out.head + piece * kEach;
+      unsigned w[kWords];
+      if constexpr (kFour) {
+        const unsigned s = scales_to_half(static_cast<unsigned short>(u[n][2] | u[n][2] << 8));
+        unsigned h[2][4];
+        codes_to_half(u[n][0], h[0]);
+        codes_to_half(u[n][1], h[1]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const unsigned v = mul_half2(h[e / 4][e % 4], s);
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+          w[e] = pack_pair<T>(f.x * a.factor[side], f.y * a.factor[side]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < kWords; ++e) w[e] = u[n][e];
+      }
+      if (a.vec) {
+#pragma unroll
+        for (int e = 0; e < kWords; e += 4) reinterpret_cast<uint4*>(dst)[e / 4] = make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
+      } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int e = 0; e < kWords; ++e) dst[e] = __uint_as_float(w[e]);
+      } else {
+        unsigned short* const to = reinterpret_cast<unsigned short*>(dst);
+#pragma unroll
+        for (int e = 0; e < kWords; ++e) to[2 * e] = static_cast<unsigned short>(w[e]), to[2 * e + 1] = static_cast<unsigned short>(w[e] >> 16);
+      }
+    }
+  }
+}
+
+// ---- host side ----------------------------------------------------------------------
+
+struct FourPlan {
+  int NB, HB, blocks, warps, rs;
+  double most;  // stages that there can be
+  size_t unit_bytes, ml_bytes, bytes;
+};
+
+FourPlan make_plan(const ra_paged_kv& c, int heads) {
+  FourPlan p = {};
+  const int G = (heads + c.kv_heads - 1) / c.kv_heads;
+  p.NB = G > 8 ? 2 : 1;
+  p.HB = (G + 8 * p.NB - 1) / (8 * p.NB);
+  p.warps = c.head_dim * p.NB <= 128 ? 8 : 4;
+  const size_t units = static_cast<size_t>(c.kv_heads) * c.batch * p.HB;
+  const long long room = static_cast<long long>(c.max_pages) * c.page_size;
+  p.most = static_cast<double>(units) * ((room + 31) / 32);
+  const int wave = kBlocksPerSm * sm_count();
+  p.blocks = p.most < static_cast<double>(wave) * p.warps ? (static_cast<int>(p.most) + p.warps - 1) / p.warps : wave;
+  p.rs = std::min(8 * p.NB, G);
+  auto whole = [](size_t n) { return (n + 127) & ~static_cast<size_t>(127); };
+  const size_t rows = (units + static_cast<size_t>(p.blocks) * p.warps) * p.rs;
+  p.unit_bytes = whole(units * sizeof(int2));
+  p.ml_bytes = whole(rows * sizeof(float2));
+  p.bytes = p.unit_bytes + p.ml_bytes + rows * c.head_dim * sizeof(float);
+  return p;
+}
+
+template <typename T, int D, int NB>
+int launch_four(const FourArgs& a, const FourPlan& p, cudaStream_t stream) {
+  if (p.blocks > 0) {
+    const int rc = launch_main<paged_4bit_kernel<T, D, NB>, FourBlock<D, NB>>(p.blocks, stream, a);
+    if (rc != RA_OK) return rc;
+  }
+  return launch_fold<T, D, 8 * NB>(a.p, stream);
+}
+
+bool power_of_two(float f) { return f >= 1.0f / (1 << 30) && f <= 1 << 30 && std::exp2(std::round(std::log2(f))) == f; }
+
+}  // namespace
+
+int check_paged_4bit(const ra_paged_kv& c, float k_scale, float v_scale, const char* what) {
+  RAB_REQUIRE(c.dtype == RA_F16 || c.dtype == RA_BF16, RA_ERR_INVALID, "%s: rows are fp16 or bf16, got dtype %d", what, c.dtype);
+  RAB_REQUIRE(c.head_dim == 32 || c.head_dim == 64 || c.head_dim == 128 || c.head_dim == 256, RA_ERR_UNSUPPORTED,
+              "%s: unsupported head_dim=%d (supported: 32, 64, 128, 256)", what, c.head_dim);
+  RAB_REQUIRE(power_of_two(k_scale) && power_of_two(v_scale), RA_ERR_INVALID,
+              "%s: k_scale and v_scale are powers of two from 2^-30 to 2^30", what);
+  return check_paged(c, what);
+}
+
+namespace {
+
+int check_decode(const ra_paged_kv& c, int heads, float k_scale, float v_scale) {
+  const char* const what = "paged_decode_4bit";
+  const int rc = check_paged_4bit(c, k_scale, v_scale, what);
+  if (rc != RA_OK) return rc;
+  RAB_REQUIRE(heads >= c.kv_heads && heads <= 4096, RA_ERR_INVALID, "%s: bad heads", what);
+  RAB_REQUIRE(static_cast<long long>(c.batch) * heads < (1ll << 24), RA_ERR_INVALID, "%s: too many rows", what);
+  RAB_REQUIRE(static_cast<long long>(c.num_pages) * c.kv_heads < (1ll << 31) - 1, RA_ERR_INVALID, "%s: too many pages", what);
+  return RA_OK;
+}
+
+// The entry points that read rows back. `kFour`: out of a cache in 4 bits.
+template <bool kFour>
+int read_rows(const char* what, const ra_paged_kv* cache, float k_scale, float v_scale, const int* ends, const int* start,
+              const ra_rows* k_out, const ra_rows* v_out, int rows, cudaStream_t stream) {
+  RAB_REQUIRE(cache && k_out && v_out, RA_ERR_INVALID, "%s: null argument", what);
+  ra_paged_kv c = *cache;
+  c.lens = ends;  // (lengths are not read)
+  int rc = RA_OK;
+  if (kFour) {
+    rc = check_paged_4bit(c, k_scale, v_scale, what);
+  } else {
+    RAB_REQUIRE(c.dtype == RA_F32 || c.dtype == RA_F16 || c.dtype == RA_BF16, RA_ERR_INVALID, "%s: unknown dtype %d", what, c.dtype);
+    RAB_REQUIRE(c.head_dim == 32 || c.head_dim == 64 || c.head_dim == 128 || c.head_dim == 256, RA_ERR_UNSUPPORTED,
+                "%s: unsupported head_dim=%d (supported: 32, 64, 128, 256)", what, c.head_dim);
+    rc = check_paged(c, what);
+  }
+  if (rc == RA_OK) rc = check_lists(c, what);
+  if (rc != RA_OK) return rc;
+  RAB_REQUIRE(rows >= 0, RA_ERR_INVALID, "%s: bad shape", what);
+  RAB_REQUIRE(c.kv_heads <= 1 << 16, RA_ERR_INVALID, "%s: bad heads", what);
+  if (c.batch == 0 || rows == 0) return RA_OK;
+  const int es = c.dtype == RA_F32 ? 4 : 2;
+  RAB_REQUIRE(k_out->data && v_out->data, RA_ERR_INVALID, "%s: null argument", what);
+  RAB_REQUIRE(((reinterpret_cast<uintptr_t>(k_out->data) | reinterpret_cast<uintptr_t>(v_out->data)) & (es - 1u)) == 0 &&
+                  (reinterpret_cast<uintptr_t>(start) & 3u) == 0,
+              RA_ERR_INVALID, "%s: rows or start are not aligned to their elements", what);
+  ReadArgs a;
+  std::memset(&a, 0, sizeof(a));
+  const ra_rows* out[2] = {k_out, v_out};
+  unsigned long long all = 0;
+  for (int i = 0; i < 2; ++i) {
+    a.out[i] = {static_cast<char*>(out[i]->data), out[i]->row_stride, out[i]->head_stride};
+    all |= reinterpret_cast<uintptr_t>(out[i]->data);
+    if (rows > 1) all |= static_cast<unsigned long long>(out[i]->row_stride) * es;
+    if (c.kv_heads > 1) all |= static_cast<unsigned long long>(out[i]->head_stride) * es;
+  }
+  a.vec = (all & 15u) == 0;
+  a.pages[0] = static_cast<const char*>(c.k);
+  a.pages[1] = static_cast<const char*>(c.v);
+  a.table = c.page_table;
+  a.table_stride = c.table_stride;
+  a.ends = ends;
+  a.start = start;
+  a.rows = rows;
+  a.num_pages = c.num_pages;
+  a.max_pages = c.max_pages;
+  a.shift = page_shift(c.page_size);
+  a.B = c.batch;
+  a.kvH = c.kv_heads;
+  a.factor[0] = k_scale;
+  a.factor[1] = v_scale;
+  auto go = [&](auto t, auto d) -> int {
+    RAB_CUDA(launch_overlapped(paged_read_kernel<decltype(t), d(), kFour>, dim3((static_cast<unsigned>(rows) + kReadTokens - 1) / kReadTokens),
+                               dim3(kReadThreads), 0, stream, a));
+    return RA_OK;
+  };
+  auto by_dim = [&](auto t) -> int {
+    if (c.head_dim == 32) return go(t, std::integral_constant<int, 32>());
+    if (c.head_dim == 64) return go(t, std::integral_constant<int, 64>());
+    if (c.head_dim == 128) return go(t, std::integral_constant<int, 128>());
+    return go(t, std::integral_constant<int, 256>());
+  };
+  if constexpr (!kFour) {
+    if (c.dtype == RA_F32) return by_dim(float());
+  }
+  return c.dtype == RA_BF16 ? by_dim(__nv_bfloat16()) : by_dim(__half());
+}
+
+}  // namespace
+}  // namespace rab
+
+using namespace rab;
+
+extern "C" {
+
+size_t ra_paged_decode_4bit_workspace_bytes(const ra_paged_kv* cache, int heads) {
+  if (!cache || check_decode(*cache, heads, 1.f, 1.f) != RA_OK) return 0;
+  ra_paged_kv c = *cache;
+  if (c.num_pages == 0) c.max_pages = 0;
+  return make_plan(c, heads).bytes;
+}
+
+int ra_paged_decode_4bit(const ra_paged_kv* cache, float k_scale, float v_scale, const void* q, int heads, void* out, float* lse,
+                         void* workspace, size_t workspace_bytes, ra_stream stream_) {
+  const char* const what = "paged_decode_4bit";
+  RAB_REQUIRE(cache != nullptr, RA_ERR_INVALID, "%s: null argument", what);
+  int rc = check_decode(*cache, heads, k_scale, v_scale);
+  if (rc == RA_OK) rc = check_lists(*cache, what);
+  if (rc != RA_OK) return rc;
+  if (cache->batch == 0) return RA_OK;
+  RAB_REQUIRE(q && out, RA_ERR_INVALID, "%s: null argument", what);
+  RAB_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0, RA_ERR_INVALID,
+              "%s: q and out must be 16-byte aligned", what);
+  RAB_REQUIRE((reinterpret_cast<uintptr_t>(lse) & 3u) == 0, RA_ERR_INVALID, "%s: lse is not aligned to its elements", what);
+  ra_paged_kv c = *cache;
+  if (c.num_pages == 0) c.max_pages = 0;  // (holds no keys, whatever the tables say)
+  const FourPlan p = make_plan(c, heads);
+  RAB_REQUIRE(p.most < 2147483648.0 * std::max(p.blocks * p.warps, 1), RA_ERR_INVALID, "%s: too many keys", what);
+  RAB_REQUIRE(workspace && workspace_bytes >= p.bytes && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, RA_ERR_OVERFLOW,
+              "%s: workspace too small or not 16-byte aligned", what);
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  unsigned char* const ws = static_cast<unsigned char*>(workspace);
+  FourArgs f;
+  std::memset(&f, 0, sizeof(f));
+  f.k_factor = k_scale;
+  f.v_factor = v_scale;
+  PagedArgs& a = f.p;
+  a.q = q;
+  a.k = c.k;
+  a.v = c.v;
+  a.out = out;
+  a.lse = lse;
+  a.table = c.page_table;
+  a.table_stride = c.table_stride;
+  a.lens = c.lens;
+  a.num_pages = c.num_pages;
+  a.max_pages = c.max_pages;
+  a.shift = page_shift(c.page_size);
+  a.B = c.batch;
+  a.H = heads;
+  a.kvH = c.kv_heads;
+  a.G = (heads + c.kv_heads - 1) / c.kv_heads;
+  a.HB = p.HB;
+  a.rs = p.rs;
+  a.scale_log2 = kLog2e / std::sqrt(static_cast<float>(c.head_dim));
+  a.unit_parts = reinterpret_cast<int2*>(ws);
+  a.part_ml = reinterpret_cast<float2*>(ws + p.unit_bytes);
+  a.part_o = reinterpret_cast<float*>(ws + p.unit_bytes + p.ml_bytes);
+  a.status = device_status_ptr();
+  RAB_REQUIRE(a.status != nullptr, RA_ERR_CUDA, "%s: no device status word", what);
+  a.wait_ns = tcgen::tc_wait_limit_ns();
+  a.shares = p.blocks * p.warps;
+  const int stall = tcgen::tc_stall_after();
+  a.missing = stall > 0 ? 16 : stall == 0 ? -1 : 0;
+  auto go = [&](auto t, auto d) -> int {
+    using T = decltype(t);
+    return p.NB == 1 ? launch_four<T, d(), 1>(f, p, stream) : launch_four<T, d(), 2>(f, p, stream);
+  };
+  auto by_dim = [&](auto t) -> int {
+    if (c.head_dim == 32) return go(t, std::integral_constant<int, 32>());
+    if (c.head_dim == 64) return go(t, std::integral_constant<int, 64>());
+    if (c.head_dim == 128) return go(t, std::integral_constant<int, 128>());
+    return go(t, std::integral_constant<int, 256>());
+  };
+  return c.dtype == RA_BF16 ? by_dim(__nv_bfloat16()) : by_dim(__half());
+}
+
+int ra_paged_read(const ra_paged_kv* cache, const int* ends, const int* start, const ra_rows* k_out, const ra_rows* v_out, int rows,
+                  ra_stream stream) {
+  return read_rows<false>("paged_read", cache, 1.f, 1.f, ends, start, k_out, v_out, rows, static_cast<cudaStream_t>(stream));
+}
+
+int ra_paged_read_4bit(const ra_paged_kv* cache, float k_scale, float v_scale, const int* ends, const int* start,
+                       const ra_rows* k_out, const ra_rows* v_out, int rows, ra_stream stream) {
+  return read_rows<true>("paged_read_4bit", cache, k_scale, v_scale, ends, start, k_out, v_out, rows, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"
