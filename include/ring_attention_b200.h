@@ -68,6 +68,7 @@ typedef struct ra_segmap {
 } ra_segmap;
 
 typedef void* ra_stream; /* a cudaStream_t */
+struct ra_rows;           /* rows with strides of their own, see below */
 
 RA_API const char* ra_last_error(void);
 RA_API int ra_version(void);
@@ -249,6 +250,20 @@ RA_API int ra_prefill_host(int dtype, const void* q_host, const void* k_host, co
                            float* out_host, float* lse_host, const ra_shape* shape,
                            const ra_segmap* qmap, const ra_segmap* kmap, int pos_stride,
                            unsigned flags, long long doc_len);
+
+/* Attention over packed sequences of unlike lengths, 16 bits in and out: q and out are (rows, heads, head_dim), k and v (key rows,
+ * kv heads, head_dim), with any strides whose rows and heads begin at multiples of 16 bytes and do not overlap (a fused projection's
+ * output as it is; batch_stride is not used). Sequence b of shape->batch has query rows ends[b] to ends[b + 1] of the shape->seq_q
+ * there are and key rows k_ends[b] to k_ends[b + 1] of shape->seq_k (device, batch + 1 each, rising; k_ends NULL: ends). With `causal`, query i of a
+ * sequence sees its keys j <= i + keys - queries: a whole prompt, or a prompt's next rows behind those that a cache has of it
+ * (ra_paged_read brings them). lse (heads, seq_q; fp32, or NULL) gets the log of the sum of exponentials. A row that sees no key gives zeros and
+ * -inf; rows of no sequence stay as they are. heads is a multiple of kv heads. Sums and the softmax are held in 32 bits, the weights of the sum over V are rounded
+ * to dtype as in ra_attention_step_fp16, and the result once. What is not finite in a sequence's K or V does not reach other
+ * sequences; in its own, a value with weight 0 may reach queries of the same 128 keys. A bounded wait that runs out is reported as of the step kernels, and
+ * rows that are not finished then stay as they are. out must not share memory with q, k or v. */
+RA_API int ra_packed_attention(int dtype, const struct ra_rows* q, const struct ra_rows* k, const struct ra_rows* v,
+                               const struct ra_rows* out, float* lse, const ra_shape* shape, const int* ends, const int* k_ends,
+                               int causal, ra_stream stream);
 
 /* ------------------------------------------------------------------- decode ---- */
 

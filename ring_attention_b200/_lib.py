@@ -211,6 +211,7 @@ _SIG = {
                                   C.POINTER(NormRope), _P]),
     "ra_paged_decode_workspace_bytes": (C.c_size_t, [C.POINTER(PagedKV), C.c_int, C.c_int]),
     "ra_paged_decode": (C.c_int, [C.POINTER(PagedKV), _P, C.c_int, _P, C.c_int, _P, _P, _P, C.c_size_t, _P]),
+    "ra_packed_attention": (C.c_int, [C.c_int, _ROWS, _ROWS, _ROWS, _ROWS, _P, C.POINTER(Shape), _P, _P, C.c_int, _P]),
     "ra_paged_read": (C.c_int, [C.POINTER(PagedKV), _P, _P, _ROWS, _ROWS, C.c_int, _P]),
     "ra_paged_append_4bit": (C.c_int, [C.POINTER(PagedKV), C.c_float, C.c_float, _ROWS, _ROWS, C.c_int, _P, _ROWS, _ROWS, C.c_int,
                                        C.POINTER(NormRope), _P]),

@@ -672,6 +672,29 @@ def _packed_rows(t, shape, dtype, out=False):
     return PACK_ROWS(t.data_ptr(), 0, sh, sr)
 
 
+def packed_attention(q, k, v, ends, out, *, k_ends=None, causal=True, lse=None):
+    """Attention over packed sequences of unlike lengths, fp16 or bf16: q and out are (rows, heads, head_dim), k and v (key rows,
+    kv_heads, head_dim), with any strides whose rows and heads begin at multiples of 16 bytes (slices of a fused projection go in
+    as they are); heads is a multiple of kv_heads, query head h reads KV head h % kv_heads. Sequence b has query rows ends[b] to
+    ends[b + 1] and key rows k_ends[b] to k_ends[b + 1] ((batch + 1,), int32, rising; None: those of ``ends``); with ``causal`` its query i sees
+    its keys j <= i + keys - queries: whole prompts, or the next rows of prompts behind what ``paged_read`` brings of them. ``lse``
+    ((heads, rows), fp32) gets the log-sum-exp. A row that sees no key gives zeros and -inf; rows of no sequence stay as they are."""
+    dev = _on_device(q, k, v, ends, k_ends, out, lse)
+    shape, kv_shape, dt = q.shape, k.shape, q.dtype
+    if len(shape) != 3 or len(kv_shape) != 3 or kv_shape[2] != shape[2] or (dt is not torch.float16 and dt is not torch.bfloat16):
+        raise ValueError("packed_attention: expected (rows, heads, head_dim) queries in fp16 or bf16 and keys with as many elements a row")
+    rows, H, D = shape
+    B = ends.numel() - 1
+    if B < 0:
+        raise ValueError("packed_attention: ends has batch + 1 elements")
+    if lse is not None and (lse.shape != (H, rows) or lse.dtype != torch.float32):
+        raise ValueError("packed_attention: lse is (heads, rows) in fp32")
+    check(packed("ra_packed_attention")(_DT[dt], _packed_rows(q, shape, dt), _packed_rows(k, kv_shape, dt), _packed_rows(v, kv_shape, dt),
+                                        _packed_rows(out, shape, dt, True), _ptr(lse), PACK_SHAPE(B, H, rows, kv_shape[0], D, kv_shape[1]),
+                                        _int32(ends, (B + 1,), "ends"), _int32(k_ends, (B + 1,), "k_ends") if k_ends is not None else None,
+                                        int(causal), _raw_stream(dev)))
+
+
 def paged_read(k_pages, v_pages, page_table, ends, k_out, v_out, *, start=None):
     """Rows of sequences out of a paged KV cache (see ``paged_append``), one sequence's behind the other's, as ``packed_attention``
     reads them: rows ends[b] to ends[b + 1] of k_out and v_out ((rows, kv_heads, head_dim), contiguous rows) get rows
