@@ -8,15 +8,17 @@
 //
 // An item is a block of query tokens of one sequence and a KV head. A query tile of 128 rows holds the same tokens of `pack` query heads
 // that share the KV head (one box of a 4-D tensor map), so that a tile has as few keys behind the diagonal as can be, and a sequence of 32
-// tokens fills one where four heads share a KV head; a block takes two tiles of neighbouring tokens (head_dim 256: one). The blocks
-// of one wave stay for the whole call and take the items, the most key tiles first, one after the other: tensor memory, barriers and rings
-// are set up once, and the next item's queries, keys and first scores come while the rows of the last one are written.
+// tokens fills one where four heads share a KV head; a block takes two tiles of neighbouring tokens (head_dim 256: one). The items
+// are numbered, those with the most key tiles first, and the blocks of one wave stay for the whole call and take one after the other:
+// tensor memory, barriers and rings are set up once, and the next item's queries, keys and first scores come while the rows of the last
+// one are written.
 //
 // Roles (384 threads; head_dim 256: 256): warp 0 copies with TMA, warps 1 and 2 issue tcgen05.mma (2: only where P has a place of its own,
 // head_dim 64), warp 3 finds the items, warps 4 to 7 and 8 to 11 are the softmax of either tile, a row a thread.
 //
-// Key tiles are counted from the sequence's first key. Of the last one only as many products are made as it has keys, in steps of 16; the
-// rest of the last step, which is the next sequence's, is put out of V's tile before. A value that is not finite reaches the queries of its own
+// Key tiles are counted from the sequence's first key. Of a query tile's last one only as many products are made as its rows see keys, in
+// steps of 16, and only the halves of its scores that a warp's rows see are worked on; what a last step has of the next sequence is put
+// out of V's tile before. A value that is not finite reaches the queries of its own
 // sequence whose weight for it is 0 only within that tile.
 #include <atomic>
 #include <type_traits>
@@ -37,7 +39,7 @@ struct PackedArgs {
   const int* ends;              // sequence b has query rows ends[b] to ends[b + 1]
   const int* k_ends;            // and keys
   int rows, k_rows, B, H, kvH, G;
-  int pack, tile_tokens, token_shift;  // heads of a tile, its tokens, and log2 of a block's tokens
+  int pack, tile_tokens, tile_shift, token_shift;  // heads of a tile, its tokens and their log2, and log2 of a block's tokens
   int head_sets;                       // ceil(G / pack)
   int causal;
   int* status;
@@ -60,17 +62,21 @@ struct PackedCfg {
   static constexpr int kBN = D == 256 ? 64 : 128;  // keys of a tile
   static constexpr int kBoxes = D / 64;
   static constexpr int kQBytes = kBM * D * 2, kKvBytes = kBN * D * 2;
-  static constexpr int kStages = D == 64 ? 6 : 4;
+  static constexpr int kStages = D == 64 ? 8 : 4;
   // head_dim 64: P has a place of its own and the next scores go out while P is made; 128: P overwrites S; 256: two score buffers, the
   // next but one scores go out behind the products with P that overwrites theirs
   static constexpr bool kEarlyS = D == 64, kDoubleS = D == 256, kOrdered = D == 128;
   static constexpr int kColS0 = 0, kColS1 = 128, kColO0 = 256, kColO1 = 256 + D;
   static constexpr int kColP0 = kEarlyS ? 384 : kColS0, kColP1 = kEarlyS ? 448 : kColS1;
+  // registers of the copying and issuing warps' threads and of the softmax threads (128 and 256, of 168 each at the start)
+  static constexpr int kRegsLo = D == 64 ? 104 : 72, kRegsHi = D == 64 ? 200 : 216;
+  static_assert(128 * kRegsLo + 256 * kRegsHi <= 384 * 168, "registers");
   static constexpr int kOffKv = kTiles * kQBytes;
   static constexpr int kOffOut = kOffKv + kStages * kKvBytes;  // rows on their way out: 4 KB a warp
   static constexpr int kOffBar = kOffOut + kTiles * 4 * 4096;
-  static constexpr int kNumBars = 4 + 2 * kStages + 8 + 4;
-  static constexpr int kOffItem = kOffBar + kNumBars * 8;
+  static constexpr int kNumBars = 4 + 2 * kStages + 8 + 6;
+  static constexpr int kOffNext = (kOffBar + kNumBars * 8 + 15) & ~15;  // the hardware's answer, see next_block
+  static constexpr int kOffItem = kOffNext + 16;
   static constexpr int kSmemBytes = kOffItem + 2 * static_cast<int>(sizeof(Item)) + 16 + 1024;
   static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
@@ -117,15 +123,14 @@ struct Items {
   const PackedArgs& a;
   int lane, of_block;  // items of a block of tokens
   Seq mine;            // lane's among the first 32 sequences
-  int level;           // key tiles of the last item found
+  int top, level;      // key tiles: the most, those of the last item found
   __device__ Items(const PackedArgs& a_, int lane_) : a(a_), lane(lane_), of_block(a_.kvH * a_.head_sets) {
     mine = Seq{0, 0, 0, 0, 0};
     if (lane < a.B) mine = sequence(a, lane);
-    level = 0;
     int most = mine.k_len;
     for (int b = lane + 32; b < a.B; b += 32) most = max(most, sequence(a, b).k_len);
     most = __reduce_max_sync(0xffffffffu, most);
-    level = (most + kBN - 1) / kBN;
+    top = level = (most + kBN - 1) / kBN;
   }
   __device__ Seq of(int b) const { return b < 32 ? mine : b < a.B ? sequence(a, b) : Seq{0, 0, 0, 0, 0}; }
   __device__ long long count(int c) const {  // blocks with c key tiles or more
@@ -134,13 +139,14 @@ struct Items {
     for (int b0 = 32; b0 < a.B; b0 += 32) sum += __reduce_add_sync(0xffffffffu, blocks_from<kBN>(a, of(b0 + lane), c));
     return sum;
   }
-  // (numbers rise from call to call)
+  // (quick where numbers rise from call to call)
   __device__ Item find(long long i) {
     Item it = {};
     const long long block = i / of_block;
-    if (count(level) <= block) {
-      if (count(0) <= block) return it;
-      int lo = 0, hi = level;  // count(lo) > block >= count(hi)
+    const bool lower = count(level) <= block;
+    if (lower || count(level + 1) > block) {
+      if (lower && count(0) <= block) return it;
+      int lo = lower ? 0 : level + 1, hi = lower ? level : top + 1;  // count(lo) > block >= count(hi)
       while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
         if (count(mid) > block) lo = mid;
@@ -187,6 +193,34 @@ __device__ inline void tma_load_4d(unsigned dst, const CUtensorMap* map, unsigne
       : "memory");
 }
 
+// Takes the next block of the grid that has not begun in its place: *number is its number; *more: there was one (if not, no further one
+// may be asked for). The answer goes to 16 bytes at `room` and `bar`; n counts the calls. Run by a warp; false: the wait ran out.
+template <typename Wait>
+__device__ inline bool take_block(unsigned room, unsigned bar, int n, unsigned* number, bool* more, Wait wait) {
+  if ((threadIdx.x & 31) == 0) {
+    mbar_expect_tx(bar, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(room), "r"(bar)
+                 : "memory");
+  }
+  __syncwarp();
+  if (!wait(bar, n & 1, 14, n)) return false;
+  unsigned got, x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 answer;\n\t"
+      "ld.shared.b128 answer, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, answer;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, answer;\n\t}"
+      : "=r"(got), "=r"(x)
+      : "r"(room)
+      : "memory");
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (the next answer comes behind this reading)
+  __syncwarp();
+  *more = got != 0;
+  *number = x;
+  return true;
+}
+
 // ---- kernel -------------------------------------------------------------------------
 
 // DR: head_dim of the tensors: D, or 32 on the 64-wide kernel, whose copies bring zeros for the upper half of every row.
@@ -206,6 +240,7 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
   const unsigned s_full = kv_free + 8 * C::kStages, s_free = s_full + 16;                // [2]
   const unsigned p_full = s_free + 16, o_done = p_full + 16;                             // [2]
   const unsigned item_full = o_done + 16, item_free = item_full + 16;                    // [2]
+  const unsigned next_full = item_free + 16, copied = next_full + 8;
   volatile Item* const items = reinterpret_cast<volatile Item*>(smem + C::kOffItem);
   unsigned* const tmem_slot = reinterpret_cast<unsigned*>(smem + C::kOffItem + 2 * sizeof(Item));
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -228,6 +263,8 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
       mbar_init(kv_full + 8 * s, 1);
       mbar_init(kv_free + 8 * s, C::kEarlyS ? 2 : 1);
     }
+    mbar_init(next_full, 1);
+    mbar_init(copied, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_map(&map_q);
@@ -250,28 +287,45 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, a.status, which, n, a.wait_ns)) != 0;
   };
   // The n-th item of this block; false: there is none, or the block gives up.
-  auto next_item = [&](int n, Item* it) {
-    if (!wait(item_full + 8 * (n & 1), (n >> 1) & 1, 11, n)) return false;
+  auto item_at = [&](int n) {
     const volatile Item& from = items[n & 1];
-    it->there = from.there, it->q0 = from.q0, it->q_len = from.q_len, it->k0 = from.k0, it->k_len = from.k_len;
-    it->token0 = from.token0, it->kv = from.kv, it->head = from.head;
+    Item it;
+    it.there = from.there, it.q0 = from.q0, it.q_len = from.q_len, it.k0 = from.k0, it.k_len = from.k_len;
+    it.token0 = from.token0, it.kv = from.kv, it.head = from.head;
+    return it;
+  };
+  auto give_item_back = [&](int n) {
     __syncwarp();
     if (lane == 0) mbar_arrive(item_free + 8 * (n & 1));
+  };
+  auto next_item = [&](int n, Item* it) {
+    if (!wait(item_full + 8 * (n & 1), (n >> 1) & 1, 11, n)) return false;
+    *it = item_at(n);
+    give_item_back(n);
     return it->there != 0;
   };
   auto tiles_of = [&](const Item& it, int w) { return w < C::kTiles ? (tile_keys<D>(a, it, w) + kBN - 1) / kBN : 0; };
 
   if (warp < 4) {
-    if constexpr (C::kTiles == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if constexpr (C::kTiles == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsLo));
     if (gone) {
     } else if (warp == 3) {
       // ------------------------------------------------------------------ items ----
+      // The grid has a block for every item that there can be, of which one for each SM runs. Its first item is that of its own number;
+      // then it takes over the numbers of blocks that have not begun, in the order in which they would, as long as there are any.
       Items<kBN> list(a, lane);
-      bool ok = true;
+      bool ok = true, more = true;
+      int taken = 0;
+      unsigned number = blockIdx.x;
       for (int n = 0; ok; ++n) {
-        // to and fro over the blocks, so that each gets items of all sizes
-        const int at = (n & 1) ? static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x);
-        const Item it = list.find(static_cast<long long>(n) * gridDim.x + at);
+        Item it = {};
+        if (more) it = list.find(number);
+        // (the rest of the grid has nothing to do: it is taken over as well, so that it does not have to begin)
+        while (more && !it.there && ok) {
+          ok = take_block(base + C::kOffNext, next_full, taken++, &number, &more, wait);
+          if (ok && more) it = list.find(number);
+        }
+        if (!ok) break;
         if (n >= 2) ok = wait(item_free + 8 * (n & 1), ((n >> 1) + 1) & 1, 12, n);
         if (!ok) break;
         if (lane == 0) {
@@ -282,10 +336,12 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
         }
         __syncwarp();
         if (!it.there) break;
+        // not before the item's last copy is on its way: what is taken early is another block's late
+        ok = wait(copied, n & 1, 15, n) && take_block(base + C::kOffNext, next_full, taken++, &number, &more, wait);
       }
     } else if (warp == 0) {
       // ----------------------------------------------------------------- copies ----
-      int ring = 0, q_uses[2] = {0, 0};
+      unsigned ring = 0, q_uses[2] = {0, 0};
       bool ok = true;
       Item it;
       for (int n = 0; ok && next_item(n, &it); ++n) {
@@ -303,9 +359,9 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
         }
         for (int t = 0; t < n_tiles && ok; ++t)
           for (int which = 0; which < 2 && ok; ++which, ++ring) {
-            const int slot = ring % C::kStages, use = ring / C::kStages;
+            const unsigned slot = ring % C::kStages, use = ring / C::kStages;
             if (use > 0) ok = wait(kv_free + 8 * slot, (use + 1) & 1, 1, ring);
-            if (a.stall_after >= 0 && ring >= a.stall_after) ok = false;  // (test hook)
+            if (a.stall_after >= 0 && static_cast<int>(ring) >= a.stall_after) ok = false;  // (test hook)
             if (ok && lane == 0) {
               mbar_expect_tx(kv_full + 8 * slot, C::kKvBytes);
               for (int bx = 0; bx < C::kBoxes; ++bx)
@@ -314,32 +370,37 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
             }
           }
         __syncwarp();
+        if (ok && lane == 0) mbar_arrive(copied);
       }
     } else if (warp == 1 || C::kEarlyS) {
       // --------------------------------------------------------------- products ----
       constexpr unsigned kFmt = kBf16 ? 1u : 0u;
-      constexpr unsigned idesc_s = make_idesc(kFmt, 0, kBN, kBM), idesc_pv = make_idesc(kFmt, 1, D, kBM);
+      constexpr unsigned idesc_pv = make_idesc(kFmt, 1, D, kBM);
       constexpr unsigned kBox = (kBM * 128) >> 4, kKvBox = (kBN * 128) >> 4;
       const unsigned long long qd0 = desc_kmajor(base), kd0 = desc_kmajor(s_kv), vd0 = desc_mnmajor(s_kv, kBN * 128, 1024);
-      int ring = 0;  // key tiles of this block so far, twice
-      auto slot_of = [&](int i) { return i % C::kStages; };
-      auto wait_kv = [&](int i) { return wait(kv_full + 8 * slot_of(i), (i / C::kStages) & 1, 4, i); };
-      auto put_s = [&](int i, unsigned col, int w) {  // S = Q_w K^T of ring item i
+      unsigned ring = 0;  // key tiles of this block so far, twice
+      auto slot_of = [&](unsigned i) { return i % C::kStages; };
+      auto wait_kv = [&](unsigned i) { return wait(kv_full + 8 * slot_of(i), (i / C::kStages) & 1, 4, i); };
+      auto put_s = [&](unsigned i, unsigned col, int w, int steps) {  // S = Q_w K^T of ring item i, of `steps` times 16 keys
+        const unsigned idesc_s = make_idesc(kFmt, 0, 16, kBM) + (static_cast<unsigned>(steps - 1) << 18);
         const unsigned long long qd = qd0 + static_cast<unsigned long long>(w * (C::kQBytes >> 4));
         const unsigned long long kd = kd0 + static_cast<unsigned long long>(slot_of(i) * (C::kKvBytes >> 4));
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks)
           mma_ss(tmem + col, qd + (ks / 4) * kBox + (ks % 4) * 2, kd + (ks / 4) * kKvBox + (ks % 4) * 2, idesc_s, ks > 0);
       };
-      auto put_pv = [&](int i, unsigned col_o, unsigned col_p, int steps, bool acc) {  // O += P V, `steps` times 16 keys
+      auto put_pv = [&](unsigned i, unsigned col_o, unsigned col_p, int steps, bool acc) {  // O += P V, `steps` times 16 keys
         const unsigned long long vd = vd0 + static_cast<unsigned long long>(slot_of(i) * (C::kKvBytes >> 4));
+        if (steps == kBN / 16) {
 #pragma unroll
-        for (int ks = 0; ks < kBN / 16; ++ks)
-          if (ks < steps) mma_ts(tmem + col_o, tmem + col_p + ks * 8, vd + ks * (2048 >> 4), idesc_pv, acc || ks > 0);
+          for (int ks = 0; ks < kBN / 16; ++ks) mma_ts(tmem + col_o, tmem + col_p + ks * 8, vd + ks * (2048 >> 4), idesc_pv, acc || ks > 0);
+        } else {
+          for (int ks = 0; ks < steps; ++ks) mma_ts(tmem + col_o, tmem + col_p + ks * 8, vd + ks * (2048 >> 4), idesc_pv, acc || ks > 0);
+        }
       };
       // V's rows behind the sequence's last key, as far as the last step of 16 reaches (its weights there are 0, but 0 times what another
       // sequence has there need not be). Both issuing warps may do it: they write the same zeros.
-      auto clear_v = [&](int i, int keys) {
+      auto clear_v = [&](unsigned i, int keys) {
         if (keys >= kBN || keys % 16 == 0) return;
         const unsigned tile = s_kv + slot_of(i) * C::kKvBytes + keys * 128;
         for (int x = lane; x < (16 - keys % 16) * 8 * C::kBoxes; x += 32)
@@ -355,7 +416,9 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
       for (int n = 0; ok && next_item(n, &it); ++n) {
         const int n_of[2] = {tiles_of(it, 0), tiles_of(it, 1)}, n_tiles = max(n_of[0], n_of[1]);
         auto keys_of = [&](int t) { return it.k_len - t * kBN; };  // of the sequence, from a tile on
-        auto steps_of = [&](int t) { return min(kBN, (keys_of(t) + 15) & ~15) / 16; };
+        const int seen_of[2] = {tile_keys<D>(a, it, 0), C::kTiles == 2 ? tile_keys<D>(a, it, 1) : 0};
+        // keys of tile t that some row of query tile w sees, in steps of 16
+        auto steps_of = [&](int t, int w) { return min(kBN, (seen_of[w] - t * kBN + 15) & ~15) / 16; };
         if constexpr (C::kOrdered) {
           // One warp issues for both tiles in turn: P.V of tile t and, behind it, the scores of tile t + 1 over the P that it read.
           ok = n_tiles == 0 || wait_kv(ring);
@@ -365,7 +428,7 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
             if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
-              put_s(ring, w == 0 ? C::kColS0 : C::kColS1, w);
+              put_s(ring, w == 0 ? C::kColS0 : C::kColS1, w, steps_of(0, w));
               tc_commit(s_full + 8 * w);
               if (n_of[w] == 1) tc_commit(q_free + 8 * w);
               if (w == 1 || n_of[1] == 0) tc_commit(kv_free + 8 * slot_of(ring));
@@ -373,7 +436,7 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
             __syncwarp();
           }
           for (int t = 0; t < n_tiles && ok; ++t) {
-            const int iv = ring + 2 * t + 1, ik = iv + 1;
+            const unsigned iv = ring + 2 * t + 1, ik = iv + 1;
             ok = wait_kv(iv) && (t + 1 >= n_tiles || wait_kv(ik));
             if (!ok) break;
             clear_v(iv, keys_of(t));
@@ -383,10 +446,10 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
               if (!ok) break;
               tc_fence_after();
               if (elect_one()) {
-                put_pv(iv, w == 0 ? C::kColO0 : C::kColO1, w == 0 ? C::kColP0 : C::kColP1, steps_of(t), t > 0);
+                put_pv(iv, w == 0 ? C::kColO0 : C::kColO1, w == 0 ? C::kColP0 : C::kColP1, steps_of(t, w), t > 0);
                 const bool last_v = w == 1 || t >= n_of[1];
                 if (t + 1 < n_of[w]) {
-                  put_s(ik, w == 0 ? C::kColS0 : C::kColS1, w);
+                  put_s(ik, w == 0 ? C::kColS0 : C::kColS1, w, steps_of(t + 1, w));
                   tc_commit(s_full + 8 * w);
                   if (t + 2 == n_of[w]) tc_commit(q_free + 8 * w);
                 } else {
@@ -406,7 +469,7 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
             tc_fence_after();
             if (elect_one()) {
               const int buf = s_uses & 1;
-              put_s(ring + 2 * t, buf * kBN, 0);
+              put_s(ring + 2 * t, buf * kBN, 0, steps_of(t, 0));
               tc_commit(s_full + 8 * buf);
               tc_commit(kv_free + 8 * slot_of(ring + 2 * t));
               if (t + 1 == n_tiles) tc_commit(q_free);
@@ -423,7 +486,7 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
             clear_v(ring + 2 * t + 1, keys_of(t));
             tc_fence_after();
             if (elect_one()) {
-              put_pv(ring + 2 * t + 1, C::kColO0, (p_uses[0] & 1) * kBN, steps_of(t), t > 0);
+              put_pv(ring + 2 * t + 1, C::kColO0, (p_uses[0] & 1) * kBN, steps_of(t, 0), t > 0);
               tc_commit(o_done);
               tc_commit(kv_free + 8 * slot_of(ring + 2 * t + 1));
             }
@@ -436,11 +499,11 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
           const int w = warp - 1, mine = n_of[w];
           const unsigned col_s = w == 0 ? C::kColS0 : C::kColS1;
           auto do_s = [&](int t) {
-            const int i = ring + 2 * t;
+            const unsigned i = ring + 2 * t;
             if (!wait_kv(i)) return false;
             tc_fence_after();
             if (elect_one()) {
-              put_s(i, col_s, w);
+              put_s(i, col_s, w, steps_of(t, w));
               tc_commit(s_full + 8 * w);
               tc_commit(kv_free + 8 * slot_of(i));
               if (t + 1 == mine) tc_commit(q_free + 8 * w);
@@ -448,7 +511,7 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
             __syncwarp();
             return true;
           };
-          auto give_back = [&](int i) {  // a tile of the other query tile alone: its place goes back unread
+          auto give_back = [&](unsigned i) {  // a tile of the other query tile alone: its place goes back unread
             if (!wait_kv(i)) return false;
             if (lane == 0) mbar_arrive(kv_free + 8 * slot_of(i));
             __syncwarp();
@@ -456,7 +519,7 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
           };
           if (mine > 0) ok = wait(q_full + 8 * w, q_uses[0]++ & 1, 3, n) && do_s(0);
           for (int t = 0; t < n_tiles && ok; ++t) {
-            const int iv = ring + 2 * t + 1;
+            const unsigned iv = ring + 2 * t + 1;
             if (t < mine) {
               if (t + 1 < mine) ok = wait(s_free + 8 * w, p_uses[0] & 1, 9, t) && do_s(t + 1);
               ok = ok && wait(p_full + 8 * w, p_uses[0] & 1, 6, t) && wait_kv(iv);
@@ -465,7 +528,7 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
               clear_v(iv, keys_of(t));
               tc_fence_after();
               if (elect_one()) {
-                put_pv(iv, w == 0 ? C::kColO0 : C::kColO1, w == 0 ? C::kColP0 : C::kColP1, steps_of(t), t > 0);
+                put_pv(iv, w == 0 ? C::kColO0 : C::kColO1, w == 0 ? C::kColP0 : C::kColP1, steps_of(t, w), t > 0);
                 tc_commit(o_done + 8 * w);
                 tc_commit(kv_free + 8 * slot_of(iv));
               }
@@ -479,7 +542,7 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
       }
     }
   } else {
-    if constexpr (C::kTiles == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if constexpr (C::kTiles == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsHi));
     // ----------------------------------------------------------------- softmax ----
     const int w = (warp - 4) >> 2;
     const int row = ((warp & 3) << 5) + lane;
@@ -491,14 +554,27 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
     const float scale_log2 = rsqrtf(static_cast<float>(DR)) * kLog2e;
     bool ok = !gone;
     unsigned uses = 0, items_of = 0;  // key tiles and items of this query tile so far
-    Item it;
-    for (int n = 0; ok && next_item(n, &it); ++n) {
-      const int head = row / a.tile_tokens, token = it.token0 + w * a.tile_tokens + row % a.tile_tokens;
-      const bool valid = token < it.q_len && it.head + head < a.G;
+    // (what the rows' way out wants of the item is read again behind the tile loop, which has no registers for it)
+    auto place = [&](const Item& it, int* head, int* token) {
+      *head = it.head + (row >> a.tile_shift);
+      *token = it.token0 + (w << a.tile_shift) + (row & (a.tile_tokens - 1));
+      return *token < it.q_len && *head < a.G;
+    };
+    for (int n = 0; ok; ++n) {
+      ok = wait(item_full + 8 * (n & 1), (n >> 1) & 1, 11, n);
+      if (!ok) break;
+      int n_own, see;
+      bool valid;
+      {
+        const Item it = item_at(n);
+        if (!it.there) break;
+        int head, token;
+        valid = place(it, &head, &token);
+        n_own = tiles_of(it, w);
+        // keys that the row sees (a row that there is not: all, with weights of 0, so that it asks for no mask)
+        see = !valid ? 0x7fffffff : a.causal ? min(it.k_len, token + 1 + it.k_len - it.q_len) : it.k_len;
+      }
       const bool any_valid = __any_sync(0xffffffffu, valid) != 0;
-      const int n_own = tiles_of(it, w);
-      // keys that the row sees (a row that there is not: all, with weights of 0, so that it asks for no mask)
-      const int see = !valid ? 0x7fffffff : a.causal ? min(it.k_len, token + 1 + it.k_len - it.q_len) : it.k_len;
       float m_ref = valid ? -INFINITY : 1e30f, l_run = 0.f;
       for (int j = 0; j < n_own && ok; ++j, ++uses) {
         const int buf = C::kDoubleS ? uses & 1 : 0;
@@ -522,99 +598,118 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
           mbar_arrive(p_full + 8 * w);
           continue;
         }
-        float s[kBN];
-        if constexpr (kBN == 128) tmem_ld128(t_s, s);
-        else tmem_ld64(t_s + buf * kBN, s);
-        if constexpr (C::kEarlyS) {
-          tc_fence_before();
-          mbar_arrive(s_free + 8 * w);
-        }
         const int hi = min(max(see - j * kBN, 0), kBN);  // columns that the row sees
-        if (!__all_sync(0xffffffffu, hi == kBN)) {
-#pragma unroll
-          for (int i = 0; i < kBN; ++i) s[i] = i < hi ? s[i] : -INFINITY;
-        }
-        // P = 2^(s scale - m_ref) and the row sum; m_ref is moved only when a tile's sum says so (see step_tc.cu)
-        const float2 scale2 = make_float2(scale_log2, scale_log2);
-        float2 sum_a, sum_b;
-        auto half_tile = [&](int h, float neg_m) {
-          const float2 negm2 = make_float2(neg_m, neg_m);
-          unsigned pk[32];
-#pragma unroll
-          for (int i = 0; i < 64; i += 4) {
-            const int c = h * 64 + i;
-            const float2 x0 = ffma2(make_float2(s[c], s[c + 1]), scale2, negm2);
-            const float2 x1 = ffma2(make_float2(s[c + 2], s[c + 3]), scale2, negm2);
-            const float2 p0 = make_float2(ex2(x0.x), ex2(x0.y)), p1 = make_float2(ex2(x1.x), ex2(x1.y));
-            sum_a = fadd2(sum_a, p0);
-            sum_b = fadd2(sum_b, p1);
-            pk[i / 2] = pack_pair<T>(p0.x, p0.y);
-            pk[i / 2 + 1] = pack_pair<T>(p1.x, p1.y);
+        const bool full = __all_sync(0xffffffffu, hi == kBN) != 0;
+        // The first kCols columns of the tile (64 of 128 where no row of the warp sees more: the others' weights are 0); false: gave up.
+        auto work = [&](auto cols) {
+          constexpr int kCols = decltype(cols)::value;
+          float s[kCols];
+          if constexpr (kCols == 128) tmem_ld128(t_s, s);
+          else tmem_ld64(t_s + buf * kBN, s);
+          if constexpr (C::kEarlyS) {
+            tc_fence_before();
+            mbar_arrive(s_free + 8 * w);
           }
-          tmem_st32u(t_p + buf * kBN + h * 32, &pk[0]);
-        };
-        auto whole_tile = [&]() {
-          const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;
-          sum_a = sum_b = make_float2(0.f, 0.f);
+          if (!full) {
 #pragma unroll
-          for (int h = 0; h < kBN / 64; ++h) half_tile(h, neg_m);
-          return (sum_a.x + sum_a.y) + (sum_b.x + sum_b.y);
+            for (int i = 0; i < kCols; ++i) s[i] = i < hi ? s[i] : -INFINITY;
+          }
+          // P = 2^(s scale - m_ref) and the row sum; m_ref is moved only when a tile's sum says so (see step_tc.cu)
+          const float2 scale2 = make_float2(scale_log2, scale_log2);
+          float2 sum_a, sum_b;
+          auto half_tile = [&](int h, float neg_m) {
+            const float2 negm2 = make_float2(neg_m, neg_m);
+            unsigned pk[32];
+#pragma unroll
+            for (int i = 0; i < 64; i += 4) {
+              const int c = h * 64 + i;
+              const float2 x0 = ffma2(make_float2(s[c], s[c + 1]), scale2, negm2);
+              const float2 x1 = ffma2(make_float2(s[c + 2], s[c + 3]), scale2, negm2);
+              const float2 p0 = make_float2(ex2(x0.x), ex2(x0.y)), p1 = make_float2(ex2(x1.x), ex2(x1.y));
+              sum_a = fadd2(sum_a, p0);
+              sum_b = fadd2(sum_b, p1);
+              pk[i / 2] = pack_pair<T>(p0.x, p0.y);
+              pk[i / 2 + 1] = pack_pair<T>(p1.x, p1.y);
+            }
+            tmem_st32u(t_p + buf * kBN + h * 32, &pk[0]);
+          };
+          auto whole_tile = [&]() {
+            const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;
+            sum_a = sum_b = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int h = 0; h < kCols / 64; ++h) half_tile(h, neg_m);
+            if constexpr (kCols < kBN) {
+              unsigned none[32];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) none[i] = 0u;
+              tmem_st32u(t_p + 32, &none[0]);
+            }
+            return (sum_a.x + sum_a.y) + (sum_b.x + sum_b.y);
+          };
+          bool need = m_ref == -INFINITY && hi > 0;  // this row's reference has to move
+          bool slow = __any_sync(0xffffffffu, need) != 0;
+          float row_sum = 0.f;
+          [[maybe_unused]] bool waited = slow;
+          if (C::kEarlyS || slow) wait_pv();
+          if (!ok) return;
+          if (!slow) {
+            row_sum = whole_tile();
+            need = !(row_sum <= kRowSumLimit) && valid;  // (NaN too)
+            slow = __any_sync(0xffffffffu, need) != 0;
+            if (C::kDoubleS && slow) wait_pv(), waited = true;  // O has to be at rest
+            if (!ok) return;
+          }
+          // Rows that need it move their reference, the others keep theirs, so that no row's result hangs on which rows share its warp.
+          // Those that have one and were not asked yet, because another's first tile is here, may need it in turn.
+#pragma unroll 1
+          for (int pass = 0; slow && pass < 2; ++pass) {
+            float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
+#pragma unroll
+            for (int i = 4; i < kCols; i += 8) {
+              m0 = max3(m0, s[i], s[i + 1]);
+              m1 = max3(m1, s[i + 2], s[i + 3]);
+              if (i + 4 < kCols) {
+                m2 = max3(m2, s[i + 4], s[i + 5]);
+                m3 = max3(m3, s[i + 6], s[i + 7]);
+              }
+            }
+            const float tile_max = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * scale_log2;
+            float alpha = 1.f;
+            bool rescale = false;
+            if (need && tile_max > m_ref) {
+              if (m_ref > -INFINITY) {
+                alpha = ex2(m_ref - tile_max);
+                rescale = true;
+              }
+              m_ref = tile_max;
+            }
+            if (j > 0 && __any_sync(0xffffffffu, rescale)) {
+              l_run *= alpha;
+#pragma unroll 1
+              for (int c = 0; c < D / 32; ++c) {
+                float o[32];
+                tmem_ld32(t_o + c * 32, o);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] *= alpha;
+                tmem_st32(t_o + c * 32, o);
+              }
+            }
+            row_sum = whole_tile();
+            need = !(row_sum <= kRowSumLimit) && valid;
+            slow = __any_sync(0xffffffffu, need) != 0;
+          }
+          l_run += row_sum;
+          if constexpr (C::kDoubleS) {  // (keeps step with the barrier, which tells the latest phase from the one before alone)
+            if (!waited) wait_pv();
+          }
         };
-        bool need = m_ref == -INFINITY && hi > 0;  // this row's reference has to move
-        bool slow = __any_sync(0xffffffffu, need) != 0;
-        float row_sum = 0.f;
-        if (C::kEarlyS || slow) wait_pv();
+        if constexpr (kBN == 128) {
+          if (!full && !__any_sync(0xffffffffu, valid && hi > 64)) work(std::integral_constant<int, 64>());
+          else work(std::integral_constant<int, 128>());
+        } else {
+          work(std::integral_constant<int, 64>());
+        }
         if (!ok) break;
-        if (!slow) {
-          row_sum = whole_tile();
-          need = !(row_sum <= kRowSumLimit) && valid;  // (NaN too)
-          slow = __any_sync(0xffffffffu, need) != 0;
-          if (C::kDoubleS && slow) wait_pv();  // O has to be at rest
-          if (!ok) break;
-        }
-        // Rows that need it move their reference, the others keep theirs, so that no row's result hangs on which rows share its warp. Those
-        // that have one and were not asked yet, because another's first tile is here, may need it in turn.
-#pragma unroll 1
-        for (int pass = 0; pass < 2 && __any_sync(0xffffffffu, need); ++pass) {
-          float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
-#pragma unroll
-          for (int i = 4; i < kBN; i += 8) {
-            m0 = max3(m0, s[i], s[i + 1]);
-            m1 = max3(m1, s[i + 2], s[i + 3]);
-            if (i + 4 < kBN) {
-              m2 = max3(m2, s[i + 4], s[i + 5]);
-              m3 = max3(m3, s[i + 6], s[i + 7]);
-            }
-          }
-          const float tile_max = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * scale_log2;
-          float alpha = 1.f;
-          bool rescale = false;
-          if (need && tile_max > m_ref) {
-            if (m_ref > -INFINITY) {
-              alpha = ex2(m_ref - tile_max);
-              rescale = true;
-            }
-            m_ref = tile_max;
-          }
-          if (j > 0 && __any_sync(0xffffffffu, rescale)) {
-            l_run *= alpha;
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              float o[32];
-              tmem_ld32(t_o + c * 32, o);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] *= alpha;
-              tmem_st32(t_o + c * 32, o);
-            }
-          }
-          row_sum = whole_tile();
-          need = !(row_sum <= kRowSumLimit) && valid;
-        }
-        l_run += row_sum;
-        if constexpr (C::kDoubleS) {  // (keeps step with the barrier, which tells the latest phase from the one before alone)
-          if (!slow) wait_pv();
-          if (!ok) break;
-        }
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(p_full + 8 * w);
@@ -627,45 +722,54 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
         tc_fence_after();
         ++items_of;
       }
+      const Item it = item_at(n);
+      give_item_back(n);
       if (!any_valid) continue;
+      int head, token;
+      place(it, &head, &token);
       // (scores of NaN alone set no reference, but the row is NaN and not one without keys)
       const bool have = n_own > 0 && (m_ref > -INFINITY || l_run != l_run);
       const float inv = have ? 1.f / l_run : 0.f;
-      const int h = (it.head + head) * a.kvH + it.kv;
-      const long long at = (it.q0 + token) * a.out_row + h * a.out_head;  // (of a valid row)
-      if (a.lse && valid) a.lse[static_cast<size_t>(h) * a.rows + it.q0 + token] = !have ? -INFINITY : l_run > 0.f ? m_ref * kLn2 + logf(l_run) : l_run;
+      if (a.lse && valid)
+        a.lse[static_cast<size_t>(head * a.kvH + it.kv) * a.rows + it.q0 + token] = !have ? -INFINITY : l_run > 0.f ? m_ref * kLn2 + logf(l_run) : l_run;
+      const unsigned rows_there = __ballot_sync(0xffffffffu, valid);
       // 64 columns at a time through shared memory, so that 8 lanes write 128 bytes of a row side by side
       constexpr int kCols = DR < 64 ? DR : 64, kLanes = kCols / 8, kRowsPer = 32 / kLanes;
+      // (the lane out of its register, volatile: what hangs on threadIdx the compiler works out in front of the tile loop, and carries
+      // through it in registers that the loop lacks)
+      int lane_out;
+      asm volatile("mov.u32 %0, %%laneid;" : "=r"(lane_out));
+      const int piece = lane_out % kLanes, first = lane_out / kLanes;
 #pragma unroll 1
       for (int pass = 0; pass < DR / kCols; ++pass) {
+        float o[64];
+        if (n_own > 0) {
+          if constexpr (kCols == 64) tmem_ld64(t_o + pass * kCols, o);
+          else tmem_ld32(t_o, reinterpret_cast<float(&)[32]>(o));
+        } else {
 #pragma unroll
-        for (int c = 0; c < kCols / 32; ++c) {
-          float o[32];
-          if (n_own > 0) {
-            tmem_ld32(t_o + pass * kCols + c * 32, o);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = 0.f;
-          }
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = have ? o[i] * inv : 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 + (((c * 4 + i) ^ (lane & 7)) << 4)),
-                         "r"(pack_pair<T>(o[8 * i], o[8 * i + 1])), "r"(pack_pair<T>(o[8 * i + 2], o[8 * i + 3])),
-                         "r"(pack_pair<T>(o[8 * i + 4], o[8 * i + 5])), "r"(pack_pair<T>(o[8 * i + 6], o[8 * i + 7]))
-                         : "memory");
+          for (int i = 0; i < kCols; ++i) o[i] = 0.f;
         }
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) o[i] = have ? o[i] * inv : 0.f;
+#pragma unroll
+        for (int i = 0; i < kCols / 8; ++i)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane_out * 128 + ((i ^ (lane_out & 7)) << 4)),
+                       "r"(pack_pair<T>(o[8 * i], o[8 * i + 1])), "r"(pack_pair<T>(o[8 * i + 2], o[8 * i + 3])),
+                       "r"(pack_pair<T>(o[8 * i + 4], o[8 * i + 5])), "r"(pack_pair<T>(o[8 * i + 6], o[8 * i + 7]))
+                       : "memory");
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < 32 / kRowsPer; ++i) {
-          const int r = i * kRowsPer + lane / kLanes, piece = lane % kLanes;
+          const int r = i * kRowsPer + first, of_tile = ((warp & 3) << 5) + r;
+          const int h = (it.head + (of_tile >> a.tile_shift)) * a.kvH + it.kv;
+          const int q = it.q0 + it.token0 + (w << a.tile_shift) + (of_tile & (a.tile_tokens - 1));
           uint4 v;
           asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                        : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                        : "r"(stage + r * 128 + ((piece ^ (r & 7)) << 4)));
-          const long long to = __shfl_sync(0xffffffffu, at, r);
-          if (__shfl_sync(0xffffffffu, valid, r)) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + to + pass * kCols + piece * 8) = v;
+          if (rows_there >> r & 1u)
+            *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + q * a.out_row + h * a.out_head + pass * kCols + piece * 8) = v;
         }
         __syncwarp();
       }
@@ -727,6 +831,7 @@ int launch_packed(const ra_rows& q, const ra_rows& k, const ra_rows& v, PackedAr
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   a.pack = heads_per_tile(a.G, (a.rows + a.B - 1) / a.B);
   a.tile_tokens = kBM / a.pack;
+  while ((1 << a.tile_shift) < a.tile_tokens) ++a.tile_shift;
   a.head_sets = (a.G + a.pack - 1) / a.pack;
   a.token_shift = 0;
   while ((1 << a.token_shift) < C::kTiles * a.tile_tokens) ++a.token_shift;
@@ -754,8 +859,8 @@ int launch_packed(const ra_rows& q, const ra_rows& k, const ra_rows& v, PackedAr
   }
   // (as many items as there can be)
   const long long most = ((static_cast<long long>(a.rows) >> a.token_shift) + a.B) * a.kvH * a.head_sets;
-  const unsigned grid = static_cast<unsigned>(std::min<long long>(most, sm_count()));
-  RAB_CUDA(launch_overlapped(kern, dim3(grid), dim3(C::kThreads), C::kSmemBytes, stream, mq, mk, mv, a));
+  RAB_REQUIRE(most < 1ll << 31, RA_ERR_INVALID, "packed_attention: too many rows, sequences and heads");
+  RAB_CUDA(launch_overlapped(kern, dim3(static_cast<unsigned>(most)), dim3(C::kThreads), C::kSmemBytes, stream, mq, mk, mv, a));
   return RA_OK;
 }
 
