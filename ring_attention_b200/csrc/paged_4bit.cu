@@ -27,25 +27,112 @@ struct FourArgs {
   float k_factor, v_factor;
 };
 
+// The list of stages is one of kGrain keys each, so that short calls divide over all warps; a copy takes as many of them, up to GR, as a
+// share has left of a unit, because what surrounds a copy costs some 300 instructions and 16 keys of 128 columns 280.
+constexpr int kGrain = 32;
+constexpr int four_warps(int D, int NB) { return D * NB <= 128 ? 6 : 4; }  // of a block
+
 template <int D, int NB>
 struct FourBlock {
-  static constexpr bool kBulk = true, kFour = true;
-  static constexpr int SR = 32, RU = 8 * NB;
+  static constexpr int GR = D >= 256 ? 1 : D == 128 ? 2 : 4, SR = GR * kGrain, RU = 8 * NB;
   // accumulators and queries: (D / 4 + D / 8) NB registers
-  static constexpr int kWarps = D * NB <= 128 ? 8 : 4, kThreads = kWarps * 32;
-  static constexpr int kBoxes = 1;
+  static constexpr int kWarps = four_warps(D, NB), kThreads = kWarps * 32;
   static constexpr int kCodeBytes = D / 2, kScaleBytes = D / 16, kRowBytes = kCodeBytes + kScaleBytes;
   static constexpr int kTileBytes = SR * kRowBytes;  // per tensor: codes, then scales
-  static constexpr int kStages = 110 * 1024 / kWarps / (2 * kTileBytes) < 8 ? 110 * 1024 / kWarps / (2 * kTileBytes) : 8;
+  static constexpr int kMost = 110 * 1024 / kWarps / (2 * kTileBytes);
+  static constexpr int kStages = kMost < 4 ? kMost : 4;
   static constexpr int kRingBytes = 2 * kStages * kTileBytes;
-  static constexpr int kOffInfo = (kWarps * kRingBytes + 15) & ~15;
-  static constexpr int kOffBar = kOffInfo + kWarps * kStages * static_cast<int>(sizeof(StageInfo));
+  static constexpr int kOffInfo = kWarps * kRingBytes;
+  static constexpr int kOffBar = kOffInfo + kWarps * kStages * 32;
   static constexpr int kOffRoom = (kOffBar + kWarps * kStages * 8 + 15) & ~15;
   static constexpr int kOffFlag = kOffRoom + static_cast<int>(sizeof(ScanRoom<kWarps>));
   static constexpr int kSmemBytes = kOffFlag + 8;
-  static_assert(kTileBytes % 16 == 0 && kStages >= 3 && sizeof(StageInfo) % 4 == 0, "the ring");
-  static_assert((kWarps * kStages * sizeof(StageInfo)) % 8 == 0, "the barriers");
+  static_assert(kTileBytes % 16 == 0 && kStages >= 2 && sizeof(StageInfo) == 32, "the ring");
   static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two blocks to an SM");
+};
+
+// A warp's ring: while a place is worked on, the others' copies are on their way.
+template <typename C>
+struct FourRing {
+  const PagedArgs& a;
+  unsigned char* tiles;  // shared memory: the ring, what there is to know of its places, its barriers
+  int4* info;
+  unsigned full;
+  volatile int* gave_up;
+  Walk<kGrain> w;  // the next grain to copy
+  int total, per, next, first_st;
+  // this lane's copies: piece `piece` of the rows, of K's or V's codes or scales
+  const unsigned char* from;
+  unsigned to, row_bytes, rows, offset;
+  int kind, page;  // (page: of its next copy, -1: none)
+  __device__ inline void look_up() {
+    const int at = (w.st * kGrain + static_cast<int>(offset)) >> a.shift;
+    page = -1;
+    if (next < total && kind < 4 && static_cast<int>(offset) < w.left() && at < a.max_pages) page = a.table[w.b * a.table_stride + at];
+  }
+  __device__ inline void begin(unsigned base) {
+    const unsigned lane = threadIdx.x & 31, shift = a.shift < 5 ? a.shift : 5, pieces = C::SR >> shift;
+    rows = 1u << shift;
+    offset = lane % pieces * rows;
+    kind = lane / pieces;
+    const int which = kind >> 1;  // 0: codes, 1: scales
+    row_bytes = which == 0 ? C::kCodeBytes : C::kScaleBytes;
+    from = static_cast<const unsigned char*>((kind & 1) == 0 ? a.k : a.v) + (which == 0 ? 0 : C::kCodeBytes << a.shift);
+    to = base + (kind & 1) * C::kTileBytes + (which == 0 ? 0 : C::SR * C::kCodeBytes) + offset * row_bytes;
+    first_st = w.st;
+    next = 0;
+    look_up();
+    for (int s = 0; s < C::kStages; ++s) copy(s);
+  }
+  // Copies the next grains, if there are any, to a place that is free.
+  __device__ inline void copy(int slot) {
+    if (next >= total) return;
+    const int grains = min(min(C::GR, total - next), w.n - w.st), keys = min(grains * kGrain, w.left());
+    if (w.st == 0) {
+      first_st = 0;
+      // the warp with a unit's first grain says which shares have parts of it: its own and those that the rest reaches into
+      const int here = min(w.n, total - next);
+      if ((threadIdx.x & 31) == 0)
+        a.unit_parts[w.uid] = make_int2(static_cast<int>(blockIdx.x * C::kWarps + (threadIdx.x >> 5)), 1 + (w.n - here + per - 1) / per);
+    }
+    const bool there = page >= 0 && page < a.num_pages && static_cast<int>(offset) < keys;
+    const unsigned lanes = __ballot_sync(0xffffffffu, there);
+    if ((threadIdx.x & 31) == 0) {
+      // blocks of 16 keys that are there
+      unsigned blocks = lanes & ((1u << (C::SR / rows)) - 1u);
+      if (rows == 32) blocks = (blocks & 1u) * 3u | (blocks & 2u) * 6u | (blocks & 4u) * 12u | (blocks & 8u) * 24u;
+      const bool ends = w.st + grains == w.n;
+      const int last = ends && first_st == 0 ? 2 : ends || next + grains == total;
+      info[2 * slot] = make_int4(w.b, w.kvh, w.hb, w.uid);
+      info[2 * slot + 1] = make_int4(keys, static_cast<int>(blocks), w.st == first_st, last);
+      tcgen::mbar_expect_tx(full + 8 * slot, 2 * C::kRowBytes * rows * __popc(lanes & ((1u << (C::SR / rows)) - 1u)) + a.missing);
+    }
+    __syncwarp();
+    if (there) {
+      const int row = (w.st * kGrain + static_cast<int>(offset)) & ((1 << a.shift) - 1);
+      tcgen::bulk_load(to + 2 * slot * C::kTileBytes,
+                       from + ((static_cast<size_t>(page) * a.kvH + w.kvh) << a.shift) * C::kRowBytes + row * row_bytes, row_bytes * rows,
+                       full + 8 * slot);
+    }
+    next += grains;
+    w.st += grains - 1;
+    if (next < total) {
+      w.next(a);
+      look_up();
+    }
+  }
+  __device__ inline StageInfo at(int s) const {
+    const int4 x = info[2 * (s % C::kStages)], y = info[2 * (s % C::kStages) + 1];
+    StageInfo u;
+    u.b = x.x, u.kvh = x.y, u.hb = x.z, u.uid = x.w;
+    u.keys = y.x, u.pages = y.y, u.first = y.z, u.last = y.w;
+    return u;
+  }
+  // Waits for copy s; false: the warp gives up.
+  __device__ inline bool wait(int s) {
+    return __all_sync(0xffffffffu, tcgen::mbar_wait(full + 8 * (s % C::kStages), (s / C::kStages) & 1, gave_up, a.status, 3, s,
+                                                    a.wait_ns)) != 0;
+  }
 };
 
 // The eight codes of a word as fp16 pairs, neighbours together.
@@ -74,31 +161,21 @@ __device__ inline unsigned transposed(unsigned a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-template <typename T>
-__device__ inline float element(const T* p) {
-  return static_cast<float>(*p);
-}
 
 // Words of shared memory, N of them.
 template <int N>
-__device__ inline void load_words(unsigned addr, unsigned* w) {
-  if constexpr (N == 4)
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr) : "memory");
-  else if constexpr (N == 2)
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr) : "memory");
-  else
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr) : "memory");
+__device__ inline void load_words(const unsigned char* p, unsigned (&w)[N]) {
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const unsigned*>(p);
+  }
 }
-__device__ inline unsigned load_u16(unsigned addr) {
-  unsigned short v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
-  return v;
-}
-__device__ inline unsigned load_u8(unsigned addr) {
-  unsigned v;
-  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
-}
+__device__ inline unsigned load_u16(const unsigned char* p) { return *reinterpret_cast<const unsigned short*>(p); }
 
 // Where the products' places are. Lane (g, j) of a fragment has its rows g and g + 8 and its columns 2 j, 2 j + 1, 2 j + 8, 2 j + 9.
 // Key at place p of 16: p ^ (p >> 2 & 1), so that the keys 2 j differ in the rest by four, as do the keys g of half a warp: with the
@@ -122,7 +199,21 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
   constexpr int RU = C::RU, kSteps = D / 16, kTiles = D / 16;
   extern __shared__ __align__(1024) unsigned char smem[];
   const PagedArgs& a = args.p;
-  paged_block<C>(a, nullptr, nullptr, smem, [&](Ring<C>& ring, int warp) {
+  const unsigned base = tcgen::smem_u32(smem);
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  volatile int* const gave_up = reinterpret_cast<volatile int*>(smem + C::kOffFlag);
+  let_next_start();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kWarps * C::kStages; ++s) tcgen::mbar_init(base + C::kOffBar + 8 * s, 1);
+    *gave_up = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  wait_for_previous();
+  FourRing<C> ring{a, smem + warp * C::kRingBytes, reinterpret_cast<int4*>(smem + C::kOffInfo) + 2 * warp * C::kStages,
+                   base + C::kOffBar + warp * C::kStages * 8, gave_up};
+  ring.total = find_share<kGrain, C::kWarps>(a, warp, &ring.w, &ring.per, reinterpret_cast<ScanRoom<C::kWarps>*>(smem + C::kOffRoom));
+  auto walk = [&]() {
+    ring.begin(base + warp * C::kRingBytes);
     const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
     const int key_g = key_at(g), key_0 = key_at(2 * j), key_1 = key_at(2 * j + 1);
     const int turn_g = four_turn(key_g, D), turn_0 = four_turn(key_0, D), turn_1 = four_turn(key_1, D);
@@ -139,10 +230,11 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
     unsigned qb[NB][kSteps][2];
     float o[NB][kTiles][4];
     float m_run[NB][2], l_run[NB][2], factor[NB][2];  // of heads 2 j and 2 j + 1 of the eight
-    const int total = ring.total;
-    for (int s = 0; s < total; ++s) {
+    int left = ring.total;
+    for (int s = 0; left > 0; ++s) {
       const int slot = s % C::kStages;
-      const StageInfo u = ring.info[slot];
+      const StageInfo u = ring.at(s);
+      left -= (u.keys + kGrain - 1) / kGrain;
       if (u.first) {  // (while the copy is on its way)
         // Q as B fragments, fp16: a row is brought to a largest magnitude of 1 to 2 by a power of two, which leaves all of it
         // that counts: fp16 rows and bf16 ones lose nothing above 2^-14 of their largest element, and below it less than 2^-25 of that.
@@ -151,11 +243,20 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
           int b, h;
           const bool is = unit_row<RU>(a, u, nb * 8 + g, &b, &h);
           const T* const src = static_cast<const T*>(a.q) + (is ? static_cast<size_t>(b) * a.H + h : 0) * D;
-          float most = 0.f;
+          uint2 raw[kSteps];
 #pragma unroll
           for (int st = 0; st < kSteps; ++st)
+            raw[st] = is ? *reinterpret_cast<const uint2*>(src + Cols::k_column(st, j)) : make_uint2(0u, 0u);
+          auto pair = [&](unsigned u) {
+            if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&u));
+            else return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+          };
+          float most = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(is ? element(src + Cols::k_column(st, j) + e) : 0.f));
+          for (int st = 0; st < kSteps; ++st) {
+            const float2 x = pair(raw[st].x), y = pair(raw[st].y);
+            most = fmaxf(most, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y))));
+          }
           most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
           most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
           // 2^-e by the exponent's bits (rows of zeros, of what is below 2^-100 or not finite: as they are)
@@ -165,9 +266,9 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
           const float up = plain ? 1.f : 1.f / down;
 #pragma unroll
           for (int st = 0; st < kSteps; ++st) {
-            const T* const x = src + Cols::k_column(st, j);
-            qb[nb][st][0] = is ? pack_pair<__half>(element(x) * down, element(x + 1) * down) : 0u;
-            qb[nb][st][1] = is ? pack_pair<__half>(element(x + 2) * down, element(x + 3) * down) : 0u;
+            const float2 x = pair(raw[st].x), y = pair(raw[st].y);
+            qb[nb][st][0] = pack_pair<__half>(x.x * down, x.y * down);
+            qb[nb][st][1] = pack_pair<__half>(y.x * down, y.y * down);
           }
           const float f = up * args.k_factor * a.scale_log2;
           factor[nb][0] = __shfl_sync(0xffffffffu, f, 8 * j);
@@ -179,34 +280,33 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
         }
       }
       if (!ring.wait(s)) return;
-      const unsigned k_tile = ring.tiles + 2 * slot * C::kTileBytes, v_tile = k_tile + C::kTileBytes;
+      const unsigned char *const k_tile = ring.tiles + 2 * slot * C::kTileBytes, *const v_tile = k_tile + C::kTileBytes;
 #pragma unroll 1
-      for (int key0 = 0; key0 < C::SR; key0 += 16) {
+      for (int key0 = 0; key0 < u.keys; key0 += 16) {
         const int n_valid = u.keys - key0;  // keys from here on
-        if (n_valid <= 0) break;
         if (!(u.pages >> (key0 / 16) & 1u)) continue;
         // S^T = K Q^T: keys g and g + 8 of the tile, heads 2 j and 2 j + 1
         float sc[NB][4];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
-        const unsigned k_codes = k_tile + key0 * C::kCodeBytes;
-        const unsigned k_scales = k_tile + C::SR * C::kCodeBytes + (key0 + key_g) * C::kScaleBytes;
+        const unsigned char* const k_codes = k_tile + key0 * C::kCodeBytes;
+        const unsigned char* const k_scales = k_tile + C::SR * C::kCodeBytes + (key0 + key_g) * C::kScaleBytes;
 #pragma unroll
         for (int p = 0; p < kKPieces; ++p) {
           unsigned w[2][kKWords];
 #pragma unroll
-          for (int r = 0; r < 2; ++r) load_words<kKWords>(k_codes + r * 8 * C::kCodeBytes + k_at[p], w[r]);
+          for (int r = 0; r < 2; ++r) load_words(k_codes + k_at[p] + r * 8 * C::kCodeBytes, w[r]);
           // scales of the lane's blocks, two to a piece of 32 columns
           unsigned sk[2][2];
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const unsigned at = k_scales + r * 8 * C::kScaleBytes;
+            const unsigned char* const at = k_scales + r * 8 * C::kScaleBytes;
             if constexpr (D >= 128) {
-              const unsigned both = scales_to_half(static_cast<unsigned short>(load_u16(at + 8 * p + 2 * j)));
+              const unsigned both = scales_to_half(static_cast<unsigned short>(load_u16(at + 2 * j + 8 * p)));
               sk[r][0] = __byte_perm(both, both, 0x1010);
               sk[r][1] = __byte_perm(both, both, 0x3232);
             } else {
-              const unsigned one = load_u8(at + (D == 64 ? j : j / 2));
+              const unsigned one = at[D == 64 ? j : j / 2];
               sk[r][0] = sk[r][1] = scales_to_half(static_cast<unsigned short>(one | one << 8));
             }
           }
@@ -228,12 +328,16 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
             }
           }
         }
-        const bool in0 = key_g < n_valid, in1 = key_g + 8 < n_valid;
+        const bool whole = n_valid >= 16, in0 = key_g < n_valid, in1 = key_g + 8 < n_valid;
         bool more = false;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sc[nb][i] = (i < 2 ? in0 : in1) ? sc[nb][i] * factor[nb][i & 1] : -INFINITY;
+          for (int i = 0; i < 4; ++i) sc[nb][i] *= factor[nb][i & 1];
+          if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[nb][i] = (i < 2 ? in0 : in1) ? sc[nb][i] : -INFINITY;
+          }
           more = more || fmaxf(sc[nb][0], sc[nb][2]) > m_run[nb][0] || fmaxf(sc[nb][1], sc[nb][3]) > m_run[nb][1];
         }
         if (__any_sync(0xffffffffu, more)) {  // rare after the first stages
@@ -275,32 +379,40 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
           pb[nb][1] = transposed(pack_pair<__half>(p[2], p[3]));
         }
         // O^T += V^T P^T
-        const unsigned v_codes = v_tile + key0 * C::kCodeBytes;
-        const unsigned v_scales = v_tile + C::SR * C::kCodeBytes + key0 * C::kScaleBytes;
+        const unsigned char* const v_codes = v_tile + key0 * C::kCodeBytes;
+        const unsigned char* const v_scales = v_tile + C::SR * C::kCodeBytes + key0 * C::kScaleBytes;
         unsigned va[2][2][kTiles];  // [keys 2 j.., 2 j + 8..][rows g, g + 8][tile]: pairs of keys
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           unsigned w[2][kVWords];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const unsigned at = v_codes + r * 8 * C::kCodeBytes + v_at[e];
-            if constexpr (D >= 64) load_words<kVWords>(at, w[e]);
+            const unsigned char* const at = v_codes + v_at[e] + r * 8 * C::kCodeBytes;
+            if constexpr (D >= 64) load_words(at, w[e]);
             else w[e][0] = load_u16(at);
           }
           // the scales of the two keys, of the block of row g and of that of row g + 8 (head_dim 256: the next block); 0 for
           // keys that are not the sequence's, whose bytes may be anything
           unsigned sv[2];
           {
-            const bool is0 = key_0 + 8 * r < n_valid, is1 = key_1 + 8 * r < n_valid;
-            const unsigned at0 = v_scales + (key_0 + 8 * r) * C::kScaleBytes, at1 = v_scales + (key_1 + 8 * r) * C::kScaleBytes;
+            const unsigned char *const at0 = v_scales + key_0 * C::kScaleBytes + r * 8 * C::kScaleBytes,
+                                *const at1 = v_scales + key_1 * C::kScaleBytes + r * 8 * C::kScaleBytes;
+            unsigned s0, s1;
             if constexpr (D == 256) {
-              const unsigned s0 = is0 ? load_u16(at0 + 2 * g) : 0u, s1 = is1 ? load_u16(at1 + 2 * g) : 0u;
+              s0 = load_u16(at0 + 2 * g), s1 = load_u16(at1 + 2 * g);
+            } else {
+              constexpr int kLanes = 128 / D;  // lanes to a block
+              s0 = at0[g / kLanes], s1 = at1[g / kLanes];
+            }
+            if (!whole) {
+              s0 = key_0 + 8 * r < n_valid ? s0 : 0u;
+              s1 = key_1 + 8 * r < n_valid ? s1 : 0u;
+            }
+            if constexpr (D == 256) {
               const unsigned both = __byte_perm(s0, s1, 0x5140);  // (s0.lo, s1.lo, s0.hi, s1.hi)
               sv[0] = scales_to_half(static_cast<unsigned short>(both));
               sv[1] = scales_to_half(static_cast<unsigned short>(both >> 16));
             } else {
-              constexpr int kLanes = 128 / D;  // lanes to a block
-              const unsigned s0 = is0 ? load_u8(at0 + g / kLanes) : 0u, s1 = is1 ? load_u8(at1 + g / kLanes) : 0u;
               sv[0] = sv[1] = scales_to_half(static_cast<unsigned short>(s0 | s1 << 8));
             }
           }
@@ -329,7 +441,7 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
         }
       }
       __syncwarp();
-      if (s > 0) ring.copy_next((s - 1) % C::kStages);
+      ring.copy(slot);
       if (u.last) {
         const size_t part = (static_cast<size_t>(blockIdx.x) * C::kWarps + warp + u.uid) * a.rs;
 #pragma unroll
@@ -368,7 +480,14 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
           }
       }
     }
-  });
+  };
+  // (behind a launch that gave up nothing is computed; the fold writes nothing then either)
+  if (ring.total > 0 && a.missing >= 0 && __shfl_sync(0xffffffffu, *reinterpret_cast<volatile int*>(a.status), 0) == 0) walk();
+  __syncthreads();
+  if (*gave_up) {  // give copies in flight time to land
+    const unsigned long long t0 = tcgen::global_ns();
+    while (tcgen::global_ns() - t0 < 1000000ull) __nanosleep(1000);
+  }
 }
 
 // ---- rows back out of a cache --------------------------------------------------------
@@ -494,10 +613,10 @@ FourPlan make_plan(const ra_paged_kv& c, int heads) {
   const int G = (heads + c.kv_heads - 1) / c.kv_heads;
   p.NB = G > 8 ? 2 : 1;
   p.HB = (G + 8 * p.NB - 1) / (8 * p.NB);
-  p.warps = c.head_dim * p.NB <= 128 ? 8 : 4;
+  p.warps = four_warps(c.head_dim, p.NB);
   const size_t units = static_cast<size_t>(c.kv_heads) * c.batch * p.HB;
   const long long room = static_cast<long long>(c.max_pages) * c.page_size;
-  p.most = static_cast<double>(units) * ((room + 31) / 32);
+  p.most = static_cast<double>(units) * ((room + kGrain - 1) / kGrain);
   const int wave = kBlocksPerSm * sm_count();
   p.blocks = p.most < static_cast<double>(wave) * p.warps ? (static_cast<int>(p.most) + p.warps - 1) / p.warps : wave;
   p.rs = std::min(8 * p.NB, G);

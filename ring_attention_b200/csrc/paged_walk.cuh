@@ -228,7 +228,7 @@ constexpr int kMmaRows = 16;
 // 128 bytes each, four / eight warps 294 / 178, of 32 rows of 64 bytes, eight warps, 138.
 template <typename T, int D, int kRows_, int kExtraBytes>
 struct PagedBlock {
-  static constexpr bool kBulk = sizeof(T) == 4, kFour = false;
+  static constexpr bool kBulk = sizeof(T) == 4;
   static constexpr int SR = stage_keys(kBulk, D), RU = kRows_;
   static constexpr int kWarps = block_warps(kBulk, D), kThreads = kWarps * 32;
   static constexpr int kBoxes = kBulk || D <= 64 ? 1 : D / 64;
@@ -317,17 +317,7 @@ struct Ring {
       tcgen::mbar_expect_tx(full + 8 * slot, 2 * C::kRowBytes * rows() * __popc(there) + a.missing);
     }
     __syncwarp();
-    if constexpr (C::kFour) {
-      // a tensor's codes and its scales lie apart in a page, and here
-      const int which = at / 2;
-      if (at < 4 && head >= 0) {
-        const unsigned bytes = which == 0 ? C::kCodeBytes : C::kScaleBytes;
-        tcgen::bulk_load(tiles + (2 * slot + at % 2) * C::kTileBytes + which * C::SR * C::kCodeBytes + first * bytes,
-                         static_cast<const unsigned char*>(at % 2 == 0 ? a.k : a.v) + (static_cast<size_t>(head) << a.shift) * C::kRowBytes +
-                             (static_cast<size_t>(which * C::kCodeBytes) << a.shift) + row * bytes,
-                         bytes * rows(), full + 8 * slot);
-      }
-    } else if constexpr (C::kBulk) {
+    if constexpr (C::kBulk) {
       if (tensor < 2 && head >= 0)
         tcgen::bulk_load(tiles + (2 * slot + tensor) * C::kTileBytes + first * C::kRowBytes,
                          static_cast<const unsigned char*>(tensor == 0 ? a.k : a.v) +
