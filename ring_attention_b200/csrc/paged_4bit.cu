@@ -43,11 +43,12 @@ struct FourBlock {
   static constexpr int kStages = kMost < 4 ? kMost : 4;
   static constexpr int kRingBytes = 2 * kStages * kTileBytes;
   static constexpr int kOffInfo = kWarps * kRingBytes;
-  static constexpr int kOffBar = kOffInfo + kWarps * kStages * 32;
+  static constexpr int kOffUnits = kOffInfo + ((kWarps * kStages * 4 + 15) & ~15);
+  static constexpr int kOffBar = kOffUnits + kWarps * kStages * 16;
   static constexpr int kOffRoom = (kOffBar + kWarps * kStages * 8 + 15) & ~15;
   static constexpr int kOffFlag = kOffRoom + static_cast<int>(sizeof(ScanRoom<kWarps>));
   static constexpr int kSmemBytes = kOffFlag + 8;
-  static_assert(kTileBytes % 16 == 0 && kStages >= 2 && sizeof(StageInfo) == 32, "the ring");
+  static_assert(kTileBytes % 16 == 0 && kStages >= 2, "the ring");
   static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two blocks to an SM");
 };
 
@@ -55,20 +56,39 @@ struct FourBlock {
 template <typename C>
 struct FourRing {
   const PagedArgs& a;
-  unsigned char* tiles;  // shared memory: the ring, what there is to know of its places, its barriers
-  int4* info;
+  unsigned char* tiles;  // shared memory: the ring, what there is to know of its places (see Info), the units of their keys, barriers
+  unsigned* info;
+  int4* units;
   unsigned full;
   volatile int* gave_up;
-  Walk<kGrain> w;  // the next grain to copy
-  int total, per, next, first_st;
+  Walk<kGrain> w;  // the unit whose grains are copied
+  int total, per, next;
+  // of the warp's part of that unit: grains that are left, keys of the unit that are, the next key, whether nothing is copied yet
+  int run, left, at;
+  bool fresh, whole;  // (whole: the part is all of the unit)
+  const int* table;
   // this lane's copies: piece `piece` of the rows, of K's or V's codes or scales
   const unsigned char* from;
   unsigned to, row_bytes, rows, offset;
   int kind, page;  // (page: of its next copy, -1: none)
-  __device__ inline void look_up() {
-    const int at = (w.st * kGrain + static_cast<int>(offset)) >> a.shift;
-    page = -1;
-    if (next < total && kind < 4 && static_cast<int>(offset) < w.left() && at < a.max_pages) page = a.table[w.b * a.table_stride + at];
+
+  // What a warp has to know of a place when its copy has landed: keys (8 bits), blocks of 16 keys that are there (8), first of its part of
+  // the unit (1), last of it (1: yes, 2: yes, and the part is the result).
+  static constexpr int kBlocks = 8, kFirst = 16, kLast = 17;
+
+  __device__ inline void begin_part() {
+    run = min(w.n - w.st, total - next);
+    left = w.left();
+    at = w.st * kGrain;
+    fresh = true;
+    whole = w.st == 0 && run == w.n;
+    table = a.table + w.b * a.table_stride;
+    // the warp with a unit's first grain says which shares have parts of it: its own and those that the rest reaches into
+    if (w.st == 0 && (threadIdx.x & 31) == 0)
+      a.unit_parts[w.uid] = make_int2(static_cast<int>(blockIdx.x * C::kWarps + (threadIdx.x >> 5)), 1 + (w.n - run + per - 1) / per);
+  }
+  __device__ inline void look_up() {  // (the keys of a unit lie in its table)
+    page = run > 0 && kind < 4 && static_cast<int>(offset) < left ? table[(at + static_cast<int>(offset)) >> a.shift] : -1;
   }
   __device__ inline void begin(unsigned base) {
     const unsigned lane = threadIdx.x & 31, shift = a.shift < 5 ? a.shift : 5, pieces = C::SR >> shift;
@@ -79,54 +99,43 @@ struct FourRing {
     row_bytes = which == 0 ? C::kCodeBytes : C::kScaleBytes;
     from = static_cast<const unsigned char*>((kind & 1) == 0 ? a.k : a.v) + (which == 0 ? 0 : C::kCodeBytes << a.shift);
     to = base + (kind & 1) * C::kTileBytes + (which == 0 ? 0 : C::SR * C::kCodeBytes) + offset * row_bytes;
-    first_st = w.st;
     next = 0;
+    begin_part();
     look_up();
     for (int s = 0; s < C::kStages; ++s) copy(s);
   }
   // Copies the next grains, if there are any, to a place that is free.
   __device__ inline void copy(int slot) {
-    if (next >= total) return;
-    const int grains = min(min(C::GR, total - next), w.n - w.st), keys = min(grains * kGrain, w.left());
-    if (w.st == 0) {
-      first_st = 0;
-      // the warp with a unit's first grain says which shares have parts of it: its own and those that the rest reaches into
-      const int here = min(w.n, total - next);
-      if ((threadIdx.x & 31) == 0)
-        a.unit_parts[w.uid] = make_int2(static_cast<int>(blockIdx.x * C::kWarps + (threadIdx.x >> 5)), 1 + (w.n - here + per - 1) / per);
-    }
-    const bool there = page >= 0 && page < a.num_pages && static_cast<int>(offset) < keys;
-    const unsigned lanes = __ballot_sync(0xffffffffu, there);
+    if (run == 0) return;
+    const int grains = min(C::GR, run), keys = min(grains * kGrain, left);
+    const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages) && static_cast<int>(offset) < keys;
+    const unsigned pieces = __ballot_sync(0xffffffffu, there && kind == 0);
     if ((threadIdx.x & 31) == 0) {
-      // blocks of 16 keys that are there
-      unsigned blocks = lanes & ((1u << (C::SR / rows)) - 1u);
-      if (rows == 32) blocks = (blocks & 1u) * 3u | (blocks & 2u) * 6u | (blocks & 4u) * 12u | (blocks & 8u) * 24u;
-      const bool ends = w.st + grains == w.n;
-      const int last = ends && first_st == 0 ? 2 : ends || next + grains == total;
-      info[2 * slot] = make_int4(w.b, w.kvh, w.hb, w.uid);
-      info[2 * slot + 1] = make_int4(keys, static_cast<int>(blocks), w.st == first_st, last);
-      tcgen::mbar_expect_tx(full + 8 * slot, 2 * C::kRowBytes * rows * __popc(lanes & ((1u << (C::SR / rows)) - 1u)) + a.missing);
+      unsigned blocks = pieces;
+      if (rows == 32) blocks = (pieces & 1u) * 3u | (pieces & 2u) * 6u | (pieces & 4u) * 12u | (pieces & 8u) * 24u;
+      info[slot] = static_cast<unsigned>(keys) | blocks << kBlocks | static_cast<unsigned>(fresh) << kFirst |
+                   (run > grains ? 0u : whole ? 2u : 1u) << kLast;
+      if (fresh) units[slot] = make_int4(w.b, w.kvh, w.hb, w.uid);
+      tcgen::mbar_expect_tx(full + 8 * slot, 2 * C::kRowBytes * rows * __popc(pieces) + a.missing);
     }
     __syncwarp();
     if (there) {
-      const int row = (w.st * kGrain + static_cast<int>(offset)) & ((1 << a.shift) - 1);
+      const int row = (at + static_cast<int>(offset)) & ((1 << a.shift) - 1);
       tcgen::bulk_load(to + 2 * slot * C::kTileBytes,
                        from + ((static_cast<size_t>(page) * a.kvH + w.kvh) << a.shift) * C::kRowBytes + row * row_bytes, row_bytes * rows,
                        full + 8 * slot);
     }
+    fresh = false;
+    at += grains * kGrain;
+    left -= grains * kGrain;
     next += grains;
-    w.st += grains - 1;
-    if (next < total) {
+    run -= grains;
+    if (run == 0 && next < total) {  // on to the next unit
+      w.st = w.n - 1;
       w.next(a);
-      look_up();
+      begin_part();
     }
-  }
-  __device__ inline StageInfo at(int s) const {
-    const int4 x = info[2 * (s % C::kStages)], y = info[2 * (s % C::kStages) + 1];
-    StageInfo u;
-    u.b = x.x, u.kvh = x.y, u.hb = x.z, u.uid = x.w;
-    u.keys = y.x, u.pages = y.y, u.first = y.z, u.last = y.w;
-    return u;
+    look_up();
   }
   // Waits for copy s; false: the warp gives up.
   __device__ inline bool wait(int s) {
@@ -197,6 +206,7 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
   using C = FourBlock<D, NB>;
   using Cols = FourCols<D>;
   constexpr int RU = C::RU, kSteps = D / 16, kTiles = D / 16;
+  constexpr int kT = D * NB <= 256 ? 2 : 1;  // tiles of 16 keys at a time: two, as far as the registers go
   extern __shared__ __align__(1024) unsigned char smem[];
   const PagedArgs& a = args.p;
   const unsigned base = tcgen::smem_u32(smem);
@@ -209,8 +219,8 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   wait_for_previous();
-  FourRing<C> ring{a, smem + warp * C::kRingBytes, reinterpret_cast<int4*>(smem + C::kOffInfo) + 2 * warp * C::kStages,
-                   base + C::kOffBar + warp * C::kStages * 8, gave_up};
+  FourRing<C> ring{a, smem + warp * C::kRingBytes, reinterpret_cast<unsigned*>(smem + C::kOffInfo) + warp * C::kStages,
+                   reinterpret_cast<int4*>(smem + C::kOffUnits) + warp * C::kStages, base + C::kOffBar + warp * C::kStages * 8, gave_up};
   ring.total = find_share<kGrain, C::kWarps>(a, warp, &ring.w, &ring.per, reinterpret_cast<ScanRoom<C::kWarps>*>(smem + C::kOffRoom));
   auto walk = [&]() {
     ring.begin(base + warp * C::kRingBytes);
@@ -230,12 +240,18 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
     unsigned qb[NB][kSteps][2];
     float o[NB][kTiles][4];
     float m_run[NB][2], l_run[NB][2], factor[NB][2];  // of heads 2 j and 2 j + 1 of the eight
+    float m_off[NB][2];                               // m_run, or 0 where nothing has been seen
     int left = ring.total;
+    StageInfo u = {};
     for (int s = 0; left > 0; ++s) {
       const int slot = s % C::kStages;
-      const StageInfo u = ring.at(s);
-      left -= (u.keys + kGrain - 1) / kGrain;
-      if (u.first) {  // (while the copy is on its way)
+      const unsigned known = ring.info[slot];
+      const int keys = known & 0xff, last = known >> FourRing<C>::kLast & 3u;
+      const unsigned blocks = known >> FourRing<C>::kBlocks & 0xffu;
+      left -= (keys + kGrain - 1) / kGrain;
+      if (known >> FourRing<C>::kFirst & 1u) {  // (while the copy is on its way)
+        const int4 x = ring.units[slot];
+        u.b = x.x, u.kvh = x.y, u.hb = x.z, u.uid = x.w;
         // Q as B fragments, fp16: a row is brought to a largest magnitude of 1 to 2 by a power of two, which leaves all of it
         // that counts: fp16 rows and bf16 ones lose nothing above 2^-14 of their largest element, and below it less than 2^-25 of that.
 #pragma unroll
@@ -276,69 +292,80 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
 #pragma unroll
           for (int i = 0; i < kTiles; ++i) o[nb][i][0] = o[nb][i][1] = o[nb][i][2] = o[nb][i][3] = 0.f;
           m_run[nb][0] = m_run[nb][1] = -INFINITY;
+          m_off[nb][0] = m_off[nb][1] = 0.f;
           l_run[nb][0] = l_run[nb][1] = 0.f;  // this lane's share of the sums
         }
       }
       if (!ring.wait(s)) return;
       const unsigned char *const k_tile = ring.tiles + 2 * slot * C::kTileBytes, *const v_tile = k_tile + C::kTileBytes;
 #pragma unroll 1
-      for (int key0 = 0; key0 < u.keys; key0 += 16) {
-        const int n_valid = u.keys - key0;  // keys from here on
-        if (!(u.pages >> (key0 / 16) & 1u)) continue;
-        // S^T = K Q^T: keys g and g + 8 of the tile, heads 2 j and 2 j + 1
-        float sc[NB][4];
+      for (int key0 = 0; key0 < keys; key0 += 16 * kT) {
+        constexpr unsigned kAll = (1u << kT) - 1u;
+        const unsigned there = blocks >> (key0 / 16) & kAll;
+        if (there == 0) continue;
+        const bool whole = there == kAll && keys - key0 >= 16 * kT;  // (if not: see_of, keys of a tile that are there)
+        auto see_of = [&](int t) { return (there >> t & 1u) ? keys - key0 - 16 * t : 0; };
+        // S^T = K Q^T: keys g and g + 8 of a tile, heads 2 j and 2 j + 1
+        float sc[kT][NB][4];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
-        const unsigned char* const k_codes = k_tile + key0 * C::kCodeBytes;
-        const unsigned char* const k_scales = k_tile + C::SR * C::kCodeBytes + (key0 + key_g) * C::kScaleBytes;
+        for (int t = 0; t < kT; ++t)
 #pragma unroll
-        for (int p = 0; p < kKPieces; ++p) {
-          unsigned w[2][kKWords];
+          for (int nb = 0; nb < NB; ++nb) sc[t][nb][0] = sc[t][nb][1] = sc[t][nb][2] = sc[t][nb][3] = 0.f;
 #pragma unroll
-          for (int r = 0; r < 2; ++r) load_words(k_codes + k_at[p] + r * 8 * C::kCodeBytes, w[r]);
-          // scales of the lane's blocks, two to a piece of 32 columns
-          unsigned sk[2][2];
+        for (int p = 0; p < kKPieces; ++p)
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const unsigned char* const at = k_scales + r * 8 * C::kScaleBytes;
-            if constexpr (D >= 128) {
-              const unsigned both = scales_to_half(static_cast<unsigned short>(load_u16(at + 2 * j + 8 * p)));
-              sk[r][0] = __byte_perm(both, both, 0x1010);
-              sk[r][1] = __byte_perm(both, both, 0x3232);
-            } else {
-              const unsigned one = at[D == 64 ? j : j / 2];
-              sk[r][0] = sk[r][1] = scales_to_half(static_cast<unsigned short>(one | one << 8));
-            }
-          }
+          for (int t = 0; t < kT; ++t) {
+            const unsigned char* const k_codes = k_tile + (key0 + 16 * t) * C::kCodeBytes;
+            const unsigned char* const k_scales = k_tile + C::SR * C::kCodeBytes + (key0 + 16 * t + key_g) * C::kScaleBytes;
+            unsigned w[2][kKWords];
 #pragma unroll
-          for (int i = 0; i < kKWords; ++i) {
-            unsigned h[2][4];
+            for (int r = 0; r < 2; ++r) load_words(k_codes + k_at[p] + r * 8 * C::kCodeBytes, w[r]);
+            // scales of the lane's blocks, two to a piece of 32 columns
+            unsigned sk[2][2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              codes_to_half(w[r][i], h[r]);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) h[r][e] = mul_half2(h[r][e], sk[r][i / 2]);
+              const unsigned char* const at = k_scales + r * 8 * C::kScaleBytes;
+              if constexpr (D >= 128) {
+                const unsigned both = scales_to_half(static_cast<unsigned short>(load_u16(at + 2 * j + 8 * p)));
+                sk[r][0] = __byte_perm(both, both, 0x1010);
+                sk[r][1] = __byte_perm(both, both, 0x3232);
+              } else {
+                const unsigned one = at[D == 64 ? j : j / 2];
+                sk[r][0] = sk[r][1] = scales_to_half(static_cast<unsigned short>(one | one << 8));
+              }
             }
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const unsigned ka[4] = {h[0][2 * e], h[1][2 * e], h[0][2 * e + 1], h[1][2 * e + 1]};
-              const int st = p * 8 + 2 * i + e;
+            for (int i = 0; i < kKWords; ++i) {
+              unsigned h[2][4];
 #pragma unroll
-              for (int nb = 0; nb < NB; ++nb) mma16816<__half>(sc[nb], ka, qb[nb][st][0], qb[nb][st][1]);
+              for (int r = 0; r < 2; ++r) {
+                codes_to_half(w[r][i], h[r]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) h[r][e] = mul_half2(h[r][e], sk[r][i / 2]);
+              }
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const unsigned ka[4] = {h[0][2 * e], h[1][2 * e], h[0][2 * e + 1], h[1][2 * e + 1]};
+                const int st = p * 8 + 2 * i + e;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) mma16816<__half>(sc[t][nb], ka, qb[nb][st][0], qb[nb][st][1]);
+              }
             }
           }
-        }
-        const bool whole = n_valid >= 16, in0 = key_g < n_valid, in1 = key_g + 8 < n_valid;
         bool more = false;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
+          float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sc[nb][i] *= factor[nb][i & 1];
-          if (!whole) {
+          for (int t = 0; t < kT; ++t) {
+            if (!whole) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sc[nb][i] = (i < 2 ? in0 : in1) ? sc[nb][i] : -INFINITY;
+              for (int i = 0; i < 4; ++i) sc[t][nb][i] = key_g + (i < 2 ? 0 : 8) < see_of(t) ? sc[t][nb][i] : -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top[i & 1] = fmaxf(top[i & 1], sc[t][nb][i]);
           }
-          more = more || fmaxf(sc[nb][0], sc[nb][2]) > m_run[nb][0] || fmaxf(sc[nb][1], sc[nb][3]) > m_run[nb][1];
+          more = more || top[0] * factor[nb][0] > m_run[nb][0] || top[1] * factor[nb][1] > m_run[nb][1];
         }
         if (__any_sync(0xffffffffu, more)) {  // rare after the first stages
 #pragma unroll
@@ -346,13 +373,16 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
             float f[2];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              float mx = fmaxf(sc[nb][c], sc[nb][2 + c]);
+              float mx = -INFINITY;
+#pragma unroll
+              for (int t = 0; t < kT; ++t) mx = fmaxf(mx, fmaxf(sc[t][nb][c], sc[t][nb][2 + c]));
 #pragma unroll
               for (int d = 4; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-              const float mn = fmaxf(m_run[nb][c], mx);
+              const float mn = fmaxf(m_run[nb][c], mx * factor[nb][c]);  // (factors are above 0)
               f[c] = m_run[nb][c] == -INFINITY ? 0.f : ex2(m_run[nb][c] - mn);
               l_run[nb][c] = m_run[nb][c] == -INFINITY ? l_run[nb][c] : l_run[nb][c] * f[c];  // (0, or NaN to keep)
               m_run[nb][c] = mn;
+              m_off[nb][c] = mn == -INFINITY ? 0.f : mn;
             }
 #pragma unroll
             for (int i = 0; i < kTiles; ++i) {
@@ -364,37 +394,36 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
           }
         }
         // P^T as the B fragments of the second product, rounded to fp16 (l is not): 2^-12 of a weight
-        unsigned pb[NB][2];
+        unsigned pb[kT][NB][2];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          float p[4];
+        for (int t = 0; t < kT; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float m = m_run[nb][i & 1];
-            p[i] = ex2(sc[nb][i] - (m == -INFINITY ? 0.f : m));
+          for (int nb = 0; nb < NB; ++nb) {
+            float p[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = ex2(fmaf(sc[t][nb][i], factor[nb][i & 1], -m_off[nb][i & 1]));
+            l_run[nb][0] += p[0] + p[2];
+            l_run[nb][1] += p[1] + p[3];
+            pb[t][nb][0] = transposed(pack_pair<__half>(p[0], p[1]));
+            pb[t][nb][1] = transposed(pack_pair<__half>(p[2], p[3]));
           }
-          l_run[nb][0] += p[0] + p[2];
-          l_run[nb][1] += p[1] + p[3];
-          pb[nb][0] = transposed(pack_pair<__half>(p[0], p[1]));
-          pb[nb][1] = transposed(pack_pair<__half>(p[2], p[3]));
-        }
         // O^T += V^T P^T
-        const unsigned char* const v_codes = v_tile + key0 * C::kCodeBytes;
-        const unsigned char* const v_scales = v_tile + C::SR * C::kCodeBytes + key0 * C::kScaleBytes;
-        unsigned va[2][2][kTiles];  // [keys 2 j.., 2 j + 8..][rows g, g + 8][tile]: pairs of keys
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          unsigned w[2][kVWords];
+        for (int t = 0; t < kT; ++t) {
+          const unsigned char* const v_codes = v_tile + (key0 + 16 * t) * C::kCodeBytes;
+          const unsigned char* const v_scales = v_tile + C::SR * C::kCodeBytes + (key0 + 16 * t) * C::kScaleBytes;
+          unsigned h[2][kVWords][2][4], sv[2][2];  // [keys 2 j.., 2 j + 8..]: the codes of two keys, column by column; the scales
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const unsigned char* const at = v_codes + v_at[e] + r * 8 * C::kCodeBytes;
-            if constexpr (D >= 64) load_words(at, w[e]);
-            else w[e][0] = load_u16(at);
-          }
-          // the scales of the two keys, of the block of row g and of that of row g + 8 (head_dim 256: the next block); 0 for
-          // keys that are not the sequence's, whose bytes may be anything
-          unsigned sv[2];
-          {
+          for (int r = 0; r < 2; ++r) {
+            unsigned w[2][kVWords];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const unsigned char* const at = v_codes + v_at[e] + r * 8 * C::kCodeBytes;
+              if constexpr (D >= 64) load_words(at, w[e]);
+              else w[e][0] = load_u16(at);
+            }
+            // the scales of the two keys, of the block of row g and of that of row g + 8 (head_dim 256: the next block); 0 for
+            // keys that are not the sequence's, whose bytes may be anything
             const unsigned char *const at0 = v_scales + key_0 * C::kScaleBytes + r * 8 * C::kScaleBytes,
                                 *const at1 = v_scales + key_1 * C::kScaleBytes + r * 8 * C::kScaleBytes;
             unsigned s0, s1;
@@ -405,44 +434,38 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
               s0 = at0[g / kLanes], s1 = at1[g / kLanes];
             }
             if (!whole) {
-              s0 = key_0 + 8 * r < n_valid ? s0 : 0u;
-              s1 = key_1 + 8 * r < n_valid ? s1 : 0u;
+              s0 = key_0 + 8 * r < see_of(t) ? s0 : 0u;
+              s1 = key_1 + 8 * r < see_of(t) ? s1 : 0u;
             }
             if constexpr (D == 256) {
               const unsigned both = __byte_perm(s0, s1, 0x5140);  // (s0.lo, s1.lo, s0.hi, s1.hi)
-              sv[0] = scales_to_half(static_cast<unsigned short>(both));
-              sv[1] = scales_to_half(static_cast<unsigned short>(both >> 16));
+              sv[r][0] = scales_to_half(static_cast<unsigned short>(both));
+              sv[r][1] = scales_to_half(static_cast<unsigned short>(both >> 16));
             } else {
-              sv[0] = sv[1] = scales_to_half(static_cast<unsigned short>(s0 | s1 << 8));
+              sv[r][0] = sv[r][1] = scales_to_half(static_cast<unsigned short>(__byte_perm(s0, s1, 0x0040)));
+            }
+            // the codes of the two keys change places so that those of a column lie in a byte
+#pragma unroll
+            for (int i = 0; i < kVWords; ++i) {
+              const unsigned even = (w[0][i] & 0x0f0f0f0fu) | ((w[1][i] << 4) & 0xf0f0f0f0u);
+              const unsigned odd = ((w[0][i] >> 4) & 0x0f0f0f0fu) | (w[1][i] & 0xf0f0f0f0u);
+              codes_to_half(even, h[r][i][0]);
+              codes_to_half(odd, h[r][i][1]);
             }
           }
-          // the codes of the two keys change places so that those of a column lie in a byte
-          unsigned h[kVWords][2][4];
 #pragma unroll
-          for (int i = 0; i < kVWords; ++i) {
-            const unsigned even = (w[0][i] & 0x0f0f0f0fu) | ((w[1][i] << 4) & 0xf0f0f0f0u);
-            const unsigned odd = ((w[0][i] >> 4) & 0x0f0f0f0fu) | (w[1][i] & 0xf0f0f0f0u);
-            codes_to_half(even, h[i][0]);
-            codes_to_half(odd, h[i][1]);
+          for (int i = 0; i < kTiles; ++i) {
+            constexpr int x = Cols::v_other;  // from the column of row g to that of row g + 8
+            const unsigned av[4] = {mul_half2(h[0][i / 8][i % 2][i % 8 / 2], sv[0][0]), mul_half2(h[0][(i + x) / 8][(i + x) % 2][(i + x) % 8 / 2], sv[0][1]),
+                                    mul_half2(h[1][i / 8][i % 2][i % 8 / 2], sv[1][0]), mul_half2(h[1][(i + x) / 8][(i + x) % 2][(i + x) % 8 / 2], sv[1][1])};
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) mma16816<__half>(o[nb][i], av, pb[t][nb][0], pb[t][nb][1]);
           }
-#pragma unroll
-          for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const int col = i + x * Cols::v_other;  // of the lane's
-              va[r][x][i] = mul_half2(h[col / 8][col % 2][col % 8 / 2], sv[x]);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
-          const unsigned av[4] = {va[0][0][i], va[0][1][i], va[1][0][i], va[1][1][i]};
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) mma16816<__half>(o[nb][i], av, pb[nb][0], pb[nb][1]);
         }
       }
       __syncwarp();
       ring.copy(slot);
-      if (u.last) {
+      if (last) {
         const size_t part = (static_cast<size_t>(blockIdx.x) * C::kWarps + warp + u.uid) * a.rs;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
@@ -454,7 +477,7 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
             const int r = nb * 8 + 2 * j + c;
             int b, h;
             if (!unit_row<RU>(a, u, r, &b, &h)) continue;
-            const bool result = u.last == 2;
+            const bool result = last == 2;
             const float f = !result ? args.v_factor : l == 0.f ? 0.f : args.v_factor / l;  // (no key seen: O is 0 as well)
             constexpr int kEach = D / 16;  // columns side by side of row g, as many of row g + 8 behind them
 #pragma unroll
