@@ -573,6 +573,9 @@ int launch_forward(int dtype, int head_dim, int inter, const Args& a, unsigned t
   });
 }
 
+template <typename T>
+int launch_plain_4bit(int head_dim, const Args& a, unsigned tokens, cudaStream_t stream);  // append_4bit.cu
+
 // Rows of k, v and q of new tokens to a paged cache and q_out (see ra_paged_append, ra_paged_append_4bit).
 template <bool kFour>
 int append_rows(const char* what, const ra_paged_kv* cache, const ra_rows* k, const ra_rows* v, int rows, const int* counts,
@@ -611,6 +614,13 @@ int append_rows(const char* what, const ra_paged_kv* cache, const ra_rows* k, co
   a.page_shift = page_shift(cache->page_size);
   a.scale[1] = k_scale;
   a.scale[2] = v_scale;
+  if constexpr (kFour) {
+    if (!q && !a.w[1] && a.rot_dim == 0) {
+      const unsigned tokens = static_cast<unsigned>(cache->batch) * a.S;
+      return cache->dtype == RA_F16 ? launch_plain_4bit<__half>(cache->head_dim, a, tokens, static_cast<cudaStream_t>(stream))
+                                    : launch_plain_4bit<__nv_bfloat16>(cache->head_dim, a, tokens, static_cast<cudaStream_t>(stream));
+    }
+  }
   return launch_forward<true, kFour>(cache->dtype, cache->head_dim, inter, a, static_cast<unsigned>(cache->batch) * a.S, static_cast<cudaStream_t>(stream));
 }
 

@@ -52,6 +52,10 @@ struct FourBlock {
   static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two blocks to an SM");
 };
 
+// The reference of the weights is moved only when a score runs this far above it (in log2): weights of up to 2^8 are as exact in fp16
+// as those below 1, and with sixteen heads some maximum moves in nearly every one of a share's first tiles, at 200 instructions each time.
+constexpr float kSlack = 8.f;
+
 // A warp's ring: while a place is worked on, the others' copies are on their way.
 template <typename C>
 struct FourRing {
@@ -365,9 +369,9 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
 #pragma unroll
             for (int i = 0; i < 4; ++i) top[i & 1] = fmaxf(top[i & 1], sc[t][nb][i]);
           }
-          more = more || top[0] * factor[nb][0] > m_run[nb][0] || top[1] * factor[nb][1] > m_run[nb][1];
+          more = more || top[0] * factor[nb][0] > m_run[nb][0] + kSlack || top[1] * factor[nb][1] > m_run[nb][1] + kSlack;
         }
-        if (__any_sync(0xffffffffu, more)) {  // rare after the first stages
+        if (__any_sync(0xffffffffu, more)) {  // rare after a unit's first keys
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
             float f[2];
@@ -531,18 +535,22 @@ struct ReadArgs {
   float factor[2];
 };
 
-// A block has kTokens rows of the results: it finds out whose they are and where, and copies them for all heads, 16 bytes of a row a
-// thread, or (4 bits) one block of 16 elements. Bound by memory: a row comes in once and goes out once.
-constexpr int kReadThreads = 256, kReadTokens = 8;
+// A block has as many rows of the results as threads share out: it finds out whose they are and where, and a thread copies 16 bytes of a
+// row, or (4 bits) one block of 16 elements, for one head after the other, `per` of the list of K's heads and V's, four at a time. Bound
+// by memory: a row comes in once and goes out once.
+constexpr int kReadThreads = 256, kReadAhead = 4;
+template <typename T, bool kFour>
+constexpr int read_pieces(int D) { return kFour ? D / 16 : D * static_cast<int>(sizeof(T)) / 16; }
+
 template <typename T, int D, bool kFour>
-__global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const __grid_constant__ ReadArgs a) {
-  constexpr int kEach = kFour ? 16 : 16 / static_cast<int>(sizeof(T)), kPieces = D / kEach, kOf = kReadTokens * kPieces;
-  constexpr int kWords = kEach * static_cast<int>(sizeof(T)) / 4, kAhead = 4;
-  __shared__ long long place_of[kReadTokens];
+__global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const __grid_constant__ ReadArgs a, int per) {
+  constexpr int kPieces = read_pieces<T, kFour>(D), kTokens = kReadThreads / kPieces, kEach = D / kPieces;
+  constexpr int kWords = kEach * static_cast<int>(sizeof(T)) / 4;
+  __shared__ long long place_of[kTokens];
   let_next_start();
   wait_for_previous();
-  const int token0 = static_cast<int>(blockIdx.x) * kReadTokens;
-  if (threadIdx.x < kReadTokens) {
+  const int token0 = static_cast<int>(blockIdx.x) * kTokens;
+  if (threadIdx.x < kTokens) {
     const int i = token0 + static_cast<int>(threadIdx.x);
     long long place = -2;  // a row of the results that is no sequence's stays as it is
     if (i < a.rows && i >= a.ends[0] && i < a.ends[a.B]) {
@@ -558,55 +566,72 @@ __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const __grid_c
     place_of[threadIdx.x] = place;
   }
   __syncthreads();
-  const int total = 2 * a.kvH * kOf;
-  for (int i0 = threadIdx.x; i0 < total; i0 += kAhead * kReadThreads) {
-    unsigned u[kAhead][kFour ? 3 : kWords];
+  const int token = threadIdx.x / kPieces, piece = threadIdx.x % kPieces;
+  const long long place = place_of[token];
+  if (place == -2) return;
+  const bool there = place >= 0;  // (a row that there is not is zeros)
+  const int row = static_cast<int>(place) & ((1 << a.shift) - 1);
+  const size_t page_head = there ? static_cast<size_t>(place >> a.shift) : 0;
+  [[maybe_unused]] const int code_at = row * (D / 2) + ((piece / 2) ^ four_turn(row, D)) * 16 + piece % 2 * 8;
+  [[maybe_unused]] const int scale_at = (D / 2 << a.shift) + row * (D / 16) + piece;
+  const int end = min((static_cast<int>(blockIdx.y) + 1) * per, 2 * a.kvH);
+  for (int h0 = static_cast<int>(blockIdx.y) * per; h0 < end; h0 += kReadAhead) {
+    unsigned u[kReadAhead][kFour ? 3 : 4];
 #pragma unroll
-    for (int n = 0; n < kAhead; ++n) {
-      const int i = i0 + n * kReadThreads;
-      if (i >= total) break;
-      const int side_head = i / kOf, token = i % kOf / kPieces, piece = i % kPieces;
-      const int side = side_head >= a.kvH, head = side_head - side * a.kvH;
-      const long long place = place_of[token];
+    for (int n = 0; n < kReadAhead; ++n) {
 #pragma unroll
-      for (int w = 0; w < (kFour ? 3 : kWords); ++w) u[n][w] = 0u;  // a row that there is not is zeros
-      if (place < 0) continue;
+      for (int w = 0; w < (kFour ? 3 : 4); ++w) u[n][w] = 0u;
+      if (h0 + n >= end || !there) continue;
+      const bool v = h0 + n >= a.kvH;
+      const size_t head = page_head + (h0 + n - (v ? a.kvH : 0));
+      const char* const pages = v ? a.pages[1] : a.pages[0];
       if constexpr (kFour) {
-        const int row = static_cast<int>(place) & ((1 << a.shift) - 1);
-        const char* const page = a.pages[side] + (((place >> a.shift) + head) << a.shift) * four_row_bytes(D);
-        const uint2 c = *reinterpret_cast<const uint2*>(page + row * (D / 2) + ((piece / 2) ^ four_turn(row, D)) * 16 + piece % 2 * 8);
+        const char* const from = pages + (head << a.shift) * four_row_bytes(D);
+        const uint2 c = *reinterpret_cast<const uint2*>(from + code_at);
         u[n][0] = c.x, u[n][1] = c.y;
-        u[n][2] = static_cast<unsigned char>(page[(D / 2 << a.shift) + row * (D / 16) + piece]);
+        u[n][2] = static_cast<unsigned char>(from[scale_at]);
       } else {
-        const uint4 v = *reinterpret_cast<const uint4*>(
-            a.pages[side] + ((place + (static_cast<long long>(head) << a.shift)) * D + piece * kEach) * sizeof(T));
-        u[n][0] = v.x, u[n][1] = v.y, u[n][2] = v.z, u[n][3] = v.w;
+        const uint4 x = *reinterpret_cast<const uint4*>(pages + (((head << a.shift) + row) * D + piece * kEach) * sizeof(T));
+        u[n][0] = x.x, u[n][1] = x.y, u[n][2] = x.z, u[n][3] = x.w;
       }
     }
 #pragma unroll
-    for (int n = 0; n < kAhead; ++n) {
-      const int i = i0 + n * kReadThreads;
-      if (i >= total) break;
-      const int side_head = i / kOf, token = i % kOf / kPieces, piece = i % kPieces;
-      const int side = side_head >= a.kvH, head = side_head - side * a.kvH;
-      if (place_of[token] == -2) continue;
-      const ReadRows out = a.out[side];
-      T* const dst = reinterpret_cast<T*>(out.data) + (token0 + token) * out.row + head * out.head + piece * kEach;
+    for (int n = 0; n < kReadAhead; ++n) {
+      if (h0 + n >= end) break;
+      const bool v = h0 + n >= a.kvH;
+      const ReadRows& out = v ? a.out[1] : a.out[0];
+      T* const dst = reinterpret_cast<T*>(out.data) + static_cast<long long>(token0 + token) * out.row +
+                     (h0 + n - (v ? a.kvH : 0)) * out.head + piece * kEach;
       unsigned w[kWords];
       if constexpr (kFour) {
         const unsigned s = scales_to_half(static_cast<unsigned short>(u[n][2] | u[n][2] << 8));
+        const float f = v ? a.factor[1] : a.factor[0];
         unsigned h[2][4];
         codes_to_half(u[n][0], h[0]);
         codes_to_half(u[n][1], h[1]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const unsigned v = mul_half2(h[e / 4][e % 4], s);
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
-          w[e] = pack_pair<T>(f.x * a.factor[side], f.y * a.factor[side]);
+          const unsigned x = mul_half2(h[e / 4][e % 4], s);
+          const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&x));
+          w[e] = pack_pair<T>(y.x * f, y.y * f);
         }
       } else {
 #pragma unroll
         for (int e = 0; e < kWords; ++e) w[e] = u[n][e];
+      }
+      if constexpr (kFour) {
+        // Two lanes have 64 bytes side by side; they exchange halves, so that a store of the warp has whole 32-byte sectors (four prompts of
+        // 20000 to 32768 rows, 8 KV heads of 128 in bf16: 127 -> 92 us).
+        if (a.vec) {
+          const bool odd = threadIdx.x & 1;
+          unsigned r[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) r[e] = __shfl_xor_sync(0xffffffffu, odd ? w[e] : w[4 + e], 1);
+          uint4* const to = reinterpret_cast<uint4*>(dst) - (odd ? 2 : 0) + (odd ? 1 : 0);  // (of the even lane's block, and 32 bytes behind it)
+          to[0] = odd ? make_uint4(r[0], r[1], r[2], r[3]) : make_uint4(w[0], w[1], w[2], w[3]);
+          to[2] = odd ? make_uint4(w[4], w[5], w[6], w[7]) : make_uint4(r[0], r[1], r[2], r[3]);
+          continue;
+        }
       }
       if (a.vec) {
 #pragma unroll
@@ -737,8 +762,15 @@ int read_rows(const char* what, const ra_paged_kv* cache, float k_scale, float v
   a.factor[0] = k_scale;
   a.factor[1] = v_scale;
   auto go = [&](auto t, auto d) -> int {
-    RAB_CUDA(launch_overlapped(paged_read_kernel<decltype(t), d(), kFour>, dim3((static_cast<unsigned>(rows) + kReadTokens - 1) / kReadTokens),
-                               dim3(kReadThreads), 0, stream, a));
+    constexpr unsigned kTokens = kReadThreads / read_pieces<decltype(t), kFour>(d());
+    const unsigned blocks = (static_cast<unsigned>(rows) + kTokens - 1) / kTokens;
+    // all heads a block, whose place it finds but once, or, where that leaves SMs without enough blocks, fewer
+    const int heads = 2 * c.kv_heads, room = 8 * sm_count();
+    int per = heads;
+    while (per > kReadAhead && static_cast<long long>(blocks) * ((heads + per - 1) / per) < room) per = (per + 1) / 2;
+    RAB_REQUIRE((heads + per - 1) / per <= 65535, RA_ERR_INVALID, "%s: bad heads", what);
+    RAB_CUDA(launch_overlapped(paged_read_kernel<decltype(t), d(), kFour>, dim3(blocks, static_cast<unsigned>((heads + per - 1) / per)),
+                               dim3(kReadThreads), 0, stream, a, per));
     return RA_OK;
   };
   auto by_dim = [&](auto t) -> int {
