@@ -117,47 +117,58 @@ __device__ inline int blocks_from(const PackedArgs& a, const Seq& s, int c) {
   return first >= s.blocks ? 0 : s.blocks - static_cast<int>(first);
 }
 
-// The items by their number, those with the most key tiles first, then by sequence, block, and KV head and set of heads. Run by a warp.
+// The items by their number, those with the most key tiles first, then by sequence, block, and KV head and set of heads. Run by a warp. What
+// it has counted and where it has got to among the sequences it keeps, so that many sequences are gone over once for each number of key
+// tiles and not for each item.
 template <int kBN>
 struct Items {
   const PackedArgs& a;
   int lane, of_block;  // items of a block of tokens
   Seq mine;            // lane's among the first 32 sequences
   int top, level;      // key tiles: the most, those of the last item found
+  long long from, above;  // blocks with `level` key tiles or more, and with more than them
+  int chunk;              // sequences chunk to chunk + 31 have had `passed` blocks of just this level before them
+  long long passed;
   __device__ Items(const PackedArgs& a_, int lane_) : a(a_), lane(lane_), of_block(a_.kvH * a_.head_sets) {
     mine = Seq{0, 0, 0, 0, 0};
     if (lane < a.B) mine = sequence(a, lane);
     int most = mine.k_len;
     for (int b = lane + 32; b < a.B; b += 32) most = max(most, sequence(a, b).k_len);
     most = __reduce_max_sync(0xffffffffu, most);
-    top = level = (most + kBN - 1) / kBN;
+    top = (most + kBN - 1) / kBN;
+    to_level(top);
   }
   __device__ Seq of(int b) const { return b < 32 ? mine : b < a.B ? sequence(a, b) : Seq{0, 0, 0, 0, 0}; }
   __device__ long long count(int c) const {  // blocks with c key tiles or more
-    int n = blocks_from<kBN>(a, mine, c);
-    long long sum = __reduce_add_sync(0xffffffffu, n);
+    long long sum = __reduce_add_sync(0xffffffffu, blocks_from<kBN>(a, mine, c));
     for (int b0 = 32; b0 < a.B; b0 += 32) sum += __reduce_add_sync(0xffffffffu, blocks_from<kBN>(a, of(b0 + lane), c));
     return sum;
   }
-  // (quick where numbers rise from call to call)
+  __device__ void to_level(int c) {
+    level = c;
+    from = count(c);
+    above = count(c + 1);
+    chunk = 0;
+    passed = 0;
+  }
   __device__ Item find(long long i) {
     Item it = {};
     const long long block = i / of_block;
-    const bool lower = count(level) <= block;
-    if (lower || count(level + 1) > block) {
-      if (lower && count(0) <= block) return it;
-      int lo = lower ? 0 : level + 1, hi = lower ? level : top + 1;  // count(lo) > block >= count(hi)
+    if (from <= block || above > block) {
+      if (from <= block && (level == 0 || count(0) <= block)) return it;
+      int lo = from <= block ? 0 : level + 1, hi = from <= block ? level : top + 1;  // count(lo) > block >= count(hi)
       while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
         if (count(mid) > block) lo = mid;
         else hi = mid;
       }
-      level = lo;
+      to_level(lo);
     }
-    long long at = block - count(level + 1);  // among the blocks of just this level
-    for (int b0 = 0; b0 < a.B; b0 += 32) {
-      const Seq s = of(b0 + lane);
-      const int above = blocks_from<kBN>(a, s, level + 1), n = blocks_from<kBN>(a, s, level) - above;
+    if (block - above < passed) chunk = 0, passed = 0;
+    for (; chunk < a.B; chunk += 32) {
+      const long long at = block - above - passed;  // among the blocks of just this level from here on
+      const Seq s = of(chunk + lane);
+      const int more = blocks_from<kBN>(a, s, level + 1), n = blocks_from<kBN>(a, s, level) - more;
       int upto = n;
 #pragma unroll
       for (int d = 1; d < 32; d *= 2) {
@@ -166,20 +177,20 @@ struct Items {
       }
       const unsigned has = __ballot_sync(0xffffffffu, upto > at);
       if (has) {
-        const int from = __ffs(static_cast<int>(has)) - 1;
+        const int src = __ffs(static_cast<int>(has)) - 1;
         const int m = static_cast<int>(i - block * of_block);
         it.there = 1;
-        it.q0 = __shfl_sync(0xffffffffu, s.q0, from);
-        it.q_len = __shfl_sync(0xffffffffu, s.q_len, from);
-        it.k0 = __shfl_sync(0xffffffffu, s.k0, from);
-        it.k_len = __shfl_sync(0xffffffffu, s.k_len, from);
-        const int nth = static_cast<int>(at) - __shfl_sync(0xffffffffu, upto - n, from);
-        it.token0 = (__shfl_sync(0xffffffffu, s.blocks - above, from) - 1 - nth) << a.token_shift;
+        it.q0 = __shfl_sync(0xffffffffu, s.q0, src);
+        it.q_len = __shfl_sync(0xffffffffu, s.q_len, src);
+        it.k0 = __shfl_sync(0xffffffffu, s.k0, src);
+        it.k_len = __shfl_sync(0xffffffffu, s.k_len, src);
+        const int nth = static_cast<int>(at) - __shfl_sync(0xffffffffu, upto - n, src);
+        it.token0 = (__shfl_sync(0xffffffffu, s.blocks - more, src) - 1 - nth) << a.token_shift;
         it.kv = m % a.kvH;
         it.head = m / a.kvH * a.pack;
         return it;
       }
-      at -= __shfl_sync(0xffffffffu, upto, 31);
+      passed += __shfl_sync(0xffffffffu, upto, 31);
     }
     return it;
   }
