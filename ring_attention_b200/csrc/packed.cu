@@ -55,34 +55,39 @@ struct Item {
   int kv, head;   // KV head, first of the tile's heads inside the group
 };
 
-template <int D>
+// kOne: one query tile a block and two blocks to an SM, for short sequences, of which a block's second tile would have few rows or none:
+// two blocks are in different places of an item, so that one's copies and rows' way out run under the other's softmax.
+template <int D, bool kOne>
 struct PackedCfg {
-  static constexpr int kTiles = D == 256 ? 1 : 2;
+  static_assert(!kOne || D <= 128, "two blocks to an SM");
+  static constexpr int kTiles = D == 256 || kOne ? 1 : 2;
   static constexpr int kThreads = 128 + 128 * kTiles;
   static constexpr int kBN = D == 256 ? 64 : 128;  // keys of a tile
   static constexpr int kBoxes = D / 64;
   static constexpr int kQBytes = kBM * D * 2, kKvBytes = kBN * D * 2;
-  static constexpr int kStages = D == 64 ? 8 : 4;
+  static constexpr int kStages = (D == 64 ? 8 : 4) / (kOne ? 2 : 1);
   // head_dim 64: P has a place of its own and the next scores go out while P is made; 128: P overwrites S; 256: two score buffers, the
   // next but one scores go out behind the products with P that overwrites theirs
   static constexpr bool kEarlyS = D == 64, kDoubleS = D == 256, kOrdered = D == 128;
-  static constexpr int kColS0 = 0, kColS1 = 128, kColO0 = 256, kColO1 = 256 + D;
-  static constexpr int kColP0 = kEarlyS ? 384 : kColS0, kColP1 = kEarlyS ? 448 : kColS1;
-  // registers of the copying and issuing warps' threads and of the softmax threads (128 and 256, of 168 each at the start)
-  static constexpr int kRegsLo = D == 64 ? 104 : 72, kRegsHi = D == 64 ? 200 : 216;
-  static_assert(128 * kRegsLo + 256 * kRegsHi <= 384 * 168, "registers");
+  static constexpr int kCols = kOne ? 256 : 512;  // of tensor memory
+  static constexpr int kColS0 = 0, kColS1 = 128, kColO0 = kOne ? 128 : 256, kColO1 = 256 + D;
+  static constexpr int kColP0 = !kEarlyS ? kColS0 : kOne ? 192 : 384, kColP1 = kEarlyS ? 448 : kColS1;
+  // registers of the copying and issuing warps' threads and of the softmax threads: of 168 each at the start, or, two blocks to an SM, 128
+  // (head_dim 256: 255 each, nothing to share out)
+  static constexpr int kRegsLo = kOne ? 56 : D == 64 ? 104 : 72, kRegsHi = kOne ? 200 : D == 64 ? 200 : 216;
+  static constexpr bool kShare = D != 256;
+  static_assert(!kShare || 128 * kRegsLo + 128 * kTiles * kRegsHi <= kThreads * (kOne ? 128 : 168), "registers");
   static constexpr int kOffKv = kTiles * kQBytes;
   static constexpr int kOffOut = kOffKv + kStages * kKvBytes;  // rows on their way out: 4 KB a warp
   static constexpr int kOffBar = kOffOut + kTiles * 4 * 4096;
   static constexpr int kNumBars = 4 + 2 * kStages + 8 + 6;
   static constexpr int kOffNext = (kOffBar + kNumBars * 8 + 15) & ~15;  // the hardware's answer, see next_block
   static constexpr int kOffItem = kOffNext + 16;
-  static constexpr int kSmemBytes = kOffItem + 2 * static_cast<int>(sizeof(Item)) + 16 + 1024;
-  static_assert(kSmemBytes <= 232448, "shared memory budget");
+  static constexpr int kSmemBytes = kOffItem + 2 * static_cast<int>(sizeof(Item)) + 16;
+  static_assert((kOne ? 2 : 1) * (kSmemBytes + 1024) <= 228 * 1024, "shared memory");
 };
 
 // Key tiles that query tile w of an item needs (0: none, or no rows), and its keys.
-template <int D>
 __device__ inline int tile_keys(const PackedArgs& a, const Item& it, int w) {
   const int first = it.token0 + w * a.tile_tokens;
   if (first >= it.q_len) return 0;
@@ -235,16 +240,14 @@ __device__ inline bool take_block(unsigned room, unsigned bar, int n, unsigned* 
 // ---- kernel -------------------------------------------------------------------------
 
 // DR: head_dim of the tensors: D, or 32 on the 64-wide kernel, whose copies bring zeros for the upper half of every row.
-template <int D, int DR, typename T>
-__global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
+template <int D, int DR, typename T, bool kOne>
+__global__ void __launch_bounds__(PackedCfg<D, kOne>::kThreads, kOne ? 2 : 1)
     packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PackedArgs a) {
-  using C = PackedCfg<D>;
+  using C = PackedCfg<D, kOne>;
   constexpr int kBN = C::kBN;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  extern __shared__ unsigned char smem_raw[];
-  unsigned char* const smem =
-      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  extern __shared__ __align__(1024) unsigned char smem[];
   const unsigned base = smem_u32(smem), s_kv = base + C::kOffKv, bars = base + C::kOffBar;
   const unsigned q_full = bars, q_free = bars + 16;                                      // [2] each
   const unsigned kv_full = bars + 32, kv_free = kv_full + 8 * C::kStages;                // [kStages]
@@ -257,7 +260,7 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  constexpr int kItemReaders = 2 + (C::kEarlyS ? 1 : 0) + 4 * C::kTiles;
+  constexpr int kIssuers = C::kEarlyS ? C::kTiles : 1, kItemReaders = 1 + kIssuers + 4 * C::kTiles;
   let_next_start();
   if (tid == 0) {
     for (int w = 0; w < 2; ++w) {
@@ -272,7 +275,7 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
     }
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(kv_full + 8 * s, 1);
-      mbar_init(kv_free + 8 * s, C::kEarlyS ? 2 : 1);
+      mbar_init(kv_free + 8 * s, kIssuers);
     }
     mbar_init(next_full, 1);
     mbar_init(copied, 1);
@@ -283,7 +286,8 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
     prefetch_map(&map_v);
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(C::kCols)
+                 : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
@@ -315,10 +319,10 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
     give_item_back(n);
     return it->there != 0;
   };
-  auto tiles_of = [&](const Item& it, int w) { return w < C::kTiles ? (tile_keys<D>(a, it, w) + kBN - 1) / kBN : 0; };
+  auto tiles_of = [&](const Item& it, int w) { return w < C::kTiles ? (tile_keys(a, it, w) + kBN - 1) / kBN : 0; };
 
   if (warp < 4) {
-    if constexpr (C::kTiles == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsLo));
+    if constexpr (C::kShare) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsLo));
     if (gone) {
     } else if (warp == 3) {
       // ------------------------------------------------------------------ items ----
@@ -383,7 +387,7 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
         __syncwarp();
         if (ok && lane == 0) mbar_arrive(copied);
       }
-    } else if (warp == 1 || C::kEarlyS) {
+    } else if (warp <= kIssuers) {
       // --------------------------------------------------------------- products ----
       constexpr unsigned kFmt = kBf16 ? 1u : 0u;
       constexpr unsigned idesc_pv = make_idesc(kFmt, 1, D, kBM);
@@ -427,7 +431,7 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
       for (int n = 0; ok && next_item(n, &it); ++n) {
         const int n_of[2] = {tiles_of(it, 0), tiles_of(it, 1)}, n_tiles = max(n_of[0], n_of[1]);
         auto keys_of = [&](int t) { return it.k_len - t * kBN; };  // of the sequence, from a tile on
-        const int seen_of[2] = {tile_keys<D>(a, it, 0), C::kTiles == 2 ? tile_keys<D>(a, it, 1) : 0};
+        const int seen_of[2] = {tile_keys(a, it, 0), C::kTiles == 2 ? tile_keys(a, it, 1) : 0};
         // keys of tile t that some row of query tile w sees, in steps of 16
         auto steps_of = [&](int t, int w) { return min(kBN, (seen_of[w] - t * kBN + 15) & ~15) / 16; };
         if constexpr (C::kOrdered) {
@@ -553,7 +557,7 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
       }
     }
   } else {
-    if constexpr (C::kTiles == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsHi));
+    if constexpr (C::kShare) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsHi));
     // ----------------------------------------------------------------- softmax ----
     const int w = (warp - 4) >> 2;
     const int row = ((warp & 3) << 5) + lane;
@@ -795,7 +799,7 @@ __global__ void __launch_bounds__(PackedCfg<D>::kThreads, 1)
       while (global_ns() - t0 < 1000000ull) __nanosleep(1000);
     }
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::kCols) : "memory");
   }
 }
 
@@ -836,14 +840,10 @@ bool rows_for_tma(const ra_rows& r, int head_dim, int heads, int rows) {
          (heads <= 1 || r.head_stride < 1ll << 32) && (rows <= 1 || r.row_stride < 1ll << 32);
 }
 
-template <int D, int DR, typename T>
-int launch_packed(const ra_rows& q, const ra_rows& k, const ra_rows& v, PackedArgs a, cudaStream_t stream) {
-  using C = PackedCfg<D>;
+template <int D, int DR, typename T, bool kOne>
+int launch_tiles(const ra_rows& q, const ra_rows& k, const ra_rows& v, PackedArgs a, cudaStream_t stream) {
+  using C = PackedCfg<D, kOne>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  a.pack = heads_per_tile(a.G, (a.rows + a.B - 1) / a.B);
-  a.tile_tokens = kBM / a.pack;
-  while ((1 << a.tile_shift) < a.tile_tokens) ++a.tile_shift;
-  a.head_sets = (a.G + a.pack - 1) / a.pack;
   a.token_shift = 0;
   while ((1 << a.token_shift) < C::kTiles * a.tile_tokens) ++a.token_shift;
   CUtensorMap mq, mk, mv;
@@ -860,7 +860,7 @@ int launch_packed(const ra_rows& q, const ra_rows& k, const ra_rows& v, PackedAr
   rc = make_rows_map(&mk, kBf16, k.data, 3, kdims, ks, kbox);
   if (rc == RA_OK) rc = make_rows_map(&mv, kBf16, v.data, 3, kdims, vs, kbox);
   if (rc != RA_OK) return rc;
-  auto kern = packed_kernel<D, DR, T>;
+  auto kern = packed_kernel<D, DR, T, kOne>;
   static std::atomic<unsigned long long> smem_set{0};  // once per device and instantiation
   int dev = 0;
   RAB_CUDA(cudaGetDevice(&dev));
@@ -873,6 +873,22 @@ int launch_packed(const ra_rows& q, const ra_rows& k, const ra_rows& v, PackedAr
   RAB_REQUIRE(most < 1ll << 31, RA_ERR_INVALID, "packed_attention: too many rows, sequences and heads");
   RAB_CUDA(launch_overlapped(kern, dim3(static_cast<unsigned>(most)), dim3(C::kThreads), C::kSmemBytes, stream, mq, mk, mv, a));
   return RA_OK;
+}
+
+template <int D, int DR, typename T>
+int launch_packed(const ra_rows& q, const ra_rows& k, const ra_rows& v, PackedArgs a, cudaStream_t stream) {
+  const long long tokens = (a.rows + a.B - 1) / a.B;
+  a.pack = heads_per_tile(a.G, tokens);
+  a.tile_tokens = kBM / a.pack;
+  while ((1 << a.tile_shift) < a.tile_tokens) ++a.tile_shift;
+  a.head_sets = (a.G + a.pack - 1) / a.pack;
+  if constexpr (D <= 128) {
+    // Sequences of one query tile on average, at head_dim 64 and below of two, are taken a tile a block. us a call of 16384 rows, two tiles a
+    // block / one: H32/kvH8 D128, sequences of 16 rows (half a tile) 301 / 211, 32 rows 151 / 117, 64 rows 93 / 93, 128 rows 87 / 103; H24/kvH6 D64,
+    // 32 rows (a tile) 125 / 79, 64 rows 66 / 59, 128 rows 63 / 66; H16 D64, 128 rows (a tile) 88 / 50, 256 rows 69 / 60, 512 rows 76 / 74.
+    if (tokens <= (D == 64 ? 2 : 1) * a.tile_tokens) return launch_tiles<D, DR, T, true>(q, k, v, a, stream);
+  }
+  return launch_tiles<D, DR, T, false>(q, k, v, a, stream);
 }
 
 }  // namespace

@@ -362,6 +362,9 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
           float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
           for (int t = 0; t < kT; ++t) {
+            // (rounded before the difference to the reference, so that the largest score's is 0 however large it is)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[t][nb][i] *= factor[nb][i & 1];
             if (!whole) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) sc[t][nb][i] = key_g + (i < 2 ? 0 : 8) < see_of(t) ? sc[t][nb][i] : -INFINITY;
@@ -369,7 +372,7 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
 #pragma unroll
             for (int i = 0; i < 4; ++i) top[i & 1] = fmaxf(top[i & 1], sc[t][nb][i]);
           }
-          more = more || top[0] * factor[nb][0] > m_run[nb][0] + kSlack || top[1] * factor[nb][1] > m_run[nb][1] + kSlack;
+          more = more || top[0] > m_run[nb][0] + kSlack || top[1] > m_run[nb][1] + kSlack;
         }
         if (__any_sync(0xffffffffu, more)) {  // rare after a unit's first keys
 #pragma unroll
@@ -382,7 +385,7 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
               for (int t = 0; t < kT; ++t) mx = fmaxf(mx, fmaxf(sc[t][nb][c], sc[t][nb][2 + c]));
 #pragma unroll
               for (int d = 4; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-              const float mn = fmaxf(m_run[nb][c], mx * factor[nb][c]);  // (factors are above 0)
+              const float mn = fmaxf(m_run[nb][c], mx);
               f[c] = m_run[nb][c] == -INFINITY ? 0.f : ex2(m_run[nb][c] - mn);
               l_run[nb][c] = m_run[nb][c] == -INFINITY ? l_run[nb][c] : l_run[nb][c] * f[c];  // (0, or NaN to keep)
               m_run[nb][c] = mn;
@@ -405,7 +408,7 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
           for (int nb = 0; nb < NB; ++nb) {
             float p[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = ex2(fmaf(sc[t][nb][i], factor[nb][i & 1], -m_off[nb][i & 1]));
+            for (int i = 0; i < 4; ++i) p[i] = ex2(sc[t][nb][i] - m_off[nb][i & 1]);
             l_run[nb][0] += p[0] + p[2];
             l_run[nb][1] += p[1] + p[3];
             pb[t][nb][0] = transposed(pack_pair<__half>(p[0], p[1]));
