@@ -356,6 +356,29 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
               }
             }
           }
+        // V's bytes are on their way while the weights are worked out, as far as the registers go
+        constexpr bool kEarlyV = D * NB <= 128;
+        unsigned vw[kT][2][2][kVWords], vs[kT][2][2];  // [tile][keys 2 j.., 2 j + 8..][key]: words of codes, bytes of scales
+        auto load_v = [&](int t) {
+          const unsigned char* const v_codes = v_tile + (key0 + 16 * t) * C::kCodeBytes;
+          const unsigned char* const v_scales = v_tile + C::SR * C::kCodeBytes + (key0 + 16 * t) * C::kScaleBytes;
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const unsigned char* const at = v_codes + v_at[e] + r * 8 * C::kCodeBytes;
+              if constexpr (D >= 64) load_words(at, vw[t][r][e]);
+              else vw[t][r][e][0] = load_u16(at);
+              const unsigned char* const of = v_scales + (e == 0 ? key_0 : key_1) * C::kScaleBytes + r * 8 * C::kScaleBytes;
+              constexpr int kLanes = D == 256 ? 1 : 128 / D;  // lanes to a block
+              if constexpr (D == 256) vs[t][r][e] = load_u16(of + 2 * g);
+              else vs[t][r][e] = of[g / kLanes];
+            }
+        };
+        if constexpr (kEarlyV) {
+#pragma unroll
+          for (int t = 0; t < kT; ++t) load_v(t);
+        }
         bool more = false;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -417,29 +440,14 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
         // O^T += V^T P^T
 #pragma unroll
         for (int t = 0; t < kT; ++t) {
-          const unsigned char* const v_codes = v_tile + (key0 + 16 * t) * C::kCodeBytes;
-          const unsigned char* const v_scales = v_tile + C::SR * C::kCodeBytes + (key0 + 16 * t) * C::kScaleBytes;
+          if constexpr (!kEarlyV) load_v(t);
           unsigned h[2][kVWords][2][4], sv[2][2];  // [keys 2 j.., 2 j + 8..]: the codes of two keys, column by column; the scales
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            unsigned w[2][kVWords];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const unsigned char* const at = v_codes + v_at[e] + r * 8 * C::kCodeBytes;
-              if constexpr (D >= 64) load_words(at, w[e]);
-              else w[e][0] = load_u16(at);
-            }
+            auto& w = vw[t][r];
             // the scales of the two keys, of the block of row g and of that of row g + 8 (head_dim 256: the next block); 0 for
             // keys that are not the sequence's, whose bytes may be anything
-            const unsigned char *const at0 = v_scales + key_0 * C::kScaleBytes + r * 8 * C::kScaleBytes,
-                                *const at1 = v_scales + key_1 * C::kScaleBytes + r * 8 * C::kScaleBytes;
-            unsigned s0, s1;
-            if constexpr (D == 256) {
-              s0 = load_u16(at0 + 2 * g), s1 = load_u16(at1 + 2 * g);
-            } else {
-              constexpr int kLanes = 128 / D;  // lanes to a block
-              s0 = at0[g / kLanes], s1 = at1[g / kLanes];
-            }
+            unsigned s0 = vs[t][r][0], s1 = vs[t][r][1];
             if (!whole) {
               s0 = key_0 + 8 * r < see_of(t) ? s0 : 0u;
               s1 = key_1 + 8 * r < see_of(t) ? s1 : 0u;
