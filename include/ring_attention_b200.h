@@ -260,7 +260,8 @@ RA_API int ra_prefill_host(int dtype, const void* q_host, const void* k_host, co
  * -inf; rows of no sequence stay as they are. heads is a multiple of kv heads. Sums and the softmax are held in 32 bits, the weights of the sum over V are rounded
  * to dtype as in ra_attention_step_fp16, and the result once. What is not finite in a sequence's K or V does not reach other
  * sequences; in its own, a value with weight 0 may reach queries of the same 128 keys. A bounded wait that runs out is reported as of the step kernels, and
- * rows that are not finished then stay as they are. out must not share memory with q, k or v. */
+ * rows that are not finished then stay as they are. Scores are held in 32 bits as they come: beyond some 2^26 nothing is promised. out
+ * must not share memory with q, k or v. */
 RA_API int ra_packed_attention(int dtype, const struct ra_rows* q, const struct ra_rows* k, const struct ra_rows* v,
                                const struct ra_rows* out, float* lse, const ra_shape* shape, const int* ends, const int* k_ends,
                                int causal, ra_stream stream);

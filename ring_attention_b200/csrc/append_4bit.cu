@@ -8,8 +8,8 @@ namespace rab {
 namespace {
 
 // Rows that are neither normed nor turned, and no queries: a thread makes the codes of one block of 16 elements of kAhead heads at a time.
-// us a call, four prompts' chunks of 2060 to 4099 tokens, 8 KV heads of 128 in fp16: PLAIN_US, in the other kernel, whose threads have registers
-// for angles and weights, OTHER_US.
+// us on the device, chunks of 2500 to 4099 tokens of four prompts, 8 KV heads of 128 in fp16 (69 MB, 10.5 at the copy's rate): 20, and in the
+// other kernel, whose threads hold angles and weights and of which two blocks fit an SM, 33.
 constexpr int kPlainThreads = 256, kPlainAhead = 4;
 template <typename T, int D>
 __global__ void __launch_bounds__(kPlainThreads) plain_4bit_kernel(const __grid_constant__ Args a, unsigned total, int per) {

@@ -13,8 +13,17 @@
 // tensor memory, barriers and rings are set up once, and the next item's queries, keys and first scores come while the rows of the last
 // one are written.
 //
-// Roles (384 threads; head_dim 256: 256): warp 0 copies with TMA, warps 1 and 2 issue tcgen05.mma (2: only where P has a place of its own,
-// head_dim 64), warp 3 finds the items, warps 4 to 7 and 8 to 11 are the softmax of either tile, a row a thread.
+// Measured (graph; floor at 1643 TFLOP/s): 16 prompts of up to 4099 rows H32/kvH8 D128 bf16 897 us, 980 TFLOP/s (535 us), chunks of up to 1531 rows behind
+// up to 16384 of four prompts 693, 1144 (483), two documents of up to 32768 rows H8 D64 fp16 2062, 788 (988: there the exp unit is the bound);
+// 13 prompts of up to 200 rows H24/kvH6 D64 14.5: two items one after the other on some SMs, each a chain of copy, scores, softmax, product
+// and way out of some 6 us. The items dealt in advance, to and fro over the blocks, instead of taken over as they go: B1 H8 S32768 D64
+// 1574 -> 1412 us, D128 2102 -> 1972.
+//
+// Roles (384 threads; head_dim 256 and one tile a block: 256): warp 0 copies with TMA, warps 1 and 2 issue tcgen05.mma (2: only where P has a place of its own,
+// head_dim 64), warp 3 finds the items, warps 4 to 7 and 8 to 11 are the softmax of either tile, a row a thread. (One
+// warp of each pair that shares a scheduler in its exponentials while the other waits, by barriers, was slower: head_dim 64 247 -> 302 us for
+// 2 x 18944 rows. How registers are shared out matters less for spills than for the order of instructions that follows: 72 / 216, 88 / 208
+// and 104 / 200 at head_dim 64 247, 253, 230 us, at 128 281, 279, 283.)
 //
 // Key tiles are counted from the sequence's first key. Of a query tile's last one only as many products are made as its rows see keys, in
 // steps of 16, and only the halves of its scores that a warp's rows see are worked on; what a last step has of the next sequence is put

@@ -95,6 +95,24 @@ def test_long_sequences(dtype, H, kvH, D, causal):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,kvH,D", [(40, 1, 64), (64, 2, 128), (34, 2, 32), (20, 1, 256)])
+def test_more_heads_than_a_tile_takes(dtype, H, kvH, D):
+    check(dtype, problem(41, dtype, H, kvH, D, [150, 3, 40]))
+    check(dtype, problem(44, dtype, H, kvH, D, [1, 2, 1, 1], [1, 40, 300, 129]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,kvH,D", [(4, 1, 64), (2, 2, 128), (2, 1, 256), (4, 2, 32)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_a_long_sequence_among_short_ones(dtype, H, kvH, D, causal):
+    """By the average a call of short sequences; one is long, and some have long keys."""
+    lens = [1] * 200 + [2500] + [2] * 100
+    check(dtype, problem(47, dtype, H, kvH, D, lens), causal)
+    k_lens = [1] * 200 + [2600] + [2 + 300 * (i % 50 == 0) for i in range(100)]
+    check(dtype, problem(50, dtype, H, kvH, D, lens, k_lens), causal)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("D", [32, 64, 128, 256])
 def test_rows_with_strides(dtype, D):
     """Slices of a fused projection, heads before rows, results inside wider ones, a tensor of one row."""
