@@ -892,10 +892,13 @@ int launch_packed(const ra_rows& q, const ra_rows& k, const ra_rows& v, PackedAr
   while ((1 << a.tile_shift) < a.tile_tokens) ++a.tile_shift;
   a.head_sets = (a.G + a.pack - 1) / a.pack;
   if constexpr (D <= 128) {
-    // Sequences of one query tile on average, at head_dim 64 and below of two, are taken a tile a block. us a call of 16384 rows, two tiles a
+    // Sequences of one query tile on average, at head_dim 64 and below of two if their keys are few, are taken a tile a block. us a call of 16384 rows, two tiles a
     // block / one: H32/kvH8 D128, sequences of 16 rows (half a tile) 301 / 211, 32 rows 151 / 117, 64 rows 93 / 93, 128 rows 87 / 103; H24/kvH6 D64,
-    // 32 rows (a tile) 125 / 79, 64 rows 66 / 59, 128 rows 63 / 66; H16 D64, 128 rows (a tile) 88 / 50, 256 rows 69 / 60, 512 rows 76 / 74.
-    if (tokens <= (D == 64 ? 2 : 1) * a.tile_tokens) return launch_tiles<D, DR, T, true>(q, k, v, a, stream);
+    // 32 rows (a tile) 125 / 79, 64 rows 66 / 59, 128 rows 63 / 66; H16 D64, 128 rows (a tile) 88 / 50, 256 rows 69 / 60, 512 rows 76 / 74. 64 chunks on 8192 keys: H32/kvH8 D128, 32 rows 437 / 389; H24/kvH6 D64, 64 rows
+    // (two tiles) 327 / 426.
+    constexpr int kFewKeys = 512;
+    const bool two = D == 64 && a.k_rows <= static_cast<long long>(kFewKeys) * a.B;
+    if (tokens <= (two ? 2 : 1) * a.tile_tokens) return launch_tiles<D, DR, T, true>(q, k, v, a, stream);
   }
   return launch_tiles<D, DR, T, false>(q, k, v, a, stream);
 }
