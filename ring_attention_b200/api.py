@@ -589,8 +589,9 @@ def qk_norm_rope_backward(q, k, dq_out, dk_out, dq, dk, *, dq_weight=None, dk_we
         workspace.nbytes if need else 0, _raw_stream(dev)))
 
 
-def _paged_kv(k_pages, v_pages, page_table, lens):
-    """(ra_paged_kv, kv heads, page size, head_dim, batch) of the tensors (see ``paged_append``)."""
+def _paged_kv(k_pages, v_pages, page_table, lens, lens_at=None):
+    """(ra_paged_kv, kv heads, page size, head_dim, batch) of the tensors (see ``paged_append``); lens_at: the address of what stands in
+    the place of lens."""
     shape, (B, most) = k_pages.shape, page_table.shape
     if len(shape) != 4 or shape != v_pages.shape or k_pages.dtype != v_pages.dtype or \
             not (k_pages.is_contiguous() and v_pages.is_contiguous()):
@@ -598,7 +599,7 @@ def _paged_kv(k_pages, v_pages, page_table, lens):
     n, kvH, page, D = shape
     return PACK_PAGED_KV(_dtype(k_pages), n, kvH, page, D, k_pages.data_ptr(), v_pages.data_ptr(), B, most,
                          page_table.stride(0), _int32(page_table, (B, most), "page_table"),
-                         _int32(lens, (B,), "lens")), kvH, page, D, B
+                         _int32(lens, (B,), "lens") if lens_at is None else lens_at), kvH, page, D, B
 
 
 def _append(name, dt, c_heads, c_dim, c_batch, k, v, counts, rope, positions, k_weight, q, q_out, q_weight, eps):
@@ -703,7 +704,7 @@ def paged_read(k_pages, v_pages, page_table, ends, k_out, v_out, *, start=None):
     dev = _on_device(k_pages, v_pages, page_table, ends, start, k_out, v_out)
     B = page_table.shape[0]
     at = _int32(ends, (B + 1,), "ends")
-    cache, kvH, _, D, _ = _paged_kv(k_pages, v_pages, page_table, ends[:B])
+    cache, kvH, _, D, _ = _paged_kv(k_pages, v_pages, page_table, None, at)
     shape = (k_out.shape[0], kvH, D)
     check(packed("ra_paged_read")(cache, at, _int32(start, (B,), "start") if start is not None else None,
                                   _packed_rows(k_out, shape, k_pages.dtype, True), _packed_rows(v_out, shape, k_pages.dtype, True),
@@ -718,24 +719,27 @@ def pages_4bit(num_pages, kv_heads, page_size, head_dim, device="cuda"):
     return torch.zeros((num_pages, kv_heads, page_size * head_dim * 9 // 16), dtype=torch.uint8, device=device)
 
 
-def _paged_4bit(k_pages, v_pages, page_table, lens, head_dim, dtype):
-    """(ra_paged_kv, kv heads, batch) of a cache in 4 bits whose rows have head_dim elements and come and go in dtype."""
+_UINT8 = torch.uint8
+_FOUR_DT = {torch.float16: RA_F16, torch.bfloat16: RA_BF16}
+
+
+def _paged_4bit(k_pages, v_pages, page_table, lens, head_dim, dtype, lens_at=None):
+    """(ra_paged_kv, kv heads, batch) of a cache in 4 bits whose rows have head_dim elements and come and go in dtype; lens_at as for
+    ``_paged_kv``."""
     shape, (B, most) = k_pages.shape, page_table.shape
-    if len(shape) != 3 or shape != v_pages.shape or k_pages.dtype != torch.uint8 or v_pages.dtype != torch.uint8 or \
+    if len(shape) != 3 or shape != v_pages.shape or k_pages.dtype is not _UINT8 or v_pages.dtype is not _UINT8 or \
             not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         raise ValueError("k_pages and v_pages: expected contiguous uint8 (num_pages, kv_heads, page_size * head_dim * 9 / 16) tensors alike")
     n, kvH, size = shape
     page, rest = divmod(16 * size, 9 * head_dim) if head_dim > 0 else (0, 1)
     if rest:
         raise ValueError("the pages do not hold whole rows of the head_dim")
-    return PACK_PAGED_KV(_dtype_of_4bit(dtype), n, kvH, page, head_dim, k_pages.data_ptr(), v_pages.data_ptr(), B, most,
-                         page_table.stride(0), _int32(page_table, (B, most), "page_table"), _int32(lens, (B,), "lens")), kvH, B
-
-
-def _dtype_of_4bit(dtype):
-    if dtype is not torch.float16 and dtype is not torch.bfloat16:
+    code = _FOUR_DT.get(dtype)
+    if code is None:
         raise ValueError(f"a cache in 4 bits takes rows in fp16 or bf16, got {dtype}")
-    return _DT[dtype]
+    return PACK_PAGED_KV(code, n, kvH, page, head_dim, k_pages.data_ptr(), v_pages.data_ptr(), B, most,
+                         page_table.stride(0), _int32(page_table, (B, most), "page_table"),
+                         _int32(lens, (B,), "lens") if lens_at is None else lens_at), kvH, B
 
 
 def paged_append_4bit(k, v, k_pages, v_pages, page_table, lens, *, k_scale=1.0, v_scale=1.0, counts=None, rope=None, positions=None,
@@ -758,7 +762,7 @@ def paged_read_4bit(k_pages, v_pages, page_table, ends, k_out, v_out, *, start=N
     B = page_table.shape[0]
     at = _int32(ends, (B + 1,), "ends")
     rows, kvH, D = k_out.shape
-    cache, c_heads, _ = _paged_4bit(k_pages, v_pages, page_table, ends[:B], D, k_out.dtype)
+    cache, c_heads, _ = _paged_4bit(k_pages, v_pages, page_table, None, D, k_out.dtype, at)
     shape = (rows, c_heads, D)
     check(packed("ra_paged_read_4bit")(cache, k_scale, v_scale, at, _int32(start, (B,), "start") if start is not None else None,
                                        _packed_rows(k_out, shape, k_out.dtype, True), _packed_rows(v_out, shape, k_out.dtype, True),
