@@ -749,7 +749,7 @@ def paged_append_4bit(k, v, k_pages, v_pages, page_table, lens, *, k_scale=1.0, 
     Scales are in units of k_scale and v_scale, powers of two that every call on the cache is given alike: 1 serves rows whose largest
     elements are between about 0.1 and 2688. What is held is the nearest to the row as ``paged_append`` would store it."""
     dev = _on_device(k, v, k_pages, v_pages, page_table, lens, counts, positions, k_weight, q, q_out, q_weight)
-    D = k.shape[3]
+    D = k.shape[-1]
     cache, kvH, B = _paged_4bit(k_pages, v_pages, page_table, lens, D, k.dtype)
     check(packed("ra_paged_append_4bit")(cache, k_scale, v_scale,
                                          *_append("paged_append_4bit", k.dtype, kvH, D, B, k, v, counts, rope, positions, k_weight, q,

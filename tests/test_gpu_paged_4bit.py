@@ -563,3 +563,13 @@ def test_wrapper_refusals():
                 lambda: api.paged_read(k, v, t, i32([0, 40]), to, to)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_append_wants_four_dimensions():
+    rows, pages = torch.zeros(4, 16, 64, dtype=torch.bfloat16, device="cuda"), api.pages_4bit(2, 4, 16, 64)
+    with pytest.raises(ValueError):
+        api.paged_append_4bit(rows, rows, pages, pages, i32([[0]]), i32([0]))
+    with pytest.raises(ValueError):
+        api.paged_read_4bit(pages, pages, i32([[0]]), i32([0, 4]), rows[0], rows[0])
+    with pytest.raises(ValueError):
+        api.paged_decode_4bit(rows[:, :, 0], pages, pages, i32([[0]]), i32([4]), rows[:, :, 0])
