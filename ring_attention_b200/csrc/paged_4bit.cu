@@ -403,7 +403,8 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
 #pragma unroll
             for (int i = 0; i < 4; ++i) top[i & 1] = fmaxf(top[i & 1], sc[t][nb][i]);
           }
-          more = more || top[0] > m_run[nb][0] + kSlack || top[1] > m_run[nb][1] + kSlack;
+          // (the difference is exact where the sum may round to a score a step of 2^4 above the reference: a weight of 2^16)
+          more = more || top[0] - m_run[nb][0] > kSlack || top[1] - m_run[nb][1] > kSlack;
         }
         if (__any_sync(0xffffffffu, more)) {  // rare after a unit's first keys
 #pragma unroll

@@ -573,3 +573,30 @@ def test_append_wants_four_dimensions():
         api.paged_read_4bit(pages, pages, i32([[0]]), i32([0, 4]), rows[0], rows[0])
     with pytest.raises(ValueError):
         api.paged_decode_4bit(rows[:, :, 0], pages, pages, i32([[0]]), i32([4]), rows[:, :, 0])
+
+
+def test_scores_one_step_above_the_reference():
+    """Scores (in log2) of 2^27 to 2^28, where steps are 16: a key whose score is one step above the reference has all the weight, as a
+    weight of 2^16 is beyond fp16. Keys 0 and 16 of a warp's share, read one after the other; every other key's score is 0."""
+    D, page = 256, 32
+    scale = np.float32(1.4426950408889634) / np.float32(16.0) * np.float32(2.0 ** 20)
+    found = []
+    for s0 in range(112, 127):
+        for t, code in ((1.0, 2), (2.0, 4), (4.0, 6)):
+            a, b = 6 * ref.E4M3[s0], 6 * ref.E4M3[s0] + t * 2.0 ** -13
+            if np.float32(b) != b:
+                continue
+            m, s = np.float32(a) * scale, np.float32(b) * scale
+            if 2.0 ** 27 <= m and s < 2.0 ** 28 and s - m == 16 and np.float32(m + np.float32(8.0)) == s:
+                found.append((s0, code))
+    assert found
+    for dtype in DTYPES:
+        for s0, code in found:
+            q = np.zeros((1, 16, D))
+            q[..., 0], q[..., 128] = 1.0, 2.0 ** -13
+            codes, scales = np.zeros((2, 1, 1, page, D), np.uint8), np.full((2, 1, 1, page, D // 16), 56, np.uint8)  # (56: 1.0)
+            scales[0, 0, 0, :, 0] = s0
+            codes[0, 0, 0, [0, 16], 0], codes[0, 0, 0, 16, 128], codes[1, 0, 0, 16] = 7, code, 2
+            raw = [ref.join_pages(c, s) for c, s in zip(codes, scales)]
+            out, lse = run(dtype, q, raw, np.array([[0]]), [32], (2.0 ** 20, 1.0))
+            assert (out == 1).all() and torch.isfinite(lse).all()
