@@ -460,7 +460,7 @@ RA_API int ra_paged_read_4bit(const ra_paged_kv* cache, float k_scale, float v_s
 
 /* ra_paged_decode over such a cache, without shared pages. q and out are of cache->dtype. The cached values enter both products
  * exactly; the queries do but for elements less than 2^-14 of their row's largest, which lose less than 2^-25 of that; the weights of the sum
- * over V are rounded to fp16, and the result once. A wait that ran out is treated as there.
+ * over V are rounded to 11 bits, those below 2^-21 of the largest to multiples of 2^-31 of it, and the result once. A wait that ran out is treated as there.
  * `workspace`: ra_paged_decode_4bit_workspace_bytes(...) bytes, 16-byte aligned, of this call's launches alone. */
 RA_API size_t ra_paged_decode_4bit_workspace_bytes(const ra_paged_kv* cache, int heads);
 RA_API int ra_paged_decode_4bit(const ra_paged_kv* cache, float k_scale, float v_scale, const void* q, int heads, void* out, float* lse,

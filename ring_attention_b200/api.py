@@ -771,7 +771,8 @@ def paged_read_4bit(k_pages, v_pages, page_table, ends, k_out, v_out, *, start=N
 
 def paged_decode_4bit(q, k_pages, v_pages, page_table, lens, out, *, k_scale=1.0, v_scale=1.0, lse=None, workspace=None):
     """``paged_decode`` over a cache in 4 bits (see ``paged_append_4bit``), without shared pages: q and out are (batch, heads,
-    head_dim) in fp16 or bf16. The values that the cache holds enter exactly; the weights of the sum over V are rounded to fp16."""
+    head_dim) in fp16 or bf16. The values that the cache holds enter exactly; the weights of the sum over V are rounded to 11 bits, those
+    below 2^-21 of the largest to multiples of 2^-31 of it."""
     dev = _on_device(q, k_pages, v_pages, page_table, lens, out, lse, workspace)
     shape = q.shape
     if len(shape) != 3 or shape[0] != page_table.shape[0]:

@@ -60,9 +60,11 @@ struct FourBlock {
   static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two blocks to an SM");
 };
 
-// The reference of the weights is moved only when a score runs this far above it (in log2): weights of up to 2^8 are as exact in fp16
-// as those below 1, and with sixteen heads some maximum moves in nearly every one of a share's first tiles, at 200 instructions each time.
-constexpr float kSlack = 8.f;
+// The reference of the weights is moved only when a score runs kSlack above it (in log2): with sixteen heads some maximum moves in nearly
+// every one of a share's first tiles, at 200 instructions each time. The reference's own weight is 2^kLift, because what is 2^-25 and less
+// is 0 in fp16 while it counts in the weights' sum: so those below 2^-32 of the reference's do, not those below 2^-25 (of 300000 keys
+// that may be 1 %). Together 2^14 at most, and 2^15 where the reference less kLift is rounded: fp16 goes up to 2^16.
+constexpr float kSlack = 7.f, kLift = 7.f;
 
 // A warp's ring: while a place is worked on, the others' copies are on their way.
 template <typename C>
@@ -252,7 +254,7 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
     unsigned qb[NB][kSteps][2];
     float o[NB][kTiles][4];
     float m_run[NB][2], l_run[NB][2], factor[NB][2];  // of heads 2 j and 2 j + 1 of the eight
-    float m_off[NB][2];                               // m_run, or 0 where nothing has been seen
+    float m_off[NB][2];                               // m_run - kLift, or 0 where nothing has been seen
     int left = ring.total;
     StageInfo u = {};
     for (int s = 0; left > 0; ++s) {
@@ -418,10 +420,11 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
 #pragma unroll
               for (int d = 4; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
               const float mn = fmaxf(m_run[nb][c], mx);
-              f[c] = m_run[nb][c] == -INFINITY ? 0.f : ex2(m_run[nb][c] - mn);
+              const float off = mn == -INFINITY ? 0.f : mn - kLift;
+              f[c] = m_run[nb][c] == -INFINITY ? 0.f : ex2(m_off[nb][c] - off);
               l_run[nb][c] = m_run[nb][c] == -INFINITY ? l_run[nb][c] : l_run[nb][c] * f[c];  // (0, or NaN to keep)
               m_run[nb][c] = mn;
-              m_off[nb][c] = mn == -INFINITY ? 0.f : mn;
+              m_off[nb][c] = off;
             }
 #pragma unroll
             for (int i = 0; i < kTiles; ++i) {
@@ -432,7 +435,7 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
             }
           }
         }
-        // P^T as the B fragments of the second product, rounded to fp16 (l is not): 2^-12 of a weight
+        // P^T as the B fragments of the second product, rounded to fp16 (l is not): off by 2^-11 of a weight, or by 2^-32 of the reference's
         unsigned pb[kT][NB][2];
 #pragma unroll
         for (int t = 0; t < kT; ++t)
@@ -520,9 +523,9 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
               }
             }
             if (g == 0) {
-              if (!result) a.part_ml[part + r] = make_float2(m_run[nb][c], l);
+              if (!result) a.part_ml[part + r] = make_float2(m_run[nb][c] == -INFINITY ? -INFINITY : m_off[nb][c], l);
               else if (a.lse)
-                a.lse[static_cast<size_t>(b) * a.H + h] = l > 0.f ? m_run[nb][c] * kLn2 + logf(l) : l == 0.f ? -INFINITY : l;
+                a.lse[static_cast<size_t>(b) * a.H + h] = l > 0.f ? m_off[nb][c] * kLn2 + logf(l) : l == 0.f ? -INFINITY : l;
             }
           }
       }

@@ -600,3 +600,24 @@ def test_scores_one_step_above_the_reference():
             raw = [ref.join_pages(c, s) for c, s in zip(codes, scales)]
             out, lse = run(dtype, q, raw, np.array([[0]]), [32], (2.0 ** 20, 1.0))
             assert (out == 1).all() and torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("H", [2, 16])
+def test_small_weights_count(dtype, D, H):
+    """One key takes nearly all of the weight and has a V of zeros, 31 others some 2^-25.6 of its weight each: the result is theirs.
+    A weight is off by half of fp16's smallest step where the reference's is 2^7, so by 2^-32 of the reference's."""
+    rng, page, f = np.random.default_rng(22), 16, 2.0 ** 10
+    q, table, lens = np.ones((1, H, D)), np.array([[1, 0]]), [32]
+    k, v = 0.03 * rng.standard_normal((2, 1, page, D)), np.abs(rng.standard_normal((2, 1, page, D))) + 0.5
+    k[1, 0, 0], v[1, 0, 0] = 25.6 * np.log(2) / np.sqrt(D), 0.0
+    raw = [ref.join_pages(*ref.encode(x * g, g)) for x, g in ((k, 1.0), (v, f))]
+    values = [ref.values(p, page, D, g) for p, g in zip(raw, (1.0, f))]
+    out, err, lse, lse_err = want(q, *values, table, lens, torch.float32)
+    assert (out > 0).all()
+    err = err + 2.0 ** -11 * out + 2.0 ** -32 * values[1][:, 0].sum((0, 1))
+    assert (err < 0.05 * out).all()
+    got = run(dtype, q, raw, table, lens, (1.0, f))
+    check(got[0], out, err, dtype, "out")
+    assert (np.abs(got[1].double().cpu().numpy() - lse) <= lse_err).all()
