@@ -300,7 +300,8 @@ __global__ void __launch_bounds__(FourBlock<D, NB>::kThreads, 2) paged_4bit_kern
             qb[nb][st][0] = pack_pair<__half>(x.x * down, x.y * down);
             qb[nb][st][1] = pack_pair<__half>(y.x * down, y.y * down);
           }
-          const float f = up * args.k_factor * a.scale_log2;
+          // (kept finite, so that scores of 0 stay 0 where queries and K's factor are beyond 32 bits together)
+          const float f = fminf(up * (args.k_factor * a.scale_log2), 3.402823466e+38f);
           factor[nb][0] = __shfl_sync(0xffffffffu, f, 8 * j);
           factor[nb][1] = __shfl_sync(0xffffffffu, f, 8 * j + 4);
 #pragma unroll

@@ -621,3 +621,18 @@ def test_small_weights_count(dtype, D, H):
     got = run(dtype, q, raw, table, lens, (1.0, f))
     check(got[0], out, err, dtype, "out")
     assert (np.abs(got[1].double().cpu().numpy() - lse) <= lse_err).all()
+
+
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+def test_the_largest_queries_on_keys_of_zeros(D):
+    """Queries and a factor whose product is beyond 32 bits: keys of zeros have scores of 0 all the same, and the key with the largest
+    score all the weight."""
+    q = np.full((1, 4, D), 2.0 ** 110)
+    codes, scales = np.zeros((2, 1, 2, 16, D), np.uint8), np.full((2, 1, 2, 16, D // 16), 56, np.uint8)  # (56: 1.0)
+    codes[1] = 2
+    raw = [ref.join_pages(c, s) for c, s in zip(codes, scales)]
+    out, lse = run(torch.bfloat16, q, raw, np.array([[0]]), [9], (2.0 ** 30, 1.0))
+    assert (out == 1).all() and ((lse - np.log(9)).abs() <= 2.0 ** -21).all()
+    codes[0, :, :, 5, 0], scales[0, :, :, 5, 0], codes[1, :, :, 5] = 1, 1, 3  # a score of 2^-10, 2^30 and 2^110 over sqrt(D)
+    out, lse = run(torch.bfloat16, q, [ref.join_pages(c, s) for c, s in zip(codes, scales)], np.array([[0]]), [9], (2.0 ** 30, 1.0))
+    assert (out == 1.5).all()
