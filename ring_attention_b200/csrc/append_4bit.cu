@@ -16,7 +16,7 @@ __global__ void __launch_bounds__(kPlainThreads) plain_4bit_kernel(const __grid_
   constexpr int L = D / 16;
   let_next_start();
   wait_for_previous();
-  const unsigned token = (blockIdx.x * kPlainThreads + threadIdx.x) / L;
+  const unsigned token = blockIdx.x * (kPlainThreads / L) + threadIdx.x / L;  // (threads may be more than 2^32)
   const int block = threadIdx.x % L;
   if (token >= total) return;
   const int b = static_cast<int>(token / a.S), t = static_cast<int>(token - static_cast<unsigned>(b) * a.S);
@@ -65,7 +65,7 @@ int launch_plain_4bit(int head_dim, const Args& a, unsigned tokens, cudaStream_t
     const unsigned blocks = (tokens + kTokens - 1) / kTokens;
     // as many heads a thread as loads are on their way, or, where that leaves SMs without a block, one
     const int heads = 2 * a.heads[1];
-    const int per = blocks * ((heads + kPlainAhead - 1) / kPlainAhead) >= 2u * sm_count() ? kPlainAhead : 1;
+    const int per = static_cast<long long>(blocks) * ((heads + kPlainAhead - 1) / kPlainAhead) >= 2ll * sm_count() ? kPlainAhead : 1;
     RAB_REQUIRE((heads + per - 1) / per <= 65535, RA_ERR_INVALID, "paged_append_4bit: bad heads");
     RAB_CUDA(launch_overlapped(plain_4bit_kernel<T, d()>, dim3(blocks, static_cast<unsigned>((heads + per - 1) / per)),
                                dim3(kPlainThreads), 0, stream, a, tokens, per));

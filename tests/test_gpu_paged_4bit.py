@@ -636,3 +636,17 @@ def test_the_largest_queries_on_keys_of_zeros(D):
     codes[0, :, :, 5, 0], scales[0, :, :, 5, 0], codes[1, :, :, 5] = 1, 1, 3  # a score of 2^-10, 2^30 and 2^110 over sqrt(D)
     out, lse = run(torch.bfloat16, q, [ref.join_pages(c, s) for c, s in zip(codes, scales)], np.array([[0]]), [9], (2.0 ** 30, 1.0))
     assert (out == 1.5).all()
+
+
+@pytest.mark.parametrize("D,tokens", [(256, (1 << 28) + 5), (128, (1 << 29) + 5)])
+def test_more_threads_than_32_bits_count(D, tokens):
+    """As many tokens as wrap a count of their threads; all but the last five lie before the sequence's first row."""
+    dtype, page = torch.bfloat16, 16
+    row = gpu(np.random.default_rng(23).standard_normal((1, 1, 1, D)), dtype)
+    pages = [api.pages_4bit(1, 1, page, D) for _ in range(2)]
+    x = row.expand(1, 1, tokens, D)
+    api.paged_append_4bit(x, x, *pages, i32([[0]]), i32([5 - tokens]))
+    held = ref.decode(*ref.encode(row.double().cpu().numpy()[0, 0, 0], 1.0), 1.0)
+    for p in pages:
+        got = ref.values(p.cpu().numpy(), page, D, 1.0)[0, 0]
+        assert (got[:5] == held).all() and (got[5:] == 0).all()
