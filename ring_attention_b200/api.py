@@ -715,17 +715,20 @@ def paged_read(k_pages, v_pages, page_table, ends, k_out, v_out, *, start=None):
 
 
 def pages_4bit(num_pages, kv_heads, page_size, head_dim, device="cuda"):
-    """Empty pages of K or V for ``paged_append_4bit``: (num_pages, kv_heads, page_size * head_dim * 9 / 16) bytes."""
-    return torch.zeros((num_pages, kv_heads, page_size * head_dim * 9 // 16), dtype=torch.uint8, device=device)
+    """Empty pages of K or V for ``paged_append_4bit``: (num_pages, kv_heads, page_size * head_dim * 9 / 16) bytes. The tensor keeps the
+    page_size for the calls that get it; they are told it by keyword where they get a view of it, or pages made elsewhere."""
+    pages = torch.zeros((num_pages, kv_heads, page_size * head_dim * 9 // 16), dtype=torch.uint8, device=device)
+    pages.page_size_4bit = page_size
+    return pages
 
 
 _UINT8 = torch.uint8
 _FOUR_DT = {torch.float16: RA_F16, torch.bfloat16: RA_BF16}
 
 
-def _paged_4bit(k_pages, v_pages, page_table, lens, head_dim, dtype, lens_at=None):
+def _paged_4bit(k_pages, v_pages, page_table, lens, head_dim, dtype, lens_at=None, page_size=None):
     """(ra_paged_kv, kv heads, batch) of a cache in 4 bits whose rows have head_dim elements and come and go in dtype; lens_at as for
-    ``_paged_kv``."""
+    ``_paged_kv``. The bytes of a page are as many rows of some other head_dim, too: page_size, where it is known, has to be theirs."""
     shape, (B, most) = k_pages.shape, page_table.shape
     if len(shape) != 3 or shape != v_pages.shape or k_pages.dtype is not _UINT8 or v_pages.dtype is not _UINT8 or \
             not (k_pages.is_contiguous() and v_pages.is_contiguous()):
@@ -734,6 +737,9 @@ def _paged_4bit(k_pages, v_pages, page_table, lens, head_dim, dtype, lens_at=Non
     page, rest = divmod(16 * size, 9 * head_dim) if head_dim > 0 else (0, 1)
     if rest:
         raise ValueError("the pages do not hold whole rows of the head_dim")
+    if page_size is not None and page_size != page or getattr(k_pages, "page_size_4bit", page) != page or \
+            getattr(v_pages, "page_size_4bit", page) != page:
+        raise ValueError(f"pages with {page} rows of head_dim {head_dim} to a head: not the page_size that they have")
     code = _FOUR_DT.get(dtype)
     if code is None:
         raise ValueError(f"a cache in 4 bits takes rows in fp16 or bf16, got {dtype}")
@@ -743,33 +749,35 @@ def _paged_4bit(k_pages, v_pages, page_table, lens, head_dim, dtype, lens_at=Non
 
 
 def paged_append_4bit(k, v, k_pages, v_pages, page_table, lens, *, k_scale=1.0, v_scale=1.0, counts=None, rope=None, positions=None,
-                      k_weight=None, q=None, q_out=None, q_weight=None, eps=1e-6):
+                      k_weight=None, q=None, q_out=None, q_weight=None, eps=1e-6, page_size=None):
     """``paged_append`` to a cache in 4 bits: k_pages and v_pages are those of ``pages_4bit``, k and v fp16 or bf16. 16 elements of a row
     share a scale in e4m3 (their largest magnitude / 6), an element is held as one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (with a sign) times it.
     Scales are in units of k_scale and v_scale, powers of two that every call on the cache is given alike: 1 serves rows whose largest
-    elements are between about 0.1 and 2688. What is held is the nearest to the row as ``paged_append`` would store it."""
+    elements are between about 0.1 and 2688. What is held is the nearest to the row as ``paged_append`` would store it. Of pages that
+    ``pages_4bit`` did not return as they are (a view, bytes from elsewhere) ``page_size`` says how many rows they have, and rows of
+    another head_dim are refused; without it that is what their bytes make of the rows' head_dim."""
     dev = _on_device(k, v, k_pages, v_pages, page_table, lens, counts, positions, k_weight, q, q_out, q_weight)
     D = k.shape[-1]
-    cache, kvH, B = _paged_4bit(k_pages, v_pages, page_table, lens, D, k.dtype)
+    cache, kvH, B = _paged_4bit(k_pages, v_pages, page_table, lens, D, k.dtype, None, page_size)
     check(packed("ra_paged_append_4bit")(cache, k_scale, v_scale,
                                          *_append("paged_append_4bit", k.dtype, kvH, D, B, k, v, counts, rope, positions, k_weight, q,
                                                   q_out, q_weight, eps), _raw_stream(dev)))
 
 
-def paged_read_4bit(k_pages, v_pages, page_table, ends, k_out, v_out, *, start=None, k_scale=1.0, v_scale=1.0):
+def paged_read_4bit(k_pages, v_pages, page_table, ends, k_out, v_out, *, start=None, k_scale=1.0, v_scale=1.0, page_size=None):
     """``paged_read`` out of a cache in 4 bits (see ``paged_append_4bit``): the values that the cache holds, in fp16 or bf16."""
     dev = _on_device(k_pages, v_pages, page_table, ends, start, k_out, v_out)
     B = page_table.shape[0]
     at = _int32(ends, (B + 1,), "ends")
     rows, kvH, D = k_out.shape
-    cache, c_heads, _ = _paged_4bit(k_pages, v_pages, page_table, None, D, k_out.dtype, at)
+    cache, c_heads, _ = _paged_4bit(k_pages, v_pages, page_table, None, D, k_out.dtype, at, page_size)
     shape = (rows, c_heads, D)
     check(packed("ra_paged_read_4bit")(cache, k_scale, v_scale, at, _int32(start, (B,), "start") if start is not None else None,
                                        _packed_rows(k_out, shape, k_out.dtype, True), _packed_rows(v_out, shape, k_out.dtype, True),
                                        rows, _raw_stream(dev)))
 
 
-def paged_decode_4bit(q, k_pages, v_pages, page_table, lens, out, *, k_scale=1.0, v_scale=1.0, lse=None, workspace=None):
+def paged_decode_4bit(q, k_pages, v_pages, page_table, lens, out, *, k_scale=1.0, v_scale=1.0, lse=None, workspace=None, page_size=None):
     """``paged_decode`` over a cache in 4 bits (see ``paged_append_4bit``), without shared pages: q and out are (batch, heads,
     head_dim) in fp16 or bf16. The values that the cache holds enter exactly; the weights of the sum over V are rounded to 11 bits, those
     below 2^-21 of the largest to multiples of 2^-31 of it."""
@@ -778,7 +786,7 @@ def paged_decode_4bit(q, k_pages, v_pages, page_table, lens, out, *, k_scale=1.0
     if len(shape) != 3 or shape[0] != page_table.shape[0]:
         raise ValueError("paged_decode_4bit: q does not fit the cache")
     B, H, D = shape
-    cache, _, _ = _paged_4bit(k_pages, v_pages, page_table, lens, D, q.dtype)
+    cache, _, _ = _paged_4bit(k_pages, v_pages, page_table, lens, D, q.dtype, None, page_size)
     if out.shape != shape or out.dtype != q.dtype or \
             lse is not None and (lse.shape != (B, H) or lse.dtype != torch.float32):
         raise ValueError("paged_decode_4bit: out is like q, lse (batch, heads) in fp32")

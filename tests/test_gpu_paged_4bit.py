@@ -650,3 +650,31 @@ def test_more_threads_than_32_bits_count(D, tokens):
     for p in pages:
         got = ref.values(p.cpu().numpy(), page, D, 1.0)[0, 0]
         assert (got[:5] == held).all() and (got[5:] == 0).all()
+
+
+def test_pages_of_another_head_dim_are_refused():
+    """Pages made for rows of 128 elements would hold twice as many of 64 to the byte: refused where pages_4bit made them, and of any
+    pages where the call says page_size."""
+    dtype, page = torch.bfloat16, 16
+    marked = [api.pages_4bit(2, 2, page, 128) for _ in range(2)]
+    plain = [p[:] for p in marked]  # (views do not say what they were made for)
+    table, lens, ends = i32([[0]]), i32([4]), i32([0, 4])
+    for D in (32, 64, 256):
+        rows, q, to = (torch.zeros(s, dtype=dtype, device="cuda") for s in ((1, 2, 3, D), (1, 4, D), (4, 2, D)))
+        for pages, kw in ((marked, {}), (plain, {"page_size": page}), (marked, {"page_size": page}), ([plain[0], marked[1]], {})):
+            for bad in (lambda: api.paged_append_4bit(rows, rows, *pages, table, lens, **kw),
+                        lambda: api.paged_decode_4bit(q, *pages, table, lens, torch.empty_like(q), **kw),
+                        lambda: api.paged_read_4bit(*pages, table, ends, to, to.clone(), **kw)):
+                with pytest.raises(ValueError, match="head_dim|page_size"):
+                    bad()
+    assert all((p == 0).all() for p in marked)
+    rows, q, to = (torch.ones(s, dtype=dtype, device="cuda") for s in ((1, 2, 4, 128), (1, 4, 128), (4, 2, 128)))
+    for pages, kw in ((marked, {}), (plain, {"page_size": page}), (plain, {}), (marked, {"page_size": page})):
+        api.paged_append_4bit(rows, rows, *pages, table, i32([0]), **kw)
+        outs = [torch.zeros_like(to) for _ in range(2)]
+        api.paged_read_4bit(*pages, table, ends, *outs, **kw)
+        out = torch.zeros_like(q)
+        api.paged_decode_4bit(q, *pages, table, lens, out, **kw)
+        assert all((x == 6 * 11 / 64).all() for x in (*outs, out))  # (of 1: 1 / 6 is nearest to 11 / 64, 64 / 11 to 6)
+        with pytest.raises(ValueError):
+            api.paged_read_4bit(*pages, table, ends, *outs, page_size=32)

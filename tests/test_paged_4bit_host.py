@@ -159,3 +159,15 @@ def test_wrapper_refusals():
         api._packed_rows(torch.zeros(4, 2, 64).expand(4, 2, 64)[:, :1].expand(4, 2, 64), (4, 2, 64), torch.float32, True)
     with pytest.raises(ValueError):
         api._packed_rows(torch.zeros(4, 64, 2).transpose(1, 2), (4, 2, 64), torch.float32)
+
+
+def test_pages_say_what_they_were_made_for():
+    pages = api.pages_4bit(3, 2, 16, 128, device="cpu")
+    table, lens = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    assert api._paged_4bit(pages, pages, table, lens, 128, torch.float16)[1:] == (2, 1)
+    for D in (32, 64, 256):
+        with pytest.raises(ValueError):
+            api._paged_4bit(pages, pages, table, lens, D, torch.float16)
+        with pytest.raises(ValueError):
+            api._paged_4bit(pages[:], pages[:], table, lens, D, torch.float16, page_size=16)
+    assert api._paged_4bit(pages[:], pages[:], table, lens, 128, torch.float16, page_size=16)[1:] == (2, 1)
