@@ -435,7 +435,8 @@ RA_API int ra_debug_paged_route(const ra_paged_kv* cache, int heads, int shared_
 /* Rows of sequences out of a paged cache, one sequence's behind the other's, as ra_packed_attention reads them: row i of k_out and
  * v_out ((rows, kv_heads, head_dim) of the cache's dtype; batch_stride is not used), for ends[b] <= i < ends[b + 1], gets row
  * start[b] + i - ends[b] of sequence b (`ends`: device, batch + 1, rising; `start`: device, batch; NULL: 0). A row that the cache does not hold
- * is zeros; rows before ends[0] and from ends[batch] on stay as they are. cache->lens is not read and may be NULL. */
+ * is zeros; rows before ends[0] and from ends[batch] on stay as they are. Rows of a result must not overlap. cache->lens is not read and
+ * may be NULL. */
 RA_API int ra_paged_read(const ra_paged_kv* cache, const int* ends, const int* start, const ra_rows* k_out, const ra_rows* v_out,
                          int rows, ra_stream stream);
 

@@ -77,6 +77,22 @@ inline cudaError_t launch_overlapped(void (*kern)(P...), dim3 grid, dim3 block, 
 }
 #endif
 
+// Whether no two of (rows, heads, head_dim) rows share memory (batch_stride is not used). Mostly one stride steps over all of the other's
+// rows; where neither does, the rows nearest to each head's first are looked at.
+inline bool rows_apart(const ra_rows& r, int head_dim, int heads, int rows) {
+  using Wide = __int128;
+  const Wide row = r.row_stride < 0 ? -static_cast<Wide>(r.row_stride) : static_cast<Wide>(r.row_stride);
+  const Wide head = r.head_stride < 0 ? -static_cast<Wide>(r.head_stride) : static_cast<Wide>(r.head_stride);
+  if ((rows > 1 && row < head_dim) || (heads > 1 && head < head_dim)) return false;
+  if (rows <= 1 || heads <= 1 || row >= head * (heads - 1) + head_dim || head >= row * (rows - 1) + head_dim) return true;
+  for (int h = 1; h < heads; ++h) {
+    const Wide at = head * h, n = at / row;
+    if (n >= rows) break;  // (this head and those behind it lie behind all rows of the first)
+    if (at - n * row < head_dim || (n + 1 < rows && (n + 1) * row - at < head_dim)) return false;
+  }
+  return true;
+}
+
 inline int kv_heads_of(const ra_shape& s) { return s.kv_heads > 0 ? s.kv_heads : s.heads; }
 
 // ---- device status word ----------------------------------------------------------

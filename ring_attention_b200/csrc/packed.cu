@@ -840,7 +840,7 @@ int heads_per_tile(int G, long long tokens) {
   return best;
 }
 
-// Rows that TMA can copy: 16-byte aligned, and rows or heads apart that do not overlap.
+// Rows that TMA can copy: 16-byte aligned, and strides of a row or more.
 bool rows_for_tma(const ra_rows& r, int head_dim, int heads, int rows) {
   unsigned long long all = reinterpret_cast<uintptr_t>(r.data);
   if (heads > 1) all |= static_cast<unsigned long long>(r.head_stride) * 2;
@@ -925,6 +925,7 @@ extern "C" int ra_packed_attention(int dtype, const ra_rows* q, const ra_rows* k
               RA_ERR_INVALID, "%s: ends, k_ends or lse are not aligned to their elements", what);
   RAB_REQUIRE(rows_for_tma(*q, D, H, shape->seq_q) && rows_for_tma(*out, D, H, shape->seq_q), RA_ERR_INVALID,
               "%s: rows and heads must begin at multiples of 16 bytes and not overlap", what);
+  RAB_REQUIRE(rows_apart(*out, D, H, shape->seq_q), RA_ERR_INVALID, "%s: rows of the result overlap", what);
   // without keys nothing is copied, but the maps want an address: the queries'
   const ra_rows none = {q->data, 0, D, static_cast<long long>(kvH) * D};
   const ra_rows& kr = shape->seq_k > 0 ? *k : none;

@@ -760,6 +760,8 @@ int read_rows(const char* what, const ra_paged_kv* cache, float k_scale, float v
   RAB_REQUIRE(((reinterpret_cast<uintptr_t>(k_out->data) | reinterpret_cast<uintptr_t>(v_out->data)) & (es - 1u)) == 0 &&
                   (reinterpret_cast<uintptr_t>(start) & 3u) == 0,
               RA_ERR_INVALID, "%s: rows or start are not aligned to their elements", what);
+  RAB_REQUIRE(rows_apart(*k_out, c.head_dim, c.kv_heads, rows) && rows_apart(*v_out, c.head_dim, c.kv_heads, rows), RA_ERR_INVALID,
+              "%s: rows of a result overlap", what);
   ReadArgs a;
   std::memset(&a, 0, sizeof(a));
   const ra_rows* out[2] = {k_out, v_out};

@@ -62,3 +62,19 @@ def test_strides_of_one_row_or_head_do_not_count(name):
     """(the call goes on to the device, which is not there: not a refusal of its arguments)"""
     rc = call(**{name: rows(row=3, head=5)}, seq_q=1, seq_k=1, heads=1, kv_heads=1)
     assert rc in (0, 2), lib().ra_last_error()
+
+
+@pytest.mark.cpu_only
+def test_rows_of_a_result_share_no_memory():
+    """Head h + 1 of a row may not be head h of the next; interleaved rows that only look so are none of that."""
+    D = 64
+    for row, head in ((64, 64), (128, 64), (64, 128), (192, 64), (200, 72), (128, 128), (128, 136)):
+        refused(call(out=rows(row=row, head=head)), 1, "overlap")
+    # heads side by side, rows side by side, rows with room, and two heads whose rows lie between one another's
+    for row, head, more in ((256, 64, {}), (64, 6400, {}), (264, 64, {}), (128, 64, dict(heads=2)), (128, 192, dict(heads=2)),
+                            (128, 64 * 201, dict(heads=2)), (64, 64, dict(seq_q=1)), (64, 64, dict(heads=1, kv_heads=1))):
+        rc = call(out=rows(row=row, head=head), **more)
+        assert rc in (0, 2), lib().ra_last_error()
+    # (rows that are only read may lie as they like)
+    for name in ("q", "k", "v"):
+        assert call(**{name: rows(row=64, head=64)}) in (0, 2), lib().ra_last_error()

@@ -171,3 +171,20 @@ def test_pages_say_what_they_were_made_for():
         with pytest.raises(ValueError):
             api._paged_4bit(pages[:], pages[:], table, lens, D, torch.float16, page_size=16)
     assert api._paged_4bit(pages[:], pages[:], table, lens, 128, torch.float16, page_size=16)[1:] == (2, 1)
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.cpu_only
+def test_rows_read_back_share_no_memory(four):
+    L = lib()
+
+    def call(row, head, n=5, other=False, **c):
+        cache, one, two = paged(lens=None, **c), C.byref(Rows(P, 0, head, row)), C.byref(Rows(P, 0, 64, 128))
+        args = (P, None, two, one) if other else (P, None, one, two)
+        return L.ra_paged_read_4bit(cache, 1.0, 1.0, *args, n, None) if four else L.ra_paged_read(cache, *args, n, None)
+
+    for row, head in ((0, 64), (128, 0), (64, 64), (127, 64), (-100, 64), (128, 256), (192, -192), (32, 6400)):
+        for other in (False, True):
+            refused(call(row, head, other=other), 1, "overlap")
+    for row, head, more in ((128, 64, {}), (-128, 64, {}), (64, 320, {}), (128, 192, {}), (0, 64, dict(n=1)), (64, 0, dict(kv_heads=1))):
+        assert call(row, head, **more) in (0, 2), L.ra_last_error()
