@@ -132,8 +132,9 @@ __device__ inline int blocks_from(const PackedArgs& a, const Seq& s, int c) {
 }
 
 // The items by their number, those with the most key tiles first, then by sequence, block, and KV head and set of heads. Run by a warp. What
-// it has counted and where it has got to among the sequences it keeps, so that many sequences are gone over once for each number of key
-// tiles and not for each item.
+// it has counted and where it has got to among the sequences it keeps, so that many sequences are gone over a few times for each number of
+// key tiles and not for each item, nor for each number behind the last one (the grid has room for a block more of every sequence: of 32768
+// places with one sequence of 300 rows among them, 8 KV heads, those were 886 a block, and other warps' waits ran out).
 template <int kBN>
 struct Items {
   const PackedArgs& a;
@@ -141,6 +142,7 @@ struct Items {
   Seq mine;            // lane's among the first 32 sequences
   int top, level;      // key tiles: the most, those of the last item found
   long long from, above;  // blocks with `level` key tiles or more, and with more than them
+  long long all = -1;     // blocks, once they have been counted
   int chunk;              // sequences chunk to chunk + 31 have had `passed` blocks of just this level before them
   long long passed;
   __device__ Items(const PackedArgs& a_, int lane_) : a(a_), lane(lane_), of_block(a_.kvH * a_.head_sets) {
@@ -169,7 +171,11 @@ struct Items {
     Item it = {};
     const long long block = i / of_block;
     if (from <= block || above > block) {
-      if (from <= block && (level == 0 || count(0) <= block)) return it;
+      if (from <= block) {
+        if (level == 0) return it;
+        if (all < 0) all = count(0);
+        if (all <= block) return it;
+      }
       int lo = from <= block ? 0 : level + 1, hi = from <= block ? level : top + 1;  // count(lo) > block >= count(hi)
       while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;

@@ -379,3 +379,22 @@ def test_wrapper_refusals():
                 lambda: api.packed_attention(torch.empty(25, 4, 68, dtype=q.dtype, device="cuda")[..., :64], k, v, e, out)):
         with pytest.raises(RingAttentionError):
             bad()
+
+
+def test_many_places_without_a_sequence():
+    """One prompt and 32767 places that have none: no wait comes near a limit of 50 ms while blocks go through what there is not."""
+    dtype, H, D, n, B = torch.bfloat16, 8, 64, 300, 32768
+    q, k, v, _, _ = problem(53, dtype, H, H, D, [n])
+    ends = np.full(B + 1, n)
+    ends[0] = 0
+    L = lib()
+    api.device_status()
+    try:
+        L.ra_debug_set_wait_limit_ns(50_000_000)
+        out, lse = run(q, k, v, ends)
+        torch.cuda.synchronize()
+        assert api.device_status()[0] == 0
+    finally:
+        L.ra_debug_set_wait_limit_ns(0)
+        api.device_status()
+    compare(dtype, q, k, v, [0, n], [0, n], True, out, lse)
