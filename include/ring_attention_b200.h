@@ -257,7 +257,7 @@ RA_API int ra_prefill_host(int dtype, const void* q_host, const void* k_host, co
  * there are and key rows k_ends[b] to k_ends[b + 1] of shape->seq_k (device, batch + 1 each, rising; k_ends NULL: ends). With `causal`, query i of a
  * sequence sees its keys j <= i + keys - queries: a whole prompt, or a prompt's next rows behind those that a cache has of it
  * (ra_paged_read brings them). lse (heads, seq_q; fp32, or NULL) gets the log of the sum of exponentials. A row that sees no key gives zeros and
- * -inf; rows of no sequence stay as they are. heads is a multiple of kv heads. Sums and the softmax are held in 32 bits, the weights of the sum over V are rounded
+ * -inf; rows of no sequence stay as they are. heads is a multiple of kv heads; batch is 2^22 and batch * heads 2^25 at most. Sums and the softmax are held in 32 bits, the weights of the sum over V are rounded
  * to dtype as in ra_attention_step_fp16, and the result once. What is not finite in a sequence's K or V does not reach other
  * sequences; in its own, a value with weight 0 may reach queries of the same 128 keys. A bounded wait that runs out is reported as of the step kernels, and
  * rows that are not finished then stay as they are. Scores are held in 32 bits as they come: beyond some 2^26 nothing is promised. out

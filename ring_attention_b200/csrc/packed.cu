@@ -924,7 +924,11 @@ extern "C" int ra_packed_attention(int dtype, const ra_rows* q, const ra_rows* k
               "%s: unsupported head_dim=%d (supported: 32, 64, 128, 256)", what, D);
   RAB_REQUIRE(shape->batch >= 0 && shape->seq_q >= 0 && shape->seq_k >= 0, RA_ERR_INVALID, "%s: bad shape", what);
   RAB_REQUIRE(H > 0 && kvH > 0 && H % kvH == 0 && H <= 1 << 16, RA_ERR_INVALID, "%s: heads are a multiple of kv_heads", what);
-  RAB_REQUIRE(shape->seq_q <= (1 << 30) && shape->seq_k <= (1 << 30) && shape->batch <= (1 << 30), RA_ERR_INVALID, "%s: too many rows", what);
+  RAB_REQUIRE(shape->seq_q <= (1 << 30) && shape->seq_k <= (1 << 30), RA_ERR_INVALID, "%s: too many rows", what);
+  // Blocks take the numbers of places without rows over one after the other, some 2.3 us each (32768 places with one sequence of 300 rows among them,
+  // 8 KV heads: 2.0 ms), while their other warps wait: so many that this takes half a second of the 2 s that a wait may.
+  RAB_REQUIRE(shape->batch <= (1 << 22) && static_cast<long long>(shape->batch) * H <= (1 << 25), RA_ERR_INVALID, "%s: too many sequences",
+              what);
   if (shape->batch == 0 || shape->seq_q == 0) return RA_OK;
   RAB_REQUIRE(ends && q->data && out->data && (shape->seq_k == 0 || (k->data && v->data)), RA_ERR_INVALID, "%s: null argument", what);
   RAB_REQUIRE(((reinterpret_cast<uintptr_t>(ends) | reinterpret_cast<uintptr_t>(k_ends) | reinterpret_cast<uintptr_t>(lse)) & 3u) == 0,

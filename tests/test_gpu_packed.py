@@ -398,3 +398,18 @@ def test_many_places_without_a_sequence():
         L.ra_debug_set_wait_limit_ns(0)
         api.device_status()
     compare(dtype, q, k, v, [0, n], [0, n], True, out, lse)
+
+
+@pytest.mark.parametrize("H", [1, 8])
+def test_as_many_places_as_a_call_takes(H):
+    """2^22 places, of which the first and the last have a prompt: no wait runs out."""
+    dtype, D, B = torch.bfloat16, 64, 1 << 22
+    q, k, v, _, _ = problem(56, dtype, H, H, D, [300, 70])
+    ends = torch.full((B + 1,), 300, dtype=torch.int32, device="cuda")
+    ends[0], ends[B] = 0, 370
+    out, lse = torch.full_like(q, 7.0), torch.full((H, 370), 7.0, device="cuda")
+    api.device_status()
+    api.packed_attention(q, k, v, ends, out, lse=lse)
+    torch.cuda.synchronize()
+    assert api.device_status()[0] == 0
+    compare(dtype, q, k, v, [0, 300, 370], [0, 300, 370], True, out, lse)

@@ -78,3 +78,11 @@ def test_rows_of_a_result_share_no_memory():
     # (rows that are only read may lie as they like)
     for name in ("q", "k", "v"):
         assert call(**{name: rows(row=64, head=64)}) in (0, 2), lib().ra_last_error()
+
+
+def test_more_places_than_waits_have_time_for():
+    """(batch 0 comes before it: nothing to do)"""
+    refused(call(batch=(1 << 22) + 1, heads=1, kv_heads=1), 1, "too many")
+    refused(call(batch=1 << 22, heads=9, kv_heads=1), 1, "too many")
+    refused(call(batch=1 << 30, heads=1, kv_heads=1), 1, "too many")
+    refused(call(batch=1 << 20, heads=33, kv_heads=33), 1, "too many")
