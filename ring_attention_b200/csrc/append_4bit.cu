@@ -8,8 +8,9 @@ namespace rab {
 namespace {
 
 // Rows that are neither normed nor turned, and no queries: a thread makes the codes of one block of 16 elements of kAhead heads at a time.
-// us on the device, chunks of 2500 to 4099 tokens of four prompts, 8 KV heads of 128 in fp16 (69 MB, 10.5 at the copy's rate): 20, and in the
-// other kernel, whose threads hold angles and weights and of which two blocks fit an SM, 33.
+// us in a graph, chunks of 2349 to 4099 tokens of four prompts, 8 KV heads of 128 in fp16 (10.3 at the copy's rate): 16, and in the other
+// kernel, whose threads hold angles and weights and of which two blocks fit an SM, with K's norm and rotation 24; with those of 32 query
+// heads on top, as a step of a server has them, 67 (42.5), where paged_append to a cache in 16 bits takes 61.
 constexpr int kPlainThreads = 256, kPlainAhead = 4;
 template <typename T, int D>
 __global__ void __launch_bounds__(kPlainThreads) plain_4bit_kernel(const __grid_constant__ Args a, unsigned total, int per) {

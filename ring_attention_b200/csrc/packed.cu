@@ -13,17 +13,25 @@
 // tensor memory, barriers and rings are set up once, and the next item's queries, keys and first scores come while the rows of the last
 // one are written.
 //
-// Measured (graph; floor at 1643 TFLOP/s): 16 prompts of up to 4099 rows H32/kvH8 D128 bf16 897 us, 980 TFLOP/s (535 us), chunks of up to 1531 rows behind
-// up to 16384 of four prompts 693, 1144 (483), two documents of up to 32768 rows H8 D64 fp16 2062, 788 (988: there the exp unit is the bound);
-// 13 prompts of up to 200 rows H24/kvH6 D64 14.5: two items one after the other on some SMs, each a chain of copy, scores, softmax, product
-// and way out of some 6 us. The items dealt in advance, to and fro over the blocks, instead of taken over as they go: B1 H8 S32768 D64
-// 1574 -> 1412 us, D128 2102 -> 1972.
+// Measured, us a launch in a CUDA graph, and the floor at the measured rate of a matrix product (1643 TFLOP/s):
 //
-// Roles (384 threads; head_dim 256 and one tile a block: 256): warp 0 copies with TMA, warps 1 and 2 issue tcgen05.mma (2: only where P has a place of its own,
-// head_dim 64), warp 3 finds the items, warps 4 to 7 and 8 to 11 are the softmax of either tile, a row a thread. (One
-// warp of each pair that shares a scheduler in its exponentials while the other waits, by barriers, was slower: head_dim 64 247 -> 302 us for
-// 2 x 18944 rows. How registers are shared out matters less for spills than for the order of instructions that follows: 72 / 216, 88 / 208
-// and 104 / 200 at head_dim 64 247, 253, 230 us, at 128 281, 279, 283.)
+//   16 prompts of up to 4099 rows, H32/kvH8 D128 bf16                   850 to 900   535
+//   4 chunks of up to 1531 rows behind up to 16384, H32/kvH8 D128 bf16  655 to 695   483
+//   2 documents of up to 32768 rows, H8 D64 fp16                        2060 to 2130 989 (1310 by the exp unit)
+//   13 prompts of up to 200 rows, H24/kvH6 D64 bf16                     15 to 16     1.8
+//   B1 H8 S8192, D32 / 64 / 128 / 256 bf16                              111 / 113 / 120 / 289
+//
+// The short ones are two items one after the other on some SMs, each a chain of copy, scores, softmax, product and way out of some 6 us.
+// Items that blocks take over as they go replace a share dealt in advance, to and fro over the blocks: B1 H8 S32768 D64 1574 -> 1412 us, D128
+// 2102 -> 1972.
+//
+// Roles (384 threads; head_dim 256 and one tile a block: 256): warp 0 copies with TMA, warps 1 and 2 issue tcgen05.mma (2: only where P has
+// a place of its own, head_dim 64), warp 3 finds the items, warps 4 to 7 and 8 to 11 are the softmax of either tile, a row a thread.
+//
+// Two things that were slower: turns of the two softmax warps of a scheduler, by barriers (head_dim 64, 2 x 18944 rows: 247 -> 302 us); and other
+// splits of the registers, which change the order of instructions more than the spills (72 / 216, 88 / 208, 104 / 200 of them at head_dim 64
+// 247, 253, 230 us, at 128 281, 279, 283). Bytes spilled (stores / loads): head_dim 64 68 / 176, 128 72 / 76, 256 none; one tile a block, whose
+// threads start with 128 registers, 108 / 260 and 272 / 392.
 //
 // Key tiles are counted from the sequence's first key. Of a query tile's last one only as many products are made as its rows see keys, in
 // steps of 16, and only the halves of its scores that a warp's rows see are worked on; what a last step has of the next sequence is put
@@ -898,10 +906,17 @@ int launch_packed(const ra_rows& q, const ra_rows& k, const ra_rows& v, PackedAr
   while ((1 << a.tile_shift) < a.tile_tokens) ++a.tile_shift;
   a.head_sets = (a.G + a.pack - 1) / a.pack;
   if constexpr (D <= 128) {
-    // Sequences of one query tile on average, at head_dim 64 and below of two if their keys are few, are taken a tile a block. us a call of 16384 rows, two tiles a
-    // block / one: H32/kvH8 D128, sequences of 16 rows (half a tile) 301 / 211, 32 rows 151 / 117, 64 rows 93 / 93, 128 rows 87 / 103; H24/kvH6 D64,
-    // 32 rows (a tile) 125 / 79, 64 rows 66 / 59, 128 rows 63 / 66; H16 D64, 128 rows (a tile) 88 / 50, 256 rows 69 / 60, 512 rows 76 / 74. 64 chunks on 8192 keys: H32/kvH8 D128, 32 rows 437 / 389; H24/kvH6 D64, 64 rows
-    // (two tiles) 327 / 426.
+    // Sequences of one query tile on average, and at head_dim 64 and below of two if their keys are few, are taken a tile a block. us in a
+    // graph, a tile a block / two:
+    //   16384 rows, H32/kvH8 D128 (a tile is 32 tokens), sequences of 16, 32, 64, 128 rows: 162 / 252, 91 / 127, 87 / 81, 102 / 87
+    //   16384 rows, H24/kvH6 D64 (32 tokens), sequences of 32, 64, 128 rows: 57 / 101, 54 / 55, 62 / 61
+    //   16384 rows, H16 D64 (128 tokens), sequences of 128, 256, 512 rows: 49 / 85, 56 / 67, 69 / 75
+    //   64 chunks on 8192 keys, 32 rows of H32/kvH8 D128: 416 / 552, 64 rows of H24/kvH6 D64: 366 / 328
+    // A call of few sequences, where all items run at once, feels it little: 5 to 40 prompts of up to 50 to 200 rows 0.85 to 1.11.
+    // The host knows rows and places but no lengths: a place without a sequence counts as a short one, room without rows as rows. One
+    // prompt of 8192 rows in 1, 16, 256 places (H32/kvH8 D128), as chosen: 432, 482, 625 us, the last 525 with two tiles a block; a fixed
+    // number of places well above the sequences of most steps, or a long prompt among hundreds of short ones, pays for it here and in the
+    // finder of items, which goes over all places for every number of key tiles.
     constexpr int kFewKeys = 512;
     const bool two = D == 64 && a.k_rows <= static_cast<long long>(kFewKeys) * a.B;
     if (tokens <= (two ? 2 : 1) * a.tile_tokens) return launch_tiles<D, DR, T, true>(q, k, v, a, stream);

@@ -16,12 +16,17 @@
 // conversion and their scales one multiplication.
 //
 // What bounds it: 290 warp instructions to 16 keys of 128 columns (116 of them V's, 82 K's), of which the conversions, V's change of places
-// and the scores' comparisons, 130, are the ALU pipe's at half rate. Alone, without copies, that took 92 us where the copies alone took 77 (64
-// sequences of up to 8191 rows, H32/kvH8 D128, 454 MB; 69 at the copy's rate); together 111 us, 4.1 TB/s, 59 % of the issue slots, three
-// warps a scheduler. Four sequences of up to 262144 rows 202 us, 4.7 TB/s (the same rows in 16 bits: 502 us). head_dim 256 with 16 heads to a
-// KV head has two warps a scheduler (255 registers) and the latency of each instruction: 5 sequences of up to 33333 rows 50 us (11.5).
-// Eight warps a block with copies of 32 keys instead of six with 64: 114 and 216 us.
-// Times in this file are of launches one behind the other in a CUDA graph.
+// and the scores' comparisons, 130, are the ALU pipe's at half rate: 59 % of the issue slots, three warps a scheduler. Without copies, 64
+// sequences of up to 8191 rows (H32/kvH8 D128, 454 MB) took 92 us, the copies alone 77.
+//
+// Measured, us in a CUDA graph, and the floor of the cache's bytes at the copy's rate:
+//
+//   64 sequences of up to 8191 rows, H32/kvH8 D128         111   69
+//   64 sequences of 4096 to 8191, H32/kvH8 D32, 64, 128    53, 71, 104   17, 35, 69 (the instructions of a row are nearly as many)
+//   4 sequences of up to 262144 rows, H32/kvH8 D128        202   145 (the same rows in 16 bits: 502)
+//   5 sequences of up to 33333 rows, H32/kvH2 D256         50    11.5 (16 heads: 255 registers, two warps a scheduler, 102 bytes spilled)
+//
+// Eight warps a block with copies of 32 keys instead of six with 64: 114 and 216 us for the first and the third.
 #include "paged_walk.cuh"
 
 namespace rab {
