@@ -259,7 +259,7 @@ RA_API int ra_prefill_host(int dtype, const void* q_host, const void* k_host, co
  * (ra_paged_read brings them). lse (heads, seq_q; fp32, or NULL) gets the log of the sum of exponentials. A row that sees no key gives zeros and
  * -inf; rows of no sequence stay as they are. heads is a multiple of kv heads; batch is 2^22 and batch * heads 2^25 at most. Sums and the softmax are held in 32 bits, the weights of the sum over V are rounded
  * to dtype as in ra_attention_step_fp16, and the result once. What is not finite in a sequence's K or V does not reach other
- * sequences; in its own, a value with weight 0 may reach queries of the same 128 keys. A bounded wait that runs out is reported as of the step kernels, and
+ * sequences; in its own, a value of V may reach queries that do not see it yet, from up to 254 keys before it. A bounded wait that runs out is reported as of the step kernels, and
  * rows that are not finished then stay as they are. Scores are held in 32 bits as they come: beyond some 2^26 nothing is promised. out
  * must not share memory with q, k or v. */
 RA_API int ra_packed_attention(int dtype, const struct ra_rows* q, const struct ra_rows* k, const struct ra_rows* v,

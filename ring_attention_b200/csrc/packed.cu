@@ -35,8 +35,8 @@
 //
 // Key tiles are counted from the sequence's first key. Of a query tile's last one only as many products are made as its rows see keys, in
 // steps of 16, and only the halves of its scores that a warp's rows see are worked on; what a last step has of the next sequence is put
-// out of V's tile before. A value that is not finite reaches the queries of its own
-// sequence whose weight for it is 0 only within that tile.
+// out of V's tile before. A value of V that is not finite reaches queries of its own sequence whose weight for it is 0 where their query
+// tile takes its key tile: 127 keys in front of it and 127 tokens in front of those at most.
 #include <atomic>
 #include <type_traits>
 

@@ -413,3 +413,23 @@ def test_as_many_places_as_a_call_takes(H):
     torch.cuda.synchronize()
     assert api.device_status()[0] == 0
     compare(dtype, q, k, v, [0, 300, 370], [0, 300, 370], True, out, lse)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,kvH,D", [(2, 2, 32), (2, 2, 64), (8, 2, 64), (2, 2, 128), (4, 1, 128), (2, 2, 256)])
+@pytest.mark.parametrize("before", [0, 1, 64, 127])
+def test_how_far_a_value_that_is_not_finite_reaches(dtype, H, kvH, D, before):
+    """Queries that see it, and none that is 255 keys or more before it."""
+    n, at = 900, 700
+    q, k, v, ends, k_ends = problem(59, dtype, H, kvH, D, [n], [n + before])
+    clean = run(q, k, v, ends, k_ends)
+    v = v.clone()
+    v[at, 0, 3] = float("inf")
+    out, lse = run(q, k, v, ends, k_ends)
+    assert torch.equal(lse, clean[1])
+    assert kvH == 1 or torch.equal(out[:, 1::kvH], clean[0][:, 1::kvH])
+    first = at - before  # the first query that sees it
+    assert not torch.isfinite(out[first:, ::kvH, 3]).any()
+    keep = torch.arange(D, device="cuda") != 3
+    assert torch.equal(out[..., keep], clean[0][..., keep])
+    assert torch.equal(out[:first - 254], clean[0][:first - 254])
